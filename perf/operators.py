@@ -1,0 +1,350 @@
+"""The measured cases of the block-scaled FP8 linears and of what stands around them in a block.
+
+Five operators, each over its range of sizes: the e4m3 quant with one scale per block of 128 (``quant``), SwiGLU with that
+quant behind it (``silu``), the FP8 product of block-scaled operands (``gemm``), the same product grouped by expert with
+ragged row counts that only the device knows (``grouped``), and the RMSNorm of queries and keys per head with the position
+rotation in the same pass (``qk``).
+
+``run`` is one pass: with ``own`` through ``h3_tp2_amd.ops``, otherwise in elementary torch operations in fp32, rounded
+once.  ``exact`` restates the definitions in float64.
+"""
+from __future__ import annotations
+
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+E4M3 = torch.float8_e4m3fn
+BLOCK = 128
+FP8_MAX = 448.0
+MIN_SCALE = 1.0 / (448.0 * 512.0)
+EPS = 1e-6
+_TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+def listed():
+    return [
+        # the out projection's input of a long clip on one rank: activations, ragged token count
+        dict(name="quant_act_m42848", kind="quant", M=42848, K=7168, rows=1, dtype="bf16"),
+        # a checkpoint's QKV weight brought to 128 x 128 blocks
+        dict(name="quant_weight_21504", kind="quant", M=21504, K=5376, rows=128, dtype="bf16"),
+        # the experts' gate|up products of a few decoded tokens
+        dict(name="silu_m64", kind="silu", M=64, F=2048, dtype="bf16"),
+        # the H3 MLP's gate|up product of one rank's tokens
+        dict(name="silu_m18880", kind="silu", M=18880, F=14336, dtype="bf16"),
+        # one token through the QKV projection: the weight is read once, launches and the host count
+        dict(name="gemm_m1", kind="gemm", M=1, K=5376, N=21504, dtype="bf16", bias=False, tokens_first=False),
+        # a short ragged sequence through the out projection, fp16 with a bias, scales in [M, blocks] order
+        dict(name="gemm_m200", kind="gemm", M=200, K=7168, N=5376, dtype="fp16", bias=True, tokens_first=True),
+        # one rank's tokens of a clip through the QKV projection
+        dict(name="gemm_m18880", kind="gemm", M=18880, K=5376, N=21504, dtype="bf16", bias=False, tokens_first=False),
+        # decode: two rows per expert on average, most of the time is the experts' weights
+        dict(name="grouped_m64_e32", kind="grouped", M=64, E=32, K=4096, N=2048, spare=0, dtype="bf16"),
+        # a chunk of a prompt in a buffer of fixed capacity: ragged experts, rows behind the last one stay as they were
+        dict(name="grouped_m4100_e16", kind="grouped", M=4100, E=16, K=4096, N=4096, spare=117, dtype="bf16"),
+        # a long prompt, about a thousand rows per expert
+        dict(name="grouped_m32768_e32", kind="grouped", M=32768, E=32, K=4096, N=4096, spare=0, dtype="bf16"),
+        # decode: eight sequences at their own positions, grouped-query heads, whole-head rotation
+        dict(name="qk_t8", kind="qk", T=8, H=32, Hk=8, D=128, R=128, positions=True, interleaved=False, dtype="bf16"),
+        # the H3 heads (128, 96 of them rotated) of one rank's tokens, q and k read out of the QKV product
+        dict(name="qk_t18880", kind="qk", T=18880, H=56, Hk=56, D=128, R=96, positions=False, interleaved=False,
+             dtype="bf16"),
+    ]
+
+
+# (K, N) of the linears that the framework's models have, and of small and odd ones
+_LINEARS = ((5376, 21504), (7168, 5376), (14336, 5376), (4096, 6144), (1536, 4608), (1536, 1536), (1200, 2064),
+            (528, 720))
+_EXPERTS = ((4096, 2048), (2048, 4096), (4096, 4096), (1536, 4608), (1200, 1040))
+
+
+def _log_int(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    kind = rng.choices(("quant", "silu", "gemm", "grouped", "qk"), (2, 2, 4, 4, 3))[0]
+    dtype = "fp16" if rng.random() < 0.25 else "bf16"
+    if kind == "quant":
+        if rng.random() < 0.3:
+            K, N = rng.choice(_LINEARS)
+            return dict(kind=kind, M=N - 16 * rng.randrange(8), K=K, rows=128, dtype=rng.choice(("bf16", "fp16", "fp32")))
+        return dict(kind=kind, M=_log_int(rng, 1, 42848), K=16 * _log_int(rng, 16, 448), rows=1, dtype=dtype)
+    if kind == "silu":
+        return dict(kind=kind, M=_log_int(rng, 1, 18880), F=16 * _log_int(rng, 16, 896), dtype=dtype)
+    if kind == "gemm":
+        K, N = rng.choice(_LINEARS)
+        if rng.random() < 0.15:
+            dtype = "fp32"
+        return dict(kind=kind, M=_log_int(rng, 1, 18880), K=K, N=N, dtype=dtype, bias=rng.random() < 0.3,
+                    tokens_first=rng.random() < 0.25)
+    if kind == "grouped":
+        K, N = rng.choice(_EXPERTS)
+        M = _log_int(rng, 8, 32768)
+        return dict(kind=kind, M=M, E=rng.choice((3, 8, 16, 32)), K=K, N=N, spare=rng.randrange(M // 4) if rng.random() < 0.5 else 0,
+                    dtype=dtype)
+    D = rng.choice((64, 128, 256))
+    Hk = rng.choice((1, 2, 8, 28))
+    return dict(kind=kind, T=_log_int(rng, 1, 18880), H=Hk * rng.choice((1, 2, 4)), Hk=Hk, D=D,
+                R=rng.choice((D, D // 2, D // 4 * 3)), positions=rng.random() < 0.5, interleaved=rng.random() < 0.4, dtype=dtype)
+
+
+# ---- inputs ----------------------------------------------------------------------------------------------------------
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(int(seed))
+
+
+def _randn(g, *shape):
+    return torch.randn(*shape, generator=g, device="cuda")
+
+
+def _activations(g, M, K):
+    """fp32 activations [M, K] as a linear meets them: rows of log-normal magnitude, 0.1 % outlier channels x40."""
+    x = _randn(g, M, K)
+    x *= torch.exp(_randn(g, M, 1))
+    x[:, torch.randperm(K, generator=g, device="cuda")[:max(1, K // 1000)]] *= 40.0
+    return x
+
+
+def _spread(s, rows, K):
+    """Block scales [ceil(n / r), ceil(K / 128)] laid over the rows x K values they belong to (r = 1 or 128)."""
+    r = BLOCK if s.shape[0] != rows else 1
+    return s.repeat_interleave(r, 0)[:rows].repeat_interleave(BLOCK, 1)[:, :K]
+
+
+def _pad_blocks(x, rows):
+    """x [M, K] in fp32, padded with zeros to whole blocks and seen as [row blocks, rows, column blocks, 128]."""
+    M, K = x.shape
+    x = torch.nn.functional.pad(x.float(), (0, -K % BLOCK, 0, -M % rows))
+    return x.view(x.shape[0] // rows, rows, x.shape[1] // BLOCK, BLOCK)
+
+
+def _quant(x, rows):
+    """The plain quant: e4m3 codes [M, K] and one fp32 scale per block of rows x 128."""
+    M, K = x.shape
+    b = _pad_blocks(x, rows)
+    s = (b.abs().amax(dim=(1, 3)) / FP8_MAX).clamp_min(MIN_SCALE)
+    inv = 1.0 / s
+    q = (b * inv[:, None, :, None]).clamp(-FP8_MAX, FP8_MAX).to(E4M3)
+    return q.view(-1, b.shape[2] * BLOCK)[:M, :K].contiguous(), s
+
+
+def _weight(g, N, K):
+    return _quant(_randn(g, N, K) * 0.02, BLOCK)
+
+
+def prepare(case, seed):
+    g = _gen(seed)
+    kind = case["kind"]
+    dt = _TYPES[case["dtype"]]
+    st = dict(kind=kind, dtype=dt)
+    if kind == "quant":
+        st["rows"] = case["rows"]
+        x = _activations(g, case["M"], case["K"]) if case["rows"] == 1 else _randn(g, case["M"], case["K"]) * 0.02
+        st["x"] = x.to(dt)
+    elif kind == "silu":
+        st["x"] = (_randn(g, case["M"], 2 * case["F"]) * torch.exp(0.5 * _randn(g, case["M"], 1))).to(dt)
+    elif kind == "gemm":
+        a, sa = _quant(_activations(g, case["M"], case["K"]), 1)
+        # token-contiguous scales as the quant writes them, or [M, blocks] rows as another producer may
+        st["a"], st["sa"] = a, sa if case["tokens_first"] else sa.t().contiguous().t()
+        st["w"], st["sw"] = _weight(g, case["N"], case["K"])
+        st["bias"] = _randn(g, case["N"]).mul_(0.1).to(dt) if case["bias"] else None
+    elif kind == "grouped":
+        M, E, K, N = case["M"], case["E"], case["K"], case["N"]
+        a, sa = _quant(_activations(g, M, K), 1)
+        st["a"], st["sa"] = a, sa.t().contiguous().t()
+        w, sw = _weight(g, E * N, K) if N % BLOCK == 0 else zip(*(_weight(g, N, K) for _ in range(E)))
+        st["w"] = w.view(E, N, K) if N % BLOCK == 0 else torch.stack(w)
+        st["sw"] = sw.view(E, N // BLOCK, -1) if N % BLOCK == 0 else torch.stack(sw)
+        # the rows of each expert: a router's uneven choices, a tenth of the experts with none
+        p = torch.exp(0.4 * _randn(g, E)) * (torch.rand(E, generator=g, device="cuda") > 0.1)
+        p[int(seed) % E] += 0.5
+        pick = torch.multinomial(p, M - case["spare"], replacement=True, generator=g)
+        sizes = torch.bincount(pick, minlength=E)
+        st["offsets"] = torch.nn.functional.pad(sizes.cumsum(0), (1, 0)).to(torch.int32)
+        st["most"] = int(sizes.max())
+        # the buffer of fixed capacity that the program keeps
+        st["out"] = _randn(g, M, N).to(dt) if case["spare"] else None
+    else:
+        T, H, Hk, D, R = (case[k] for k in ("T", "H", "Hk", "D", "R"))
+        qkv = (_randn(g, T, (H + 2 * Hk) * D) * torch.exp(0.5 * _randn(g, T, 1))).to(dt)
+        st["q"] = qkv[:, :H * D].view(T, H, D)
+        st["k"] = qkv[:, H * D:(H + Hk) * D].view(T, Hk, D)
+        st["wq"], st["wk"] = (1.0 + 0.1 * _randn(g, D)).to(dt), (1.0 + 0.1 * _randn(g, D)).to(dt)
+        rows = 4096 if case["positions"] else T
+        at = torch.arange(rows, device="cuda")[:, None].double()
+        ang = at * torch.exp(torch.arange(R // 2, device="cuda").double() * (-math.log(10000.0) / (R // 2)))
+        st["table"] = torch.cat((ang.cos(), ang.sin()), dim=1).float()
+        st["positions"] = torch.randint(0, rows, (T,), generator=g, device="cuda") if case["positions"] else None
+        st["interleaved"] = case["interleaved"]
+    return st
+
+
+# ---- one pass --------------------------------------------------------------------------------------------------------
+
+def _ops():
+    path = os.path.join(os.getcwd(), "minimax-h3-2x-dgx-spark-tp2_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    from h3_tp2_amd import ops
+    return ops
+
+
+def run(st):
+    return _run_own(st, _ops()) if own else _run_plain(st)
+
+
+def _run_own(st, ops):
+    kind = st["kind"]
+    if kind == "quant":
+        return ops.quant_blocks(st["x"], rows=st["rows"])
+    if kind == "silu":
+        return ops.silu_mul_quant_blocks(st["x"])
+    if kind == "gemm":
+        return ops.gemm_blocks(st["a"], st["w"], st["sa"], st["sw"], st["dtype"], st["bias"])
+    if kind == "grouped":
+        return ops.grouped_gemm_blocks(st["a"], st["w"], st["sa"], st["sw"], st["offsets"], st["dtype"], out=st["out"])
+    return ops.qk_norm_rope(st["q"], st["k"], st["wq"], st["wk"], st["table"], EPS, positions=st["positions"],
+                            interleaved=st["interleaved"])
+
+
+def _norm_rope(x, w, table, interleaved):
+    T, heads, D = x.shape
+    h = table.shape[1] // 2
+    x = x.float()
+    n = x * torch.rsqrt(x.square().mean(dim=2, keepdim=True) + EPS) * w.float()
+    c, s = table[:, None, :h], table[:, None, h:]
+    if interleaved:
+        a, b = n[..., 0:2 * h:2], n[..., 1:2 * h:2]
+        rot = torch.stack((a * c - b * s, b * c + a * s), dim=3).flatten(2)
+    else:
+        a, b = n[..., :h], n[..., h:2 * h]
+        rot = torch.cat((a * c - b * s, b * c + a * s), dim=2)
+    return torch.cat((rot, n[..., 2 * h:]), dim=2)
+
+
+def _run_plain(st):
+    kind, dt = st["kind"], st["dtype"]
+    if kind == "quant":
+        return _quant(st["x"], st["rows"])
+    if kind == "silu":
+        g, u = st["x"].float().chunk(2, dim=1)
+        return _quant(g / (1.0 + torch.exp(-g)) * u, 1)
+    if kind == "gemm":
+        (M, K), N = st["a"].shape, st["w"].shape[0]
+        y = (st["a"].float() * _spread(st["sa"], M, K)) @ (st["w"].float() * _spread(st["sw"], N, K)).t()
+        return (y if st["bias"] is None else y + st["bias"].float()).to(dt)
+    if kind == "grouped":
+        # every expert's rows padded to the largest expert's count, one batched product, the rows picked out again
+        (M, K), (E, N, _), off, most = st["a"].shape, st["w"].shape, st["offsets"].long(), st["most"]
+        a = st["a"].float() * st["sa"].repeat_interleave(BLOCK, 1)[:, :K]
+        at = (off[:-1, None] + torch.arange(most, device=off.device)).clamp_max(M - 1)
+        s = st["sw"].repeat_interleave(BLOCK, 1)[:, :N].transpose(1, 2).repeat_interleave(BLOCK, 1)[:, :K]
+        y = torch.bmm(a[at], st["w"].view(torch.uint8).transpose(1, 2).contiguous().view(E4M3).float() * s)
+        row = torch.arange(M, device=off.device)
+        e = (torch.searchsorted(off, row, right=True) - 1).clamp_max(E - 1)
+        y = y[e, (row - off[e]).clamp_max(most - 1)].to(dt)
+        return y if st["out"] is None else torch.where((row < off[-1])[:, None], y, st["out"])
+    table = st["table"] if st["positions"] is None else st["table"][st["positions"]]
+    return tuple(_norm_rope(st[x], st["w" + x], table, st["interleaved"]).to(dt) for x in ("q", "k"))
+
+
+# ---- what a pass cannot do without -----------------------------------------------------------------------------------
+
+def work(case):
+    kind = case["kind"]
+    e = 4 if case["dtype"] == "fp32" else 2
+    if kind == "quant":
+        M, K = case["M"], case["K"]
+        return dict(bytes=(e + 1) * M * K + 4 * math.ceil(M / case["rows"]) * math.ceil(K / BLOCK), flops=3 * M * K)
+    if kind == "silu":
+        M, F = case["M"], case["F"]
+        return dict(bytes=5 * M * F + 4 * M * math.ceil(F / BLOCK), flops=8 * M * F)
+    if kind in ("gemm", "grouped"):
+        M, K, N = case["M"] - case.get("spare", 0), case["K"], case["N"]
+        E = case.get("E", 1)
+        if kind == "grouped":
+            E = min(E, M)                              # experts without rows are not read
+        kb, nb = math.ceil(K / BLOCK), math.ceil(N / BLOCK)
+        return dict(bytes=M * K + 4 * M * kb + E * (N * K + 4 * nb * kb) + e * M * N, flops=2 * M * N * K)
+    heads = case["H"] + case["Hk"]
+    return dict(bytes=4 * case["T"] * (heads * case["D"] + case["R"]), flops=8 * case["T"] * heads * case["D"])
+
+
+# ---- the same in float64 ---------------------------------------------------------------------------------------------
+
+_CHUNK = 4096
+
+
+def _quant64(x, rows):
+    """Codes and scales of float64 values block by block, ragged edges cut rather than padded."""
+    M, K = x.shape
+    q, cols = torch.empty(M, K, dtype=torch.float64, device=x.device), []
+    for k in range(0, K, BLOCK):
+        c = x[:, k:k + BLOCK].abs().amax(dim=1)
+        if rows > 1:
+            c = torch.stack([p.max() for p in c.split(rows)])
+        s = torch.maximum(c / FP8_MAX, torch.full_like(c, MIN_SCALE))
+        each = s.repeat_interleave(rows)[:M, None]
+        q[:, k:k + BLOCK] = (x[:, k:k + BLOCK] / each).clamp(-FP8_MAX, FP8_MAX).to(E4M3).double()
+        cols.append(s)
+    return q, torch.stack(cols, dim=1)
+
+
+def _product64(a, sa, w, sw, bias=None):
+    """The sum over blocks of the scaled products of the codes."""
+    M, K = a.shape
+    N = w.shape[0]
+    parts = []
+    for m in range(0, M, _CHUNK):
+        y = torch.zeros(min(_CHUNK, M - m), N, dtype=torch.float64, device=a.device)
+        for b in range(sa.shape[1]):
+            k = slice(b * BLOCK, min(K, (b + 1) * BLOCK))
+            col = sw[:, b].double().repeat_interleave(BLOCK)[:N]
+            y += (a[m:m + _CHUNK, k].double() @ w[:, k].double().t()) * col * sa[m:m + _CHUNK, b].double()[:, None]
+        parts.append(y if bias is None else y + bias.double())
+    return torch.cat(parts)
+
+
+def _rotate64(x, w, table, interleaved):
+    """Norm and rotation as complex numbers: the pair (a, b) times cos + i sin."""
+    T, heads, D = x.shape
+    h = table.shape[1] // 2
+    x = x.double()
+    n = x / torch.sqrt(x.pow(2).sum(dim=2, keepdim=True) / D + EPS) * w.double()
+    pairs = n[..., :2 * h].reshape(T, heads, h, 2) if interleaved else n[..., :2 * h].reshape(T, heads, 2, h).transpose(2, 3)
+    z = torch.view_as_complex(pairs.contiguous()) * torch.complex(table[:, :h].double(), table[:, h:].double())[:, None]
+    r = torch.view_as_real(z)
+    n[..., :2 * h] = r.flatten(2) if interleaved else r.transpose(2, 3).flatten(2)
+    return n
+
+
+def exact(case, seed):
+    st = prepare(case, seed)
+    kind = st["kind"]
+    if kind == "quant":
+        return _quant64(st["x"].double(), st["rows"])
+    if kind == "silu":
+        F = case["F"]
+        parts = [_quant64(x[:, :F] * torch.sigmoid(x[:, :F]) * x[:, F:], 1)
+                 for x in (c.double() for c in st["x"].split(_CHUNK))]
+        return tuple(torch.cat(p) for p in zip(*parts))
+    if kind == "gemm":
+        return _product64(st["a"], st["sa"], st["w"], st["sw"], st["bias"])
+    if kind == "grouped":
+        y = torch.zeros(case["M"], case["N"], dtype=torch.float64, device="cuda") if st["out"] is None else st["out"].double()
+        off = st["offsets"].tolist()
+        for e in range(case["E"]):
+            r = slice(off[e], off[e + 1])
+            if r.start < r.stop:
+                y[r] = _product64(st["a"][r], st["sa"][r], st["w"][e], st["sw"][e])
+        return y
+    table = st["table"] if st["positions"] is None else st["table"].index_select(0, st["positions"])
+    return tuple(torch.cat([_rotate64(x[t:t + _CHUNK], w, table[t:t + _CHUNK], st["interleaved"])
+                            for t in range(0, case["T"], _CHUNK)]) for x, w in ((st["q"], st["wq"]), (st["k"], st["wk"])))
