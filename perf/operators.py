@@ -78,8 +78,6 @@ def draw(rng):
         return dict(kind=kind, M=_log_int(rng, 1, 18880), F=16 * _log_int(rng, 16, 896), dtype=dtype)
     if kind == "gemm":
         K, N = rng.choice(_LINEARS)
-        if rng.random() < 0.15:
-            dtype = "fp32"
         return dict(kind=kind, M=_log_int(rng, 1, 18880), K=K, N=N, dtype=dtype, bias=rng.random() < 0.3,
                     tokens_first=rng.random() < 0.25)
     if kind == "grouped":
