@@ -264,6 +264,55 @@ typedef struct h3fp8_group {
 int h3fp8_grouped_gemm(const h3fp8_group* groups, int n_groups, void* stream);
 
 /*
+ * The block-scaled FP8 linear: operands with one scale per block of 128 (no counterpart in the reference, whose path has
+ * one scale per token and one per channel).
+ *
+ *   h3fp8_quant_blocks           x [M, K] bf16 / fp16 / fp32 (dtype) -> q [M, K] e4m3fn and one fp32 scale per block of
+ *                                `rows` (1: activations, 128: weights) x 128: scale = max(max|x| / 448, 1/(448*512)), q =
+ *                                e4m3fn_rne(clamp(x * (1/scale), +-448)), NaN propagating.  The scale of row block i and
+ *                                column block j is at scale[i * ss_m + j * ss_k].
+ *   h3fp8_silu_mul_quant_blocks  x [M, 2F] = [gate | up] bf16 / fp16 -> the 1 x 128 quant of g / (1 + exp(-g)) * u, held in
+ *                                fp32 until its code: q [M, F], scale as above.
+ *   h3fp8_gemm_blocks            y[m, n] = round(sum_b sa[m * sa_m + b * sa_k] * sw[(n / 128) * sw_n + b * sw_k] * P_b (+
+ *                                bias[n])), P_b the product over the 128 columns of block b; fp32, b ascending; y bf16 or
+ *                                fp16 (out_dtype), bias [N] in that type or NULL.
+ *   h3fp8_grouped_gemm_blocks    the same product by expert: w [E, N, K] (expert stride w_e), sw [E, N / 128, K / 128]
+ *                                (strides sw_e, sw_n, sw_k), rows offsets[e] .. offsets[e + 1] - 1 of a by w[e].  offsets:
+ *                                [E + 1] int32 / int64 (idx_bytes 4 / 8) on the device, non-decreasing; the host never
+ *                                reads them, and offsets outside [0, M] count as its ends.  Rows of y that no expert has
+ *                                are left as they were.
+ * K, N, F multiples of 16 (a last block of fewer than 128 has a scale of its own); a, w rows 16-byte aligned; y rows
+ * 16-byte aligned with a stride that is a multiple of 8; x rows 16-byte and q rows 8-byte aligned.
+ */
+int h3fp8_quant_blocks(const void* x, int64_t ldx, int dtype, int64_t M, int64_t K, int rows, void* q, int64_t ldq,
+                       float* scale, int64_t ss_m, int64_t ss_k, void* stream);
+int h3fp8_silu_mul_quant_blocks(const void* x, int64_t ldx, int dtype, int64_t M, int64_t F, void* q, int64_t ldq,
+                                float* scale, int64_t ss_m, int64_t ss_k, void* stream);
+int h3fp8_gemm_blocks(const void* a, int64_t lda, const void* w, int64_t ldw, const float* sa, int64_t sa_m, int64_t sa_k,
+                      const float* sw, int64_t sw_n, int64_t sw_k, const void* bias, void* y, int64_t ldy, int out_dtype,
+                      int64_t M, int64_t N, int64_t K, void* stream);
+int h3fp8_grouped_gemm_blocks(const void* a, int64_t lda, const void* w, int64_t w_e, int64_t ldw, const float* sa,
+                              int64_t sa_m, int64_t sa_k, const float* sw, int64_t sw_e, int64_t sw_n, int64_t sw_k,
+                              const void* offsets, int idx_bytes, void* y, int64_t ldy, int out_dtype, int64_t M, int64_t N,
+                              int64_t K, int64_t E, void* stream);
+
+/*
+ * RMSNorm of queries and keys per head with the position rotation in the same pass: q [T, H, D], k [T, Hk, D] bf16 / fp16
+ * (dtype) with token and head strides, D = 64, 128 or 256, dims contiguous.  n = x / sqrt(sum x^2 / D + eps) * weight, then
+ * pair p of the first R dims (half-split: dims p and p + R/2; interleaved: 2p and 2p + 1) rotated by cos = table[pos, p],
+ * sin = table[pos, R/2 + p]: (a cos - b sin, b cos + a sin); fp32 throughout, rounded once.  table [P, R] fp32 or bf16; pos =
+ * positions[t * pos_stride] (int32 / int64: pos_bytes 4 / 8) or t (positions NULL).  A position outside [0, P) is not read
+ * through: that token's outputs are NaN.  R a multiple of 16 (interleaved: of 2), 0: the norm alone.  The outputs may be the
+ * inputs themselves (with the same strides).  The fused consumer of the two-pass product is h3fp8_scale_qk_norm_rope (h3_tp2/
+ * fp8_consumers.py:424-461), which reproduces a stock kernel's rounding of n to bf16.
+ */
+int h3fp8_qk_norm_rope(const void* q, int64_t q_t, int64_t q_h, const void* k, int64_t k_t, int64_t k_h, int dtype, int64_t T,
+                       int H, int Hk, int D, const void* q_weight, const void* k_weight, const void* table, int64_t ld_table,
+                       int table_dtype, int64_t P, int R, int interleaved, const void* positions, int64_t pos_stride,
+                       int pos_bytes, float eps, void* out_q, int64_t oq_t, int64_t oq_h, void* out_k, int64_t ok_t,
+                       int64_t ok_h, void* stream);
+
+/*
  * Self-checks used by the install probe and the tests (no reference counterpart beyond its install probes,
  * h3_tp2/fp8_cutlass.py:196-249):
  *   h3fp8_selfcheck_e4m3   converts every fp32 bit pattern with |x| <= 448 (and the NaNs) with the hardware cvt used

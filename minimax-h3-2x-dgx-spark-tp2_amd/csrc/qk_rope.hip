@@ -1,0 +1,204 @@
+// RMSNorm of queries and keys per head with the position rotation in the same pass (gfx950).
+//
+// Per token t and head, x of D dims (D = 64, 128 or 256), R of them rotated (half = R / 2 pairs):
+//   n_d = x_d / sqrt(sum x^2 / D + eps) * w_d                                    (fp32)
+//   half-split:   pair p = dims (p, p + half);   interleaved: pair p = dims (2p, 2p + 1)
+//   (a, b) -> (a cos_p - b sin_p, b cos_p + a sin_p), cos | sin = table[pos], pos = positions[t] or t
+// rounded once to the input's type: unlike the fused consumer of the two-pass product (consumers.hip), which reproduces a
+// stock kernel that rounds n to bf16 before it rotates.
+//
+// HBM-bound: every head is read and written once.  A lane holds 8 consecutive dims (16-byte loads and stores), D / 8 lanes
+// a head, so a wave holds 512 / D heads of one token at a time and takes the token's q heads and then its k heads; the
+// rotation's table entries of the lane's dims are loaded once per token and kept.  The sum of squares is an xor butterfly
+// over the head's lanes.  The half-split partner of dim d is 16-byte aligned with it when half % 8 == 0, so it is one lane
+// exchange per dim; the interleaved partner is in the lane.
+#include "h3fp8_common.h"
+
+namespace {
+
+using namespace h3;
+
+struct QkRopeArgs {
+    const uint16_t* q;
+    const uint16_t* k;
+    int64_t q_t, q_h, k_t, k_h;                 // strides (elements) of tokens and heads
+    uint16_t* oq;
+    uint16_t* ok;
+    int64_t oq_t, oq_h, ok_t, ok_h;
+    const uint16_t* wq;
+    const uint16_t* wk;
+    const void* table;                          // [P, R]: cos of the half pairs, then sin
+    int64_t ld_table;
+    const void* positions;                      // null: the token's own number
+    int64_t pos_stride;
+    int pos_bytes;
+    int64_t P;
+    int64_t T;
+    int H, Hk, half;
+    float eps;
+    int per;                                    // passes (512 / D heads each) a wave takes
+    int chunks;                                 // waves per token
+};
+
+template <bool FP16>
+__device__ __forceinline__ void widen8(v4u v, float f[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[2 * i] = FP16 ? fp16_to_f32(v[i] & 0xffffu) : u2f(v[i] << 16);
+        f[2 * i + 1] = FP16 ? fp16_to_f32(v[i] >> 16) : u2f(v[i] & 0xffff0000u);
+    }
+}
+
+template <bool FP16>
+__device__ __forceinline__ v4u narrow8(const float f[8]) {
+    v4u v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        v[i] = FP16 ? fp16_rne(f[2 * i]) | (fp16_rne(f[2 * i + 1]) << 16) : cvt_bf16x2(f[2 * i], f[2 * i + 1]);
+    return v;
+}
+
+template <bool TF32>
+__device__ __forceinline__ float table_at(const void* row, int i) {
+    return TF32 ? reinterpret_cast<const float*>(row)[i] : bf16_to_f32(reinterpret_cast<const uint16_t*>(row)[i]);
+}
+
+template <int D, bool FP16, bool TF32, bool INTER>
+__global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkRopeArgs a) {
+    constexpr int LPH = D / 8, HPW = 64 / LPH;              // lanes per head, heads per pass
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int64_t unit = (int64_t)blockIdx.x * 4 + wave;
+    const int64_t t = unit / a.chunks;
+    if (t >= a.T) return;
+    const int pass0 = (int)(unit - t * a.chunks) * a.per;
+    const int j = lane % LPH, sub = lane / LPH;             // the lane's 8 dims 8j .. 8j + 7 of head `sub` of a pass
+    const int heads = a.H + a.Hk;
+    const int passes = min(pass0 + a.per, (heads + HPW - 1) / HPW);
+    int64_t pos = t;
+    if (a.positions)
+        pos = a.pos_bytes == 8 ? reinterpret_cast<const int64_t*>(a.positions)[t * a.pos_stride]
+                               : (int64_t)reinterpret_cast<const int32_t*>(a.positions)[t * a.pos_stride];
+    const bool known = pos >= 0 && pos < a.P;               // else the outputs are NaN and the table is not read
+    const int half = a.half;
+    // cos and the signed sin of each of the lane's dims: out_d = n_d cos + partner_d sin (1 and 0 past the rotated dims)
+    float cs[8], sn[8];
+    const char* row = reinterpret_cast<const char*>(a.table) + (known ? pos : 0) * a.ld_table * (TF32 ? 4 : 2);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int d = 8 * j + e;
+        cs[e] = 1.0f;
+        sn[e] = 0.0f;
+        if (d < 2 * half) {
+            const int p = INTER ? d >> 1 : (d < half ? d : d - half);
+            const bool minus = INTER ? !(d & 1) : d < half;
+            const float s = table_at<TF32>(row, half + p);
+            cs[e] = table_at<TF32>(row, p);
+            sn[e] = minus ? -s : s;
+        }
+        if (!known) cs[e] = __builtin_nanf("");
+    }
+    const bool rotated = 8 * j < 2 * half;                  // half-split: half % 8 == 0, a lane is wholly in or out
+    const int partner = INTER ? 0 : (lane - j) + (8 * j < half ? j + half / 8 : j - half / 8);
+    for (int ps = pass0; ps < passes; ++ps) {
+        const int h = ps * HPW + sub;
+        const bool live = h < heads, isq = h < a.H;
+        const uint16_t* src = isq ? a.q + t * a.q_t + (int64_t)h * a.q_h : a.k + t * a.k_t + (int64_t)(h - a.H) * a.k_h;
+        v4u v = {0u, 0u, 0u, 0u}, w = {0u, 0u, 0u, 0u};
+        if (live) {
+            v = *reinterpret_cast<const v4u*>(src + 8 * j);
+            w = *reinterpret_cast<const v4u*>((isq ? a.wq : a.wk) + 8 * j);
+        }
+        float x[8], g[8];
+        widen8<FP16>(v, x);
+        widen8<FP16>(w, g);
+        float ss = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(x[e], x[e], ss);
+#pragma unroll
+        for (int o = LPH / 2; o >= 1; o >>= 1) ss += __shfl_xor(ss, o, 64);
+        const float r = 1.0f / __builtin_sqrtf(ss * (1.0f / D) + a.eps);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = x[e] * r * g[e];
+        float y[8];
+        if (INTER) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                y[e] = 8 * j + e < 2 * half ? __builtin_fmaf(x[e], cs[e], x[e ^ 1] * sn[e]) : x[e] * cs[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float o = __shfl(x[e], rotated ? partner : lane, 64);
+                y[e] = rotated ? __builtin_fmaf(x[e], cs[e], o * sn[e]) : x[e] * cs[e];
+            }
+        }
+        if (!live) continue;
+        uint16_t* dst = isq ? a.oq + t * a.oq_t + (int64_t)h * a.oq_h : a.ok + t * a.ok_t + (int64_t)(h - a.H) * a.ok_h;
+        *reinterpret_cast<v4u*>(dst + 8 * j) = narrow8<FP16>(y);
+    }
+}
+
+template <int D, bool FP16, bool TF32>
+int launch_qk(const QkRopeArgs& a, bool interleaved, dim3 grid, hipStream_t st) {
+    if (interleaved) hipLaunchKernelGGL((qk_norm_rope_kernel<D, FP16, TF32, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((qk_norm_rope_kernel<D, FP16, TF32, false>), grid, dim3(256), 0, st, a);
+    H3_CHECK_HIP(hipGetLastError());
+    return H3FP8_OK;
+}
+
+template <int D>
+int launch_head(QkRopeArgs a, bool fp16, bool tf32, bool interleaved, hipStream_t st) {
+    const int passes = (a.H + a.Hk + 512 / D - 1) / (512 / D);
+    a.per = passes;
+    a.chunks = 1;
+    const int64_t units = a.T * a.chunks;
+    H3_REQUIRE(units < ((int64_t)1 << 33), "h3fp8_qk_norm_rope: too many tokens");
+    const dim3 grid((unsigned)((units + 3) / 4));
+    if (fp16) return tf32 ? launch_qk<D, true, true>(a, interleaved, grid, st) : launch_qk<D, true, false>(a, interleaved, grid, st);
+    return tf32 ? launch_qk<D, false, true>(a, interleaved, grid, st) : launch_qk<D, false, false>(a, interleaved, grid, st);
+}
+
+bool rows_ok(const void* p, int64_t st_t, int64_t st_h) {
+    return ((uintptr_t)p & 15) == 0 && st_t >= 0 && st_h >= 0 && st_t % 8 == 0 && st_h % 8 == 0;
+}
+
+}  // namespace
+
+extern "C" int h3fp8_qk_norm_rope(const void* q, int64_t q_t, int64_t q_h, const void* k, int64_t k_t, int64_t k_h, int dtype,
+                                  int64_t T, int H, int Hk, int D, const void* q_weight, const void* k_weight,
+                                  const void* table, int64_t ld_table, int table_dtype, int64_t P, int R, int interleaved,
+                                  const void* positions, int64_t pos_stride, int pos_bytes, float eps, void* out_q,
+                                  int64_t oq_t, int64_t oq_h, void* out_k, int64_t ok_t, int64_t ok_h, void* stream) {
+    H3_REQUIRE(T >= 0 && H >= 0 && Hk >= 0 && P >= 0, "h3fp8_qk_norm_rope: negative size");
+    H3_REQUIRE(D == 64 || D == 128 || D == 256, "h3fp8_qk_norm_rope: head size %d (64, 128 or 256)", D);
+    H3_REQUIRE(R >= 0 && R <= D && R % (interleaved ? 2 : 16) == 0,
+               "h3fp8_qk_norm_rope: %d rotated dims of %d (half-split: a multiple of 16, interleaved: of 2)", R, D);
+    H3_REQUIRE(dtype == H3FP8_DT_BF16 || dtype == H3FP8_DT_FP16, "h3fp8_qk_norm_rope: bad dtype %d", dtype);
+    H3_REQUIRE(table_dtype == H3FP8_DT_BF16 || table_dtype == H3FP8_DT_F32, "h3fp8_qk_norm_rope: the table is fp32 or bf16");
+    if (T == 0 || (int64_t)H + Hk == 0) return H3FP8_OK;
+    H3_REQUIRE(H <= (1 << 20) && Hk <= (1 << 20), "h3fp8_qk_norm_rope: too many heads");
+    H3_REQUIRE((H == 0 || (q && out_q && q_weight)) && (Hk == 0 || (k && out_k && k_weight)) && (R == 0 || table),
+               "h3fp8_qk_norm_rope: null pointer");
+    H3_REQUIRE((H == 0 || (rows_ok(q, q_t, q_h) && rows_ok(out_q, oq_t, oq_h) && ((uintptr_t)q_weight & 15) == 0)) &&
+                   (Hk == 0 || (rows_ok(k, k_t, k_h) && rows_ok(out_k, ok_t, ok_h) && ((uintptr_t)k_weight & 15) == 0)),
+               "h3fp8_qk_norm_rope: q, k, their outputs and the weights need 16-byte alignment and token and head strides "
+               "that are multiples of 8 elements");
+    H3_REQUIRE(R == 0 || (ld_table >= R && ((uintptr_t)table & (table_dtype == H3FP8_DT_F32 ? 3 : 1)) == 0),
+               "h3fp8_qk_norm_rope: the table's row stride must be >= %d", R);
+    H3_REQUIRE(positions ? pos_bytes == 4 || pos_bytes == 8 : P >= T || R == 0,
+               "h3fp8_qk_norm_rope: positions must be int32 or int64, and without them the table needs a row per token");
+    QkRopeArgs a{};
+    a.q = (const uint16_t*)q; a.q_t = q_t; a.q_h = q_h;
+    a.k = (const uint16_t*)k; a.k_t = k_t; a.k_h = k_h;
+    a.oq = (uint16_t*)out_q; a.oq_t = oq_t; a.oq_h = oq_h;
+    a.ok = (uint16_t*)out_k; a.ok_t = ok_t; a.ok_h = ok_h;
+    a.wq = (const uint16_t*)q_weight; a.wk = (const uint16_t*)k_weight;
+    a.table = table; a.ld_table = ld_table; a.P = R ? P : T;
+    a.positions = R ? positions : nullptr; a.pos_stride = pos_stride; a.pos_bytes = pos_bytes;
+    a.T = T; a.H = H; a.Hk = Hk; a.half = R / 2; a.eps = eps;
+    const bool fp16 = dtype == H3FP8_DT_FP16, tf32 = table_dtype == H3FP8_DT_F32;
+    hipStream_t st = (hipStream_t)stream;
+    if (D == 64) return launch_head<64>(a, fp16, tf32, interleaved != 0, st);
+    if (D == 128) return launch_head<128>(a, fp16, tf32, interleaved != 0, st);
+    return launch_head<256>(a, fp16, tf32, interleaved != 0, st);
+}

@@ -66,6 +66,13 @@ _SIGS = {
                                    I64, I64, P, I64, I64, P], I),
     "h3fp8_scale_bias_cast": ([P, I64, P, I64, P, I64, P, P, I64, I, I64, I64, P], I),
     "h3fp8_grouped_gemm": ([ctypes.POINTER(Group), I, P], I),
+    "h3fp8_quant_blocks": ([P, I64, I, I64, I64, I, P, I64, P, I64, I64, P], I),
+    "h3fp8_silu_mul_quant_blocks": ([P, I64, I, I64, I64, P, I64, P, I64, I64, P], I),
+    "h3fp8_gemm_blocks": ([P, I64, P, I64, P, I64, I64, P, I64, I64, P, P, I64, I, I64, I64, I64, P], I),
+    "h3fp8_grouped_gemm_blocks": ([P, I64, P, I64, I64, P, I64, I64, P, I64, I64, I64, P, I, P, I64, I, I64, I64, I64,
+                                   I64, P], I),
+    "h3fp8_qk_norm_rope": ([P, I64, I64, P, I64, I64, I, I64, I, I, I, P, P, P, I64, I, I64, I, I, P, I64, I,
+                            ctypes.c_float, P, I64, I64, P, I64, I64, P], I),
     "h3fp8_selfcheck_e4m3": ([ctypes.POINTER(ctypes.c_uint64), ctypes.POINTER(ctypes.c_uint64)], I),
     "h3fp8_selfcheck_bf16": ([ctypes.POINTER(ctypes.c_uint64), ctypes.POINTER(ctypes.c_uint64)], I),
     "h3fp8_copy_silu_table": ([P, P], I),

@@ -651,6 +651,218 @@ def grouped_gemm(problems):  # noqa: ANN001,ANN201
     return outs
 
 
+# ---- the block-scaled linear: one scale per block of 128 ------------------------------------------------------------
+
+BLOCK = 128                     # columns of a block (and rows, of a weight's)
+
+
+def _blocks(n: int) -> int:
+    return (n + BLOCK - 1) // BLOCK
+
+
+def _axes(t: torch.Tensor) -> tuple:
+    """Strides, those of a size-1 axis (which torch leaves arbitrary) as 0."""
+    return tuple(st if n > 1 else 0 for st, n in zip(t.stride(), t.shape))
+
+
+def _call_on(t: torch.Tensor, name: str, *args) -> None:
+    """The entry point on ``t``'s device and that device's current stream, whichever device is the current one."""
+    if t.get_device() == torch.cuda.current_device():
+        _lib.call(name, *args, _stream(t))
+    else:
+        with torch.cuda.device(t.device):
+            _lib.call(name, *args, _stream(t))
+
+
+def _same_device(name: str, *ts) -> None:  # noqa: ANN002
+    """Every operand on the first one's GPU."""
+    _need_cuda(*ts)
+    for t in ts[1:]:
+        if t is not None and t.device != ts[0].device:
+            raise ValueError(f"{name}: every operand must be on {ts[0].device}, got one on {t.device}")
+
+
+def _block_outputs(name: str, like: torch.Tensor, M: int, K: int, rows: int, q: torch.Tensor | None,
+                   scale: torch.Tensor | None):
+    """q [M, K] and the block scales [ceil(M / rows), ceil(K / 128)]: allocated (scales of 1 x 128 blocks with the tokens
+    contiguous, the order the product reads them in) or the caller's, the scales in any strides."""
+    MB, KB = -(-M // rows), _blocks(K)
+    if q is None:
+        q = torch.empty((M, K), device=like.device, dtype=E4M3)
+    else:
+        check_buffer(q, "q", (M, K), E4M3, like.device)
+    if scale is None:
+        scale = torch.empty((KB, MB), device=like.device, dtype=torch.float32).t() if rows == 1 else \
+            torch.empty((MB, KB), device=like.device, dtype=torch.float32)
+    else:
+        if scale.dtype != torch.float32 or tuple(scale.shape) != (MB, KB) or scale.device != like.device:
+            raise ValueError(f"{name}: scale must be float32 ({MB}, {KB}) on {like.device}, got {scale.dtype} "
+                             f"{tuple(scale.shape)} on {scale.device}")
+        if any(n > 1 and st < 1 for st, n in zip(scale.stride(), scale.shape)):
+            raise ValueError(f"{name}: the entries of scale must not overlap")
+    return q, scale
+
+
+def quant_blocks(x: torch.Tensor, rows: int = 1, q: torch.Tensor | None = None, scale: torch.Tensor | None = None):
+    """e4m3 quant with one scale per block of ``rows`` x 128 (1: activations, 128: weights) of a bf16 / fp16 / fp32 [M, K]
+    tensor, K a multiple of 16: (q e4m3fn [M, K], scale fp32 [ceil(M / rows), ceil(K / 128)]).  Blocks at the edge are
+    smaller.  The 1 x 128 scales come with strides (1, M), tokens contiguous, the order ``gemm_blocks`` reads best."""
+    if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.dtype not in _DT:
+        raise ValueError("quant_blocks takes a bf16, fp16 or fp32 [M, K] tensor")
+    if rows not in (1, BLOCK):
+        raise ValueError(f"quant_blocks: blocks have 1 or {BLOCK} rows, got {rows}")
+    M, K = x.shape
+    if K % 16:
+        raise ValueError(f"quant_blocks: K must be a multiple of 16, got {K}")
+    ldx = _rows(x, "x")
+    _need_cuda(x)
+    q, scale = _block_outputs("quant_blocks", x, M, K, rows, q, scale)
+    _call_on(x, "h3fp8_quant_blocks", x.data_ptr(), ldx, _DT[x.dtype], M, K, rows, q.data_ptr(), _rows(q, "q"),
+             scale.data_ptr(), *_axes(scale))
+    return q, scale
+
+
+def silu_mul_quant_blocks(x: torch.Tensor, q: torch.Tensor | None = None, scale: torch.Tensor | None = None):
+    """silu(gate) * up of a bf16 / fp16 [M, 2F] = [gate | up] tensor, quantised per 1 x 128 block from its fp32 value:
+    (q e4m3fn [M, F], scale fp32 [M, ceil(F / 128)] with strides (1, M)).  F a multiple of 16."""
+    if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("silu_mul_quant_blocks takes a bf16 or fp16 [M, 2F] tensor")
+    M, W = x.shape
+    if W % 32:
+        raise ValueError(f"silu_mul_quant_blocks: x must be 2F wide with F a multiple of 16, got {W}")
+    F = W // 2
+    ldx = _rows(x, "x")
+    _need_cuda(x)
+    q, scale = _block_outputs("silu_mul_quant_blocks", x, M, F, 1, q, scale)
+    _call_on(x, "h3fp8_silu_mul_quant_blocks", x.data_ptr(), ldx, _DT[x.dtype], M, F, q.data_ptr(), _rows(q, "q"),
+             scale.data_ptr(), *_axes(scale))
+    return q, scale
+
+
+def _block_scale(s: torch.Tensor, name: str, shape: tuple) -> None:
+    if not isinstance(s, torch.Tensor) or s.dtype != torch.float32 or tuple(s.shape) != shape:
+        raise ValueError(f"{name} must be float32 {shape} (one scale per block of {BLOCK}), got "
+                         f"{getattr(s, 'dtype', type(s).__name__)} {tuple(getattr(s, 'shape', ()))}")
+
+
+def _block_out(name: str, a: torch.Tensor, M: int, N: int, out_dtype: torch.dtype, out: torch.Tensor | None) -> torch.Tensor:
+    if out_dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"{name}: out_dtype must be bf16 or fp16, got {out_dtype}")
+    if out is None:
+        return torch.empty((M, N), device=a.device, dtype=out_dtype)
+    check_buffer(out, "out", (M, N), out_dtype, a.device)
+    return out
+
+
+def gemm_blocks(a: torch.Tensor, w: torch.Tensor, scale_a: torch.Tensor, scale_b: torch.Tensor,
+                out_dtype: torch.dtype = torch.bfloat16, bias: torch.Tensor | None = None,
+                out: torch.Tensor | None = None) -> torch.Tensor:
+    """y [M, N] = round(sum_b scale_a[m, b] * scale_b[n // 128, b] * (a_b @ w_b.T)[m, n] (+ bias[n])) for block-scaled e4m3
+    operands: ``a`` [M, K] with scales [M, ceil(K / 128)], the weight ``w`` [N, K] with scales [ceil(N / 128), ceil(K / 128)]
+    (``quant_blocks``; any strides), K and N multiples of 16; bf16 or fp16 out, the bias in that type."""
+    if a.dtype != E4M3 or w.dtype != E4M3:
+        raise ValueError("gemm_blocks: a and w must be float8_e4m3fn")
+    if a.dim() != 2 or w.dim() != 2 or a.shape[1] != w.shape[1]:
+        raise ValueError(f"gemm_blocks: shape mismatch: a {tuple(a.shape)}, w {tuple(w.shape)} (w is [N, K])")
+    (M, K), N = a.shape, w.shape[0]
+    _block_scale(scale_a, "scale_a", (M, _blocks(K)))
+    _block_scale(scale_b, "scale_b", (_blocks(N), _blocks(K)))
+    if bias is not None and (bias.dim() != 1 or bias.numel() != N or bias.dtype != out_dtype or not bias.is_contiguous()):
+        raise ValueError("gemm_blocks: bias must be a contiguous [N] vector in the output dtype")
+    lda, ldw = _rows(a, "a"), _rows(w, "w")
+    _same_device("gemm_blocks", a, w, scale_a, scale_b, bias)
+    y = _block_out("gemm_blocks", a, M, N, out_dtype, out)
+    _call_on(a, "h3fp8_gemm_blocks", a.data_ptr(), lda, w.data_ptr(), ldw, scale_a.data_ptr(), *_axes(scale_a),
+             scale_b.data_ptr(), *_axes(scale_b), bias.data_ptr() if bias is not None else None, y.data_ptr(),
+             _rows(y, "out"), _DT[out_dtype], M, N, K)
+    return y
+
+
+def grouped_gemm_blocks(a: torch.Tensor, w: torch.Tensor, scale_a: torch.Tensor, scale_b: torch.Tensor,
+                        offsets: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16,
+                        out: torch.Tensor | None = None) -> torch.Tensor:
+    """``gemm_blocks`` by expert: rows offsets[e] .. offsets[e + 1] - 1 of ``a`` [M, K] times ``w[e]`` of the [E, N, K]
+    weights (scales [E, ceil(N / 128), ceil(K / 128)]).  ``offsets``: int32 / int64 [E + 1] on the GPU, non-decreasing, read
+    by the kernel only (no synchronisation, capturable); an expert may have no rows.  Rows of y that no expert has are left
+    as they were in ``out`` (without ``out`` they are undefined)."""
+    if a.dtype != E4M3 or w.dtype != E4M3:
+        raise ValueError("grouped_gemm_blocks: a and w must be float8_e4m3fn")
+    if a.dim() != 2 or w.dim() != 3 or a.shape[1] != w.shape[2]:
+        raise ValueError(f"grouped_gemm_blocks: shape mismatch: a {tuple(a.shape)}, w {tuple(w.shape)} (w is [E, N, K])")
+    (M, K), (E, N, _) = a.shape, w.shape
+    if K > 1 and w.stride(2) != 1:
+        raise ValueError("grouped_gemm_blocks: the rows of w must be contiguous")
+    _block_scale(scale_a, "scale_a", (M, _blocks(K)))
+    _block_scale(scale_b, "scale_b", (E, _blocks(N), _blocks(K)))
+    if not isinstance(offsets, torch.Tensor) or offsets.dtype not in (torch.int32, torch.int64) \
+            or tuple(offsets.shape) != (E + 1,) or not offsets.is_contiguous():
+        raise ValueError(f"grouped_gemm_blocks: offsets must be a contiguous int32 / int64 [{E + 1}] vector")
+    lda = _rows(a, "a")
+    _same_device("grouped_gemm_blocks", a, w, scale_a, scale_b, offsets)
+    y = _block_out("grouped_gemm_blocks", a, M, N, out_dtype, out)
+    ldw = w.stride(1) if N > 1 else max(K, w.stride(1))
+    _call_on(a, "h3fp8_grouped_gemm_blocks", a.data_ptr(), lda, w.data_ptr(), w.stride(0) if E > 1 else 0, ldw,
+             scale_a.data_ptr(), *_axes(scale_a), scale_b.data_ptr(), *_axes(scale_b), offsets.data_ptr(),
+             offsets.element_size(), y.data_ptr(), _rows(y, "out"), _DT[out_dtype], M, N, K, E)
+    return y
+
+
+# ---- qk norm + rotation ---------------------------------------------------------------------------------------------
+
+def _heads(t: torch.Tensor, name: str) -> None:
+    if not isinstance(t, torch.Tensor) or t.dim() != 3 or t.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"{name} must be a bf16 or fp16 [T, heads, D] tensor")
+    if t.shape[2] > 1 and t.stride(2) != 1:
+        raise ValueError(f"{name}: the dims of a head must be contiguous")
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, rope_table: torch.Tensor,
+                 eps: float, positions: torch.Tensor | None = None, interleaved: bool = False,
+                 out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """RMSNorm of every head of ``q`` [T, H, D] and ``k`` [T, Hk, D] (bf16 / fp16, D = 64, 128 or 256; views of a qkv product
+    are read in place) and the rotation of its first R dims by ``rope_table`` [P, R] (fp32 / bf16: cos of the R / 2 pairs, then
+    sin) at row ``positions[t]`` (int32 / int64 [T]) or t.  Pairs are dims (p, p + R / 2), or (2p, 2p + 1) with
+    ``interleaved``.  fp32 throughout, rounded once.  A position outside the table gives NaN.  Returns (q, k) as new tensors,
+    or ``out``, which may be (q, k) themselves."""
+    _heads(q, "q")
+    _heads(k, "k")
+    (T, H, D), (Tk, Hk, Dk) = q.shape, k.shape
+    if T != Tk or D != Dk or q.dtype != k.dtype:
+        raise ValueError(f"q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} do not match")
+    if D not in (64, 128, 256):
+        raise ValueError(f"qk_norm_rope: heads of 64, 128 or 256 dims, got {D}")
+    for w, n in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if w.dtype != q.dtype or tuple(w.shape) != (D,) or not w.is_contiguous():
+            raise ValueError(f"{n} must be a contiguous {q.dtype} [{D}] vector")
+    if rope_table.dim() != 2 or rope_table.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("rope_table must be fp32 or bf16 [P, R]")
+    P, R = rope_table.shape
+    if R > D or R % (2 if interleaved else 16):
+        raise ValueError(f"rope_table: R = {R} rotated dims of {D} (a multiple of {2 if interleaved else 16})")
+    ld_table = _rows(rope_table, "rope_table")
+    if positions is None:
+        if P < T and R:
+            raise ValueError(f"rope_table has {P} rows for {T} tokens and no positions are given")
+    elif positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) != (T,):
+        raise ValueError(f"positions must be int32 / int64 [{T}]")
+    _same_device("qk_norm_rope", q, k, q_weight, k_weight, rope_table, positions)
+    if out is None:
+        out = (torch.empty((T, H, D), device=q.device, dtype=q.dtype), torch.empty((T, Hk, D), device=q.device, dtype=q.dtype))
+    else:
+        for o, t, n in ((out[0], q, "out[0]"), (out[1], k, "out[1]")):
+            check_buffer(o, n, tuple(t.shape), t.dtype, t.device)
+            if o.shape[2] > 1 and o.stride(2) != 1:
+                raise ValueError(f"{n}: the dims of a head must be contiguous")
+    oq, ok = out
+    _call_on(q, "h3fp8_qk_norm_rope", q.data_ptr(), *_axes(q)[:2], k.data_ptr(), *_axes(k)[:2], _DT[q.dtype], T, H, Hk,
+             D, q_weight.data_ptr(), k_weight.data_ptr(), rope_table.data_ptr(), ld_table, _DT[rope_table.dtype], P, R,
+             int(interleaved), positions.data_ptr() if positions is not None else None,
+             positions.stride(0) if positions is not None and T > 1 else 0,
+             positions.element_size() if positions is not None else 8, float(eps), oq.data_ptr(), *_axes(oq)[:2],
+             ok.data_ptr(), *_axes(ok)[:2])
+    return oq, ok
+
+
 # ---- self-checks ----------------------------------------------------------------------------------------------------
 
 def selfcheck_e4m3() -> tuple[int, int]:

@@ -1,0 +1,56 @@
+"""Inputs and float64 references of the block-scaled operators' tests."""
+import torch
+
+E4M3 = torch.float8_e4m3fn
+B = 128
+
+
+def cdiv(a, b):
+    return -(-a // b)
+
+
+def spread(s, rows, cols, r):
+    """Block scales laid over the values they belong to (blocks of r x 128)."""
+    return s.repeat_interleave(r, 0)[:rows].repeat_interleave(B, 1)[:, :cols]
+
+
+def codes(g, M, K, lo=-448.0, hi=448.0, integers=False, device="cuda"):
+    x = torch.randint(-4, 5, (M, K), generator=g, device=device).float() if integers else \
+        (torch.randn(M, K, generator=g, device=device) * 60.0).clamp(lo, hi)
+    return x.to(E4M3)
+
+
+def scales(g, *shape, pow2=False, device="cuda"):
+    if pow2:
+        return torch.exp2(torch.randint(-6, 3, shape, generator=g, device=device).float())
+    return torch.exp(torch.randn(shape, generator=g, device=device)) * 1e-2
+
+
+def product64(a, w, sa, sw, bias=None):
+    """(exact product, sum of |scaled products|) in float64."""
+    (M, K), N = a.shape, w.shape[0]
+    A = a.double() * spread(sa.double(), M, K, 1)
+    W = w.double() * spread(sw.double(), N, K, B)
+    y = A @ W.t()
+    return (y if bias is None else y + bias.double()), A.abs() @ W.abs().t()
+
+
+def check_product(y, y64, mag, dtype):
+    """One rounding to the output's type, and what the MFMA leaves out of a block's sum: it aligns the products of a group to
+    the largest and drops what falls below (at most 2^-12 of the sum of magnitudes, the bound the dense product's tests
+    use); the fp32 fmas over the blocks add 2^-24 each, below 2^-16 for the 112 blocks of the deepest linear."""
+    tol = y64.abs() * (torch.finfo(dtype).eps / 2) * (1 + 2 ** -10) + mag * 2.0 ** -12 + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    bad = ~((y.double() - y64).abs() <= tol)
+    assert not bad.any(), (int(bad.sum()), bad.nonzero()[:3].tolist(), float(((y.double() - y64).abs() / tol).max()))
+
+
+def quant32(x, rows=1):
+    """The definition in fp32, bit for bit what the kernels compute (x fp32, on its device).  The quotients are taken in
+    float64 and rounded to fp32, which is the correctly rounded fp32 quotient (53 >= 2 * 24 + 2 bits); torch's own fp32
+    division by a number is a product with its reciprocal on the GPU."""
+    M, K = x.shape
+    p = torch.nn.functional.pad(x, (0, -K % B, 0, -M % rows))
+    b = p.view(p.shape[0] // rows, rows, p.shape[1] // B, B)
+    s = torch.clamp_min((b.abs().amax(dim=(1, 3)).double() / 448.0).float(), 1.0 / (448.0 * 512.0))
+    q = (b * (1.0 / s.double()).float()[:, None, :, None]).clamp(-448.0, 448.0).to(E4M3)
+    return q.view(-1, p.shape[1])[:M, :K].contiguous(), s
