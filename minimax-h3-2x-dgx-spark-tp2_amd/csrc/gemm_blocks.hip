@@ -69,13 +69,14 @@ __device__ __forceinline__ bool locate_rows(const BlocksParams& p, int TT, int64
         const uint64_t past = __ballot(sum > t);
         if (past) {
             const int f = __ffsll((unsigned long long)past) - 1;
-            const int64_t first = __shfl(lo, f, 64), last = __shfl(hi, f, 64);
+            // offsets are at most M < 2^31
+            const int first = __builtin_amdgcn_readlane((int)lo, f), last = __builtin_amdgcn_readlane((int)hi, f);
             r.e = e0 + f;
-            r.row0 = first + (t - (__shfl(sum, f, 64) - __shfl(n, f, 64))) * TT;
+            r.row0 = first + (t - (__builtin_amdgcn_readlane(sum, f) - __builtin_amdgcn_readlane(n, f))) * TT;
             r.rows = (int)min<int64_t>(TT, last - r.row0);
             return true;
         }
-        t -= __shfl(sum, 63, 64);
+        t -= __builtin_amdgcn_readlane(sum, 63);
     }
     return false;
 }
@@ -123,6 +124,438 @@ __global__ void __launch_bounds__(64, 2) gemm_blocks_kernel(BlocksParams p, int 
     *reinterpret_cast<uint2*>(p.y + m * p.ldy + n) = make_uint2(o[0], o[1]);
 }
 
+// ---- the tiled form -------------------------------------------------------------------------------------------------
+//
+// A workgroup of WN x WM waves, one per CU, walks tiles of TW channels x TT tokens (persistent: tile b, b + G, ...); a wave
+// owns NI x NJ MFMA blocks, its 16 NI channels within one 128-channel weight block.  Two waves share a SIMD, so each has
+// 256 registers; acc takes 4 NI NJ of them.
+//   * Operands go global -> LDS by LDS-DMA (whole 128-byte lines, 8 rows an instruction) into NST stages of one k-block each;
+//     the loads run NST k-steps ahead of the MFMAs, across tile boundaries.
+//   * One barrier per k-step, late in it: every wave's fragment reads of stage g have returned (the stage is free: the loads
+//     of k-step g + NST follow, one per MFMA) and its share of stage g + 1 has landed (its first fragments are read behind
+//     the remaining MFMAs).  The last two channel blocks go token by token, so that a token's fragment registers are free
+//     for the next k-step's as early as possible.
+//   * The fmas of an MFMA's four results stand LAG MFMAs behind it (it needs 24 wait states), also across k-steps; per MFMA
+//     (32 cycles of the matrix pipe) they cost 16 cycles of the vector pipe.
+//   * Channel of MFMA block i, row 4 g + r: 32 (i / 2) + 8 g + 4 (i % 2) + r, so that two blocks' results of a lane are 8
+//     consecutive channels: the epilogue stores 16 bytes per lane, 64-byte pieces of a row, without going through LDS.
+//   * LDS rows are 128 bytes; logical 16-byte chunk c of row r is stored at c ^ (weights: swz_w(r), tokens: swz(r)), which
+//     puts the 16 rows of a fragment read on different banks.
+//   * Every tile has buffer descriptors of its own from its own base: rows past the tile's read zeros and store nothing,
+//     and nothing else is limited to 32-bit offsets.
+__device__ __forceinline__ int swz_w(int r) { return ((r >> 1) & 1) | (((r >> 3) & 3) << 1); }
+
+__device__ __forceinline__ void dma4_at(v4u desc, uint32_t lds_base, uint32_t voff, uint32_t soff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"
+                 :
+                 : "s"(lds_base), "v"(voff), "s"(desc), "s"(soff)
+                 : "memory", "m0");
+}
+
+constexpr int LAG = 5;
+constexpr int AHEAD = 3;                                  // channel blocks read ahead of their MFMAs
+
+template <int WN_, int WM_, int NI_, int NJ_, int NST_>
+struct BTile {
+    static constexpr int WN = WN_, WM = WM_, NI = NI_, NJ = NJ_, NST = NST_;
+    static constexpr int WAVES = WN * WM, NM = NI * NJ;
+    static constexpr int TW = 16 * NI * WN, TT = 16 * NJ * WM;
+    static constexpr int WL = TW / 8 / WAVES, AL = TT / 8 / WAVES;   // LDS-DMA instructions per wave and k-step
+    static constexpr int LOADS = WL + AL + 1;                        // ... and one for the scales
+    static constexpr int STAGE = (TW + TT) * ROWB, A_OFF = TW * ROWB;
+    static constexpr int SC_A = (TT + 63) / 64, SC_OFF = NST * STAGE, SC_STAGE = WAVES * 256;
+    static constexpr int LDS = SC_OFF + NST * SC_STAGE;
+    static constexpr int U0 = (NI - 2) * NJ;                         // MFMAs before the last two channel blocks
+    static constexpr int BAR = (NI - 1 - AHEAD) * NJ + NJ;           // the MFMA that the barrier stands behind
+    static_assert(TW % (8 * WAVES) == 0 && TT % (8 * WAVES) == 0, "whole load instructions per wave");
+    static_assert(128 % (16 * NI) == 0 && NI % 2 == 0 && NI > AHEAD && NM > LAG, "wave tile");
+    static_assert(WL <= 15 && AL <= 15 && SC_A < WAVES && LDS <= 160 * 1024 && LOADS * (NST - 2) <= 63, "LDS, scale loads, vmcnt range");
+    static constexpr int mi(int u) { return u < U0 ? u / NJ : NI - 2 + (u - U0) % 2; }
+    static constexpr int mj(int u) { return u < U0 ? u % NJ : (u - U0) / 2; }
+};
+
+// The tile whose operands are loaded next, and its k-step.
+template <class T>
+struct BCursor {
+    v4u rw, ra, rs;             // buffer descriptors of the weight rows, the token rows and this wave's scales
+    uint32_t vw[T::WL], va[T::AL];  // lane offsets of the wave's 8-row groups
+    uint32_t cut;               // bit i (weights) / 16 + j (tokens): the lane's chunk lies at or past K in the last k-step
+    uint32_t vs;                // lane offset of the scale load
+    uint32_t s_step;            // bytes between two k-blocks' scales
+    uint32_t k0, s0;            // byte offsets of the k-step: operands, scales
+    int ks, c;
+    bool valid;
+};
+
+template <class T>
+struct BFrags {
+    v8i w[2], t[T::NJ];         // the next k-step's first two channel blocks and its tokens
+    float sa[T::NJ], sw;        // ... and its scales
+};
+
+// A wave-uniform value, in a scalar register.
+__device__ __forceinline__ uint32_t uni(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+
+struct TileSpace {
+    int rt, tiles_n, total;     // row tiles, channel tiles
+    const int* tab;             // grouped: row tiles of experts 0 .. e, in LDS
+};
+
+constexpr int MAX_TAB = 2048;   // experts of the LDS table; more are counted from the offsets at every tile
+
+// The table, by one wave; returns all experts' row tiles.
+__device__ __forceinline__ int fill_table(const BlocksParams& p, int TT, int lane, int* tab) {
+    int base = 0;
+    for (int e0 = 0; e0 < p.E; e0 += 64) {
+        const int e = e0 + lane;
+        int sum = 0;
+        if (e < p.E) {
+            const int lo = (int)offset_at(p, e), hi = (int)offset_at(p, e + 1);
+            sum = hi > lo ? (int)(((int64_t)hi - lo + TT - 1) / TT) : 0;
+        }
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_up(sum, o, 64);
+            if (lane >= o) sum += v;
+        }
+        if (e < MAX_TAB && e < p.E) tab[e] = base + sum;
+        base += __builtin_amdgcn_readlane(sum, 63);
+    }
+    return base;
+}
+
+// Tile `id` of the launch: its rows and channel tile.
+template <class T, bool GROUPED>
+__device__ __forceinline__ bool tile_at(const BlocksParams& p, const TileSpace& sp, int id, int lane, TileRows& r, int& tn) {
+    if (id >= sp.total) return false;
+    int tm;
+    tile_of(id, sp.total, sp.rt, sp.tiles_n, 4, tm, tn);
+    if (!GROUPED) {
+        r.e = 0;
+        r.row0 = (int64_t)tm * T::TT;
+        r.rows = (int)min<int64_t>(T::TT, p.M - r.row0);
+        return true;
+    }
+    if (p.E > MAX_TAB) return locate_rows(p, T::TT, tm, lane, r);
+    int before = 0;
+    for (int e0 = 0; e0 < p.E; e0 += 64) {
+        const int v = e0 + lane < p.E ? sp.tab[e0 + lane] : 0x7fffffff;
+        const uint64_t past = __ballot(v > tm);
+        if (past) {
+            const int f = __builtin_ctzll(past);
+            if (f) before = __builtin_amdgcn_readlane(v, f - 1);
+            r.e = e0 + f;
+            break;
+        }
+        before = __builtin_amdgcn_readlane(v, 63);
+    }
+    const int lo = __builtin_amdgcn_readfirstlane((int)offset_at(p, r.e)), hi = __builtin_amdgcn_readfirstlane((int)offset_at(p, r.e + 1));
+    r.row0 = lo + (int64_t)(tm - before) * T::TT;
+    r.rows = (int)min<int64_t>(T::TT, hi - r.row0);
+    return true;
+}
+
+template <class T, bool GROUPED>
+__device__ __forceinline__ void cursor_tile(BCursor<T>& I, const BlocksParams& p, const TileSpace& sp, int c, int wave, int lane) {
+    I.c = c;
+    I.ks = 0;
+    I.k0 = I.s0 = 0;
+    TileRows r;
+    int tn = 0;
+    I.valid = tile_at<T, GROUPED>(p, sp, (int)blockIdx.x + c * (int)gridDim.x, lane, r, tn);
+    if (!I.valid) {                                       // the loads still run, read nothing and fill the stage with zeros
+        I.rw[2] = I.ra[2] = I.rs[2] = 0;
+        I.s_step = 0;
+        return;
+    }
+    const int n0 = tn * T::TW, nrows = min(T::TW, p.N - n0);
+    const int kb = (p.K + BK - 1) / BK;
+    I.rw = buffer_desc(p.w + r.e * p.w_e + (int64_t)n0 * p.ldw, (uint32_t)((nrows - 1) * p.ldw + p.K));
+    I.ra = buffer_desc(p.a + r.row0 * p.lda, (uint32_t)((r.rows - 1) * p.lda + p.K));
+    const bool tok = wave < T::SC_A;                      // the first wave past the token scales': the weight's
+    const int nb = (nrows + 127) / 128;
+    const float* base = tok ? p.sa + r.row0 * p.sa_m : p.sw + r.e * p.sw_e + (int64_t)(n0 / 128) * p.sw_n;
+    const int64_t st = tok ? p.sa_m : p.sw_n, sk = tok ? p.sa_k : p.sw_k;
+    const int entries = tok ? r.rows : nb, first = tok ? 64 * wave : 64 * (wave - T::SC_A);
+    I.rs = buffer_desc(base, (uint32_t)(((entries - 1) * st + (kb - 1) * sk) * 4 + 4));
+    I.vs = first + lane < entries ? (uint32_t)((first + lane) * st * 4) : OOB;
+    I.s_step = (uint32_t)(sk * 4);
+}
+
+template <class T, bool GROUPED>
+__device__ __forceinline__ void cursor_next(BCursor<T>& I, const BlocksParams& p, const TileSpace& sp, int nk, int wave, int lane) {
+    if (!I.valid) return;                                 // empty descriptors: offset 0
+    ++I.ks;
+    I.k0 += BK;
+    I.s0 += I.s_step;
+    if (__builtin_expect(I.ks == nk, 0)) cursor_tile<T, GROUPED>(I, p, sp, I.c + 1, wave, lane);
+}
+
+// What the load instructions of the cursor's k-step share: their uniform byte offsets and LDS addresses.  Fixed here in
+// scalar registers, at least five wait states ahead of the first of them (which inline asm leaves to the program).
+struct BIssue {
+    uint32_t k0, s0, w, a, sc, cut;
+};
+
+template <class T>
+__device__ __forceinline__ BIssue bissue(const BCursor<T>& I, int nk, uint32_t st, uint32_t sc, int wave) {
+    BIssue S;
+    S.k0 = uni(I.k0);
+    S.s0 = uni(I.s0);
+    S.w = uni(st + (uint32_t)(wave * T::WL * 8 * ROWB));
+    S.a = uni(st + (uint32_t)(T::A_OFF + wave * T::AL * 8 * ROWB));
+    S.sc = uni(sc + 256u * (uint32_t)wave);
+    S.cut = I.ks == nk - 1 ? I.cut : 0u;
+    asm volatile("s_nop 4" : "+s"(S.k0), "+s"(S.s0), "+s"(S.w), "+s"(S.a), "+s"(S.sc));
+    return S;
+}
+
+// Load instruction i of the k-step.  The hardware checks the lane's offset against the buffer's size less the uniform offset,
+// so that one (k0, s0) never exceeds the size: the rows are in the lane's.
+template <class T>
+__device__ __forceinline__ void bload(const BCursor<T>& I, const BIssue& S, int i) {
+    if (i < T::WL) {
+        dma16_at(I.rw, S.w + (uint32_t)(i * 8 * ROWB), I.vw[i] | ((S.cut << (31 - i)) & OOB), S.k0);
+    } else if (i < T::WL + T::AL) {
+        const int j = i - T::WL;
+        dma16_at(I.ra, S.a + (uint32_t)(j * 8 * ROWB), I.va[j] | ((S.cut << (15 - j)) & OOB), S.k0);
+    } else {
+        dma4_at(I.rs, S.sc, I.vs, S.s0);
+    }
+}
+
+__device__ __forceinline__ v8i frag16(const uint8_t* p0, const uint8_t* p1, int off) {
+    const uint4 lo = *reinterpret_cast<const uint4*>(p0 + off);
+    const uint4 hi = *reinterpret_cast<const uint4*>(p1 + off);
+    v8i f;
+    f[0] = (int)lo.x; f[1] = (int)lo.y; f[2] = (int)lo.z; f[3] = (int)lo.w;
+    f[4] = (int)hi.x; f[5] = (int)hi.y; f[6] = (int)hi.z; f[7] = (int)hi.w;
+    return f;
+}
+
+// A wave's fragment addresses within a stage: lane l reads row c = l & 15 of a block, logical chunks 2 (l >> 4), + 1.
+template <class T>
+struct BAddr {
+    uint32_t w0, w1, t0, t1, sa, sw;
+};
+
+template <class T>
+__device__ __forceinline__ BAddr<T> baddr(int wn, int wm, int lane) {
+    const int c = lane & 15, g = lane >> 4;
+    const int wr = 8 * (c >> 2) + (c & 3);                // + 32 (i / 2) + 4 (i % 2); neither changes swz_w
+    const int tr = c;                                     // + 16 j; neither changes swz
+    BAddr<T> A;
+    A.w0 = (uint32_t)((wn * 16 * T::NI + wr) * ROWB + ((2 * g) ^ swz_w(wr)) * 16);
+    A.w1 = (uint32_t)((wn * 16 * T::NI + wr) * ROWB + ((2 * g + 1) ^ swz_w(wr)) * 16);
+    A.t0 = (uint32_t)(T::A_OFF + (wm * 16 * T::NJ + tr) * ROWB + ((2 * g) ^ swz(tr)) * 16);
+    A.t1 = (uint32_t)(T::A_OFF + (wm * 16 * T::NJ + tr) * ROWB + ((2 * g + 1) ^ swz(tr)) * 16);
+    A.sa = (uint32_t)((wm * 16 * T::NJ + c) * 4);
+    A.sw = (uint32_t)(T::SC_A * 256 + (wn * 16 * T::NI / 128) * 4);
+    return A;
+}
+
+template <class T>
+__device__ __forceinline__ v8i read_w(const uint8_t* st, const BAddr<T>& A, int i) {
+    return frag16(st + A.w0, st + A.w1, (32 * (i >> 1) + 4 * (i & 1)) * ROWB);
+}
+
+template <class T>
+__device__ __forceinline__ v8i read_t(const uint8_t* st, const BAddr<T>& A, int j) {
+    return frag16(st + A.t0, st + A.t1, 16 * j * ROWB);
+}
+
+template <class T>
+__device__ __forceinline__ void bfma(v4f (&acc)[T::NI][T::NJ], const v4f& b, float s, int u) {
+    v4f& a = acc[T::mi(u)][T::mj(u)];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) a[r] = __builtin_fmaf(b[r], s, a[r]);
+    asm volatile("" : "+v"(a));                           // here, not wherever the sum is needed next
+}
+
+// One k-step: F holds its first fragments and scales and receives the next one's; pend and sp the last LAG MFMAs' results
+// and scales.  cur / nxt: this stage and the next; ld: the stage that the loads of the cursor's k-step go to (this one).
+template <class T>
+__device__ __forceinline__ void bkstep(const uint8_t* lds, uint32_t lds0, uint32_t cur, uint32_t nxt, uint32_t cur_sc, uint32_t nxt_sc,
+                                       const BCursor<T>& I, int nk, const BAddr<T>& A, int wave,
+                                       v4f (&acc)[T::NI][T::NJ], BFrags<T>& F, v4f (&pend)[LAG], float (&sp)[T::NJ]) {
+    v8i w[T::NI], t[T::NJ];
+    v4f b[T::NM];
+    float s[T::NJ];
+    const BIssue S = bissue<T>(I, nk, lds0 + cur, lds0 + cur_sc, wave);
+    w[0] = F.w[0];
+    w[1] = F.w[1];
+#pragma unroll
+    for (int j = 0; j < T::NJ; ++j) t[j] = F.t[j];
+#pragma unroll
+    for (int u = 0; u < T::NM; ++u) {
+        b[u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[T::mi(u)], t[T::mj(u)], v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);                // the fmas behind it: 25 wait states to the MFMA they read
+        if (u == LAG - 2) {
+#pragma unroll
+            for (int j = 0; j < T::NJ; ++j) s[j] = F.sa[j] * F.sw;
+        }
+        if (u < LAG) bfma<T>(acc, pend[u], sp[T::mj(T::NM - LAG + u)], T::NM - LAG + u);
+        else bfma<T>(acc, b[u - LAG], s[T::mj(u - LAG)], u - LAG);
+#pragma unroll
+        for (int i = 2; i < T::NI; ++i)                   // this stage's channel blocks, AHEAD of their MFMAs
+            if (u == (i < AHEAD ? 0 : (i - AHEAD) * T::NJ + (i == AHEAD ? 1 : 0))) w[i] = read_w<T>(lds + cur, A, i);
+        if (u == T::BAR) {
+            wait_lgkm0();                                 // this wave's reads of the stage have returned
+            __builtin_amdgcn_s_waitcnt(vmcnt_imm(T::LOADS * (T::NST - 2)));   // its share of the next one has landed
+            barrier_nofence();
+        }
+        if (u > T::BAR) {
+            constexpr int SLOTS = T::NM - 1 - T::BAR;
+#pragma unroll
+            for (int f = (u - T::BAR - 1) * T::LOADS / SLOTS; f < (u - T::BAR) * T::LOADS / SLOTS; ++f)
+                bload<T>(I, S, f);
+            if (u == T::BAR + 1) F.w[0] = read_w<T>(lds + nxt, A, 0);
+            if (u == T::BAR + 2) F.w[1] = read_w<T>(lds + nxt, A, 1);
+            if (u == T::BAR + 3) {
+#pragma unroll
+                for (int j = 0; j < T::NJ; ++j) F.sa[j] = *reinterpret_cast<const float*>(lds + nxt_sc + A.sa + 64 * j);
+                F.sw = *reinterpret_cast<const float*>(lds + nxt_sc + A.sw);
+            }
+            if (u > T::U0 && (u - T::U0) % 2 == 1) F.t[(u - T::U0) / 2] = read_t<T>(lds + nxt, A, (u - T::U0) / 2);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int k = 0; k < LAG; ++k) pend[k] = b[T::NM - LAG + k];
+#pragma unroll
+    for (int j = 0; j < T::NJ; ++j) sp[j] = s[j];
+}
+
+template <class T, bool FP16, bool BIAS>
+__device__ __forceinline__ void bstore(const BlocksParams& p, const TileRows& r, int tn, int wn, int wm, int lane,
+                                       const v4f (&acc)[T::NI][T::NJ]) {
+    const int c = lane & 15, g = lane >> 4;
+    const __amdgpu_buffer_rsrc_t yr = make_rsrc(p.y + r.row0 * p.ldy, (uint32_t)(((r.rows - 1) * p.ldy + p.N) * 2));
+    const int n0 = tn * T::TW + wn * 16 * T::NI + 8 * g;
+#pragma unroll
+    for (int q = 0; q < T::NI / 2; ++q) {
+        const int n = n0 + 32 * q;
+        const bool in = n < p.N;
+        float bias[8];
+        if (BIAS) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) bias[e] = load_bias(p.bias, (in ? n : 0) + e, FP16);
+        }
+#pragma unroll
+        for (int j = 0; j < T::NJ; ++j) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = acc[2 * q + (e >> 2)][j][e & 3] + (BIAS ? bias[e] : 0.0f);
+            v4u o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                o[e] = FP16 ? fp16_rne(v[2 * e]) | (fp16_rne(v[2 * e + 1]) << 16) : cvt_bf16x2(v[2 * e], v[2 * e + 1]);
+            const uint32_t off = (uint32_t)(wm * 16 * T::NJ + 16 * j + c) * (uint32_t)p.ldy * 2u + (uint32_t)n * 2u;
+            __builtin_amdgcn_raw_buffer_store_b128(o, yr, in ? off : OOB, 0, 0);
+        }
+    }
+}
+
+template <class T, bool FP16, bool BIAS, bool GROUPED>
+__global__ void __launch_bounds__(T::WAVES * 64, 2) gemm_blocks_tile_kernel(BlocksParams p) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[T::LDS + (GROUPED ? MAX_TAB * 4 : 0)];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int wn = wave % T::WN, wm = wave / T::WN;
+    const uint32_t lds0 = lds_addr(lds);
+    const int nk = (p.K + BK - 1) / BK, ktail = p.K % BK;
+    TileSpace sp;
+    sp.tiles_n = (p.N + T::TW - 1) / T::TW;
+    sp.rt = (int)((p.M + T::TT - 1) / T::TT);
+    sp.tab = reinterpret_cast<const int*>(lds + T::LDS);
+    if (GROUPED) {                                        // every wave counts, and writes the same table
+        sp.rt = fill_table(p, T::TT, lane, reinterpret_cast<int*>(lds + T::LDS));
+        __syncthreads();
+    }
+    sp.total = sp.rt * sp.tiles_n;
+
+    BCursor<T> I;
+    {
+        // lane l moves LDS chunk l & 7 of row l >> 3 of an 8-row group: logical chunk (l & 7) ^ swizzle(row)
+        const int lrow = lane >> 3;
+        I.cut = 0;
+#pragma unroll
+        for (int i = 0; i < T::WL; ++i) {
+            const int row = 8 * (wave * T::WL + i) + lrow, ch = (lane & 7) ^ swz_w(row);
+            I.vw[i] = (uint32_t)(row * p.ldw) + 16u * (uint32_t)ch;
+            I.cut |= ktail && 16 * ch >= ktail ? 1u << i : 0u;
+        }
+#pragma unroll
+        for (int j = 0; j < T::AL; ++j) {
+            const int row = 8 * (wave * T::AL + j) + lrow, ch = (lane & 7) ^ swz(row);
+            I.va[j] = (uint32_t)(row * p.lda) + 16u * (uint32_t)ch;
+            I.cut |= ktail && 16 * ch >= ktail ? 1u << (16 + j) : 0u;
+        }
+    }
+    I.rw = buffer_desc(nullptr, 0);
+    I.ra = I.rs = I.rw;
+    I.vs = OOB;
+    cursor_tile<T, GROUPED>(I, p, sp, 0, wave, lane);
+    if (!I.valid) return;
+#pragma unroll
+    for (int s = 0; s < T::NST; ++s) {
+        const BIssue S = bissue<T>(I, nk, lds0 + (uint32_t)s * T::STAGE, lds0 + T::SC_OFF + (uint32_t)s * T::SC_STAGE, wave);
+#pragma unroll
+        for (int i = 0; i < T::LOADS; ++i) bload<T>(I, S, i);
+        cursor_next<T, GROUPED>(I, p, sp, nk, wave, lane);
+    }
+    const BAddr<T> A = baddr<T>(wn, wm, lane);
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(T::LOADS * (T::NST - 1)));
+    barrier_nofence();
+    BFrags<T> F;
+    F.w[0] = read_w<T>(lds, A, 0);
+    F.w[1] = read_w<T>(lds, A, 1);
+#pragma unroll
+    for (int j = 0; j < T::NJ; ++j) {
+        F.t[j] = read_t<T>(lds, A, j);
+        F.sa[j] = *reinterpret_cast<const float*>(lds + T::SC_OFF + A.sa + 64 * j);
+    }
+    F.sw = *reinterpret_cast<const float*>(lds + T::SC_OFF + A.sw);
+
+    uint32_t cur = 0, cur_sc = T::SC_OFF;
+    for (int c = 0;; ++c) {
+        TileRows r;
+        int tn = 0;
+        if (!tile_at<T, GROUPED>(p, sp, (int)blockIdx.x + c * (int)gridDim.x, lane, r, tn)) break;
+        v4f acc[T::NI][T::NJ], pend[LAG];
+        float sp_[T::NJ];
+#pragma unroll
+        for (int i = 0; i < T::NI; ++i)
+#pragma unroll
+            for (int j = 0; j < T::NJ; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < LAG; ++k) pend[k] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < T::NJ; ++j) sp_[j] = 0.f;
+        for (int ks = 0; ks < nk; ++ks) {
+            const uint32_t nxt = cur == (T::NST - 1) * T::STAGE ? 0u : cur + T::STAGE;
+            const uint32_t nxt_sc = nxt == 0 ? T::SC_OFF : cur_sc + T::SC_STAGE;
+            bkstep<T>(lds, lds0, cur, nxt, cur_sc, nxt_sc, I, nk, A, wave, acc, F, pend, sp_);
+            cursor_next<T, GROUPED>(I, p, sp, nk, wave, lane);
+            cur = nxt;
+            cur_sc = nxt_sc;
+        }
+        // the last results: 24 wait states behind their MFMAs, as a dependence
+#pragma unroll
+        for (int k = 0; k < LAG; ++k) {
+            if (k == 0) asm volatile("s_nop 15\n\ts_nop 7" : "+v"(pend[LAG - 1]));
+        }
+#pragma unroll
+        for (int k = 0; k < LAG; ++k) {
+            asm volatile("" : "+v"(pend[k]));
+            bfma<T>(acc, pend[k], sp_[T::mj(T::NM - LAG + k)], T::NM - LAG + k);
+        }
+        bstore<T, FP16, BIAS>(p, r, tn, wn, wm, lane, acc);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    wait_vm0();                                           // the loads behind the last k-step have landed before the exit
+}
+
 constexpr int64_t kMaxSpan = 0x7fff0000LL;                // byte offsets within a tile are 32-bit
 
 int check(const BlocksParams& p, const char* who, int out_dtype, int64_t N, int64_t K, int64_t E) {
@@ -155,8 +588,30 @@ int64_t row_tiles(const BlocksParams& p, int TT) {
     return p.offsets ? std::min<int64_t>(p.M, p.M / TT + p.E) : full;
 }
 
+template <class T>
+int launch_tile(const BlocksParams& p, const char* who, hipStream_t st) {
+    const int64_t tiles = row_tiles(p, T::TT) * ((p.N + T::TW - 1) / T::TW);
+    H3_REQUIRE(tiles < ((int64_t)1 << 31), "%s: too many tiles for one launch", who);
+    const dim3 grid((unsigned)std::min<int64_t>(tiles, h3host::cu_count())), block(T::WAVES * 64);
+#define H3_B(FP16, BIAS, GROUPED) hipLaunchKernelGGL((gemm_blocks_tile_kernel<T, FP16, BIAS, GROUPED>), grid, block, 0, st, p)
+    if (p.offsets) {
+        if (p.fp16) H3_B(true, false, true);
+        else H3_B(false, false, true);
+    } else if (p.fp16) {
+        if (p.bias) H3_B(true, true, false);
+        else H3_B(true, false, false);
+    } else {
+        if (p.bias) H3_B(false, true, false);
+        else H3_B(false, false, false);
+    }
+#undef H3_B
+    H3_CHECK_HIP(hipGetLastError());
+    return H3FP8_OK;
+}
+
 int run(const BlocksParams& p, const char* who, hipStream_t st) {
     if (p.M == 0 || p.N == 0 || p.E == 0) return H3FP8_OK;
+    if (p.M > 16) return launch_tile<BTile<2, 4, 8, 4, 2>>(p, who, st);
     const int tiles_n = p.N / 16;
     const int64_t tiles = row_tiles(p, 16) * tiles_n;
     H3_REQUIRE(tiles < ((int64_t)1 << 31), "%s: too many tiles for one launch", who);
