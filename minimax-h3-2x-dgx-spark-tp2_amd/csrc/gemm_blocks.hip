@@ -155,9 +155,11 @@ __device__ __forceinline__ void dma4_at(v4u desc, uint32_t lds_base, uint32_t vo
 constexpr int LAG = 5;
 constexpr int AHEAD = 3;                                  // channel blocks read ahead of their MFMAs
 
-template <int WN_, int WM_, int NI_, int NJ_, int NST_>
+// SMALL: the k-step of few MFMAs (below).  WPE: waves per SIMD that the registers are to allow.
+template <int WN_, int WM_, int NI_, int NJ_, int NST_, bool SMALL_ = false, int WPE_ = 2>
 struct BTile {
-    static constexpr int WN = WN_, WM = WM_, NI = NI_, NJ = NJ_, NST = NST_;
+    static constexpr int WN = WN_, WM = WM_, NI = NI_, NJ = NJ_, NST = NST_, WPE = WPE_;
+    static constexpr bool SMALL = SMALL_, PAIRS = NI % 2 == 0;
     static constexpr int WAVES = WN * WM, NM = NI * NJ;
     static constexpr int TW = 16 * NI * WN, TT = 16 * NJ * WM;
     static constexpr int WL = TW / 8 / WAVES, AL = TT / 8 / WAVES;   // LDS-DMA instructions per wave and k-step
@@ -165,13 +167,16 @@ struct BTile {
     static constexpr int STAGE = (TW + TT) * ROWB, A_OFF = TW * ROWB;
     static constexpr int SC_A = (TT + 63) / 64, SC_OFF = NST * STAGE, SC_STAGE = WAVES * 256;
     static constexpr int LDS = SC_OFF + NST * SC_STAGE;
+    static constexpr int PER_CU = std::min(160 * 1024 / (LDS + 1024), 32 / WAVES);   // workgroups (grouped: 1 KiB of table)
     static constexpr int U0 = (NI - 2) * NJ;                         // MFMAs before the last two channel blocks
     static constexpr int BAR = (NI - 1 - AHEAD) * NJ + NJ;           // the MFMA that the barrier stands behind
     static_assert(TW % (8 * WAVES) == 0 && TT % (8 * WAVES) == 0, "whole load instructions per wave");
-    static_assert(128 % (16 * NI) == 0 && NI % 2 == 0 && NI > AHEAD && NM > LAG, "wave tile");
-    static_assert(WL <= 15 && AL <= 15 && SC_A < WAVES && LDS <= 160 * 1024 && LOADS * (NST - 2) <= 63, "LDS, scale loads, vmcnt range");
-    static constexpr int mi(int u) { return u < U0 ? u / NJ : NI - 2 + (u - U0) % 2; }
-    static constexpr int mj(int u) { return u < U0 ? u % NJ : (u - U0) / 2; }
+    static_assert(128 % (16 * NI) == 0 && (TW % 128 == 0 || 128 % TW == 0), "a wave's channels in one weight block");
+    static_assert(SMALL || (NI % 2 == 0 && NI > AHEAD && NM > LAG), "wave tile");
+    static_assert(WL <= 15 && AL <= 15 && SC_A < WAVES && LDS <= 160 * 1024 && LOADS * (NST - 1) <= 63, "LDS, scales, vmcnt range");
+    static constexpr int mi(int u) { return u < U0 || SMALL ? u / NJ : NI - 2 + (u - U0) % 2; }
+    static constexpr int mj(int u) { return u < U0 || SMALL ? u % NJ : (u - U0) / 2; }
+    __device__ static int swz_of_w(int r) { return PAIRS ? swz_w(r) : swz(r); }
 };
 
 // The tile whose operands are loaded next, and its k-step.
@@ -193,15 +198,12 @@ struct BFrags {
     float sa[T::NJ], sw;        // ... and its scales
 };
 
-// A wave-uniform value, in a scalar register.
-__device__ __forceinline__ uint32_t uni(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
-
 struct TileSpace {
     int rt, tiles_n, total;     // row tiles, channel tiles
     const int* tab;             // grouped: row tiles of experts 0 .. e, in LDS
 };
 
-constexpr int MAX_TAB = 2048;   // experts of the LDS table; more are counted from the offsets at every tile
+constexpr int MAX_TAB = 256;    // experts of the LDS table; more are counted from the offsets at every tile
 
 // The table, by one wave; returns all experts' row tiles.
 __device__ __forceinline__ int fill_table(const BlocksParams& p, int TT, int lane, int* tab) {
@@ -291,8 +293,10 @@ __device__ __forceinline__ void cursor_next(BCursor<T>& I, const BlocksParams& p
     if (__builtin_expect(I.ks == nk, 0)) cursor_tile<T, GROUPED>(I, p, sp, I.c + 1, wave, lane);
 }
 
-// What the load instructions of the cursor's k-step share: their uniform byte offsets and LDS addresses.  Fixed here in
-// scalar registers, at least five wait states ahead of the first of them (which inline asm leaves to the program).
+// What the load instructions of the cursor's k-step share: their uniform byte offsets and LDS addresses, in scalar registers
+// for inline asm (the compiler may keep a uniform value in a vector register, and does not move it back for an asm operand).
+// The wait states that asm leaves to the program: one between a vector write and its readfirstlane, two between that and a
+// vector instruction that reads the scalar, five before a memory instruction that does.
 struct BIssue {
     uint32_t k0, s0, w, a, sc, cut;
 };
@@ -300,13 +304,12 @@ struct BIssue {
 template <class T>
 __device__ __forceinline__ BIssue bissue(const BCursor<T>& I, int nk, uint32_t st, uint32_t sc, int wave) {
     BIssue S;
-    S.k0 = uni(I.k0);
-    S.s0 = uni(I.s0);
-    S.w = uni(st + (uint32_t)(wave * T::WL * 8 * ROWB));
-    S.a = uni(st + (uint32_t)(T::A_OFF + wave * T::AL * 8 * ROWB));
-    S.sc = uni(sc + 256u * (uint32_t)wave);
+    asm volatile("s_nop 0\n\tv_readfirstlane_b32 %0, %5\n\tv_readfirstlane_b32 %1, %6\n\tv_readfirstlane_b32 %2, %7\n\t"
+                 "v_readfirstlane_b32 %3, %8\n\tv_readfirstlane_b32 %4, %9\n\ts_nop 4"
+                 : "=&s"(S.k0), "=&s"(S.s0), "=&s"(S.w), "=&s"(S.a), "=&s"(S.sc)
+                 : "v"(I.k0), "v"(I.s0), "v"(st + (uint32_t)(wave * T::WL * 8 * ROWB)),
+                   "v"(st + (uint32_t)(T::A_OFF + wave * T::AL * 8 * ROWB)), "v"(sc + 256u * (uint32_t)wave));
     S.cut = I.ks == nk - 1 ? I.cut : 0u;
-    asm volatile("s_nop 4" : "+s"(S.k0), "+s"(S.s0), "+s"(S.w), "+s"(S.a), "+s"(S.sc));
     return S;
 }
 
@@ -342,11 +345,11 @@ struct BAddr {
 template <class T>
 __device__ __forceinline__ BAddr<T> baddr(int wn, int wm, int lane) {
     const int c = lane & 15, g = lane >> 4;
-    const int wr = 8 * (c >> 2) + (c & 3);                // + 32 (i / 2) + 4 (i % 2); neither changes swz_w
+    const int wr = T::PAIRS ? 8 * (c >> 2) + (c & 3) : c; // + 32 (i / 2) + 4 (i % 2), or + 16 i; neither changes the swizzle
     const int tr = c;                                     // + 16 j; neither changes swz
     BAddr<T> A;
-    A.w0 = (uint32_t)((wn * 16 * T::NI + wr) * ROWB + ((2 * g) ^ swz_w(wr)) * 16);
-    A.w1 = (uint32_t)((wn * 16 * T::NI + wr) * ROWB + ((2 * g + 1) ^ swz_w(wr)) * 16);
+    A.w0 = (uint32_t)((wn * 16 * T::NI + wr) * ROWB + ((2 * g) ^ T::swz_of_w(wr)) * 16);
+    A.w1 = (uint32_t)((wn * 16 * T::NI + wr) * ROWB + ((2 * g + 1) ^ T::swz_of_w(wr)) * 16);
     A.t0 = (uint32_t)(T::A_OFF + (wm * 16 * T::NJ + tr) * ROWB + ((2 * g) ^ swz(tr)) * 16);
     A.t1 = (uint32_t)(T::A_OFF + (wm * 16 * T::NJ + tr) * ROWB + ((2 * g + 1) ^ swz(tr)) * 16);
     A.sa = (uint32_t)((wm * 16 * T::NJ + c) * 4);
@@ -356,7 +359,7 @@ __device__ __forceinline__ BAddr<T> baddr(int wn, int wm, int lane) {
 
 template <class T>
 __device__ __forceinline__ v8i read_w(const uint8_t* st, const BAddr<T>& A, int i) {
-    return frag16(st + A.w0, st + A.w1, (32 * (i >> 1) + 4 * (i & 1)) * ROWB);
+    return frag16(st + A.w0, st + A.w1, (T::PAIRS ? 32 * (i >> 1) + 4 * (i & 1) : 16 * i) * ROWB);
 }
 
 template <class T>
@@ -426,11 +429,79 @@ __device__ __forceinline__ void bkstep(const uint8_t* lds, uint32_t lds0, uint32
     for (int j = 0; j < T::NJ; ++j) sp[j] = s[j];
 }
 
+// The k-step of small tiles, whose time is the loads': the ring is deep, the fmas stand a whole k-step behind their MFMAs (in
+// front of the next ones, which reuse their registers), and the next k-step's fragments are read behind the MFMAs into the
+// registers that those have used.
+template <class T>
+struct SFrags {
+    v8i w[T::NI], t[T::NJ];
+    float s[T::NJ], sw;
+};
+
+template <class T>
+__device__ __forceinline__ void sread(SFrags<T>& F, const uint8_t* lds, uint32_t st, uint32_t sc, const BAddr<T>& A) {
+#pragma unroll
+    for (int i = 0; i < T::NI; ++i) F.w[i] = read_w<T>(lds + st, A, i);
+#pragma unroll
+    for (int j = 0; j < T::NJ; ++j) F.t[j] = read_t<T>(lds + st, A, j);
+#pragma unroll
+    for (int j = 0; j < T::NJ; ++j) F.s[j] = *reinterpret_cast<const float*>(lds + sc + A.sa + 64 * j);
+    F.sw = *reinterpret_cast<const float*>(lds + sc + A.sw);
+}
+
+// pend, ps: the last k-step's results and scales.
+template <class T>
+__device__ __forceinline__ void skstep(const uint8_t* lds, uint32_t lds0, uint32_t cur, uint32_t nxt, uint32_t cur_sc, uint32_t nxt_sc,
+                                       const BCursor<T>& I, int nk, const BAddr<T>& A, int wave, v4f (&acc)[T::NI][T::NJ],
+                                       SFrags<T>& F, v4f (&pend)[T::NM], float (&ps)[T::NJ]) {
+    const BIssue S = bissue<T>(I, nk, lds0 + cur, lds0 + cur_sc, wave);
+    wait_lgkm0();                                         // this wave's reads of the stage have returned
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(T::LOADS * (T::NST - 2)));       // its share of the next one has landed
+    barrier_nofence();
+#pragma unroll
+    for (int f = 0; f < T::LOADS; ++f) bload<T>(I, S, f);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < T::NM; ++u) bfma<T>(acc, pend[u], ps[T::mj(u)], u);
+#pragma unroll
+    for (int j = 0; j < T::NJ; ++j) ps[j] = F.s[j] * F.sw;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < T::NM; ++u)
+        pend[u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(F.w[T::mi(u)], F.t[T::mj(u)], v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    sread<T>(F, lds, nxt, nxt_sc, A);
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 template <class T, bool FP16, bool BIAS>
 __device__ __forceinline__ void bstore(const BlocksParams& p, const TileRows& r, int tn, int wn, int wm, int lane,
                                        const v4f (&acc)[T::NI][T::NJ]) {
     const int c = lane & 15, g = lane >> 4;
     const __amdgpu_buffer_rsrc_t yr = make_rsrc(p.y + r.row0 * p.ldy, (uint32_t)(((r.rows - 1) * p.ldy + p.N) * 2));
+    if constexpr (!T::PAIRS) {                            // 4 consecutive channels a lane and block
+#pragma unroll
+        for (int i = 0; i < T::NI; ++i) {
+            const int n = tn * T::TW + wn * 16 * T::NI + 16 * i + 4 * g;
+            const bool in = n < p.N;
+            float bias[4] = {0.f, 0.f, 0.f, 0.f};
+            if (BIAS) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) bias[e] = load_bias(p.bias, (in ? n : 0) + e, FP16);
+            }
+#pragma unroll
+            for (int j = 0; j < T::NJ; ++j) {
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] + (BIAS ? bias[e] : 0.0f);
+                const v2u32 o = FP16 ? v2u32{fp16_rne(v[0]) | (fp16_rne(v[1]) << 16), fp16_rne(v[2]) | (fp16_rne(v[3]) << 16)}
+                                     : v2u32{cvt_bf16x2(v[0], v[1]), cvt_bf16x2(v[2], v[3])};
+                const uint32_t off = (uint32_t)(wm * 16 * T::NJ + 16 * j + c) * (uint32_t)p.ldy * 2u + (uint32_t)n * 2u;
+                __builtin_amdgcn_raw_buffer_store_b64(o, yr, in ? off : OOB, 0, 0);
+            }
+        }
+        return;
+    }
     const int n0 = tn * T::TW + wn * 16 * T::NI + 8 * g;
 #pragma unroll
     for (int q = 0; q < T::NI / 2; ++q) {
@@ -457,7 +528,7 @@ __device__ __forceinline__ void bstore(const BlocksParams& p, const TileRows& r,
 }
 
 template <class T, bool FP16, bool BIAS, bool GROUPED>
-__global__ void __launch_bounds__(T::WAVES * 64, 2) gemm_blocks_tile_kernel(BlocksParams p) {
+__global__ void __launch_bounds__(T::WAVES * 64) __attribute__((amdgpu_waves_per_eu(T::WPE))) gemm_blocks_tile_kernel(BlocksParams p) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[T::LDS + (GROUPED ? MAX_TAB * 4 : 0)];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -481,7 +552,7 @@ __global__ void __launch_bounds__(T::WAVES * 64, 2) gemm_blocks_tile_kernel(Bloc
         I.cut = 0;
 #pragma unroll
         for (int i = 0; i < T::WL; ++i) {
-            const int row = 8 * (wave * T::WL + i) + lrow, ch = (lane & 7) ^ swz_w(row);
+            const int row = 8 * (wave * T::WL + i) + lrow, ch = (lane & 7) ^ T::swz_of_w(row);
             I.vw[i] = (uint32_t)(row * p.ldw) + 16u * (uint32_t)ch;
             I.cut |= ktail && 16 * ch >= ktail ? 1u << i : 0u;
         }
@@ -497,7 +568,7 @@ __global__ void __launch_bounds__(T::WAVES * 64, 2) gemm_blocks_tile_kernel(Bloc
     I.vs = OOB;
     cursor_tile<T, GROUPED>(I, p, sp, 0, wave, lane);
     if (!I.valid) return;
-#pragma unroll
+#pragma unroll 1
     for (int s = 0; s < T::NST; ++s) {
         const BIssue S = bissue<T>(I, nk, lds0 + (uint32_t)s * T::STAGE, lds0 + T::SC_OFF + (uint32_t)s * T::SC_STAGE, wave);
 #pragma unroll
@@ -507,51 +578,84 @@ __global__ void __launch_bounds__(T::WAVES * 64, 2) gemm_blocks_tile_kernel(Bloc
     const BAddr<T> A = baddr<T>(wn, wm, lane);
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(T::LOADS * (T::NST - 1)));
     barrier_nofence();
-    BFrags<T> F;
-    F.w[0] = read_w<T>(lds, A, 0);
-    F.w[1] = read_w<T>(lds, A, 1);
-#pragma unroll
-    for (int j = 0; j < T::NJ; ++j) {
-        F.t[j] = read_t<T>(lds, A, j);
-        F.sa[j] = *reinterpret_cast<const float*>(lds + T::SC_OFF + A.sa + 64 * j);
-    }
-    F.sw = *reinterpret_cast<const float*>(lds + T::SC_OFF + A.sw);
-
     uint32_t cur = 0, cur_sc = T::SC_OFF;
-    for (int c = 0;; ++c) {
-        TileRows r;
-        int tn = 0;
-        if (!tile_at<T, GROUPED>(p, sp, (int)blockIdx.x + c * (int)gridDim.x, lane, r, tn)) break;
-        v4f acc[T::NI][T::NJ], pend[LAG];
-        float sp_[T::NJ];
+    auto next_stage = [&](uint32_t& n, uint32_t& n_sc) {
+        n = cur == (T::NST - 1) * T::STAGE ? 0u : cur + T::STAGE;
+        n_sc = n == 0 ? T::SC_OFF : cur_sc + T::SC_STAGE;
+    };
+    if constexpr (T::SMALL) {
+        SFrags<T> F;
+        sread<T>(F, lds, 0, T::SC_OFF, A);
+        for (int c = 0;; ++c) {
+            TileRows r;
+            int tn = 0;
+            if (!tile_at<T, GROUPED>(p, sp, (int)blockIdx.x + c * (int)gridDim.x, lane, r, tn)) break;
+            v4f acc[T::NI][T::NJ], pend[T::NM];
+            float ps[T::NJ];
 #pragma unroll
-        for (int i = 0; i < T::NI; ++i)
+            for (int u = 0; u < T::NM; ++u) acc[T::mi(u)][T::mj(u)] = pend[u] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < T::NJ; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+            for (int j = 0; j < T::NJ; ++j) ps[j] = 0.f;
+            for (int ks = 0; ks < nk; ++ks) {
+                uint32_t nxt, nxt_sc;
+                next_stage(nxt, nxt_sc);
+                skstep<T>(lds, lds0, cur, nxt, cur_sc, nxt_sc, I, nk, A, wave, acc, F, pend, ps);
+                cursor_next<T, GROUPED>(I, p, sp, nk, wave, lane);
+                cur = nxt;
+                cur_sc = nxt_sc;
+            }
+            asm volatile("s_nop 15\n\ts_nop 7" : "+v"(pend[T::NM - 1]));
 #pragma unroll
-        for (int k = 0; k < LAG; ++k) pend[k] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < T::NJ; ++j) sp_[j] = 0.f;
-        for (int ks = 0; ks < nk; ++ks) {
-            const uint32_t nxt = cur == (T::NST - 1) * T::STAGE ? 0u : cur + T::STAGE;
-            const uint32_t nxt_sc = nxt == 0 ? T::SC_OFF : cur_sc + T::SC_STAGE;
-            bkstep<T>(lds, lds0, cur, nxt, cur_sc, nxt_sc, I, nk, A, wave, acc, F, pend, sp_);
-            cursor_next<T, GROUPED>(I, p, sp, nk, wave, lane);
-            cur = nxt;
-            cur_sc = nxt_sc;
+            for (int u = 0; u < T::NM; ++u) {
+                asm volatile("" : "+v"(pend[u]));
+                bfma<T>(acc, pend[u], ps[T::mj(u)], u);
+            }
+            bstore<T, FP16, BIAS>(p, r, tn, wn, wm, lane, acc);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        // the last results: 24 wait states behind their MFMAs, as a dependence
+    } else {
+        BFrags<T> F;
+        F.w[0] = read_w<T>(lds, A, 0);
+        F.w[1] = read_w<T>(lds, A, 1);
 #pragma unroll
-        for (int k = 0; k < LAG; ++k) {
-            if (k == 0) asm volatile("s_nop 15\n\ts_nop 7" : "+v"(pend[LAG - 1]));
+        for (int j = 0; j < T::NJ; ++j) {
+            F.t[j] = read_t<T>(lds, A, j);
+            F.sa[j] = *reinterpret_cast<const float*>(lds + T::SC_OFF + A.sa + 64 * j);
         }
+        F.sw = *reinterpret_cast<const float*>(lds + T::SC_OFF + A.sw);
+
+        for (int c = 0;; ++c) {
+            TileRows r;
+            int tn = 0;
+            if (!tile_at<T, GROUPED>(p, sp, (int)blockIdx.x + c * (int)gridDim.x, lane, r, tn)) break;
+            v4f acc[T::NI][T::NJ], pend[LAG];
+            float sp_[T::NJ];
 #pragma unroll
-        for (int k = 0; k < LAG; ++k) {
-            asm volatile("" : "+v"(pend[k]));
-            bfma<T>(acc, pend[k], sp_[T::mj(T::NM - LAG + k)], T::NM - LAG + k);
+            for (int i = 0; i < T::NI; ++i)
+#pragma unroll
+                for (int j = 0; j < T::NJ; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < LAG; ++k) pend[k] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < T::NJ; ++j) sp_[j] = 0.f;
+            for (int ks = 0; ks < nk; ++ks) {
+                uint32_t nxt, nxt_sc;
+                next_stage(nxt, nxt_sc);
+                bkstep<T>(lds, lds0, cur, nxt, cur_sc, nxt_sc, I, nk, A, wave, acc, F, pend, sp_);
+                cursor_next<T, GROUPED>(I, p, sp, nk, wave, lane);
+                cur = nxt;
+                cur_sc = nxt_sc;
+            }
+            // the last results: 24 wait states behind their MFMAs, as a dependence
+            asm volatile("s_nop 15\n\ts_nop 7" : "+v"(pend[LAG - 1]));
+#pragma unroll
+            for (int k = 0; k < LAG; ++k) {
+                asm volatile("" : "+v"(pend[k]));
+                bfma<T>(acc, pend[k], sp_[T::mj(T::NM - LAG + k)], T::NM - LAG + k);
+            }
+            bstore<T, FP16, BIAS>(p, r, tn, wn, wm, lane, acc);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        bstore<T, FP16, BIAS>(p, r, tn, wn, wm, lane, acc);
-        __builtin_amdgcn_sched_barrier(0);
     }
     wait_vm0();                                           // the loads behind the last k-step have landed before the exit
 }
@@ -592,7 +696,7 @@ template <class T>
 int launch_tile(const BlocksParams& p, const char* who, hipStream_t st) {
     const int64_t tiles = row_tiles(p, T::TT) * ((p.N + T::TW - 1) / T::TW);
     H3_REQUIRE(tiles < ((int64_t)1 << 31), "%s: too many tiles for one launch", who);
-    const dim3 grid((unsigned)std::min<int64_t>(tiles, h3host::cu_count())), block(T::WAVES * 64);
+    const dim3 grid((unsigned)std::min<int64_t>(tiles, (int64_t)T::PER_CU * h3host::cu_count())), block(T::WAVES * 64);
 #define H3_B(FP16, BIAS, GROUPED) hipLaunchKernelGGL((gemm_blocks_tile_kernel<T, FP16, BIAS, GROUPED>), grid, block, 0, st, p)
     if (p.offsets) {
         if (p.fp16) H3_B(true, false, true);
@@ -611,6 +715,20 @@ int launch_tile(const BlocksParams& p, const char* who, hipStream_t st) {
 
 int run(const BlocksParams& p, const char* who, hipStream_t st) {
     if (p.M == 0 || p.N == 0 || p.E == 0) return H3FP8_OK;
+    const int form = getenv("H3_FORM") ? atoi(getenv("H3_FORM")) : -1;
+    switch (form) {
+        case 0: return launch_tile<BTile<2, 1, 1, 1, 6, true, 2>>(p, who, st);
+        case 1: return launch_tile<BTile<2, 1, 1, 2, 4, true, 2>>(p, who, st);
+        case 2: return launch_tile<BTile<2, 2, 1, 2, 6, true, 2>>(p, who, st);
+        case 3: return launch_tile<BTile<2, 2, 2, 2, 4, true, 2>>(p, who, st);
+        case 4: return launch_tile<BTile<2, 2, 4, 2, 3, true, 2>>(p, who, st);
+        case 5: return launch_tile<BTile<2, 4, 4, 2, 4, true, 2>>(p, who, st);
+        case 6: return launch_tile<BTile<2, 4, 8, 2, 3, false, 2>>(p, who, st);
+        case 7: return launch_tile<BTile<2, 4, 8, 4, 2, false, 2>>(p, who, st);
+        case 8: return launch_tile<BTile<2, 2, 1, 1, 8, true, 2>>(p, who, st);
+        case 9: return launch_tile<BTile<4, 1, 1, 2, 6, true, 2>>(p, who, st);
+        case 10: return launch_tile<BTile<2, 2, 4, 4, 2, false, 2>>(p, who, st);
+    }
     if (p.M > 16) return launch_tile<BTile<2, 4, 8, 4, 2>>(p, who, st);
     const int tiles_n = p.N / 16;
     const int64_t tiles = row_tiles(p, 16) * tiles_n;
