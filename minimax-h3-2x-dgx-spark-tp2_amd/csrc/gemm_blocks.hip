@@ -5,8 +5,8 @@
 //
 // One MFMA makes one P_b: v_mfma 16x16x128 on e4m3 from a zero accumulator, the weight rows as its A operand and the
 // tokens as its B operand, so that lane l holds channels 4 (l >> 4) + r (r = 0 .. 3) of token l & 15 and the block's scale
-// sa * sw is one number per lane: acc = fma(P_b, sa * sw, acc) in fp32, b ascending.  Every form below computes every
-// element by this sequence, so all give the same bits.
+// sa * sw is one number per lane: acc = fma(P_b, sa * sw, acc) in fp32, b ascending, and a zero sum is +0.  Every form below
+// computes every element by this sequence, so all give the same bits.
 #include <algorithm>
 
 #include "gemm_core.h"
@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(64, 2) gemm_blocks_kernel(BlocksParams p, int 
     uint32_t o[2];
     if (p.bias) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] += load_bias(p.bias, n + i, p.fp16);
+        for (int i = 0; i < 4; ++i) acc[i] = (acc[i] + 0.0f) + load_bias(p.bias, n + i, p.fp16);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -155,28 +155,51 @@ __device__ __forceinline__ void dma4_at(v4u desc, uint32_t lds_base, uint32_t vo
 constexpr int LAG = 5;
 constexpr int AHEAD = 3;                                  // channel blocks read ahead of their MFMAs
 
-// SMALL: the k-step of few MFMAs (below).  WPE: waves per SIMD that the registers are to allow.
-template <int WN_, int WM_, int NI_, int NJ_, int NST_, bool SMALL_ = false, int WPE_ = 2>
+template <int WN_, int WM_, int NI_, int NJ_, int NST_>
 struct BTile {
-    static constexpr int WN = WN_, WM = WM_, NI = NI_, NJ = NJ_, NST = NST_, WPE = WPE_;
-    static constexpr bool SMALL = SMALL_, PAIRS = NI % 2 == 0;
+    static constexpr int WN = WN_, WM = WM_, NI = NI_, NJ = NJ_, NST = NST_;
+    static constexpr bool PAIRS = NI % 2 == 0;
     static constexpr int WAVES = WN * WM, NM = NI * NJ;
     static constexpr int TW = 16 * NI * WN, TT = 16 * NJ * WM;
     static constexpr int WL = TW / 8 / WAVES, AL = TT / 8 / WAVES;   // LDS-DMA instructions per wave and k-step
-    static constexpr int LOADS = WL + AL + 1;                        // ... and one for the scales
+    static constexpr int SC_A = (TT + 63) / 64;                      // 64-token pieces of scales, one more piece: the weight's
+    static constexpr int SL = (SC_A + WAVES) / WAVES;                // ... and the scales' per wave
+    static constexpr int LOADS = WL + AL + SL;
     static constexpr int STAGE = (TW + TT) * ROWB, A_OFF = TW * ROWB;
-    static constexpr int SC_A = (TT + 63) / 64, SC_OFF = NST * STAGE, SC_STAGE = WAVES * 256;
+    static constexpr int SC_OFF = NST * STAGE, SC_STAGE = SL * WAVES * 256;
     static constexpr int LDS = SC_OFF + NST * SC_STAGE;
-    static constexpr int PER_CU = std::min(160 * 1024 / (LDS + 1024), 32 / WAVES);   // workgroups (grouped: 1 KiB of table)
+    static_assert(LDS <= 160 * 1024, "LDS");
+    __device__ static int swz_of_w(int r) { return PAIRS ? swz_w(r) : swz(r); }
+};
+
+template <int WN, int WM, int NI, int NJ, int NST>
+struct BigTile : BTile<WN, WM, NI, NJ, NST> {
+    using B = BTile<WN, WM, NI, NJ, NST>;
     static constexpr int U0 = (NI - 2) * NJ;                         // MFMAs before the last two channel blocks
     static constexpr int BAR = (NI - 1 - AHEAD) * NJ + NJ;           // the MFMA that the barrier stands behind
-    static_assert(TW % (8 * WAVES) == 0 && TT % (8 * WAVES) == 0, "whole load instructions per wave");
-    static_assert(128 % (16 * NI) == 0 && (TW % 128 == 0 || 128 % TW == 0), "a wave's channels in one weight block");
-    static_assert(SMALL || (NI % 2 == 0 && NI > AHEAD && NM > LAG), "wave tile");
-    static_assert(WL <= 15 && AL <= 15 && SC_A < WAVES && LDS <= 160 * 1024 && LOADS * (NST - 1) <= 63, "LDS, scales, vmcnt range");
-    static constexpr int mi(int u) { return u < U0 || SMALL ? u / NJ : NI - 2 + (u - U0) % 2; }
-    static constexpr int mj(int u) { return u < U0 || SMALL ? u % NJ : (u - U0) / 2; }
-    __device__ static int swz_of_w(int r) { return PAIRS ? swz_w(r) : swz(r); }
+    static_assert(NI % 2 == 0 && NI > AHEAD && B::NM > LAG && B::SL == 1 && B::TW % 128 == 0 && 128 % (16 * NI) == 0, "wave tile");
+    static_assert(B::TW % (8 * B::WAVES) == 0 && B::TT % (8 * B::WAVES) == 0 && B::WL <= 15 && B::AL <= 15, "whole loads per wave");
+    static_assert(B::LOADS * (NST - 1) <= 63, "vmcnt range");
+    static constexpr int mi(int u) { return u < U0 ? u / NJ : NI - 2 + (u - U0) % 2; }
+    static constexpr int mj(int u) { return u < U0 ? u % NJ : (u - U0) / 2; }
+};
+
+// KS: k-steps per barrier.
+template <int WN, int WM, int NI, int NJ, int NST, int KS_>
+struct SmallTile : BTile<WN, WM, NI, NJ, NST> {
+    using B = BTile<WN, WM, NI, NJ, NST>;
+    static constexpr int KS = KS_;
+    static constexpr int PIECES = B::SC_A + 1;                       // of scales: 64 tokens' each, and the weight blocks'
+    static constexpr int SL = (PIECES + B::WAVES - 1) / B::WAVES;    // ... per wave, in the first PIECES waves at least
+    static constexpr bool EVEN = PIECES % B::WAVES == 0;             // ... and in every wave
+    static constexpr int LOADS = B::WL + B::AL + SL;                 // instructions of those waves; one fewer in the others
+    static constexpr int SC_STAGE = PIECES * 256;
+    static constexpr int LDS = B::SC_OFF + NST * SC_STAGE;
+    static_assert(B::TW % (8 * B::WAVES) == 0 && B::TT % (8 * B::WAVES) == 0, "whole load instructions per wave");
+    static_assert(128 % (16 * NI) == 0 && (B::TW % 128 == 0 || 128 % B::TW == 0), "a wave's channels in one weight block");
+    static_assert(LDS <= 160 * 1024 && LOADS * (NST - 1) <= 63 && NST >= 2 * KS, "LDS, vmcnt range, ring");
+    static constexpr int mi(int u) { return u / NJ; }
+    static constexpr int mj(int u) { return u % NJ; }
 };
 
 // The tile whose operands are loaded next, and its k-step.
@@ -429,51 +452,6 @@ __device__ __forceinline__ void bkstep(const uint8_t* lds, uint32_t lds0, uint32
     for (int j = 0; j < T::NJ; ++j) sp[j] = s[j];
 }
 
-// The k-step of small tiles, whose time is the loads': the ring is deep, the fmas stand a whole k-step behind their MFMAs (in
-// front of the next ones, which reuse their registers), and the next k-step's fragments are read behind the MFMAs into the
-// registers that those have used.
-template <class T>
-struct SFrags {
-    v8i w[T::NI], t[T::NJ];
-    float s[T::NJ], sw;
-};
-
-template <class T>
-__device__ __forceinline__ void sread(SFrags<T>& F, const uint8_t* lds, uint32_t st, uint32_t sc, const BAddr<T>& A) {
-#pragma unroll
-    for (int i = 0; i < T::NI; ++i) F.w[i] = read_w<T>(lds + st, A, i);
-#pragma unroll
-    for (int j = 0; j < T::NJ; ++j) F.t[j] = read_t<T>(lds + st, A, j);
-#pragma unroll
-    for (int j = 0; j < T::NJ; ++j) F.s[j] = *reinterpret_cast<const float*>(lds + sc + A.sa + 64 * j);
-    F.sw = *reinterpret_cast<const float*>(lds + sc + A.sw);
-}
-
-// pend, ps: the last k-step's results and scales.
-template <class T>
-__device__ __forceinline__ void skstep(const uint8_t* lds, uint32_t lds0, uint32_t cur, uint32_t nxt, uint32_t cur_sc, uint32_t nxt_sc,
-                                       const BCursor<T>& I, int nk, const BAddr<T>& A, int wave, v4f (&acc)[T::NI][T::NJ],
-                                       SFrags<T>& F, v4f (&pend)[T::NM], float (&ps)[T::NJ]) {
-    const BIssue S = bissue<T>(I, nk, lds0 + cur, lds0 + cur_sc, wave);
-    wait_lgkm0();                                         // this wave's reads of the stage have returned
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm(T::LOADS * (T::NST - 2)));       // its share of the next one has landed
-    barrier_nofence();
-#pragma unroll
-    for (int f = 0; f < T::LOADS; ++f) bload<T>(I, S, f);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int u = 0; u < T::NM; ++u) bfma<T>(acc, pend[u], ps[T::mj(u)], u);
-#pragma unroll
-    for (int j = 0; j < T::NJ; ++j) ps[j] = F.s[j] * F.sw;
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int u = 0; u < T::NM; ++u)
-        pend[u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(F.w[T::mi(u)], F.t[T::mj(u)], v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
-    __builtin_amdgcn_sched_barrier(0);
-    sread<T>(F, lds, nxt, nxt_sc, A);
-    __builtin_amdgcn_sched_barrier(0);
-}
-
 template <class T, bool FP16, bool BIAS>
 __device__ __forceinline__ void bstore(const BlocksParams& p, const TileRows& r, int tn, int wn, int wm, int lane,
                                        const v4f (&acc)[T::NI][T::NJ]) {
@@ -493,7 +471,7 @@ __device__ __forceinline__ void bstore(const BlocksParams& p, const TileRows& r,
             for (int j = 0; j < T::NJ; ++j) {
                 float v[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] + (BIAS ? bias[e] : 0.0f);
+                for (int e = 0; e < 4; ++e) v[e] = (acc[i][j][e] + 0.0f) + (BIAS ? bias[e] : 0.0f);
                 const v2u32 o = FP16 ? v2u32{fp16_rne(v[0]) | (fp16_rne(v[1]) << 16), fp16_rne(v[2]) | (fp16_rne(v[3]) << 16)}
                                      : v2u32{cvt_bf16x2(v[0], v[1]), cvt_bf16x2(v[2], v[3])};
                 const uint32_t off = (uint32_t)(wm * 16 * T::NJ + 16 * j + c) * (uint32_t)p.ldy * 2u + (uint32_t)n * 2u;
@@ -516,7 +494,7 @@ __device__ __forceinline__ void bstore(const BlocksParams& p, const TileRows& r,
         for (int j = 0; j < T::NJ; ++j) {
             float v[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = acc[2 * q + (e >> 2)][j][e & 3] + (BIAS ? bias[e] : 0.0f);
+            for (int e = 0; e < 8; ++e) v[e] = (acc[2 * q + (e >> 2)][j][e & 3] + 0.0f) + (BIAS ? bias[e] : 0.0f);
             v4u o;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -528,7 +506,7 @@ __device__ __forceinline__ void bstore(const BlocksParams& p, const TileRows& r,
 }
 
 template <class T, bool FP16, bool BIAS, bool GROUPED>
-__global__ void __launch_bounds__(T::WAVES * 64) __attribute__((amdgpu_waves_per_eu(T::WPE))) gemm_blocks_tile_kernel(BlocksParams p) {
+__global__ void __launch_bounds__(T::WAVES * 64, 2) gemm_blocks_tile_kernel(BlocksParams p) {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[T::LDS + (GROUPED ? MAX_TAB * 4 : 0)];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -583,81 +561,288 @@ __global__ void __launch_bounds__(T::WAVES * 64) __attribute__((amdgpu_waves_per
         n = cur == (T::NST - 1) * T::STAGE ? 0u : cur + T::STAGE;
         n_sc = n == 0 ? T::SC_OFF : cur_sc + T::SC_STAGE;
     };
-    if constexpr (T::SMALL) {
-        SFrags<T> F;
-        sread<T>(F, lds, 0, T::SC_OFF, A);
-        for (int c = 0;; ++c) {
-            TileRows r;
-            int tn = 0;
-            if (!tile_at<T, GROUPED>(p, sp, (int)blockIdx.x + c * (int)gridDim.x, lane, r, tn)) break;
-            v4f acc[T::NI][T::NJ], pend[T::NM];
-            float ps[T::NJ];
+    BFrags<T> F;
+    F.w[0] = read_w<T>(lds, A, 0);
+    F.w[1] = read_w<T>(lds, A, 1);
 #pragma unroll
-            for (int u = 0; u < T::NM; ++u) acc[T::mi(u)][T::mj(u)] = pend[u] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int j = 0; j < T::NJ; ++j) ps[j] = 0.f;
-            for (int ks = 0; ks < nk; ++ks) {
-                uint32_t nxt, nxt_sc;
-                next_stage(nxt, nxt_sc);
-                skstep<T>(lds, lds0, cur, nxt, cur_sc, nxt_sc, I, nk, A, wave, acc, F, pend, ps);
-                cursor_next<T, GROUPED>(I, p, sp, nk, wave, lane);
-                cur = nxt;
-                cur_sc = nxt_sc;
-            }
-            asm volatile("s_nop 15\n\ts_nop 7" : "+v"(pend[T::NM - 1]));
-#pragma unroll
-            for (int u = 0; u < T::NM; ++u) {
-                asm volatile("" : "+v"(pend[u]));
-                bfma<T>(acc, pend[u], ps[T::mj(u)], u);
-            }
-            bstore<T, FP16, BIAS>(p, r, tn, wn, wm, lane, acc);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    } else {
-        BFrags<T> F;
-        F.w[0] = read_w<T>(lds, A, 0);
-        F.w[1] = read_w<T>(lds, A, 1);
-#pragma unroll
-        for (int j = 0; j < T::NJ; ++j) {
-            F.t[j] = read_t<T>(lds, A, j);
-            F.sa[j] = *reinterpret_cast<const float*>(lds + T::SC_OFF + A.sa + 64 * j);
-        }
-        F.sw = *reinterpret_cast<const float*>(lds + T::SC_OFF + A.sw);
+    for (int j = 0; j < T::NJ; ++j) {
+        F.t[j] = read_t<T>(lds, A, j);
+        F.sa[j] = *reinterpret_cast<const float*>(lds + T::SC_OFF + A.sa + 64 * j);
+    }
+    F.sw = *reinterpret_cast<const float*>(lds + T::SC_OFF + A.sw);
 
-        for (int c = 0;; ++c) {
-            TileRows r;
-            int tn = 0;
-            if (!tile_at<T, GROUPED>(p, sp, (int)blockIdx.x + c * (int)gridDim.x, lane, r, tn)) break;
-            v4f acc[T::NI][T::NJ], pend[LAG];
-            float sp_[T::NJ];
+    for (int c = 0;; ++c) {
+        TileRows r;
+        int tn = 0;
+        if (!tile_at<T, GROUPED>(p, sp, (int)blockIdx.x + c * (int)gridDim.x, lane, r, tn)) break;
+        v4f acc[T::NI][T::NJ], pend[LAG];
+        float sp_[T::NJ];
 #pragma unroll
-            for (int i = 0; i < T::NI; ++i)
+        for (int i = 0; i < T::NI; ++i)
 #pragma unroll
-                for (int j = 0; j < T::NJ; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+            for (int j = 0; j < T::NJ; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int k = 0; k < LAG; ++k) pend[k] = v4f{0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < LAG; ++k) pend[k] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < T::NJ; ++j) sp_[j] = 0.f;
-            for (int ks = 0; ks < nk; ++ks) {
-                uint32_t nxt, nxt_sc;
-                next_stage(nxt, nxt_sc);
-                bkstep<T>(lds, lds0, cur, nxt, cur_sc, nxt_sc, I, nk, A, wave, acc, F, pend, sp_);
-                cursor_next<T, GROUPED>(I, p, sp, nk, wave, lane);
-                cur = nxt;
-                cur_sc = nxt_sc;
-            }
-            // the last results: 24 wait states behind their MFMAs, as a dependence
-            asm volatile("s_nop 15\n\ts_nop 7" : "+v"(pend[LAG - 1]));
-#pragma unroll
-            for (int k = 0; k < LAG; ++k) {
-                asm volatile("" : "+v"(pend[k]));
-                bfma<T>(acc, pend[k], sp_[T::mj(T::NM - LAG + k)], T::NM - LAG + k);
-            }
-            bstore<T, FP16, BIAS>(p, r, tn, wn, wm, lane, acc);
-            __builtin_amdgcn_sched_barrier(0);
+        for (int j = 0; j < T::NJ; ++j) sp_[j] = 0.f;
+        for (int ks = 0; ks < nk; ++ks) {
+            uint32_t nxt, nxt_sc;
+            next_stage(nxt, nxt_sc);
+            bkstep<T>(lds, lds0, cur, nxt, cur_sc, nxt_sc, I, nk, A, wave, acc, F, pend, sp_);
+            cursor_next<T, GROUPED>(I, p, sp, nk, wave, lane);
+            cur = nxt;
+            cur_sc = nxt_sc;
         }
+        // the last results: 24 wait states behind their MFMAs, as a dependence
+        asm volatile("s_nop 15\n\ts_nop 7" : "+v"(pend[LAG - 1]));
+#pragma unroll
+        for (int k = 0; k < LAG; ++k) {
+            asm volatile("" : "+v"(pend[k]));
+            bfma<T>(acc, pend[k], sp_[T::mj(T::NM - LAG + k)], T::NM - LAG + k);
+        }
+        bstore<T, FP16, BIAS>(p, r, tn, wn, wm, lane, acc);
+        __builtin_amdgcn_sched_barrier(0);
     }
     wait_vm0();                                           // the loads behind the last k-step have landed before the exit
+}
+
+// ---- the forms of small tiles ---------------------------------------------------------------------------------------
+//
+// Few tiles, or few rows per tile: the time is that of streaming the operands (the weights, mostly) and of a k-step's chain of
+// barrier, fragment reads and MFMAs.  One workgroup per tile, a deep ring of stages, fragments read a whole k-step ahead (two
+// sets of registers, the loop unrolled by two) and the fmas a whole k-step behind their MFMAs.
+// The LDS is the launch's: a size that the compiler knew would let it give a lone workgroup 512 registers a lane and put the
+// MFMAs' results into the accumulation half, a copy away from the fmas.
+template <class T>
+struct SFrags {
+    v8i w[T::NI], t[T::NJ];
+    float s[T::NJ], sw;
+};
+
+template <class T>
+__device__ __forceinline__ void sread(SFrags<T>& F, const uint8_t* lds, uint32_t st, uint32_t sc, const BAddr<T>& A) {
+#pragma unroll
+    for (int j = 0; j < T::NJ; ++j) F.t[j] = read_t<T>(lds + st, A, j);
+#pragma unroll
+    for (int i = 0; i < T::NI; ++i) F.w[i] = read_w<T>(lds + st, A, i);
+#pragma unroll
+    for (int j = 0; j < T::NJ; ++j) F.s[j] = *reinterpret_cast<const float*>(lds + sc + A.sa + 64 * j);
+    F.sw = *reinterpret_cast<const float*>(lds + sc + A.sw);
+}
+
+// The tile's loads: descriptors, lane offsets at k = 0 (OOB: nothing), the next k-step's offsets, the k-steps left.
+template <class T>
+struct SLoader {
+    v4u rw, ra, rs[T::SL];
+    uint32_t vw[T::WL], va[T::AL], vs[T::SL], step[T::SL];
+    uint32_t w_bytes, a_bytes, s_bytes[T::SL];
+    uint32_t k0, s0[T::SL];
+    uint32_t dw, da, ds;
+    int left, ktail;
+    bool full;                                            // this wave loads SL pieces of scales (else one fewer)
+};
+
+template <class T>
+__device__ __forceinline__ void sload_set(SLoader<T>& L, const BlocksParams& p, const TileRows& r, int tn, int wave, int lane) {
+    const int kb = (p.K + BK - 1) / BK, lrow = lane >> 3;
+    const int n0 = tn * T::TW, nrows = min(T::TW, p.N - n0);
+    L.rw = buffer_desc(p.w + r.e * p.w_e + (int64_t)n0 * p.ldw, (uint32_t)((nrows - 1) * p.ldw + p.K));
+    L.ra = buffer_desc(p.a + r.row0 * p.lda, (uint32_t)((r.rows - 1) * p.lda + p.K));
+    L.w_bytes = L.rw[2];
+    L.a_bytes = L.ra[2];
+#pragma unroll
+    for (int i = 0; i < T::WL; ++i) {
+        const int row = 8 * (wave * T::WL + i) + lrow;
+        L.vw[i] = (uint32_t)(row * p.ldw) + 16u * (uint32_t)((lane & 7) ^ T::swz_of_w(row));
+    }
+#pragma unroll
+    for (int j = 0; j < T::AL; ++j) {
+        const int row = 8 * (wave * T::AL + j) + lrow;
+        L.va[j] = (uint32_t)(row * p.lda) + 16u * (uint32_t)((lane & 7) ^ swz(row));
+    }
+    const int nb = (nrows + 127) / 128;
+#pragma unroll
+    for (int i = 0; i < T::SL; ++i) {                     // piece q: 64 tokens' scales, piece SC_A the weight blocks'
+        const int q = wave + i * T::WAVES;
+        const bool tok = q < T::SC_A;
+        const float* base = tok ? p.sa + r.row0 * p.sa_m : p.sw + r.e * p.sw_e + (int64_t)(n0 / 128) * p.sw_n;
+        const int64_t st = tok ? p.sa_m : p.sw_n, sk = tok ? p.sa_k : p.sw_k;
+        const int entries = tok ? r.rows : nb, first = tok ? 64 * q : 64 * (q - T::SC_A);
+        L.rs[i] = buffer_desc(base, (uint32_t)(((entries - 1) * st + (kb - 1) * sk) * 4 + 4));
+        L.s_bytes[i] = L.rs[i][2];
+        L.vs[i] = first + lane < entries ? (uint32_t)((first + lane) * st * 4) : OOB;
+        L.step[i] = (uint32_t)(sk * 4);
+        L.s0[i] = 0;
+    }
+    L.k0 = 0;
+    L.left = kb;
+    L.ktail = p.K % BK;
+    L.dw = (uint32_t)(wave * T::WL * 8 * ROWB);
+    L.da = (uint32_t)(T::A_OFF + wave * T::AL * 8 * ROWB);
+    L.ds = 256u * (uint32_t)wave;
+    L.full = wave + (T::SL - 1) * T::WAVES < T::PIECES;
+}
+
+// Before the next k-step's loads.  The last k-step of a K that is no multiple of 128 cuts the lanes past K off for good; past the
+// last one the descriptors are empty and the uniform offsets 0, so that the loads read zeros.
+template <class T>
+__device__ __forceinline__ void sload_edge(SLoader<T>& L, int wave, int lane) {
+    if (__builtin_expect(L.left == 1 && L.ktail != 0, 0)) {
+        const int lrow = lane >> 3;
+#pragma unroll
+        for (int i = 0; i < T::WL; ++i)
+            if (16 * ((lane & 7) ^ T::swz_of_w(8 * (wave * T::WL + i) + lrow)) >= L.ktail) L.vw[i] = OOB;
+#pragma unroll
+        for (int j = 0; j < T::AL; ++j)
+            if (16 * ((lane & 7) ^ swz(8 * (wave * T::AL + j) + lrow)) >= L.ktail) L.va[j] = OOB;
+    }
+    const bool live = L.left > 0;
+    L.rw[2] = live ? L.w_bytes : 0;
+    L.ra[2] = live ? L.a_bytes : 0;
+    L.k0 = live ? L.k0 : 0;
+#pragma unroll
+    for (int i = 0; i < T::SL; ++i) {
+        L.rs[i][2] = live ? L.s_bytes[i] : 0;
+        L.s0[i] = live ? L.s0[i] : 0;
+    }
+}
+
+// Load instruction i of the k-step into stage `st` (scales `sc`).
+template <class T>
+__device__ __forceinline__ void sload_one(const SLoader<T>& L, uint32_t st, uint32_t sc, int i) {
+    if (i < T::WL) {
+        dma16_at(L.rw, st + L.dw + (uint32_t)(i * 8 * ROWB), L.vw[i], L.k0);
+    } else if (i < T::WL + T::AL) {
+        const int j = i - T::WL;
+        dma16_at(L.ra, st + L.da + (uint32_t)(j * 8 * ROWB), L.va[j], L.k0);
+    } else {
+        const int k = i - T::WL - T::AL;
+        if (T::EVEN || k < T::SL - 1 || L.full) dma4_at(L.rs[k], sc + L.ds + (uint32_t)(k * T::WAVES * 256), L.vs[k], L.s0[k]);
+    }
+}
+
+template <class T>
+__device__ __forceinline__ void sload_next(SLoader<T>& L) {
+    --L.left;
+    L.k0 += BK;
+#pragma unroll
+    for (int i = 0; i < T::SL; ++i) L.s0[i] += L.step[i];
+}
+
+// All but the youngest N k-steps' loads of this wave have landed.
+template <class T, int N>
+__device__ __forceinline__ void swait(const SLoader<T>& L) {
+    if (T::EVEN || L.full) __builtin_amdgcn_s_waitcnt(vmcnt_imm(T::LOADS * N));
+    else __builtin_amdgcn_s_waitcnt(vmcnt_imm((T::LOADS - 1) * N));
+    asm volatile("" ::: "memory");
+}
+
+// Places in the ring.
+template <class T>
+struct SRing {
+    uint32_t st, sc;
+};
+template <class T>
+__device__ __forceinline__ SRing<T> snext(SRing<T> r) {
+    const bool wrap = r.st == (T::NST - 1) * T::STAGE;
+    return {wrap ? 0u : r.st + T::STAGE, wrap ? (uint32_t)T::SC_OFF : r.sc + T::SC_STAGE};
+}
+
+// One k-step on the fragments F (its results go to b): the next one's are read into G; pend and ps are the results and scales of
+// the k-step before.  BAR: a barrier first, behind which the next KS k-steps have landed in every wave and the stages of the
+// last KS whose fragments are read are free.  Each k-step loads one of those (ring place `ld`), between its MFMAs and its fmas: a
+// load holds the wave up for 16 to 30 cycles, and in a burst behind the barrier they held up everything (200 x 5376 x 7168 in
+// 128 x 64 tiles: 980 cycles a k-step, most of them 54 loads in a row).
+template <class T, bool BAR>
+__device__ __forceinline__ void skstep(const uint8_t* lds, uint32_t lds0, SRing<T>& rd, SRing<T>& ld, SLoader<T>& L,
+                                       const BAddr<T>& A, int wave, int lane, v4f (&acc)[T::NI][T::NJ], const SFrags<T>& F, SFrags<T>& G,
+                                       const v4f (&pend)[T::NM], v4f (&b)[T::NM], float (&ps)[T::NJ]) {
+    wait_lgkm0();                                         // this wave's reads of F have returned
+    if (BAR) {
+        swait<T, T::NST - 2 * T::KS>(L);
+        barrier_nofence();
+    }
+    rd = snext<T>(rd);
+    sload_edge<T>(L, wave, lane);
+    sread<T>(G, lds, rd.st, rd.sc, A);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < 2 * T::NM; ++u) {
+        if (u < T::NM)
+            b[u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(F.w[T::mi(u)], F.t[T::mj(u)], v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+        else
+            bfma<T>(acc, pend[u - T::NM], ps[T::mj(u - T::NM)], u - T::NM);
+#pragma unroll
+        for (int i = u * T::LOADS / (2 * T::NM); i < (u + 1) * T::LOADS / (2 * T::NM); ++i) sload_one<T>(L, lds0 + ld.st, lds0 + ld.sc, i);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int j = 0; j < T::NJ; ++j) ps[j] = F.s[j] * F.sw;
+    sload_next<T>(L);
+    ld = snext<T>(ld);
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// The last k-step's results, 24 wait states behind their MFMAs as a dependence.
+template <class T>
+__device__ __forceinline__ void sdrain(v4f (&acc)[T::NI][T::NJ], v4f (&pend)[T::NM], const float (&ps)[T::NJ]) {
+    asm volatile("s_nop 15\n\ts_nop 7" : "+v"(pend[T::NM - 1]));
+#pragma unroll
+    for (int u = 0; u < T::NM; ++u) {
+        asm volatile("" : "+v"(pend[u]));
+        bfma<T>(acc, pend[u], ps[T::mj(u)], u);
+    }
+}
+
+extern __shared__ __attribute__((aligned(1024))) uint8_t small_lds[];
+
+template <class T, bool FP16, bool BIAS, bool GROUPED>
+__global__ void __launch_bounds__(T::WAVES * 64) __attribute__((amdgpu_waves_per_eu(2))) gemm_blocks_small_kernel(BlocksParams p, int tiles_n, int rt) {
+    const uint8_t* lds = small_lds;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int wn = wave % T::WN, wm = wave / T::WN;
+    const uint32_t lds0 = lds_addr(lds);
+    int tm, tn;
+    tile_of((int)blockIdx.x, (int)gridDim.x, rt, tiles_n, 8, tm, tn);
+    TileRows r;
+    if (GROUPED) {
+        if (!locate_rows(p, T::TT, tm, lane, r)) return;
+    } else {
+        r.e = 0;
+        r.row0 = (int64_t)tm * T::TT;
+        r.rows = (int)min<int64_t>(T::TT, p.M - r.row0);
+    }
+    SLoader<T> L;
+    sload_set<T>(L, p, r, tn, wave, lane);
+    SRing<T> rd = {0u, (uint32_t)T::SC_OFF}, ld = rd;
+#pragma unroll
+    for (int s = 0; s < T::NST - (T::KS - 1); ++s) {
+        sload_edge<T>(L, wave, lane);
+#pragma unroll
+        for (int i = 0; i < T::LOADS; ++i) sload_one<T>(L, lds0 + ld.st, lds0 + ld.sc, i);
+        sload_next<T>(L);
+        ld = snext<T>(ld);
+    }
+    const BAddr<T> A = baddr<T>(wn, wm, lane);
+    v4f acc[T::NI][T::NJ], pa[T::NM], pb[T::NM];
+    float ps[T::NJ];
+#pragma unroll
+    for (int u = 0; u < T::NM; ++u) acc[T::mi(u)][T::mj(u)] = pa[u] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < T::NJ; ++j) ps[j] = 0.f;
+    swait<T, T::NST - T::KS>(L);
+    barrier_nofence();
+    SFrags<T> F, G;
+    sread<T>(F, lds, 0, T::SC_OFF, A);
+    // in pairs: an odd count takes one more k-step, of zeros, which adds +0
+    for (int left = (p.K + 2 * BK - 1) / (2 * BK); left > 0; --left) {
+        skstep<T, true>(lds, lds0, rd, ld, L, A, wave, lane, acc, F, G, pa, pb, ps);
+        skstep<T, T::KS == 1>(lds, lds0, rd, ld, L, A, wave, lane, acc, G, F, pb, pa, ps);
+    }
+    sdrain<T>(acc, pa, ps);
+    wait_vm0();                                           // the loads behind the last k-step have landed before the exit
+    bstore<T, FP16, BIAS>(p, r, tn, wn, wm, lane, acc);
 }
 
 constexpr int64_t kMaxSpan = 0x7fff0000LL;                // byte offsets within a tile are 32-bit
@@ -696,8 +881,30 @@ template <class T>
 int launch_tile(const BlocksParams& p, const char* who, hipStream_t st) {
     const int64_t tiles = row_tiles(p, T::TT) * ((p.N + T::TW - 1) / T::TW);
     H3_REQUIRE(tiles < ((int64_t)1 << 31), "%s: too many tiles for one launch", who);
-    const dim3 grid((unsigned)std::min<int64_t>(tiles, (int64_t)T::PER_CU * h3host::cu_count())), block(T::WAVES * 64);
+    const dim3 grid((unsigned)std::min<int64_t>(tiles, h3host::cu_count())), block(T::WAVES * 64);
 #define H3_B(FP16, BIAS, GROUPED) hipLaunchKernelGGL((gemm_blocks_tile_kernel<T, FP16, BIAS, GROUPED>), grid, block, 0, st, p)
+    if (p.offsets) {
+        if (p.fp16) H3_B(true, false, true);
+        else H3_B(false, false, true);
+    } else if (p.fp16) {
+        if (p.bias) H3_B(true, true, false);
+        else H3_B(true, false, false);
+    } else {
+        if (p.bias) H3_B(false, true, false);
+        else H3_B(false, false, false);
+    }
+#undef H3_B
+    H3_CHECK_HIP(hipGetLastError());
+    return H3FP8_OK;
+}
+
+template <class T>
+int launch_small(const BlocksParams& p, const char* who, hipStream_t st) {
+    const int64_t tiles_n = (p.N + T::TW - 1) / T::TW, rt = row_tiles(p, T::TT), tiles = rt * tiles_n;
+    H3_REQUIRE(tiles < ((int64_t)1 << 31), "%s: too many tiles for one launch", who);
+    const dim3 grid((unsigned)tiles), block(T::WAVES * 64);
+#define H3_B(FP16, BIAS, GROUPED) \
+    hipLaunchKernelGGL((gemm_blocks_small_kernel<T, FP16, BIAS, GROUPED>), grid, block, T::LDS, st, p, (int)tiles_n, (int)rt)
     if (p.offsets) {
         if (p.fp16) H3_B(true, false, true);
         else H3_B(false, false, true);
@@ -717,19 +924,22 @@ int run(const BlocksParams& p, const char* who, hipStream_t st) {
     if (p.M == 0 || p.N == 0 || p.E == 0) return H3FP8_OK;
     const int form = getenv("H3_FORM") ? atoi(getenv("H3_FORM")) : -1;
     switch (form) {
-        case 0: return launch_tile<BTile<2, 1, 1, 1, 6, true, 2>>(p, who, st);
-        case 1: return launch_tile<BTile<2, 1, 1, 2, 4, true, 2>>(p, who, st);
-        case 2: return launch_tile<BTile<2, 2, 1, 2, 6, true, 2>>(p, who, st);
-        case 3: return launch_tile<BTile<2, 2, 2, 2, 4, true, 2>>(p, who, st);
-        case 4: return launch_tile<BTile<2, 2, 4, 2, 3, true, 2>>(p, who, st);
-        case 5: return launch_tile<BTile<2, 4, 4, 2, 4, true, 2>>(p, who, st);
-        case 6: return launch_tile<BTile<2, 4, 8, 2, 3, false, 2>>(p, who, st);
-        case 7: return launch_tile<BTile<2, 4, 8, 4, 2, false, 2>>(p, who, st);
-        case 8: return launch_tile<BTile<2, 2, 1, 1, 8, true, 2>>(p, who, st);
-        case 9: return launch_tile<BTile<4, 1, 1, 2, 6, true, 2>>(p, who, st);
-        case 10: return launch_tile<BTile<2, 2, 4, 4, 2, false, 2>>(p, who, st);
+        case 0: return launch_small<SmallTile<2, 1, 1, 1, 14, 2>>(p, who, st);
+        case 1: return launch_small<SmallTile<2, 1, 1, 1, 8, 1>>(p, who, st);
+        case 2: return launch_small<SmallTile<2, 1, 1, 1, 8, 2>>(p, who, st);
+        case 3: return launch_small<SmallTile<2, 1, 1, 2, 8, 2>>(p, who, st);
+        case 4: return launch_small<SmallTile<2, 2, 1, 2, 6, 2>>(p, who, st);
+        case 5: return launch_small<SmallTile<2, 2, 2, 2, 4, 1>>(p, who, st);
+        case 6: return launch_small<SmallTile<2, 2, 2, 2, 4, 2>>(p, who, st);
+        case 7: return launch_small<SmallTile<2, 2, 4, 2, 3, 1>>(p, who, st);
+        case 8: return launch_small<SmallTile<4, 2, 2, 2, 6, 2>>(p, who, st);
+        case 9: return launch_small<SmallTile<2, 2, 4, 2, 6, 2>>(p, who, st);
+        case 10: return launch_small<SmallTile<4, 1, 2, 4, 6, 2>>(p, who, st);
+        case 11: return launch_tile<BigTile<2, 4, 8, 2, 3>>(p, who, st);
+        case 12: return launch_tile<BigTile<2, 4, 8, 4, 2>>(p, who, st);
+        case 13: return launch_small<SmallTile<2, 4, 4, 2, 4, 1>>(p, who, st);
     }
-    if (p.M > 16) return launch_tile<BTile<2, 4, 8, 4, 2>>(p, who, st);
+    if (p.M > 16) return launch_tile<BigTile<2, 4, 8, 4, 2>>(p, who, st);
     const int tiles_n = p.N / 16;
     const int64_t tiles = row_tiles(p, 16) * tiles_n;
     H3_REQUIRE(tiles < ((int64_t)1 << 31), "%s: too many tiles for one launch", who);
