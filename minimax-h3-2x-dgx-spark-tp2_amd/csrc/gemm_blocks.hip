@@ -43,6 +43,17 @@ struct TileRows {
     int64_t row0;
 };
 
+// Inclusive prefix sums over the 64 lanes: within rows of 16 by shifts, then across rows.
+__device__ __forceinline__ int wave_prefix(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);        // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);        // row_bcast 15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);        // row_bcast 31 into rows 2 and 3
+    return v;
+}
+
 // Row tile t (TT rows each, no tile spans two experts, an expert without rows has none); false past the last one.  A wave
 // looks at 64 experts at a time.
 __device__ __forceinline__ bool locate_rows(const BlocksParams& p, int TT, int64_t t, int lane, TileRows& r) {
@@ -60,12 +71,7 @@ __device__ __forceinline__ bool locate_rows(const BlocksParams& p, int TT, int64
             hi = offset_at(p, e + 1);
         }
         const int n = hi > lo ? (int)((hi - lo + TT - 1) / TT) : 0;
-        int sum = n;                                      // inclusive prefix over the lanes
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int v = __shfl_up(sum, o, 64);
-            if (lane >= o) sum += v;
-        }
+        const int sum = wave_prefix(n);
         const uint64_t past = __ballot(sum > t);
         if (past) {
             const int f = __ffsll((unsigned long long)past) - 1;
@@ -79,49 +85,6 @@ __device__ __forceinline__ bool locate_rows(const BlocksParams& p, int TT, int64
         t -= __builtin_amdgcn_readlane(sum, 63);
     }
     return false;
-}
-
-// One wave per 16 channels x 16 tokens, operands from global memory.  Two waves per SIMD at least leave a wave 256 registers,
-// and the compiler then puts an MFMA's result into vector registers, where the fmas read it.
-__global__ void __launch_bounds__(64, 2) gemm_blocks_kernel(BlocksParams p, int tiles_n) {
-    const int lane = threadIdx.x;
-    const int tn = (int)(blockIdx.x % (unsigned)tiles_n);
-    TileRows r;
-    if (!locate_rows(p, 16, blockIdx.x / (unsigned)tiles_n, lane, r)) return;
-    const int c = lane & 15, g = lane >> 4;
-    const int64_t m = r.row0 + c;
-    const bool mok = c < r.rows;
-    const uint8_t* wp = p.w + r.e * p.w_e + (int64_t)(tn * 16 + c) * p.ldw + 32 * g;
-    const uint8_t* ap = p.a + (mok ? m : r.row0) * p.lda + 32 * g;
-    const float* swp = p.sw + r.e * p.sw_e + (tn * 16 / 128) * p.sw_n;
-    const float* sap = p.sa + (mok ? m : r.row0) * p.sa_m;
-    v4f acc = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < p.K; k += BK) {
-        v8i wf = {}, af = {};
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            if (k + 32 * g + 16 * i >= p.K) continue;      // K % 16 == 0: a chunk is wholly in or out
-            const int4 x = *reinterpret_cast<const int4*>(wp + k + 16 * i), y = *reinterpret_cast<const int4*>(ap + k + 16 * i);
-            wf[4 * i] = x.x; wf[4 * i + 1] = x.y; wf[4 * i + 2] = x.z; wf[4 * i + 3] = x.w;
-            af[4 * i] = y.x; af[4 * i + 1] = y.y; af[4 * i + 2] = y.z; af[4 * i + 3] = y.w;
-        }
-        const float s = sap[(k / BK) * p.sa_k] * swp[(k / BK) * p.sw_k];
-        v4f b = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, af, v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
-        asm volatile("s_nop 15\n\ts_nop 7" : "+v"(b));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(b[i], s, acc[i]);
-    }
-    if (!mok) return;
-    const int n = tn * 16 + 4 * g;
-    uint32_t o[2];
-    if (p.bias) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = (acc[i] + 0.0f) + load_bias(p.bias, n + i, p.fp16);
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-        o[i] = p.fp16 ? fp16_rne(acc[2 * i]) | (fp16_rne(acc[2 * i + 1]) << 16) : cvt_bf16x2(acc[2 * i], acc[2 * i + 1]);
-    *reinterpret_cast<uint2*>(p.y + m * p.ldy + n) = make_uint2(o[0], o[1]);
 }
 
 // ---- the tiled form -------------------------------------------------------------------------------------------------
@@ -184,11 +147,12 @@ struct BigTile : BTile<WN, WM, NI, NJ, NST> {
     static constexpr int mj(int u) { return u < U0 ? u % NJ : (u - U0) / 2; }
 };
 
-// KS: k-steps per barrier.
-template <int WN, int WM, int NI, int NJ, int NST, int KS_>
+// KS: k-steps per barrier.  NT: the weight loads carry the non-temporal hint.
+template <int WN, int WM, int NI, int NJ, int NST, int KS_, bool NT_ = false>
 struct SmallTile : BTile<WN, WM, NI, NJ, NST> {
     using B = BTile<WN, WM, NI, NJ, NST>;
     static constexpr int KS = KS_;
+    static constexpr bool NT = NT_;
     static constexpr int PIECES = B::SC_A + 1;                       // of scales: 64 tokens' each, and the weight blocks'
     static constexpr int SL = (PIECES + B::WAVES - 1) / B::WAVES;    // ... per wave, in the first PIECES waves at least
     static constexpr bool EVEN = PIECES % B::WAVES == 0;             // ... and in every wave
@@ -223,7 +187,7 @@ struct BFrags {
 
 struct TileSpace {
     int rt, tiles_n, total;     // row tiles, channel tiles
-    const int* tab;             // grouped: row tiles of experts 0 .. e, in LDS
+    const int* tab;             // grouped: row tiles of experts 0 .. e, then their first rows and the rows behind their last, in LDS
 };
 
 constexpr int MAX_TAB = 256;    // experts of the LDS table; more are counted from the offsets at every tile
@@ -233,17 +197,17 @@ __device__ __forceinline__ int fill_table(const BlocksParams& p, int TT, int lan
     int base = 0;
     for (int e0 = 0; e0 < p.E; e0 += 64) {
         const int e = e0 + lane;
-        int sum = 0;
+        int n = 0, lo = 0, hi = 0;
         if (e < p.E) {
-            const int lo = (int)offset_at(p, e), hi = (int)offset_at(p, e + 1);
-            sum = hi > lo ? (int)(((int64_t)hi - lo + TT - 1) / TT) : 0;
+            lo = (int)offset_at(p, e), hi = (int)offset_at(p, e + 1);
+            n = hi > lo ? (int)(((int64_t)hi - lo + TT - 1) / TT) : 0;
         }
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int v = __shfl_up(sum, o, 64);
-            if (lane >= o) sum += v;
+        const int sum = wave_prefix(n);
+        if (e < MAX_TAB && e < p.E) {
+            tab[e] = base + sum;
+            tab[MAX_TAB + e] = lo;
+            tab[2 * MAX_TAB + e] = hi;
         }
-        if (e < MAX_TAB && e < p.E) tab[e] = base + sum;
         base += __builtin_amdgcn_readlane(sum, 63);
     }
     return base;
@@ -274,7 +238,7 @@ __device__ __forceinline__ bool tile_at(const BlocksParams& p, const TileSpace& 
         }
         before = __builtin_amdgcn_readlane(v, 63);
     }
-    const int lo = __builtin_amdgcn_readfirstlane((int)offset_at(p, r.e)), hi = __builtin_amdgcn_readfirstlane((int)offset_at(p, r.e + 1));
+    const int lo = __builtin_amdgcn_readfirstlane(sp.tab[MAX_TAB + r.e]), hi = __builtin_amdgcn_readfirstlane(sp.tab[2 * MAX_TAB + r.e]);
     r.row0 = lo + (int64_t)(tm - before) * T::TT;
     r.rows = (int)min<int64_t>(T::TT, hi - r.row0);
     return true;
@@ -507,7 +471,7 @@ __device__ __forceinline__ void bstore(const BlocksParams& p, const TileRows& r,
 
 template <class T, bool FP16, bool BIAS, bool GROUPED>
 __global__ void __launch_bounds__(T::WAVES * 64, 2) gemm_blocks_tile_kernel(BlocksParams p) {
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[T::LDS + (GROUPED ? MAX_TAB * 4 : 0)];
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[T::LDS + (GROUPED ? 3 * MAX_TAB * 4 : 0)];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int wn = wave % T::WN, wm = wave / T::WN;
@@ -711,7 +675,8 @@ __device__ __forceinline__ void sload_edge(SLoader<T>& L, int wave, int lane) {
 template <class T>
 __device__ __forceinline__ void sload_one(const SLoader<T>& L, uint32_t st, uint32_t sc, int i) {
     if (i < T::WL) {
-        dma16_at(L.rw, st + L.dw + (uint32_t)(i * 8 * ROWB), L.vw[i], L.k0);
+        if (T::NT) dma16_at_nt(L.rw, st + L.dw + (uint32_t)(i * 8 * ROWB), L.vw[i], L.k0);
+        else dma16_at(L.rw, st + L.dw + (uint32_t)(i * 8 * ROWB), L.vw[i], L.k0);
     } else if (i < T::WL + T::AL) {
         const int j = i - T::WL;
         dma16_at(L.ra, st + L.da + (uint32_t)(j * 8 * ROWB), L.va[j], L.k0);
@@ -920,35 +885,100 @@ int launch_small(const BlocksParams& p, const char* who, hipStream_t st) {
     return H3FP8_OK;
 }
 
+// ---- which form runs --------------------------------------------------------------------------------------------------
+//
+// Small tiles, channels x tokens (one-shot workgroups), in ascending order of their area, and how many of them a CU holds:
+#define H3_SMALL_FORMS(X)                                                                                              \
+    X(F_32x16, 3, 2, 1, 1, 1, 6, 1)                                                                                    \
+    X(F_32x32, 2, 2, 1, 1, 2, 8, 2)                                                                                    \
+    X(F_64x32, 2, 2, 1, 2, 2, 5, 1)                                                                                    \
+    X(F_32x64, 2, 2, 2, 1, 2, 6, 2)                                                                                    \
+    X(F_64x64, 1, 2, 2, 2, 2, 4, 1)                                                                                    \
+    X(F_128x64, 1, 4, 2, 2, 2, 6, 2)                                                                                   \
+    X(F_128x64_PAIR, 2, 2, 2, 4, 2, 3, 1)
+enum Form {
+#define X(id, ...) id,
+    H3_SMALL_FORMS(X)
+#undef X
+    F_256x128, F_256x256
+};
+struct FormDims { int per_cu, tw, tt; };
+constexpr FormDims kForms[] = {
+#define X(id, per, WN, WM, NI, NJ, NST, KS) {per, 16 * NI * WN, 16 * NJ * WM},
+    H3_SMALL_FORMS(X)
+#undef X
+    {1, 256, 128}, {1, 256, 256}};
+
+int64_t tiles_of(int form, int64_t row_tiles, int64_t N) { return row_tiles * ((N + kForms[form].tw - 1) / kForms[form].tw); }
+
+// The large tiles by rounds over the CUs: a k-step of 256 x 256 takes 1.6 us, of 256 x 128 1.1 us (18 880 x 21 504 x 5376: 25
+// rounds of 42 k-steps in 1.87 ms; 200 x 21 504 x 5376: one round of 256 x 128 in 48.7 us).
+int large_form(int64_t rows128, int64_t rows256, int64_t N, int G) {
+    const int64_t r128 = (tiles_of(F_256x128, rows128, N) + G - 1) / G, r256 = (tiles_of(F_256x256, rows256, N) + G - 1) / G;
+    return 16 * r256 < 11 * r128 ? F_256x256 : F_256x128;
+}
+
+// One problem: the smallest form whose tiles the CUs hold at once, since the launch then lasts as long as one tile; with 16
+// tokens or fewer always 32 x 16 (the weights' bytes count).  Past that the large tiles.  64 x 32 and 64 x 64 are for
+// experts (below): 64 x 64 on one per CU holds what 32 x 64 does on two.
+// Measured with the weights in turn from copies, smaller / taken / larger form, us, M x N x K: 32 x 5376 x 7168 13.5 / 12.0 (32 x
+// 32) / 14.7; 128 x 5376 x 7168 24.5 / 20.1 (32 x 64) / 20.7; 200 x 5376 x 7168 25.3 / 23.0 (128 x 64) / 49.5 (256 x 128); 512 x
+// 6144 x 4096 28.3 / 23.2 (128 x 64 in pairs) / 31.4; 200 x 21 504 x 5376 55.6 / 48.7 (256 x 128) / 72.2.
+int dense_form(int64_t M, int64_t N, int G) {
+    if (M <= 16) return F_32x16;
+    for (int f = 0; f < F_256x128; ++f)
+        if (f != F_64x32 && f != F_64x64 && tiles_of(f, (M + kForms[f].tt - 1) / kForms[f].tt, N) <= (int64_t)kForms[f].per_cu * G) return f;
+    return large_form((M + 127) / 128, (M + 255) / 256, N, G);
+}
+
+// By expert, from the mean rows per expert, since the host does not know the counts (each expert's last tile taken as half
+// full).  While an expert has few rows the time is its weights', and a tile should hold all of its rows.  4096 x 4096 weights,
+// 32 experts, us in 32 x 16 / 64 x 32 / 64 x 64 / 256 x 128 / 256 x 256 tiles: 4 rows each 98 / 104 / 113 / 125 / 137, 8: 116 /
+// 106 / - / 124 / 139, 16: 145 / 126 / 119 / 125 / 141, 32: 217 / 157 / 150 / 130 / 145, 128: - / - / 232 / 179 / 201, 512: - / - /
+// 624 / 384 / 373.
+int grouped_form(int64_t M, int64_t N, int64_t E, int G) {
+    if (M <= 5 * E) return F_32x16;
+    if (M <= 12 * E) return F_64x32;
+    if (M <= 24 * E) return F_64x64;
+    return large_form(M / 128 + (E + 1) / 2, M / 256 + (E + 1) / 2, N, G);
+}
+
+// The non-temporal hint on the weight loads of the forms that stream them once: for more than 64 MiB of weights, of which a next
+// call finds little in the last-level cache (256 MiB) whatever this one leaves there.  With / without it, us: 1 x 21 504 x 5376
+// 19.6 / 21.7; by expert 64 rows x 32 x 2048 x 4096 46.5 / 49.7, 256 x 32 x 4096 x 4096 106 / 116 (64 x 32); but weights that are
+// still in that cache come slower: two sets of 8 x 4096 x 4096 in turn, 20 rows, 25.9 / 21.7.
+bool streams(const BlocksParams& p) { return (int64_t)p.N * p.K * std::min<int64_t>(p.E, p.M) > (64LL << 20); }
+
+int form_for(int64_t M, int64_t N, int64_t E, bool grouped, int G) { return grouped ? grouped_form(M, N, E, G) : dense_form(M, N, G); }
+
 int run(const BlocksParams& p, const char* who, hipStream_t st) {
     if (p.M == 0 || p.N == 0 || p.E == 0) return H3FP8_OK;
-    const int form = getenv("H3_FORM") ? atoi(getenv("H3_FORM")) : -1;
-    switch (form) {
-        case 0: return launch_small<SmallTile<2, 1, 1, 1, 14, 2>>(p, who, st);
-        case 1: return launch_small<SmallTile<2, 1, 1, 1, 8, 1>>(p, who, st);
-        case 2: return launch_small<SmallTile<2, 1, 1, 1, 8, 2>>(p, who, st);
-        case 3: return launch_small<SmallTile<2, 1, 1, 2, 8, 2>>(p, who, st);
-        case 4: return launch_small<SmallTile<2, 2, 1, 2, 6, 2>>(p, who, st);
-        case 5: return launch_small<SmallTile<2, 2, 2, 2, 4, 1>>(p, who, st);
-        case 6: return launch_small<SmallTile<2, 2, 2, 2, 4, 2>>(p, who, st);
-        case 7: return launch_small<SmallTile<2, 2, 4, 2, 3, 1>>(p, who, st);
-        case 8: return launch_small<SmallTile<4, 2, 2, 2, 6, 2>>(p, who, st);
-        case 9: return launch_small<SmallTile<2, 2, 4, 2, 6, 2>>(p, who, st);
-        case 10: return launch_small<SmallTile<4, 1, 2, 4, 6, 2>>(p, who, st);
-        case 11: return launch_tile<BigTile<2, 4, 8, 2, 3>>(p, who, st);
-        case 12: return launch_tile<BigTile<2, 4, 8, 4, 2>>(p, who, st);
-        case 13: return launch_small<SmallTile<2, 4, 4, 2, 4, 1>>(p, who, st);
+    const bool grouped = p.offsets != nullptr, nt = streams(p);
+    switch (form_for(p.M, p.N, p.E, grouped, h3host::cu_count())) {
+#define X(id, per, ...)                                                                                                \
+    case id:                                                                                                           \
+        if ((id == F_32x16 || id == F_64x32 || id == F_64x64) && nt)                                                   \
+            return launch_small<SmallTile<__VA_ARGS__, id == F_32x16 || id == F_64x32 || id == F_64x64>>(p, who, st);  \
+        return launch_small<SmallTile<__VA_ARGS__>>(p, who, st);
+        H3_SMALL_FORMS(X)
+#undef X
+        case F_256x128: return launch_tile<BigTile<2, 4, 8, 2, 3>>(p, who, st);
+        default: return launch_tile<BigTile<2, 4, 8, 4, 2>>(p, who, st);
     }
-    if (p.M > 16) return launch_tile<BigTile<2, 4, 8, 4, 2>>(p, who, st);
-    const int tiles_n = p.N / 16;
-    const int64_t tiles = row_tiles(p, 16) * tiles_n;
-    H3_REQUIRE(tiles < ((int64_t)1 << 31), "%s: too many tiles for one launch", who);
-    hipLaunchKernelGGL(gemm_blocks_kernel, dim3((unsigned)tiles), dim3(64), 0, st, p, tiles_n);
-    H3_CHECK_HIP(hipGetLastError());
-    return H3FP8_OK;
 }
 
 }  // namespace
+
+namespace h3host {
+// For the tests (host only): the tile, channels x tokens, that a call over M rows runs in on G CUs, and its place in the list of
+// forms.
+void gemm_blocks_plan(int64_t M, int64_t N, int64_t E, int grouped, int G, int* out) {
+    const int f = form_for(M, N, E, grouped != 0, G);
+    out[0] = kForms[f].tw;
+    out[1] = kForms[f].tt;
+    out[2] = f;
+}
+}  // namespace h3host
 
 extern "C" {
 

@@ -54,3 +54,14 @@ def quant32(x, rows=1):
     s = torch.clamp_min((b.abs().amax(dim=(1, 3)).double() / 448.0).float(), 1.0 / (448.0 * 512.0))
     q = (b * (1.0 / s.double()).float()[:, None, :, None]).clamp(-448.0, 448.0).to(E4M3)
     return q.view(-1, p.shape[1])[:M, :K].contiguous(), s
+
+
+def plan(M, N, E=1, grouped=False, cus=256):
+    """(channels, tokens) of the tile that a product over M rows runs in: the library's own rule (csrc/gemm_blocks.hip)."""
+    import ctypes
+
+    from h3_tp2_amd import _lib
+    out = (ctypes.c_int * 3)()
+    i64 = ctypes.c_int64
+    _lib.load()["_ZN6h3host16gemm_blocks_planEllliiPi"](i64(M), i64(N), i64(E), int(grouped), cus, out)
+    return tuple(out)

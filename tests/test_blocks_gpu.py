@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from _blocks import B, E4M3, cdiv, check_product, codes, product64, quant32, scales, spread
+from _blocks import B, E4M3, cdiv, check_product, codes, plan, product64, quant32, scales, spread
 
 pytestmark = pytest.mark.gpu
 BF16, FP16, F32 = torch.bfloat16, torch.float16, torch.float32
@@ -193,6 +193,63 @@ def test_gemm_blocks_empty(cuda):
         ops.gemm_blocks(z(4, 0).to(E4M3), z(64, 0).to(E4M3), z(4, 0), z(1, 0))
 
 
+# every form that a call can run in: (M, N) with the place in the library's list that its rule gives on 256 CUs
+FORMS = [(7, 400, 0), (24, 4096, 0), (30, 13008, 1), (60, 16000, 3), (300, 2576, 3), (300, 5376, 5), (500, 6160, 6),
+         (300, 21520, 7), (2050, 5376, 8)]
+
+
+@pytest.mark.parametrize("M,N,form", FORMS)
+@pytest.mark.parametrize("K", [16, 128, 272, 640])
+def test_gemm_blocks_forms(cuda, M, N, form, K):
+    """Each form at ragged rows and channels and at 1, 3 and 5 k-blocks: the exact values, and the bits of row-by-row calls."""
+    from h3_tp2_amd import ops
+    assert plan(M, N)[2] == form
+    g = gen(M + K)
+    a, w = codes(g, M, K, integers=True), codes(g, N, K, integers=True)
+    sa, sw = scales(g, M, cdiv(K, B), pow2=True), scales(g, cdiv(N, B), cdiv(K, B), pow2=True)
+    out = torch.full((M + 2, N + 16), -3.0, device=cuda, dtype=BF16)
+    y = ops.gemm_blocks(a, w, sa, sw, out=out[1:M + 1, :N])
+    assert torch.equal(y, product64(a, w, sa, sw)[0].to(BF16))
+    assert (out[0] == -3).all() and (out[M + 1] == -3).all() and (out[:, N:] == -3).all()
+    a, w, sa, sw = codes(g, M, K), codes(g, N, K), scales(g, M, cdiv(K, B)), scales(g, cdiv(N, B), cdiv(K, B))
+    y = ops.gemm_blocks(a, w, sa, sw)
+    y64, mag = product64(a, w, sa, sw)
+    check_product(y, y64, mag, BF16)
+    for m in (0, M // 2, M - 1):
+        assert torch.equal(y[m:m + 1], ops.gemm_blocks(a[m:m + 1], w, sa[m:m + 1], sw)), m
+
+
+def test_gemm_blocks_streaming_weight(cuda):
+    """More than 64 MiB of weights: the loads with the non-temporal hint, against the same rows of a slice without it."""
+    from h3_tp2_amd import ops
+    g = gen(8)
+    M, K, N = 9, 6160, 12288
+    a, w, sa, sw = codes(g, M, K), codes(g, N, K), scales(g, M, 49), scales(g, 96, 49)
+    y = ops.gemm_blocks(a, w, sa, sw)
+    assert torch.equal(y[:, :2048], ops.gemm_blocks(a, w[:2048], sa, sw[:16]))
+    assert torch.equal(y[:, -256:], ops.gemm_blocks(a, w[-256:], sa, sw[-2:]))
+    y64, mag = product64(a, w, sa, sw)
+    check_product(y, y64, mag, BF16)
+
+
+def test_gemm_blocks_extreme_scales(cuda):
+    """Scales of 0, inf and NaN in the last of an odd number of blocks, and products that round to a negative zero: every form
+    gives the bits of the single row."""
+    from h3_tp2_amd import ops
+    g = gen(9)
+    K, N = 384, 2576
+    w, sw = codes(g, N, K), scales(g, 21, 3)
+    sw[3, 2], sw[5, 2], sw[7, 2], sw[9] = 0.0, float("inf"), float("nan"), 1e-44
+    a, sa = codes(g, 300, K), scales(g, 300, 3)
+    sa[11] = 1e-30
+    y = ops.gemm_blocks(a, w, sa, sw)
+    for m in (0, 11, 299):
+        one = ops.gemm_blocks(a[m:m + 1], w, sa[m:m + 1], sw)
+        assert torch.equal(y[m:m + 1].view(torch.int16)[~one.isnan()], one.view(torch.int16)[~one.isnan()])
+        assert torch.equal(y[m:m + 1].isnan(), one.isnan())
+    assert y[0, 7 * 128].isnan() and not y[0, 5 * 128].isfinite()
+
+
 # ---- by expert ------------------------------------------------------------------------------------------------------
 
 def grouped64(a, w, sa, sw, off):
@@ -242,6 +299,42 @@ def test_grouped(cuda, name, off, M, idx, K, N):
     for e, (lo, hi) in enumerate(zip(off[:-1], off[1:])):
         if hi > lo and e < 12:
             assert torch.equal(y[lo:hi], ops.gemm_blocks(a[lo:hi], w[e], sa[lo:hi], sw[e], dt)), e
+
+
+# (rows, experts, channels, form): each form of the rule by rows per expert; more experts than the LDS table of the large tiles
+GROUPED_FORMS = [(9, 4, 400, 0), (40, 7, 272, 2), (100, 5, 400, 4), (700, 5, 400, 7), (60000, 3, 2064, 8), (9000, 300, 144, 7)]
+
+
+@pytest.mark.parametrize("M,E,N,form", GROUPED_FORMS)
+@pytest.mark.parametrize("K", [144, 512])
+def test_grouped_forms(cuda, M, E, N, form, K):
+    from h3_tp2_amd import ops
+    assert plan(M, N, E, True)[2] == form
+    g = gen(M + K)
+    a, w = codes(g, M, K, integers=True), codes(g, E * N, K, integers=True).view(E, N, K)
+    sa, sw = scales(g, M, cdiv(K, B), pow2=True), scales(g, E, cdiv(N, B), cdiv(K, B), pow2=True)
+    cuts = torch.randint(0, M + 1, (E + 1,), generator=g, device=cuda).sort()[0]
+    cuts[E // 2] = cuts[E // 2 + 1]                                    # one without rows
+    out = torch.full((M, N), -3.0, device=cuda, dtype=BF16)
+    ops.grouped_gemm_blocks(a, w, sa, sw, cuts.to(torch.int32), out=out)
+    off = cuts.tolist()
+    for e in range(E):
+        lo, hi = off[e], off[e + 1]
+        if hi > lo:
+            assert torch.equal(out[lo:hi], product64(a[lo:hi], w[e], sa[lo:hi], sw[e])[0].to(BF16)), e
+    assert (out[:off[0]] == -3).all() and (out[off[-1]:] == -3).all()
+
+
+def test_grouped_decreasing_offsets_stay_inside(cuda):
+    """Offsets that decrease are a caller's mistake: an expert whose end is before its start has no rows, and nothing outside
+    the union of the others is written."""
+    from h3_tp2_amd import ops
+    g = gen(3)
+    a, sa, w, sw = codes(g, 40, 256), scales(g, 40, 2), codes(g, 3 * 64, 256).view(3, 64, 256), scales(g, 3, 1, 2)
+    out = torch.full((40, 64), -3.0, device=cuda, dtype=BF16)
+    ops.grouped_gemm_blocks(a, w, sa, sw, torch.tensor([5, 20, 12, 15], device=cuda), out=out)
+    assert torch.equal(out[5:12], ops.gemm_blocks(a[5:12], w[0], sa[5:12], sw[0]))
+    assert (out[:5] == -3).all() and (out[20:] == -3).all()
 
 
 def test_grouped_offsets_outside_are_ends(cuda):
