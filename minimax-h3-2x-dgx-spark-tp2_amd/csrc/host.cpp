@@ -1,6 +1,7 @@
 // The host path of the common calls, natively: the argument checks, the output allocations and the C-ABI call of
 // ops.quant_rows, ops.gemm, the dispatcher's scaled product, ops.gemm_quant, ops.gemm_swiglu_quant, ops.silu_mul_quant,
-// ops.rms_quant and ops.gate_rms_quant (h3_tp2_amd/ops.py, fp8_gemm.py).
+// ops.rms_quant and ops.gate_rms_quant (h3_tp2_amd/ops.py, fp8_gemm.py), and of the block-scaled calls ops.quant_blocks,
+// ops.silu_mul_quant_blocks, ops.gemm_blocks, ops.grouped_gemm_blocks and ops.qk_norm_rope.
 //
 // Every function takes the call only in its plain form -- exact torch tensors on one GPU, the dtypes, shapes and strides
 // that the kernels read in place, no caller-supplied outputs -- and returns None for any other, which the Python path then
@@ -10,6 +11,8 @@
 #include <Python.h>
 
 #include <ATen/ops/empty.h>
+#include <ATen/ops/empty_strided.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
@@ -354,9 +357,201 @@ PyObject* gate_rms_quant(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- the block-scaled calls --------------------------------------------------------------------------------------------
+
+int dtype_code(at::ScalarType t) {
+    return t == at::kBFloat16 ? H3FP8_DT_BF16 : t == at::kHalf ? H3FP8_DT_FP16 : t == at::kFloat ? H3FP8_DT_F32 : -1;
+}
+
+bool on_current(const at::Tensor& t) { return t.device().index() == c10::hip::current_device(); }
+
+// The stride of an axis, that of a single entry (which torch leaves arbitrary) as 0.
+int64_t axis(const at::Tensor& t, int d) { return t.size(d) > 1 ? t.stride(d) : 0; }
+
+// quant_blocks(x, rows) and silu_mul_quant_blocks(x)
+PyObject* blocks_of(PyObject* arg, int64_t rows, bool swiglu) {
+    const at::Tensor* x = plain(arg);
+    if (!x || !on_current(*x)) DECLINE;
+    const int dt = dtype_code(x->scalar_type());
+    const int64_t ldx = row_stride(*x);
+    if (dt < 0 || ldx < 0 || (swiglu && dt == H3FP8_DT_F32) || x->size(1) % (swiglu ? 32 : 16)) DECLINE;
+    const int64_t M = x->size(0), K = swiglu ? x->size(1) / 2 : x->size(1), MB = (M + rows - 1) / rows, KB = (K + 127) / 128;
+    const at::Device dev = x->device();
+    at::Tensor q, s;
+    int rc;
+    {
+        pybind11::gil_scoped_release nogil;
+        q = empty(M, K, at::kFloat8_e4m3fn, dev);
+        s = rows == 1 ? at::empty_strided({M, KB}, {1, M}, at::TensorOptions().dtype(at::kFloat).device(dev))
+                      : empty(MB, KB, at::kFloat, dev);
+        float* sp = static_cast<float*>(s.data_ptr());
+        rc = swiglu ? h3fp8_silu_mul_quant_blocks(x->data_ptr(), ldx, dt, M, K, q.data_ptr(), K, sp, axis(s, 0), axis(s, 1),
+                                                  stream_of(dev))
+                    : h3fp8_quant_blocks(x->data_ptr(), ldx, dt, M, K, (int)rows, q.data_ptr(), K, sp, axis(s, 0), axis(s, 1),
+                                         stream_of(dev));
+    }
+    if (rc) return failed(swiglu ? "h3fp8_silu_mul_quant_blocks" : "h3fp8_quant_blocks", rc);
+    return tuple_of(std::move(q), std::move(s));
+}
+
+PyObject* quant_blocks(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 2 || !PyLong_CheckExact(args[1])) DECLINE;
+    const long rows = PyLong_AsLong(args[1]);
+    if (rows == -1 && PyErr_Occurred()) PyErr_Clear();
+    if (rows != 1 && rows != 128) DECLINE;
+    return blocks_of(args[0], rows, false);
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject* silu_mul_quant_blocks(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 1) DECLINE;
+    return blocks_of(args[0], 1, true);
+    END_HANDLE_TH_ERRORS
+}
+
+// The output of a block-scaled product: None (a new tensor) or the caller's, of that shape and type with contiguous rows.
+bool output_of(PyObject* arg, int64_t M, int64_t N, at::ScalarType dt, const at::Device& dev, at::Tensor* y, int64_t* ldy) {
+    if (arg == Py_None) {
+        *y = empty(M, N, dt, dev);
+        *ldy = N;
+        return true;
+    }
+    const at::Tensor* t = plain(arg);
+    if (!t || t->scalar_type() != dt || t->device() != dev || t->dim() != 2 || t->size(0) != M || t->size(1) != N) return false;
+    *y = *t;
+    *ldy = row_stride(*t);
+    return *ldy >= 0;
+}
+
+// gemm_blocks(a, w, scale_a, scale_b, out_dtype, bias, out)
+PyObject* gemm_blocks(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 7 || !THPDtype_Check(args[4])) DECLINE;
+    const at::ScalarType dt = reinterpret_cast<THPDtype*>(args[4])->scalar_type;
+    const at::Tensor* t[4];
+    for (int i = 0; i < 4; ++i) {
+        t[i] = plain(args[i]);
+        if (!t[i] || t[i]->device() != t[0]->device() || t[i]->dim() != 2) DECLINE;
+    }
+    const at::Tensor &a = *t[0], &w = *t[1], &sa = *t[2], &sw = *t[3];
+    const int64_t lda = row_stride(a), ldw = row_stride(w);
+    const void* bias;
+    if (!on_current(a) || a.scalar_type() != at::kFloat8_e4m3fn || w.scalar_type() != at::kFloat8_e4m3fn || lda < 0 || ldw < 0 ||
+        a.size(1) != w.size(1) || (dt != at::kBFloat16 && dt != at::kHalf) || sa.scalar_type() != at::kFloat ||
+        sw.scalar_type() != at::kFloat)
+        DECLINE;
+    const int64_t M = a.size(0), K = a.size(1), N = w.size(0), KB = (K + 127) / 128;
+    if (sa.size(0) != M || sa.size(1) != KB || sw.size(0) != (N + 127) / 128 || sw.size(1) != KB ||
+        !bias_of(args[5], N, dt, a.device(), &bias))
+        DECLINE;
+    at::Tensor y;
+    int64_t ldy;
+    if (!output_of(args[6], M, N, dt, a.device(), &y, &ldy)) DECLINE;
+    int rc;
+    {
+        pybind11::gil_scoped_release nogil;
+        rc = h3fp8_gemm_blocks(a.data_ptr(), lda, w.data_ptr(), ldw, static_cast<const float*>(sa.data_ptr()), axis(sa, 0),
+                               axis(sa, 1), static_cast<const float*>(sw.data_ptr()), axis(sw, 0), axis(sw, 1), bias,
+                               y.data_ptr(), ldy, dtype_code(dt), M, N, K, stream_of(a.device()));
+    }
+    if (rc) return failed("h3fp8_gemm_blocks", rc);
+    return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
+// grouped_gemm_blocks(a, w, scale_a, scale_b, offsets, out_dtype, out)
+PyObject* grouped_gemm_blocks(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 7 || !THPDtype_Check(args[5])) DECLINE;
+    const at::ScalarType dt = reinterpret_cast<THPDtype*>(args[5])->scalar_type;
+    const at::Tensor* t[5];
+    for (int i = 0; i < 5; ++i) {
+        t[i] = plain(args[i]);
+        if (!t[i] || t[i]->device() != t[0]->device()) DECLINE;
+    }
+    const at::Tensor &a = *t[0], &w = *t[1], &sa = *t[2], &sw = *t[3], &off = *t[4];
+    const int64_t lda = row_stride(a);
+    if (!on_current(a) || a.scalar_type() != at::kFloat8_e4m3fn || w.scalar_type() != at::kFloat8_e4m3fn || lda < 0 ||
+        w.dim() != 3 || w.size(0) < 1 || w.size(1) < 1 || w.size(2) != a.size(1) || w.stride(2) != 1 ||
+        (dt != at::kBFloat16 && dt != at::kHalf) || sa.scalar_type() != at::kFloat || sw.scalar_type() != at::kFloat ||
+        sa.dim() != 2 || sw.dim() != 3 || (off.scalar_type() != at::kInt && off.scalar_type() != at::kLong))
+        DECLINE;
+    const int64_t M = a.size(0), K = a.size(1), E = w.size(0), N = w.size(1), KB = (K + 127) / 128;
+    if (sa.size(0) != M || sa.size(1) != KB || sw.size(0) != E || sw.size(1) != (N + 127) / 128 || sw.size(2) != KB ||
+        off.dim() != 1 || off.size(0) != E + 1 || !off.is_contiguous())
+        DECLINE;
+    at::Tensor y;
+    int64_t ldy;
+    if (!output_of(args[6], M, N, dt, a.device(), &y, &ldy)) DECLINE;
+    int rc;
+    {
+        pybind11::gil_scoped_release nogil;
+        rc = h3fp8_grouped_gemm_blocks(a.data_ptr(), lda, w.data_ptr(), axis(w, 0), N > 1 ? w.stride(1) : std::max(K, w.stride(1)),
+                                       static_cast<const float*>(sa.data_ptr()), axis(sa, 0), axis(sa, 1),
+                                       static_cast<const float*>(sw.data_ptr()), axis(sw, 0), axis(sw, 1), axis(sw, 2),
+                                       off.data_ptr(), (int)off.element_size(), y.data_ptr(), ldy, dtype_code(dt), M, N, K, E,
+                                       stream_of(a.device()));
+    }
+    if (rc) return failed("h3fp8_grouped_gemm_blocks", rc);
+    return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
+// qk_norm_rope(q, k, q_weight, k_weight, rope_table, eps, positions, interleaved)
+PyObject* qk_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 8 || !PyFloat_CheckExact(args[5]) || !PyBool_Check(args[7])) DECLINE;
+    const at::Tensor* t[5];
+    for (int i = 0; i < 5; ++i) {
+        t[i] = plain(args[i]);
+        if (!t[i] || t[i]->device() != t[0]->device()) DECLINE;
+    }
+    const at::Tensor &q = *t[0], &k = *t[1], &tab = *t[4];
+    const at::ScalarType dt = q.scalar_type();
+    const at::Device dev = q.device();
+    const bool inter = args[7] == Py_True;
+    if (!on_current(q) || (dt != at::kBFloat16 && dt != at::kHalf) || k.scalar_type() != dt || q.dim() != 3 || k.dim() != 3 ||
+        q.size(0) < 1 || q.size(1) < 1 || k.size(1) < 1 || k.size(0) != q.size(0) || k.size(2) != q.size(2) || q.stride(2) != 1 ||
+        k.stride(2) != 1)
+        DECLINE;
+    const int64_t T = q.size(0), H = q.size(1), Hk = k.size(1), D = q.size(2);
+    const int64_t ld_table = row_stride(tab);
+    if ((D != 64 && D != 128 && D != 256) || !vector_of(*t[2], D, dt, dev) || !vector_of(*t[3], D, dt, dev) || ld_table < 0 ||
+        (tab.scalar_type() != at::kFloat && tab.scalar_type() != at::kBFloat16) || tab.size(1) > D || tab.size(1) % (inter ? 2 : 16))
+        DECLINE;
+    const at::Tensor* pos = nullptr;
+    if (args[6] == Py_None) {
+        if (tab.size(0) < T) DECLINE;
+    } else {
+        pos = plain(args[6]);
+        if (!pos || pos->device() != dev || pos->dim() != 1 || pos->size(0) != T ||
+            (pos->scalar_type() != at::kInt && pos->scalar_type() != at::kLong))
+            DECLINE;
+    }
+    at::Tensor oq, ok;
+    int rc;
+    {
+        pybind11::gil_scoped_release nogil;
+        const at::TensorOptions opt = at::TensorOptions().dtype(dt).device(dev);
+        oq = at::empty({T, H, D}, opt);
+        ok = at::empty({T, Hk, D}, opt);
+        rc = h3fp8_qk_norm_rope(q.data_ptr(), axis(q, 0), axis(q, 1), k.data_ptr(), axis(k, 0), axis(k, 1), dtype_code(dt), T, (int)H,
+                                (int)Hk, (int)D, t[2]->data_ptr(), t[3]->data_ptr(), tab.data_ptr(), ld_table,
+                                dtype_code(tab.scalar_type()), tab.size(0), (int)tab.size(1), inter, pos ? pos->data_ptr() : nullptr,
+                                pos ? axis(*pos, 0) : 0, pos ? (int)pos->element_size() : 8, (float)PyFloat_AS_DOUBLE(args[5]),
+                                oq.data_ptr(), H * D, D, ok.data_ptr(), Hk * D, D, stream_of(dev));
+    }
+    if (rc) return failed("h3fp8_qk_norm_rope", rc);
+    return tuple_of(std::move(oq), std::move(ok));
+    END_HANDLE_TH_ERRORS
+}
+
 #define METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(name)), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {METHOD(quant_rows), METHOD(scaled_mm), METHOD(gemm), METHOD(gemm_quant),
-                          METHOD(gemm_swiglu_quant), METHOD(silu_mul_quant), METHOD(rms_quant), METHOD(gate_rms_quant),
+                          METHOD(gemm_swiglu_quant), METHOD(silu_mul_quant), METHOD(rms_quant), METHOD(gate_rms_quant), METHOD(quant_blocks),
+                          METHOD(silu_mul_quant_blocks), METHOD(gemm_blocks), METHOD(grouped_gemm_blocks), METHOD(qk_norm_rope),
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", "the common calls' host path", -1, kMethods,
                        nullptr, nullptr, nullptr, nullptr};

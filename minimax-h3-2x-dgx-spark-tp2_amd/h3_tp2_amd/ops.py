@@ -707,6 +707,8 @@ def quant_blocks(x: torch.Tensor, rows: int = 1, q: torch.Tensor | None = None, 
     """e4m3 quant with one scale per block of ``rows`` x 128 (1: activations, 128: weights) of a bf16 / fp16 / fp32 [M, K]
     tensor, K a multiple of 16: (q e4m3fn [M, K], scale fp32 [ceil(M / rows), ceil(K / 128)]).  Blocks at the edge are
     smaller.  The 1 x 128 scales come with strides (1, M), tokens contiguous, the order ``gemm_blocks`` reads best."""
+    if _host is not None and q is None and scale is None and (out := _host.quant_blocks(x, rows)) is not None:
+        return out
     if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.dtype not in _DT:
         raise ValueError("quant_blocks takes a bf16, fp16 or fp32 [M, K] tensor")
     if rows not in (1, BLOCK):
@@ -725,6 +727,8 @@ def quant_blocks(x: torch.Tensor, rows: int = 1, q: torch.Tensor | None = None, 
 def silu_mul_quant_blocks(x: torch.Tensor, q: torch.Tensor | None = None, scale: torch.Tensor | None = None):
     """silu(gate) * up of a bf16 / fp16 [M, 2F] = [gate | up] tensor, quantised per 1 x 128 block from its fp32 value:
     (q e4m3fn [M, F], scale fp32 [M, ceil(F / 128)] with strides (1, M)).  F a multiple of 16."""
+    if _host is not None and q is None and scale is None and (out := _host.silu_mul_quant_blocks(x)) is not None:
+        return out
     if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError("silu_mul_quant_blocks takes a bf16 or fp16 [M, 2F] tensor")
     M, W = x.shape
@@ -760,6 +764,8 @@ def gemm_blocks(a: torch.Tensor, w: torch.Tensor, scale_a: torch.Tensor, scale_b
     """y [M, N] = round(sum_b scale_a[m, b] * scale_b[n // 128, b] * (a_b @ w_b.T)[m, n] (+ bias[n])) for block-scaled e4m3
     operands: ``a`` [M, K] with scales [M, ceil(K / 128)], the weight ``w`` [N, K] with scales [ceil(N / 128), ceil(K / 128)]
     (``quant_blocks``; any strides), K and N multiples of 16; bf16 or fp16 out, the bias in that type."""
+    if _host is not None and (y := _host.gemm_blocks(a, w, scale_a, scale_b, out_dtype, bias, out)) is not None:
+        return y
     if a.dtype != E4M3 or w.dtype != E4M3:
         raise ValueError("gemm_blocks: a and w must be float8_e4m3fn")
     if a.dim() != 2 or w.dim() != 2 or a.shape[1] != w.shape[1]:
@@ -785,6 +791,10 @@ def grouped_gemm_blocks(a: torch.Tensor, w: torch.Tensor, scale_a: torch.Tensor,
     weights (scales [E, ceil(N / 128), ceil(K / 128)]).  ``offsets``: int32 / int64 [E + 1] on the GPU, non-decreasing, read
     by the kernel only (no synchronisation, capturable); an expert may have no rows.  Rows of y that no expert has are left
     as they were in ``out`` (without ``out`` they are undefined)."""
+    if _host is not None:
+        y = _host.grouped_gemm_blocks(a, w, scale_a, scale_b, offsets, out_dtype, out)
+        if y is not None:
+            return y
     if a.dtype != E4M3 or w.dtype != E4M3:
         raise ValueError("grouped_gemm_blocks: a and w must be float8_e4m3fn")
     if a.dim() != 2 or w.dim() != 3 or a.shape[1] != w.shape[2]:
@@ -824,6 +834,10 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     sin) at row ``positions[t]`` (int32 / int64 [T]) or t.  Pairs are dims (p, p + R / 2), or (2p, 2p + 1) with
     ``interleaved``.  fp32 throughout, rounded once.  A position outside the table gives NaN.  Returns (q, k) as new tensors,
     or ``out``, which may be (q, k) themselves."""
+    if _host is not None and out is None:
+        new = _host.qk_norm_rope(q, k, q_weight, k_weight, rope_table, eps, positions, interleaved)
+        if new is not None:
+            return new
     _heads(q, "q")
     _heads(k, "k")
     (T, H, D), (Tk, Hk, Dk) = q.shape, k.shape

@@ -136,3 +136,16 @@ def test_c_entries_refuse_without_a_gpu():
     bad("h3fp8_qk_norm_rope", qk[:16] + [4] + qk[17:], "a row per token")
     bad("h3fp8_qk_norm_rope", qk[:1] + [516] + qk[2:], "multiples of 8")
     bad("h3fp8_qk_norm_rope", qk[:19] + [p, 1, 2] + qk[22:], "int32 or int64")
+
+
+def test_native_host_path_leaves_other_calls_to_python():
+    h = _lib.host()
+    assert h is not None, "the native host path is not built"
+    x = torch.zeros(4, 64, dtype=BF16)
+    assert h.quant_blocks(x, 1) is None and h.quant_blocks(x, 2) is None and h.quant_blocks(x, 2 ** 80) is None
+    assert h.silu_mul_quant_blocks(x) is None
+    assert h.gemm_blocks(x, x, x, x, BF16, None, None) is None and h.gemm_blocks(None, x, x, x, BF16, None, None) is None
+    assert h.grouped_gemm_blocks(x, x, x, x, x, BF16, None) is None
+    assert h.qk_norm_rope(x, x, x, x, x, 1e-6, None, False) is None and h.qk_norm_rope(x, x, x, x, x, 1, None, False) is None
+    for f in (h.quant_blocks, h.silu_mul_quant_blocks, h.gemm_blocks, h.grouped_gemm_blocks, h.qk_norm_rope):
+        assert f() is None

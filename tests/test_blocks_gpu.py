@@ -443,3 +443,48 @@ def test_side_streams(cuda):
                 got.append(ops.gemm_blocks(a, w, sa, sw))
     torch.cuda.synchronize()
     assert all(torch.equal(y, ref) for y in got)
+
+
+# ---- the native host path against the Python path ---------------------------------------------------------------------
+
+def _outcome(f):
+    try:
+        out = f()
+    except Exception as e:  # noqa: BLE001
+        return type(e), str(e)
+    return [(t.dtype, tuple(t.shape), t.stride(), t.contiguous().view(torch.uint8).cpu()) for t in (out if isinstance(out, tuple) else (out,))]
+
+
+def test_native_and_python_host_paths_agree(cuda, monkeypatch):
+    """The same outputs, strides among them, or the same refusal."""
+    from h3_tp2_amd import ops
+    g = gen(12)
+    x = torch.randn(9, 544, generator=g, device=cuda).to(BF16)
+    a, w, sa, sw = codes(g, 9, 272), codes(g, 400, 272), scales(g, 9, 3), scales(g, 4, 3)
+    w3, sw3, off = codes(g, 800, 272).view(2, 400, 272), scales(g, 2, 4, 3), torch.tensor([0, 4, 9], device=cuda)
+    bias = torch.randn(400, generator=g, device=cuda).to(FP16)
+    q, k, wt = x[:, :256].view(9, 2, 128), x[:, 256:384].view(9, 1, 128), torch.ones(128, device=cuda, dtype=BF16)
+    tab, pos = torch.randn(40, 96, generator=g, device=cuda), torch.arange(9, device=cuda) * 3
+    calls = [lambda: ops.quant_blocks(x), lambda: ops.quant_blocks(x, rows=128), lambda: ops.quant_blocks(x[:1]),
+             lambda: ops.quant_blocks(x.float()), lambda: ops.quant_blocks(x[:, 1:17]), lambda: ops.quant_blocks(x, rows=3),
+             lambda: ops.quant_blocks(x[:0]), lambda: ops.silu_mul_quant_blocks(x), lambda: ops.silu_mul_quant_blocks(x[:, :40]),
+             lambda: ops.silu_mul_quant_blocks(x.half()), lambda: ops.gemm_blocks(a, w, sa, sw),
+             lambda: ops.gemm_blocks(a, w, sa, sw, FP16, bias), lambda: ops.gemm_blocks(a, w, sa, sw, BF16, bias),
+             lambda: ops.gemm_blocks(a[:1], w, sa[:1], sw), lambda: ops.gemm_blocks(a, w, sa[:, :2], sw),
+             lambda: ops.gemm_blocks(a, w, sa, sw, out=torch.empty(9, 416, device=cuda, dtype=BF16)[:, :400]),
+             lambda: ops.gemm_blocks(a, w, sa, sw, out=torch.empty(9, 401, device=cuda, dtype=BF16)[:, :400]),
+             lambda: ops.grouped_gemm_blocks(a, w3, sa, sw3, off), lambda: ops.grouped_gemm_blocks(a, w3, sa, sw3, off.int(), FP16),
+             lambda: ops.grouped_gemm_blocks(a, w3[:1], sa, sw3[:1], off[:2]), lambda: ops.grouped_gemm_blocks(a, w3, sa, sw3, off[:2]),
+             lambda: ops.qk_norm_rope(q, k, wt, wt, tab, 1e-6), lambda: ops.qk_norm_rope(q, k, wt, wt, tab, 1e-6, positions=pos),
+             lambda: ops.qk_norm_rope(q[:1], k[:1], wt, wt, tab, 1e-6, positions=pos[:1].int(), interleaved=True),
+             lambda: ops.qk_norm_rope(q, k, wt, wt, tab[:4], 1e-6), lambda: ops.qk_norm_rope(q, k, wt, wt, tab[:, :90], 1e-6)]
+    for i, f in enumerate(calls):
+        got = _outcome(f)
+        with monkeypatch.context() as m:
+            m.setattr(ops, "_host", None)
+            ref = _outcome(f)
+        assert type(got) is type(ref), (i, got, ref)
+        if isinstance(got, tuple):
+            assert got == ref, i
+        else:
+            assert all(x[:3] == y[:3] and torch.equal(x[3], y[3]) for x, y in zip(got, ref)) and len(got) == len(ref), i
