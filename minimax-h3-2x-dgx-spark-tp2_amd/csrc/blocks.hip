@@ -50,18 +50,20 @@ __device__ __forceinline__ void load8(__amdgpu_buffer_rsrc_t r, uint32_t off, v4
     if (DT == H3FP8_DT_F32) t[1] = __builtin_amdgcn_raw_buffer_load_b128(r, off + 16u, 0, 2);
 }
 
-// The largest |f| as fp32 bits: the integer order of non-negative floats, every NaN above inf.
-__device__ __forceinline__ uint32_t absmax8(const float f[8]) {
-    uint32_t m = 0;
+// max(m, |a|, |b|), NaN propagating.
+__device__ __forceinline__ float max3_abs(float m, float a, float b) {
+    float r;
+    asm("v_maximum3_f32 %0, %1, |%2|, |%3|" : "=v"(r) : "v"(m), "v"(a), "v"(b));
+    return r;
+}
+
+__device__ __forceinline__ float absmax8(const float f[8], float m) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint32_t a = f2u(f[i]) & 0x7fffffffu;
-        m = m > a ? m : a;
-    }
+    for (int i = 0; i < 8; i += 2) m = max3_abs(m, f[i], f[i + 1]);
     return m;
 }
 
-// The maximum over each row of 16 lanes (rotations within the row).
+// The maximum over each row of 16 lanes (rotations within the row); non-negative floats and NaN by their bits.
 __device__ __forceinline__ uint32_t row16_max(uint32_t m) {
     uint32_t o;
     o = (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x128, 0xf, 0xf, true); m = m > o ? m : o;      // row_ror 8, 4, 2, 1
@@ -71,17 +73,26 @@ __device__ __forceinline__ uint32_t row16_max(uint32_t m) {
     return m;
 }
 
+// FINITE: the block's maximum is finite.  Then no clamp is needed: |x| <= amax, so |x (1 / scale)| <= 448 (1 + 3 2^-24), and
+// everything below 464 rounds to 448.  Otherwise the compare / select clamp, which keeps NaN.
+template <bool FINITE>
 __device__ __forceinline__ v2u codes8(const float f[8], float inv) {
     float c[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = quant_clamp(f[i], inv);
+    for (int i = 0; i < 8; ++i) c[i] = FINITE ? f[i] * inv : quant_clamp(f[i], inv);
     return v2u{e4m3x4(c[0], c[1], c[2], c[3]), e4m3x4(c[4], c[5], c[6], c[7])};
 }
 
-// g / (1 + exp(-g)) * u.  exp2 and the reciprocal are the hardware's (1 ulp each); the rounding of -g log2(e) adds
-// |g| / 2 ulp to the exponential.  A gate so low that the exponential overflows gives -0, as the division by inf does.
+// g / (1 + exp(-g)) * u.  exp(-g) = exp2(y + d): y = -g log2(e) rounded, d what the rounding and the constant's own lost, applied
+// as a factor 1 + d ln 2 (with g held to +-200, where the exponential is 0 or inf, d stays finite).  exp2 and the reciprocal are
+// the hardware's, 1 ulp each.  A gate so low that the exponential overflows gives -0, as the division by inf does.  Without d
+// the exponential is |g| / 2 ulp off and four times as many codes at a rounding border fall on its other side.
 __device__ __forceinline__ float swiglu(float g, float u) {
-    const float e = __builtin_amdgcn_exp2f(g * -1.44269504088896340736f);
+    constexpr float L = -1.44269504088896340736f, LL = -1.92596299112661746887e-8f;       // -log2(e) = L + LL
+    const float c = __builtin_amdgcn_fmed3f(g, -200.0f, 200.0f);
+    const float y = c * L;
+    const float d = __builtin_fmaf(c, LL, __builtin_fmaf(c, L, -y));
+    const float e = __builtin_amdgcn_exp2f(y) * __builtin_fmaf(d, 0.69314718055994530942f, 1.0f);
     return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
 }
 
@@ -129,8 +140,9 @@ __global__ void __launch_bounds__(256) quant_blocks_kernel(RowsArgs a) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e] = swiglu(f[e], up[e]);
         }
-        const float s = row_scale(u2f(row16_max(absmax8(f))));
-        const v2u c = codes8(f, inv_scale(s));
+        const uint32_t mx = row16_max(f2u(absmax8(f, 0.0f)));
+        const float s = row_scale(u2f(mx)), inv = inv_scale(s);
+        const v2u c = __all(mx < 0x7f800000u) ? codes8<true>(f, inv) : codes8<false>(f, inv);
         const bool live = mw + i < a.M;
         const __amdgpu_buffer_rsrc_t qr = make_rsrc(a.q + (live ? mw + i : 0) * a.ldq, live ? (uint32_t)a.K : 0u);
         __builtin_amdgcn_raw_buffer_store_b64(c, qr, in ? (uint32_t)col : OUTSIDE, 0, 16);
@@ -164,15 +176,14 @@ __global__ void __launch_bounds__(256) quant_squares_kernel(RowsArgs a) {
             if (in && m < a.M) t[i][v] = *reinterpret_cast<const v4u*>(p + 16 * v);
         }
     }
-    uint32_t mx = 0;
+    float fm = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         float f[8];
         unpack8<DT>(t[i], f);
-        const uint32_t m = absmax8(f);
-        mx = mx > m ? mx : m;
+        fm = absmax8(f, fm);
     }
-    mx = wave_max_u32(mx);
+    uint32_t mx = wave_max_u32(f2u(fm));
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = mx;
     __syncthreads();
 #pragma unroll
@@ -184,7 +195,7 @@ __global__ void __launch_bounds__(256) quant_squares_kernel(RowsArgs a) {
         const int64_t m = mb * 128 + (threadIdx.x >> 4) + 16 * i;
         float f[8];
         unpack8<DT>(t[i], f);
-        const v2u c = codes8(f, inv);
+        const v2u c = mx < 0x7f800000u ? codes8<true>(f, inv) : codes8<false>(f, inv);     // uniform
         if (in && m < a.M) *reinterpret_cast<v2u*>(a.q + m * a.ldq + col) = c;
     }
     if (threadIdx.x == 0) a.scale[mb * a.ss_m + kb * a.ss_k] = s;

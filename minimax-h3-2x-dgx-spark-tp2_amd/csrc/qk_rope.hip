@@ -8,10 +8,14 @@
 // stock kernel that rounds n to bf16 before it rotates.
 //
 // HBM-bound: every head is read and written once.  A lane holds 8 consecutive dims (16-byte loads and stores), D / 8 lanes
-// a head, so a wave holds 512 / D heads of one token at a time and takes the token's q heads and then its k heads; the
-// rotation's table entries of the lane's dims are loaded once per token and kept.  The sum of squares is an xor butterfly
-// over the head's lanes.  The half-split partner of dim d is 16-byte aligned with it when half % 8 == 0, so it is one lane
-// exchange per dim; the interleaved partner is in the lane.
+// a head, so a wave holds 512 / D heads of one token at a time (a pass): the token's q heads and then its k heads, UNROLL passes'
+// loads in flight together.  The norm weights and the table entries of the lane's dims are loaded once and kept.  The sum of
+// squares goes over the head's lanes by DPP.  The half-split partner of dim d is half = R / 2 away, a multiple of 8, so it is
+// in another lane at the same place: the lanes exchange their packed inputs (4 words instead of 8 normalised values) and each
+// normalises its partner's too; the interleaved partner is in the lane.  With few tokens a token's passes are dealt over
+// several waves, until every SIMD has two.
+#include <algorithm>
+
 #include "h3fp8_common.h"
 
 namespace {
@@ -36,6 +40,7 @@ struct QkRopeArgs {
     int64_t T;
     int H, Hk, half;
     float eps;
+    int vec;                                    // the table entries of a lane are aligned for vector loads
     int per;                                    // passes (512 / D heads each) a wave takes
     int chunks;                                 // waves per token
 };
@@ -58,10 +63,43 @@ __device__ __forceinline__ v4u narrow8(const float f[8]) {
     return v;
 }
 
-template <bool TF32>
-__device__ __forceinline__ float table_at(const void* row, int i) {
-    return TF32 ? reinterpret_cast<const float*>(row)[i] : bf16_to_f32(reinterpret_cast<const uint16_t*>(row)[i]);
+// Entries p .. p + N - 1 of a table row; VEC: 16-byte aligned there.
+template <bool TF32, bool VEC, int N>
+__device__ __forceinline__ void table_read(const char* row, int p, float f[N]) {
+    if (VEC) {
+        if (TF32) {
+#pragma unroll
+            for (int i = 0; i < N; i += 4) {
+                const v4f v = *reinterpret_cast<const v4f*>(row + 4 * (p + i));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f[i + e] = v[e];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i += 4) {
+                const uint2 v = *reinterpret_cast<const uint2*>(row + 2 * (p + i));
+                f[i] = u2f(v.x << 16); f[i + 1] = u2f(v.x & 0xffff0000u); f[i + 2] = u2f(v.y << 16); f[i + 3] = u2f(v.y & 0xffff0000u);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            f[i] = TF32 ? reinterpret_cast<const float*>(row)[p + i] : bf16_to_f32(reinterpret_cast<const uint16_t*>(row)[p + i]);
+    }
 }
+
+// The sum over a head's LPH lanes.
+template <int LPH>
+__device__ __forceinline__ float head_sum(float v) {
+    v += u2f((uint32_t)__builtin_amdgcn_mov_dpp((int)f2u(v), 0xb1, 0xf, 0xf, true));     // lane ^ 1
+    v += u2f((uint32_t)__builtin_amdgcn_mov_dpp((int)f2u(v), 0x4e, 0xf, 0xf, true));     // lane ^ 2
+    v += u2f((uint32_t)__builtin_amdgcn_mov_dpp((int)f2u(v), 0x141, 0xf, 0xf, true));    // the other four of a half row
+    if (LPH >= 16) v += u2f((uint32_t)__builtin_amdgcn_mov_dpp((int)f2u(v), 0x140, 0xf, 0xf, true));   // the other half row
+    if (LPH >= 32) v += __shfl_xor(v, 16, 64);
+    return v;
+}
+
+constexpr int UNROLL = 4;
 
 template <int D, bool FP16, bool TF32, bool INTER>
 __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkRopeArgs a) {
@@ -75,66 +113,105 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkRopeArgs a) {
     const int j = lane % LPH, sub = lane / LPH;             // the lane's 8 dims 8j .. 8j + 7 of head `sub` of a pass
     const int heads = a.H + a.Hk;
     const int passes = min(pass0 + a.per, (heads + HPW - 1) / HPW);
+    const int half = a.half;
+    const bool rotated = 8 * j < 2 * half;                  // half-split: half % 8 == 0, a lane is wholly in or out
+    const int pj = INTER || !rotated ? j : 8 * j < half ? j + half / 8 : j - half / 8;     // the partner lane of the head
+    auto load = [&](int ps) {
+        const int h = ps * HPW + sub;
+        const bool live = ps < passes && h < heads, isq = h < a.H;
+        const uint16_t* src = isq ? a.q + t * a.q_t + (int64_t)h * a.q_h : a.k + t * a.k_t + (int64_t)(h - a.H) * a.k_h;
+        return live ? __builtin_nontemporal_load(reinterpret_cast<const v4u*>(src + 8 * j)) : v4u{0u, 0u, 0u, 0u};
+    };
+    v4u v[UNROLL];
+#pragma unroll
+    for (int i = 0; i < UNROLL; ++i) v[i] = load(pass0 + i);
+    // the norm weights of the lane's dims and of its partner's, for q and for k
+    const v4u none = {0u, 0u, 0u, 0u};
+    const v4u wq = a.H ? *reinterpret_cast<const v4u*>(a.wq + 8 * j) : none, wk = a.Hk ? *reinterpret_cast<const v4u*>(a.wk + 8 * j) : none;
+    const v4u pq = INTER || !a.H ? none : *reinterpret_cast<const v4u*>(a.wq + 8 * pj);
+    const v4u pk = INTER || !a.Hk ? none : *reinterpret_cast<const v4u*>(a.wk + 8 * pj);
     int64_t pos = t;
     if (a.positions)
         pos = a.pos_bytes == 8 ? reinterpret_cast<const int64_t*>(a.positions)[t * a.pos_stride]
                                : (int64_t)reinterpret_cast<const int32_t*>(a.positions)[t * a.pos_stride];
     const bool known = pos >= 0 && pos < a.P;               // else the outputs are NaN and the table is not read
-    const int half = a.half;
     // cos and the signed sin of each of the lane's dims: out_d = n_d cos + partner_d sin (1 and 0 past the rotated dims)
     float cs[8], sn[8];
-    const char* row = reinterpret_cast<const char*>(a.table) + (known ? pos : 0) * a.ld_table * (TF32 ? 4 : 2);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int d = 8 * j + e;
-        cs[e] = 1.0f;
-        sn[e] = 0.0f;
-        if (d < 2 * half) {
-            const int p = INTER ? d >> 1 : (d < half ? d : d - half);
-            const bool minus = INTER ? !(d & 1) : d < half;
-            const float s = table_at<TF32>(row, half + p);
-            cs[e] = table_at<TF32>(row, p);
-            sn[e] = minus ? -s : s;
-        }
-        if (!known) cs[e] = __builtin_nanf("");
-    }
-    const bool rotated = 8 * j < 2 * half;                  // half-split: half % 8 == 0, a lane is wholly in or out
-    const int partner = INTER ? 0 : (lane - j) + (8 * j < half ? j + half / 8 : j - half / 8);
-    for (int ps = pass0; ps < passes; ++ps) {
-        const int h = ps * HPW + sub;
-        const bool live = h < heads, isq = h < a.H;
-        const uint16_t* src = isq ? a.q + t * a.q_t + (int64_t)h * a.q_h : a.k + t * a.k_t + (int64_t)(h - a.H) * a.k_h;
-        v4u v = {0u, 0u, 0u, 0u}, w = {0u, 0u, 0u, 0u};
-        if (live) {
-            v = *reinterpret_cast<const v4u*>(src + 8 * j);
-            w = *reinterpret_cast<const v4u*>((isq ? a.wq : a.wk) + 8 * j);
-        }
-        float x[8], g[8];
-        widen8<FP16>(v, x);
-        widen8<FP16>(w, g);
-        float ss = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(x[e], x[e], ss);
-#pragma unroll
-        for (int o = LPH / 2; o >= 1; o >>= 1) ss += __shfl_xor(ss, o, 64);
-        const float r = 1.0f / __builtin_sqrtf(ss * (1.0f / D) + a.eps);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = x[e] * r * g[e];
-        float y[8];
+    for (int e = 0; e < 8; ++e) cs[e] = known ? 1.0f : __builtin_nanf(""), sn[e] = 0.0f;
+    if (known && rotated) {
+        const char* row = reinterpret_cast<const char*>(a.table) + pos * a.ld_table * (TF32 ? 4 : 2);
         if (INTER) {
+            float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
+            if (a.vec) {
+                table_read<TF32, true, 4>(row, 4 * j, c);
+                table_read<TF32, true, 4>(row, half + 4 * j, s);
+            } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                y[e] = 8 * j + e < 2 * half ? __builtin_fmaf(x[e], cs[e], x[e ^ 1] * sn[e]) : x[e] * cs[e];
+                for (int e = 0; e < 4; ++e)
+                    if (4 * j + e < half) {
+                        table_read<TF32, false, 1>(row, 4 * j + e, c + e);
+                        table_read<TF32, false, 1>(row, half + 4 * j + e, s + e);
+                    }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) cs[e] = c[e >> 1], sn[e] = (e & 1) ? s[e >> 1] : -s[e >> 1];
         } else {
+            const int p = 8 * j < half ? 8 * j : 8 * j - half;
+            if (a.vec) {
+                table_read<TF32, true, 8>(row, p, cs);
+                table_read<TF32, true, 8>(row, half + p, sn);
+            } else {
+                table_read<TF32, false, 8>(row, p, cs);
+                table_read<TF32, false, 8>(row, half + p, sn);
+            }
+            if (8 * j < half) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float o = __shfl(x[e], rotated ? partner : lane, 64);
-                y[e] = rotated ? __builtin_fmaf(x[e], cs[e], o * sn[e]) : x[e] * cs[e];
+                for (int e = 0; e < 8; ++e) sn[e] = -sn[e];
             }
         }
-        if (!live) continue;
-        uint16_t* dst = isq ? a.oq + t * a.oq_t + (int64_t)h * a.oq_h : a.ok + t * a.ok_t + (int64_t)(h - a.H) * a.ok_h;
-        *reinterpret_cast<v4u*>(dst + 8 * j) = narrow8<FP16>(y);
+    }
+    for (int ps = pass0; ps < passes; ps += UNROLL) {
+        v4u cur[UNROLL];
+#pragma unroll
+        for (int i = 0; i < UNROLL; ++i) cur[i] = v[i];
+#pragma unroll
+        for (int i = 0; i < UNROLL; ++i) v[i] = load(ps + UNROLL + i);
+#pragma unroll
+        for (int i = 0; i < UNROLL; ++i) {
+            const int h = (ps + i) * HPW + sub;
+            const bool live = ps + i < passes && h < heads, isq = h < a.H;
+            float x[8], y[8], g[8];
+            widen8<FP16>(cur[i], x);
+            float ss = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(x[e], x[e], ss);
+            const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(head_sum<LPH>(ss), 1.0f / D, a.eps));
+            const v4u w = {isq ? wq[0] : wk[0], isq ? wq[1] : wk[1], isq ? wq[2] : wk[2], isq ? wq[3] : wk[3]};
+            widen8<FP16>(w, g);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = x[e] * r * g[e];
+            if (INTER) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    y[e] = 8 * j + e < 2 * half ? __builtin_fmaf(x[e], cs[e], x[e ^ 1] * sn[e]) : x[e] * cs[e];
+            } else {
+                v4u o;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = (uint32_t)__shfl((int)cur[i][e], lane - j + pj, 64);
+                float p[8], pg[8];
+                widen8<FP16>(o, p);
+                const v4u pw = {isq ? pq[0] : pk[0], isq ? pq[1] : pk[1], isq ? pq[2] : pk[2], isq ? pq[3] : pk[3]};
+                widen8<FP16>(pw, pg);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    y[e] = rotated ? __builtin_fmaf(x[e], cs[e], p[e] * r * pg[e] * sn[e]) : x[e] * cs[e];
+            }
+            if (live) {
+                uint16_t* dst = isq ? a.oq + t * a.oq_t + (int64_t)h * a.oq_h : a.ok + t * a.ok_t + (int64_t)(h - a.H) * a.ok_h;
+                __builtin_nontemporal_store(narrow8<FP16>(y), reinterpret_cast<v4u*>(dst + 8 * j));
+            }
+        }
     }
 }
 
@@ -149,8 +226,10 @@ int launch_qk(const QkRopeArgs& a, bool interleaved, dim3 grid, hipStream_t st) 
 template <int D>
 int launch_head(QkRopeArgs a, bool fp16, bool tf32, bool interleaved, hipStream_t st) {
     const int passes = (a.H + a.Hk + 512 / D - 1) / (512 / D);
-    a.per = passes;
-    a.chunks = 1;
+    // two waves per SIMD while there are passes to deal, then whole tokens
+    const int64_t waves = 8LL * h3host::cu_count();
+    a.per = (int)std::max<int64_t>(1, std::min<int64_t>(passes, a.T * passes / waves));
+    a.chunks = (passes + a.per - 1) / a.per;
     const int64_t units = a.T * a.chunks;
     H3_REQUIRE(units < ((int64_t)1 << 33), "h3fp8_qk_norm_rope: too many tokens");
     const dim3 grid((unsigned)((units + 3) / 4));
@@ -196,6 +275,8 @@ extern "C" int h3fp8_qk_norm_rope(const void* q, int64_t q_t, int64_t q_h, const
     a.table = table; a.ld_table = ld_table; a.P = R ? P : T;
     a.positions = R ? positions : nullptr; a.pos_stride = pos_stride; a.pos_bytes = pos_bytes;
     a.T = T; a.H = H; a.Hk = Hk; a.half = R / 2; a.eps = eps;
+    const int need = table_dtype == H3FP8_DT_F32 ? 16 : 8;      // bytes of four entries
+    a.vec = R % 8 == 0 && ld_table % 4 == 0 && ((uintptr_t)table & (need - 1)) == 0;
     const bool fp16 = dtype == H3FP8_DT_FP16, tf32 = table_dtype == H3FP8_DT_F32;
     hipStream_t st = (hipStream_t)stream;
     if (D == 64) return launch_head<64>(a, fp16, tf32, interleaved != 0, st);
