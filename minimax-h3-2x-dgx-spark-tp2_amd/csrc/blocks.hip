@@ -11,7 +11,10 @@
 // 16 lanes x 8 elements each (16-byte loads, 8-byte code stores, the maximum over 16 lanes by row rotations), and takes
 // ROWS / 4 tokens of the same four blocks, all loads in flight before the first use; the four waves of a workgroup share
 // a tile of ROWS tokens, whose scales go through LDS so that the scale tensor, token-contiguous as the product reads it,
-// is written in pieces of ROWS consecutive entries.
+// is written in pieces of ROWS consecutive entries.  ROWS = 8: quant of 42848 x 7168 bf16 141 us (6.6 TB/s), SwiGLU of 18880 x
+// 2 x 14336 204 us (6.7 TB/s), of 64 x 2 x 2048 2.8 us; with 32 rows 152, 220 and 5.3 (few and long waves), 16 rows 146
+// and 217, 4 rows 151, 230 and 2.4 (a scale line in more pieces).  128 x 128: 21504 x 5376 bf16 54 us (6.4 TB/s); with 256
+// threads of 8 loads each, behind branches, it was 64.
 #include "h3fp8_common.h"
 
 namespace {
@@ -108,7 +111,7 @@ struct RowsArgs {
     int groups;                 // groups of four blocks per row
 };
 
-constexpr int ROWS = 32;        // tokens per workgroup
+constexpr int ROWS = 8;         // tokens per workgroup
 
 template <int DT, bool SWIGLU>
 __global__ void __launch_bounds__(256) quant_blocks_kernel(RowsArgs a) {
@@ -156,29 +159,29 @@ __global__ void __launch_bounds__(256) quant_blocks_kernel(RowsArgs a) {
     }
 }
 
-// One 128 x 128 block per workgroup: thread t holds 8 columns 8 (t & 15) of rows (t >> 4) + 16 i.
+// One 128 x 128 block per workgroup: thread t holds 8 columns 8 (t & 15) of rows (t >> 4) + 32 i.  Threads past the last row
+// or column read the block's last ones again, which does not change its maximum, and store nothing.
+constexpr int SQ_THREADS = 512;
+
 template <int DT>
-__global__ void __launch_bounds__(256) quant_squares_kernel(RowsArgs a) {
-    constexpr int EB = Elem<DT>::BYTES, NV = DT == H3FP8_DT_F32 ? 2 : 1;
-    __shared__ uint32_t part[4];
+__global__ void __launch_bounds__(SQ_THREADS) quant_squares_kernel(RowsArgs a) {
+    constexpr int EB = Elem<DT>::BYTES, NV = DT == H3FP8_DT_F32 ? 2 : 1, STEP = SQ_THREADS / 16, N = 128 / STEP;
+    __shared__ uint32_t part[SQ_THREADS / 64];
     const int kb = (int)(blockIdx.x % (unsigned)a.groups);
     const int64_t mb = blockIdx.x / (unsigned)a.groups;
-    const int col = kb * 128 + 8 * (threadIdx.x & 15);
+    const int col = kb * 128 + 8 * (threadIdx.x & 15), row = (int)threadIdx.x >> 4;
+    const int rows = (int)min((int64_t)128, a.M - mb * 128);
     const bool in = col < a.K;
-    v4u t[8][NV];
+    const uint8_t* src = a.x + mb * 128 * a.ldx + (int64_t)(in ? col : a.K - 8) * EB;
+    v4u t[N][NV];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int64_t m = mb * 128 + (threadIdx.x >> 4) + 16 * i;
-        const uint8_t* p = a.x + m * a.ldx + (int64_t)col * EB;
+    for (int i = 0; i < N; ++i)
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            t[i][v] = v4u{0u, 0u, 0u, 0u};
-            if (in && m < a.M) t[i][v] = *reinterpret_cast<const v4u*>(p + 16 * v);
-        }
-    }
+        for (int v = 0; v < NV; ++v)
+            t[i][v] = __builtin_nontemporal_load(reinterpret_cast<const v4u*>(src + min(row + STEP * i, rows - 1) * a.ldx + 16 * v));
     float fm = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < N; ++i) {
         float f[8];
         unpack8<DT>(t[i], f);
         fm = absmax8(f, fm);
@@ -187,16 +190,16 @@ __global__ void __launch_bounds__(256) quant_squares_kernel(RowsArgs a) {
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = mx;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) mx = mx > part[i] ? mx : part[i];
+    for (int i = 0; i < SQ_THREADS / 64; ++i) mx = mx > part[i] ? mx : part[i];
     const float s = row_scale(u2f(mx));
     const float inv = inv_scale(s);
+    uint8_t* dst = a.q + mb * 128 * a.ldq + col;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int64_t m = mb * 128 + (threadIdx.x >> 4) + 16 * i;
+    for (int i = 0; i < N; ++i) {
         float f[8];
         unpack8<DT>(t[i], f);
-        const v2u c = mx < 0x7f800000u ? codes8<true>(f, inv) : codes8<false>(f, inv);     // uniform
-        if (in && m < a.M) *reinterpret_cast<v2u*>(a.q + m * a.ldq + col) = c;
+        const v2u c = mx < 0x7f800000u ? codes8<true>(f, inv) : codes8<false>(f, inv);     // one side for the workgroup
+        if (in && row + STEP * i < rows) *reinterpret_cast<v2u*>(dst + (row + STEP * i) * a.ldq) = c;
     }
     if (threadIdx.x == 0) a.scale[mb * a.ss_m + kb * a.ss_k] = s;
 }
@@ -225,7 +228,7 @@ int launch_rows(RowsArgs a, int dtype, hipStream_t st) {
     const dim3 grid((unsigned)blocks), block(256);
     if (dtype == H3FP8_DT_BF16) hipLaunchKernelGGL((quant_blocks_kernel<H3FP8_DT_BF16, SWIGLU>), grid, block, 0, st, a);
     else if (dtype == H3FP8_DT_FP16) hipLaunchKernelGGL((quant_blocks_kernel<H3FP8_DT_FP16, SWIGLU>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((quant_blocks_kernel<H3FP8_DT_F32, SWIGLU>), grid, block, 0, st, a);
+    else if constexpr (!SWIGLU) hipLaunchKernelGGL((quant_blocks_kernel<H3FP8_DT_F32, SWIGLU>), grid, block, 0, st, a);
     H3_CHECK_HIP(hipGetLastError());
     return H3FP8_OK;
 }
@@ -253,7 +256,7 @@ int h3fp8_quant_blocks(const void* x, int64_t ldx, int dtype, int64_t M, int64_t
     a.groups = (int)((K + 127) / 128);
     const int64_t blocks = (M + 127) / 128 * a.groups;
     H3_REQUIRE(blocks < ((int64_t)1 << 31), "h3fp8_quant_blocks: too many blocks for one launch");
-    const dim3 grid((unsigned)blocks), block(256);
+    const dim3 grid((unsigned)blocks), block(SQ_THREADS);
     if (dtype == H3FP8_DT_BF16) hipLaunchKernelGGL((quant_squares_kernel<H3FP8_DT_BF16>), grid, block, 0, st, a);
     else if (dtype == H3FP8_DT_FP16) hipLaunchKernelGGL((quant_squares_kernel<H3FP8_DT_FP16>), grid, block, 0, st, a);
     else hipLaunchKernelGGL((quant_squares_kernel<H3FP8_DT_F32>), grid, block, 0, st, a);

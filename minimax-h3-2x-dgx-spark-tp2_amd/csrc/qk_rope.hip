@@ -179,8 +179,9 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkRopeArgs a) {
         for (int i = 0; i < UNROLL; ++i) v[i] = load(ps + UNROLL + i);
 #pragma unroll
         for (int i = 0; i < UNROLL; ++i) {
+            if (ps + i >= passes) break;                    // uniform
             const int h = (ps + i) * HPW + sub;
-            const bool live = ps + i < passes && h < heads, isq = h < a.H;
+            const bool live = h < heads, isq = h < a.H;
             float x[8], y[8], g[8];
             widen8<FP16>(cur[i], x);
             float ss = 0.0f;
