@@ -331,14 +331,14 @@ struct BAddr {
 
 template <class T>
 __device__ __forceinline__ BAddr<T> baddr(int wn, int wm, int lane) {
-    const int c = lane & 15, g = lane >> 4;
+    const int c = lane & 15, g = lane >> 4, k0 = 4 * (g >> 1) + (g & 1);
     const int wr = T::PAIRS ? 8 * (c >> 2) + (c & 3) : c; // + 32 (i / 2) + 4 (i % 2), or + 16 i; neither changes the swizzle
     const int tr = c;                                     // + 16 j; neither changes swz
     BAddr<T> A;
-    A.w0 = (uint32_t)((wn * 16 * T::NI + wr) * ROWB + ((2 * g) ^ T::swz_of_w(wr)) * 16);
-    A.w1 = (uint32_t)((wn * 16 * T::NI + wr) * ROWB + ((2 * g + 1) ^ T::swz_of_w(wr)) * 16);
-    A.t0 = (uint32_t)(T::A_OFF + (wm * 16 * T::NJ + tr) * ROWB + ((2 * g) ^ swz(tr)) * 16);
-    A.t1 = (uint32_t)(T::A_OFF + (wm * 16 * T::NJ + tr) * ROWB + ((2 * g + 1) ^ swz(tr)) * 16);
+    A.w0 = (uint32_t)((wn * 16 * T::NI + wr) * ROWB + (k0 ^ T::swz_of_w(wr)) * 16);
+    A.w1 = (uint32_t)((wn * 16 * T::NI + wr) * ROWB + ((k0 + 2) ^ T::swz_of_w(wr)) * 16);
+    A.t0 = (uint32_t)(T::A_OFF + (wm * 16 * T::NJ + tr) * ROWB + (k0 ^ swz(tr)) * 16);
+    A.t1 = (uint32_t)(T::A_OFF + (wm * 16 * T::NJ + tr) * ROWB + ((k0 + 2) ^ swz(tr)) * 16);
     A.sa = (uint32_t)((wm * 16 * T::NJ + c) * 4);
     A.sw = (uint32_t)(T::SC_A * 256 + (wn * 16 * T::NI / 128) * 4);
     return A;
