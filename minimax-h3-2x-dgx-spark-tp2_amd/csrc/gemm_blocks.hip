@@ -94,10 +94,14 @@ __device__ __forceinline__ bool locate_rows(const BlocksParams& p, int TT, int64
 // 256 registers; acc takes 4 NI NJ of them.
 //   * Operands go global -> LDS by LDS-DMA (whole 128-byte lines, 8 rows an instruction) into NST stages of one k-block each;
 //     the loads run NST k-steps ahead of the MFMAs, across tile boundaries.
-//   * One barrier per k-step, late in it: every wave's fragment reads of stage g have returned (the stage is free: the loads
-//     of k-step g + NST follow, one per MFMA) and its share of stage g + 1 has landed (its first fragments are read behind
-//     the remaining MFMAs).  The last two channel blocks go token by token, so that a token's fragment registers are free
-//     for the next k-step's as early as possible.
+//   * Two barriers per k-step.  The first, when its token fragments and scales are in registers: their part of stage g is free
+//     and takes those of k-step g + NST, one load per MFMA.  The second, when its channel fragments are, and this wave's share
+//     of stage g + 1 has landed: the weights' part follows, and the next first fragments are read behind the remaining MFMAs.
+//     The last load then stands 28 of a k-step's 32 MFMAs before the wait for it.  (One barrier, the nine loads of a k-step
+//     one per MFMA behind it, the last 18 MFMAs ahead: 18 880 x 21 504 x 5376 1890 us against 1814; two loads per MFMA: 1977.)
+//     The last two channel blocks go token by token, so that a token's fragment registers are free for the next k-step's as
+//     early as possible.
+//   * A wave whose tokens all lie behind the tile's rows only loads: the other wave of its SIMD runs alone.
 //   * The fmas of an MFMA's four results stand LAG MFMAs behind it (it needs 24 wait states), also across k-steps; per MFMA
 //     (32 cycles of the matrix pipe) they cost 16 cycles of the vector pipe.
 //   * Channel of MFMA block i, row 4 g + r: 32 (i / 2) + 8 g + 4 (i % 2) + r, so that two blocks' results of a lane are 8
@@ -139,7 +143,8 @@ template <int WN, int WM, int NI, int NJ, int NST>
 struct BigTile : BTile<WN, WM, NI, NJ, NST> {
     using B = BTile<WN, WM, NI, NJ, NST>;
     static constexpr int U0 = (NI - 2) * NJ;                         // MFMAs before the last two channel blocks
-    static constexpr int BAR = (NI - 1 - AHEAD) * NJ + NJ;           // the MFMA that the barrier stands behind
+    static constexpr int EARLY = NJ;                                 // the MFMA that the first barrier stands behind
+    static constexpr int BAR = (NI - 1 - AHEAD) * NJ + NJ;           // ... and the second
     static_assert(NI % 2 == 0 && NI > AHEAD && B::NM > LAG && B::SL == 1 && B::TW % 128 == 0 && 128 % (16 * NI) == 0, "wave tile");
     static_assert(B::TW % (8 * B::WAVES) == 0 && B::TT % (8 * B::WAVES) == 0 && B::WL <= 15 && B::AL <= 15, "whole loads per wave");
     static_assert(B::LOADS * (NST - 1) <= 63, "vmcnt range");
@@ -391,14 +396,13 @@ __device__ __forceinline__ void bkstep(const uint8_t* lds, uint32_t lds0, uint32
             if (u == (i < AHEAD ? 0 : (i - AHEAD) * T::NJ + (i == AHEAD ? 1 : 0))) w[i] = read_w<T>(lds + cur, A, i);
         if (u == T::BAR) {
             wait_lgkm0();                                 // this wave's reads of the stage have returned
-            __builtin_amdgcn_s_waitcnt(vmcnt_imm(T::LOADS * (T::NST - 2)));   // its share of the next one has landed
+            __builtin_amdgcn_s_waitcnt(vmcnt_imm(T::LOADS * (T::NST - 2) + T::AL + T::SL));   // its share of the next one has landed
             barrier_nofence();
         }
+        if (u == T::EARLY) barrier_nofence();              // the first MFMAs waited for the tokens, read behind the scales
+        if (u > T::EARLY && u <= T::EARLY + T::AL + T::SL) bload<T>(I, S, T::WL + u - T::EARLY - 1);
         if (u > T::BAR) {
-            constexpr int SLOTS = T::NM - 1 - T::BAR;
-#pragma unroll
-            for (int f = (u - T::BAR - 1) * T::LOADS / SLOTS; f < (u - T::BAR) * T::LOADS / SLOTS; ++f)
-                bload<T>(I, S, f);
+            if (u <= T::BAR + T::WL) bload<T>(I, S, u - T::BAR - 1);
             if (u == T::BAR + 1) F.w[0] = read_w<T>(lds + nxt, A, 0);
             if (u == T::BAR + 2) F.w[1] = read_w<T>(lds + nxt, A, 1);
             if (u == T::BAR + 3) {
@@ -414,6 +418,33 @@ __device__ __forceinline__ void bkstep(const uint8_t* lds, uint32_t lds0, uint32
     for (int k = 0; k < LAG; ++k) pend[k] = b[T::NM - LAG + k];
 #pragma unroll
     for (int j = 0; j < T::NJ; ++j) sp[j] = s[j];
+}
+
+// The first fragments and the scales of a tile, from its first stage.
+template <class T>
+__device__ __forceinline__ void bfirst(const uint8_t* lds, uint32_t st, uint32_t sc, const BAddr<T>& A, BFrags<T>& F) {
+    F.w[0] = read_w<T>(lds + st, A, 0);
+    F.w[1] = read_w<T>(lds + st, A, 1);
+#pragma unroll
+    for (int j = 0; j < T::NJ; ++j) F.sa[j] = *reinterpret_cast<const float*>(lds + sc + A.sa + 64 * j);
+    F.sw = *reinterpret_cast<const float*>(lds + sc + A.sw);
+    __builtin_amdgcn_sched_barrier(0);                    // the tokens last, as in a k-step
+#pragma unroll
+    for (int j = 0; j < T::NJ; ++j) F.t[j] = read_t<T>(lds + st, A, j);
+}
+
+// One k-step of a wave whose tokens lie behind the tile's rows: its loads and the barriers.
+template <class T>
+__device__ __forceinline__ void bidle(uint32_t lds0, uint32_t cur, uint32_t cur_sc, const BCursor<T>& I, int nk, int wave) {
+    const BIssue S = bissue<T>(I, nk, lds0 + cur, lds0 + cur_sc, wave);
+    wait_lgkm0();
+    barrier_nofence();
+#pragma unroll
+    for (int f = T::WL; f < T::LOADS; ++f) bload<T>(I, S, f);
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(T::LOADS * (T::NST - 2) + T::AL + T::SL));
+    barrier_nofence();
+#pragma unroll
+    for (int f = 0; f < T::WL; ++f) bload<T>(I, S, f);
 }
 
 template <class T, bool FP16, bool BIAS>
@@ -515,7 +546,7 @@ __global__ void __launch_bounds__(T::WAVES * 64, 2) gemm_blocks_tile_kernel(Bloc
         const BIssue S = bissue<T>(I, nk, lds0 + (uint32_t)s * T::STAGE, lds0 + T::SC_OFF + (uint32_t)s * T::SC_STAGE, wave);
 #pragma unroll
         for (int i = 0; i < T::LOADS; ++i) bload<T>(I, S, i);
-        cursor_next<T, GROUPED>(I, p, sp, nk, wave, lane);
+            cursor_next<T, GROUPED>(I, p, sp, nk, wave, lane);
     }
     const BAddr<T> A = baddr<T>(wn, wm, lane);
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(T::LOADS * (T::NST - 1)));
@@ -526,19 +557,24 @@ __global__ void __launch_bounds__(T::WAVES * 64, 2) gemm_blocks_tile_kernel(Bloc
         n_sc = n == 0 ? T::SC_OFF : cur_sc + T::SC_STAGE;
     };
     BFrags<T> F;
-    F.w[0] = read_w<T>(lds, A, 0);
-    F.w[1] = read_w<T>(lds, A, 1);
-#pragma unroll
-    for (int j = 0; j < T::NJ; ++j) {
-        F.t[j] = read_t<T>(lds, A, j);
-        F.sa[j] = *reinterpret_cast<const float*>(lds + T::SC_OFF + A.sa + 64 * j);
-    }
-    F.sw = *reinterpret_cast<const float*>(lds + T::SC_OFF + A.sw);
+    bfirst<T>(lds, 0, T::SC_OFF, A, F);
 
     for (int c = 0;; ++c) {
         TileRows r;
         int tn = 0;
         if (!tile_at<T, GROUPED>(p, sp, (int)blockIdx.x + c * (int)gridDim.x, lane, r, tn)) break;
+        if (r.rows <= wm * 16 * T::NJ) {                  // the other waves of the SIMDs have the matrix pipes to themselves
+            for (int ks = 0; ks < nk; ++ks) {
+                uint32_t nxt, nxt_sc;
+                next_stage(nxt, nxt_sc);
+                bidle<T>(lds0, cur, cur_sc, I, nk, wave);
+                cursor_next<T, GROUPED>(I, p, sp, nk, wave, lane);
+                cur = nxt;
+                cur_sc = nxt_sc;
+            }
+            bfirst<T>(lds, cur, cur_sc, A, F);            // the next tile's, as the last k-step of the others reads them
+            continue;
+        }
         v4f acc[T::NI][T::NJ], pend[LAG];
         float sp_[T::NJ];
 #pragma unroll
