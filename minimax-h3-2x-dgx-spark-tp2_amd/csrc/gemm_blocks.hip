@@ -947,8 +947,8 @@ constexpr FormDims kForms[] = {
 
 int64_t tiles_of(int form, int64_t row_tiles, int64_t N) { return row_tiles * ((N + kForms[form].tw - 1) / kForms[form].tw); }
 
-// The large tiles by rounds over the CUs: a k-step of 256 x 256 takes 1.6 us, of 256 x 128 1.1 us (18 880 x 21 504 x 5376: 25
-// rounds of 42 k-steps in 1.87 ms; 200 x 21 504 x 5376: one round of 256 x 128 in 48.7 us).
+// The large tiles by rounds over the CUs: one of 256 x 128 tiles takes 0.66 to 0.69 of the time of one of 256 x 256 (M x 5376 x
+// 7168 in 256 x 128 / 256 x 256, us: 1024 rows 55 / 75 in one round each, 2048 103 / 80 in 2 and 1, 4096 170 / 167 in 3 and 2).
 int large_form(int64_t rows128, int64_t rows256, int64_t N, int G) {
     const int64_t r128 = (tiles_of(F_256x128, rows128, N) + G - 1) / G, r256 = (tiles_of(F_256x256, rows256, N) + G - 1) / G;
     return 16 * r256 < 11 * r128 ? F_256x256 : F_256x128;
@@ -958,8 +958,8 @@ int large_form(int64_t rows128, int64_t rows256, int64_t N, int G) {
 // tokens or fewer always 32 x 16 (the weights' bytes count).  Past that the large tiles.  64 x 32 and 64 x 64 are for
 // experts (below): 64 x 64 on one per CU holds what 32 x 64 does on two.
 // Measured with the weights in turn from copies, smaller / taken / larger form, us, M x N x K: 32 x 5376 x 7168 13.5 / 12.0 (32 x
-// 32) / 14.7; 128 x 5376 x 7168 24.5 / 20.1 (32 x 64) / 20.7; 200 x 5376 x 7168 25.3 / 23.0 (128 x 64) / 49.5 (256 x 128); 512 x
-// 6144 x 4096 28.3 / 23.2 (128 x 64 in pairs) / 31.4; 200 x 21 504 x 5376 55.6 / 48.7 (256 x 128) / 72.2.
+// 32) / 14.7; 128 x 5376 x 7168 24.5 / 20.2 (32 x 64) / 21.4; 200 x 5376 x 7168 31.5 / 22.8 (128 x 64) / 26.8; 512 x 5376 x 7168
+// 42.8 / 35.1 (128 x 64 in pairs) / 49.0; 256 x 21 504 x 5376 58.8 / 48.5 (256 x 128) / 62.0.
 int dense_form(int64_t M, int64_t N, int G) {
     if (M <= 16) return F_32x16;
     for (int f = 0; f < F_256x128; ++f)
@@ -969,13 +969,13 @@ int dense_form(int64_t M, int64_t N, int G) {
 
 // By expert, from the mean rows per expert, since the host does not know the counts (each expert's last tile taken as half
 // full).  While an expert has few rows the time is its weights', and a tile should hold all of its rows.  4096 x 4096 weights,
-// 32 experts, us in 32 x 16 / 64 x 32 / 64 x 64 / 256 x 128 / 256 x 256 tiles: 4 rows each 98 / 104 / 113 / 125 / 137, 8: 116 /
-// 106 / - / 124 / 139, 16: 145 / 126 / 119 / 125 / 141, 32: 217 / 157 / 150 / 130 / 145, 128: - / - / 232 / 179 / 201, 512: - / - /
-// 624 / 384 / 373.
+// 32 experts, us in 32 x 16 / 64 x 32 / 64 x 64 / 256 x 128 tiles: 4 rows each 101 / 112 / 121 / 122, 8: 120 / 111 / 117 / 122,
+// 16: 149 / 131 / 122 / 124, 24: 201 / 145 / 133 / 124, 48: 277 / 203 / 162 / 128; 16 experts in 64 x 64 / 256 x 128 / 256 x
+// 256: 32 rows 76 / 70 / 73, 128: 129 / 76 / 78, 200: 167 / 88 / 84, 384: - / 130 / 123.
 int grouped_form(int64_t M, int64_t N, int64_t E, int G) {
     if (M <= 5 * E) return F_32x16;
     if (M <= 12 * E) return F_64x32;
-    if (M <= 24 * E) return F_64x64;
+    if (M <= 20 * E) return F_64x64;
     return large_form(M / 128 + (E + 1) / 2, M / 256 + (E + 1) / 2, N, G);
 }
 
