@@ -224,7 +224,7 @@ template <bool SWIGLU>
 int launch_rows(RowsArgs a, int dtype, hipStream_t st) {
     a.groups = (a.K + 511) / 512;
     const int64_t blocks = (a.M + ROWS - 1) / ROWS * a.groups;
-    H3_REQUIRE(blocks < ((int64_t)1 << 31), "quant_blocks: too many rows for one launch");
+    H3_REQUIRE(blocks < ((int64_t)1 << 24), "quant_blocks: too many rows for one launch");       // 2^32 threads
     const dim3 grid((unsigned)blocks), block(256);
     if (dtype == H3FP8_DT_BF16) hipLaunchKernelGGL((quant_blocks_kernel<H3FP8_DT_BF16, SWIGLU>), grid, block, 0, st, a);
     else if (dtype == H3FP8_DT_FP16) hipLaunchKernelGGL((quant_blocks_kernel<H3FP8_DT_FP16, SWIGLU>), grid, block, 0, st, a);
@@ -255,7 +255,7 @@ int h3fp8_quant_blocks(const void* x, int64_t ldx, int dtype, int64_t M, int64_t
     if (rows == 1) return launch_rows<false>(a, dtype, st);
     a.groups = (int)((K + 127) / 128);
     const int64_t blocks = (M + 127) / 128 * a.groups;
-    H3_REQUIRE(blocks < ((int64_t)1 << 31), "h3fp8_quant_blocks: too many blocks for one launch");
+    H3_REQUIRE(blocks < ((int64_t)1 << 23), "h3fp8_quant_blocks: too many blocks for one launch");
     const dim3 grid((unsigned)blocks), block(SQ_THREADS);
     if (dtype == H3FP8_DT_BF16) hipLaunchKernelGGL((quant_squares_kernel<H3FP8_DT_BF16>), grid, block, 0, st, a);
     else if (dtype == H3FP8_DT_FP16) hipLaunchKernelGGL((quant_squares_kernel<H3FP8_DT_FP16>), grid, block, 0, st, a);

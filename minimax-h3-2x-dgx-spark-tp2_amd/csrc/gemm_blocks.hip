@@ -108,8 +108,17 @@ __device__ __forceinline__ bool locate_rows(const BlocksParams& p, int TT, int64
 //     consecutive channels: the epilogue stores 16 bytes per lane, 64-byte pieces of a row, without going through LDS.
 //   * LDS rows are 128 bytes; logical 16-byte chunk c of row r is stored at c ^ (weights: swz_w(r), tokens: swz(r)), which
 //     puts the 16 rows of a fragment read on different banks.
+//     A 16-byte read serves lanes 0-3, 12-15 and 20-27 together, and 4-11, 16-19 and 28-31: lane groups g and g ^ 1 read chunks
+//     that differ in bit 0, so that those 16 lanes meet 16 places (with chunks 2 g, 2 g + 1: twice the LDS cycles; 200 x 5376
+//     x 7168 23.7 us against 22.6).  The order of k within a block is the operands' common one and changes no product.
 //   * Every tile has buffer descriptors of its own from its own base: rows past the tile's read zeros and store nothing,
 //     and nothing else is limited to 32-bit offsets.
+// What bounds it: with operands in the caches the return path from L2 to LDS (64 KiB a k-step and CU) beside the matrix pipe,
+// busy 0.54 of the time at 2.0 GHz and 0.63 at the 1.5 GHz that the power limit leaves under a lasting load: 18 880 x 21 504 x
+// 5376 in 1780-1850 us (2.4 PFLOP/s), 32 768 rows over 32 experts of 4096 x 4096 in 550 (2.0: every expert's last tile is
+// partly empty).  With few rows per expert the weights' way from memory: 4100 rows over 16 experts 111 us; 16 x 128 rows 76 us
+// from memory, 44 from the caches.  Fetching the weights' lines into L2 some k-steps ahead by one more load per wave (a dword
+// of each line) made every case slower (1890 -> 2244 us): the requests that are under way are the limit.
 __device__ __forceinline__ int swz_w(int r) { return ((r >> 1) & 1) | (((r >> 3) & 3) << 1); }
 
 __device__ __forceinline__ void dma4_at(v4u desc, uint32_t lds_base, uint32_t voff, uint32_t soff) {
@@ -328,7 +337,8 @@ __device__ __forceinline__ v8i frag16(const uint8_t* p0, const uint8_t* p1, int 
     return f;
 }
 
-// A wave's fragment addresses within a stage: lane l reads row c = l & 15 of a block, logical chunks 2 (l >> 4), + 1.
+// A wave's fragment addresses within a stage: lane l reads row c = l & 15 of a block, logical chunks k0 and k0 + 2, k0 = 0, 1, 4, 5
+// by g = l >> 4.
 template <class T>
 struct BAddr {
     uint32_t w0, w1, t0, t1, sa, sw;
@@ -611,6 +621,8 @@ __global__ void __launch_bounds__(T::WAVES * 64, 2) gemm_blocks_tile_kernel(Bloc
 // Few tiles, or few rows per tile: the time is that of streaming the operands (the weights, mostly) and of a k-step's chain of
 // barrier, fragment reads and MFMAs.  One workgroup per tile, a deep ring of stages, fragments read a whole k-step ahead (two
 // sets of registers, the loop unrolled by two) and the fmas a whole k-step behind their MFMAs.
+// 200 x 5376 x 7168 22.6 us (128 x 64 tiles on 168 CUs, 0.4 us a k-step: 225 MB from L2 at 10 TB/s); 1 x 21 504 x 5376 19.5 us
+// (5.9 TB/s of weights); 64 rows over 32 experts of 2048 x 4096 45 us (5.9 TB/s).
 // The LDS is the launch's: a size that the compiler knew would let it give a lone workgroup 512 registers a lane and put the
 // MFMAs' results into the accumulation half, a copy away from the fmas.
 template <class T>

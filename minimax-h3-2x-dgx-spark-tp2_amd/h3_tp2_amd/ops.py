@@ -665,6 +665,34 @@ def _axes(t: torch.Tensor) -> tuple:
     return tuple(st if n > 1 else 0 for st, n in zip(t.stride(), t.shape))
 
 
+def _own_entries(t: torch.Tensor) -> bool:
+    """No two entries of ``t`` share memory (each axis steps over all that the axes of smaller strides span)."""
+    span = 1
+    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
+        if st < span:
+            return False
+        span += st * (n - 1)
+    return True
+
+
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """No entry of ``a`` lies in ``b``: [T, heads, D] tensors of one dtype whose extents are apart, or which take turns within
+    a token (views of one qkv product) or within a head."""
+    if a.numel() == 0 or b.numel() == 0:
+        return True
+    def span(t: torch.Tensor, axis: int) -> int:
+        return 1 + sum((n - 1) * st for n, st in zip(t.shape[axis:], t.stride()[axis:]))
+    d = (b.data_ptr() - a.data_ptr()) // a.element_size()
+    if d >= span(a, 0) or -d >= span(b, 0):
+        return True
+    for axis in (0, 1):
+        steps = {t.stride(i) for t in (a, b) for i in range(axis + 1) if t.shape[i] > 1}
+        st = min(steps, default=0)
+        if st and all(x % st == 0 for x in steps) and d % st >= span(a, axis + 1) and d % st + span(b, axis + 1) <= st:
+            return True
+    return False
+
+
 def _call_on(t: torch.Tensor, name: str, *args) -> None:
     """The entry point on ``t``'s device and that device's current stream, whichever device is the current one."""
     if t.get_device() == torch.cuda.current_device():
@@ -698,7 +726,7 @@ def _block_outputs(name: str, like: torch.Tensor, M: int, K: int, rows: int, q: 
         if scale.dtype != torch.float32 or tuple(scale.shape) != (MB, KB) or scale.device != like.device:
             raise ValueError(f"{name}: scale must be float32 ({MB}, {KB}) on {like.device}, got {scale.dtype} "
                              f"{tuple(scale.shape)} on {scale.device}")
-        if any(n > 1 and st < 1 for st, n in zip(scale.stride(), scale.shape)):
+        if not _own_entries(scale):
             raise ValueError(f"{name}: the entries of scale must not overlap")
     return q, scale
 
@@ -833,7 +861,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     are read in place) and the rotation of its first R dims by ``rope_table`` [P, R] (fp32 / bf16: cos of the R / 2 pairs, then
     sin) at row ``positions[t]`` (int32 / int64 [T]) or t.  Pairs are dims (p, p + R / 2), or (2p, 2p + 1) with
     ``interleaved``.  fp32 throughout, rounded once.  A position outside the table gives NaN.  Returns (q, k) as new tensors,
-    or ``out``, which may be (q, k) themselves."""
+    or ``out``, which may be (q, k) themselves and otherwise lies apart from them."""
     if _host is not None and out is None:
         new = _host.qk_norm_rope(q, k, q_weight, k_weight, rope_table, eps, positions, interleaved)
         if new is not None:
@@ -867,6 +895,12 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
             check_buffer(o, n, tuple(t.shape), t.dtype, t.device)
             if o.shape[2] > 1 and o.stride(2) != 1:
                 raise ValueError(f"{n}: the dims of a head must be contiguous")
+            if not _own_entries(o):
+                raise ValueError(f"{n}: its heads must not overlap")
+            if not (_apart(o, t) or (o.data_ptr() == t.data_ptr() and _axes(o) == _axes(t))):
+                raise ValueError(f"{n} must be its input itself or lie apart from it")
+        if not (_apart(*out) and _apart(out[0], k) and _apart(out[1], q)):
+            raise ValueError("out: q's and k's outputs must lie apart from each other and from the other's input")
     oq, ok = out
     _call_on(q, "h3fp8_qk_norm_rope", q.data_ptr(), *_axes(q)[:2], k.data_ptr(), *_axes(k)[:2], _DT[q.dtype], T, H, Hk,
              D, q_weight.data_ptr(), k_weight.data_ptr(), rope_table.data_ptr(), ld_table, _DT[rope_table.dtype], P, R,

@@ -138,6 +138,36 @@ def test_c_entries_refuse_without_a_gpu():
     bad("h3fp8_qk_norm_rope", qk[:19] + [p, 1, 2] + qk[22:], "int32 or int64")
 
 
+def test_outputs_that_share_memory_are_refused(calls):
+    """Two entries in one place, an output over the other's input, an output shifted against its own input; in place and
+    views that take turns are taken."""
+    x = torch.zeros(8, 272, dtype=BF16)
+    base = torch.zeros(64, dtype=F32)
+    for st in ((1, 1), (0, 8), (2, 3)):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.quant_blocks(x, scale=base.as_strided((8, 3), st))
+    ops.quant_blocks(x, scale=base.as_strided((8, 3), (3, 1)))
+    T, H, D = 5, 2, 64
+    w, tab = torch.zeros(D, dtype=BF16), torch.zeros(T, D)
+    qkv = torch.zeros(T, 3 * H * D, dtype=BF16)
+    q, k, v = (qkv[:, i * H * D:(i + 1) * H * D].view(T, H, D) for i in range(3))
+    pair = torch.zeros(T, H, 2, D, dtype=BF16)
+    flat = torch.zeros(T * H * D + 8, dtype=BF16)
+    run = lambda q, k, out: ops.qk_norm_rope(q, k, w, w, tab, 1e-6, out=out)            # noqa: E731
+    for a, b, out in ((q, k, (q, k)), (q, k, (v, k)), (pair[:, :, 0], pair[:, :, 1], (pair[:, :, 0], pair[:, :, 1])),
+                      (q[:1], k[:1], (q[:1], k[:1])), (q, k, (torch.empty_like(q), torch.empty_like(k))),
+                      (q[:, :1], q[:, 1:], (q[:, :1], q[:, 1:]))):
+        run(a, b, out)
+    whole = torch.zeros(T, H, D, dtype=BF16)
+    n = len(calls)
+    for a, b, out in ((q, k, (k, q)), (q, q, (q, q)), (q, k, (v, v)), (q, k, (whole[:, :1].expand(T, H, D), k)),
+                      (q, k, (k, torch.empty_like(k))),
+                      (flat[:-8].view(T, H, D), k, (flat[8:].view(T, H, D), torch.empty_like(k)))):
+        with pytest.raises(ValueError):
+            run(a, b, out)
+    assert len(calls) == n
+
+
 def test_native_host_path_leaves_other_calls_to_python():
     h = _lib.host()
     assert h is not None, "the native host path is not built"

@@ -137,3 +137,16 @@ def test_captured(cuda):
         torch.cuda.synchronize()
         r = ops.qk_norm_rope(q, k, w, w, tab, EPS, positions=pos)
         assert torch.equal(out[0], r[0]) and torch.equal(out[1], r[1])
+
+
+def test_subnormal_mean_square(cuda):
+    """A mean square below the normal fp32 range (2^-130, exact) without eps: the norm is still 1."""
+    from h3_tp2_amd import ops
+    sign = torch.where(torch.rand(9, 4, 128, generator=gen(5), device=cuda) < 0.5, -1.0, 1.0)
+    q = (sign * 2.0 ** -65).to(BF16)
+    w = (1 + 0.1 * torch.randn(128, generator=gen(6), device=cuda)).to(BF16)
+    tab = table(9, 96)
+    oq, ok = ops.qk_norm_rope(q, q.clone(), w, w, tab, 0.0)
+    y64, mag = ref64(q, w, tab, False, eps=0.0)
+    check(oq, y64, mag)
+    assert torch.equal(oq, ok)
