@@ -171,8 +171,8 @@ struct SmallTile : BTile<WN, WM, NI, NJ, NST> {
     static constexpr int SL = (PIECES + B::WAVES - 1) / B::WAVES;    // ... per wave, in the first PIECES waves at least
     static constexpr bool EVEN = PIECES % B::WAVES == 0;             // ... and in every wave
     static constexpr int LOADS = B::WL + B::AL + SL;                 // instructions of those waves; one fewer in the others
-    static constexpr int SC_STAGE = PIECES * 256;
-    static constexpr int LDS = B::SC_OFF + NST * SC_STAGE;
+    static constexpr int SC_OFF = B::STAGE, STAGE = SC_OFF + PIECES * 256;   // a stage's scales behind its operands
+    static constexpr int LDS = NST * STAGE;
     static_assert(B::TW % (8 * B::WAVES) == 0 && B::TT % (8 * B::WAVES) == 0, "whole load instructions per wave");
     static_assert(128 % (16 * NI) == 0 && (B::TW % 128 == 0 || 128 % B::TW == 0), "a wave's channels in one weight block");
     static_assert(LDS <= 160 * 1024 && LOADS * (NST - 1) <= 63 && NST >= 2 * KS, "LDS, vmcnt range, ring");
@@ -632,14 +632,14 @@ struct SFrags {
 };
 
 template <class T>
-__device__ __forceinline__ void sread(SFrags<T>& F, const uint8_t* lds, uint32_t st, uint32_t sc, const BAddr<T>& A) {
+__device__ __forceinline__ void sread(SFrags<T>& F, const uint8_t* lds, uint32_t st, const BAddr<T>& A) {
 #pragma unroll
     for (int j = 0; j < T::NJ; ++j) F.t[j] = read_t<T>(lds + st, A, j);
 #pragma unroll
     for (int i = 0; i < T::NI; ++i) F.w[i] = read_w<T>(lds + st, A, i);
 #pragma unroll
-    for (int j = 0; j < T::NJ; ++j) F.s[j] = *reinterpret_cast<const float*>(lds + sc + A.sa + 64 * j);
-    F.sw = *reinterpret_cast<const float*>(lds + sc + A.sw);
+    for (int j = 0; j < T::NJ; ++j) F.s[j] = *reinterpret_cast<const float*>(lds + st + T::SC_OFF + A.sa + 64 * j);
+    F.sw = *reinterpret_cast<const float*>(lds + st + T::SC_OFF + A.sw);
 }
 
 // The tile's loads: descriptors, lane offsets at k = 0 (OOB: nothing), the next k-step's offsets, the k-steps left.
@@ -647,8 +647,7 @@ template <class T>
 struct SLoader {
     v4u rw, ra, rs[T::SL];
     uint32_t vw[T::WL], va[T::AL], vs[T::SL], step[T::SL];
-    uint32_t w_bytes, a_bytes, s_bytes[T::SL];
-    uint32_t k0, s0[T::SL];
+    uint32_t k0, k_step, s0[T::SL];
     uint32_t dw, da, ds;
     int left, ktail;
     bool full;                                            // this wave loads SL pieces of scales (else one fewer)
@@ -660,8 +659,6 @@ __device__ __forceinline__ void sload_set(SLoader<T>& L, const BlocksParams& p, 
     const int n0 = tn * T::TW, nrows = min(T::TW, p.N - n0);
     L.rw = buffer_desc(p.w + r.e * p.w_e + (int64_t)n0 * p.ldw, (uint32_t)((nrows - 1) * p.ldw + p.K));
     L.ra = buffer_desc(p.a + r.row0 * p.lda, (uint32_t)((r.rows - 1) * p.lda + p.K));
-    L.w_bytes = L.rw[2];
-    L.a_bytes = L.ra[2];
 #pragma unroll
     for (int i = 0; i < T::WL; ++i) {
         const int row = 8 * (wave * T::WL + i) + lrow;
@@ -681,17 +678,17 @@ __device__ __forceinline__ void sload_set(SLoader<T>& L, const BlocksParams& p, 
         const int64_t st = tok ? p.sa_m : p.sw_n, sk = tok ? p.sa_k : p.sw_k;
         const int entries = tok ? r.rows : nb, first = tok ? 64 * q : 64 * (q - T::SC_A);
         L.rs[i] = buffer_desc(base, (uint32_t)(((entries - 1) * st + (kb - 1) * sk) * 4 + 4));
-        L.s_bytes[i] = L.rs[i][2];
         L.vs[i] = first + lane < entries ? (uint32_t)((first + lane) * st * 4) : OOB;
         L.step[i] = (uint32_t)(sk * 4);
         L.s0[i] = 0;
     }
     L.k0 = 0;
+    L.k_step = BK;
     L.left = kb;
     L.ktail = p.K % BK;
     L.dw = (uint32_t)(wave * T::WL * 8 * ROWB);
     L.da = (uint32_t)(T::A_OFF + wave * T::AL * 8 * ROWB);
-    L.ds = 256u * (uint32_t)wave;
+    L.ds = T::SC_OFF + 256u * (uint32_t)wave;
     L.full = wave + (T::SL - 1) * T::WAVES < T::PIECES;
 }
 
@@ -708,20 +705,25 @@ __device__ __forceinline__ void sload_edge(SLoader<T>& L, int wave, int lane) {
         for (int j = 0; j < T::AL; ++j)
             if (16 * ((lane & 7) ^ swz(8 * (wave * T::AL + j) + lrow)) >= L.ktail) L.va[j] = OOB;
     }
+}
+template <class T>
+__device__ __forceinline__ void sload_end(SLoader<T>& L) {
     const bool live = L.left > 0;
-    L.rw[2] = live ? L.w_bytes : 0;
-    L.ra[2] = live ? L.a_bytes : 0;
+    L.rw[2] = live ? L.rw[2] : 0;
+    L.ra[2] = live ? L.ra[2] : 0;
     L.k0 = live ? L.k0 : 0;
+    L.k_step = live ? BK : 0;
 #pragma unroll
     for (int i = 0; i < T::SL; ++i) {
-        L.rs[i][2] = live ? L.s_bytes[i] : 0;
+        L.rs[i][2] = live ? L.rs[i][2] : 0;
         L.s0[i] = live ? L.s0[i] : 0;
+        L.step[i] = live ? L.step[i] : 0;
     }
 }
 
-// Load instruction i of the k-step into stage `st` (scales `sc`).
+// Load instruction i of the k-step into stage `st`.
 template <class T>
-__device__ __forceinline__ void sload_one(const SLoader<T>& L, uint32_t st, uint32_t sc, int i) {
+__device__ __forceinline__ void sload_one(const SLoader<T>& L, uint32_t st, int i) {
     if (i < T::WL) {
         if (T::NT) dma16_at_nt(L.rw, st + L.dw + (uint32_t)(i * 8 * ROWB), L.vw[i], L.k0);
         else dma16_at(L.rw, st + L.dw + (uint32_t)(i * 8 * ROWB), L.vw[i], L.k0);
@@ -730,14 +732,14 @@ __device__ __forceinline__ void sload_one(const SLoader<T>& L, uint32_t st, uint
         dma16_at(L.ra, st + L.da + (uint32_t)(j * 8 * ROWB), L.va[j], L.k0);
     } else {
         const int k = i - T::WL - T::AL;
-        if (T::EVEN || k < T::SL - 1 || L.full) dma4_at(L.rs[k], sc + L.ds + (uint32_t)(k * T::WAVES * 256), L.vs[k], L.s0[k]);
+        if (T::EVEN || k < T::SL - 1 || L.full) dma4_at(L.rs[k], st + L.ds + (uint32_t)(k * T::WAVES * 256), L.vs[k], L.s0[k]);
     }
 }
 
 template <class T>
 __device__ __forceinline__ void sload_next(SLoader<T>& L) {
     --L.left;
-    L.k0 += BK;
+    L.k0 += L.k_step;
 #pragma unroll
     for (int i = 0; i < T::SL; ++i) L.s0[i] += L.step[i];
 }
@@ -750,16 +752,9 @@ __device__ __forceinline__ void swait(const SLoader<T>& L) {
     asm volatile("" ::: "memory");
 }
 
-// Places in the ring.
+// The next place in the ring.
 template <class T>
-struct SRing {
-    uint32_t st, sc;
-};
-template <class T>
-__device__ __forceinline__ SRing<T> snext(SRing<T> r) {
-    const bool wrap = r.st == (T::NST - 1) * T::STAGE;
-    return {wrap ? 0u : r.st + T::STAGE, wrap ? (uint32_t)T::SC_OFF : r.sc + T::SC_STAGE};
-}
+__device__ __forceinline__ uint32_t snext(uint32_t st) { return st == (T::NST - 1) * T::STAGE ? 0u : st + T::STAGE; }
 
 // One k-step on the fragments F (its results go to b): the next one's are read into G; pend and ps are the results and scales of
 // the k-step before.  BAR: a barrier first, behind which the next KS k-steps have landed in every wave and the stages of the
@@ -767,7 +762,7 @@ __device__ __forceinline__ SRing<T> snext(SRing<T> r) {
 // load holds the wave up for 16 to 30 cycles, and in a burst behind the barrier they held up everything (200 x 5376 x 7168 in
 // 128 x 64 tiles: 980 cycles a k-step, most of them 54 loads in a row).
 template <class T, bool BAR>
-__device__ __forceinline__ void skstep(const uint8_t* lds, uint32_t lds0, SRing<T>& rd, SRing<T>& ld, SLoader<T>& L,
+__device__ __forceinline__ void skstep(const uint8_t* lds, uint32_t lds0, uint32_t& rd, uint32_t& ld, SLoader<T>& L,
                                        const BAddr<T>& A, int wave, int lane, v4f (&acc)[T::NI][T::NJ], const SFrags<T>& F, SFrags<T>& G,
                                        const v4f (&pend)[T::NM], v4f (&b)[T::NM], float (&ps)[T::NJ]) {
     wait_lgkm0();                                         // this wave's reads of F have returned
@@ -776,8 +771,11 @@ __device__ __forceinline__ void skstep(const uint8_t* lds, uint32_t lds0, SRing<
         barrier_nofence();
     }
     rd = snext<T>(rd);
-    sload_edge<T>(L, wave, lane);
-    sread<T>(G, lds, rd.st, rd.sc, A);
+    if (__builtin_expect(L.left <= 1, 0)) {
+        sload_edge<T>(L, wave, lane);
+        sload_end<T>(L);
+    }
+    sread<T>(G, lds, rd, A);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int u = 0; u < 2 * T::NM; ++u) {
@@ -786,7 +784,7 @@ __device__ __forceinline__ void skstep(const uint8_t* lds, uint32_t lds0, SRing<
         else
             bfma<T>(acc, pend[u - T::NM], ps[T::mj(u - T::NM)], u - T::NM);
 #pragma unroll
-        for (int i = u * T::LOADS / (2 * T::NM); i < (u + 1) * T::LOADS / (2 * T::NM); ++i) sload_one<T>(L, lds0 + ld.st, lds0 + ld.sc, i);
+        for (int i = u * T::LOADS / (2 * T::NM); i < (u + 1) * T::LOADS / (2 * T::NM); ++i) sload_one<T>(L, lds0 + ld, i);
         __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
@@ -828,12 +826,13 @@ __global__ void __launch_bounds__(T::WAVES * 64) __attribute__((amdgpu_waves_per
     }
     SLoader<T> L;
     sload_set<T>(L, p, r, tn, wave, lane);
-    SRing<T> rd = {0u, (uint32_t)T::SC_OFF}, ld = rd;
+    uint32_t rd = 0, ld = 0;
 #pragma unroll
     for (int s = 0; s < T::NST - (T::KS - 1); ++s) {
         sload_edge<T>(L, wave, lane);
+        sload_end<T>(L);
 #pragma unroll
-        for (int i = 0; i < T::LOADS; ++i) sload_one<T>(L, lds0 + ld.st, lds0 + ld.sc, i);
+        for (int i = 0; i < T::LOADS; ++i) sload_one<T>(L, lds0 + ld, i);
         sload_next<T>(L);
         ld = snext<T>(ld);
     }
@@ -847,7 +846,7 @@ __global__ void __launch_bounds__(T::WAVES * 64) __attribute__((amdgpu_waves_per
     swait<T, T::NST - T::KS>(L);
     barrier_nofence();
     SFrags<T> F, G;
-    sread<T>(F, lds, 0, T::SC_OFF, A);
+    sread<T>(F, lds, 0, A);
     // in pairs: an odd count takes one more k-step, of zeros, which adds +0
     for (int left = (p.K + 2 * BK - 1) / (2 * BK); left > 0; --left) {
         skstep<T, true>(lds, lds0, rd, ld, L, A, wave, lane, acc, F, G, pa, pb, ps);
