@@ -148,9 +148,11 @@ struct BTile {
     __device__ static int swz_of_w(int r) { return PAIRS ? swz_w(r) : swz(r); }
 };
 
-template <int WN, int WM, int NI, int NJ, int NST>
+// NT (both kinds of tiles): the weight loads carry the non-temporal hint.
+template <int WN, int WM, int NI, int NJ, int NST, bool NT_ = false>
 struct BigTile : BTile<WN, WM, NI, NJ, NST> {
     using B = BTile<WN, WM, NI, NJ, NST>;
+    static constexpr bool NT = NT_;
     static constexpr int U0 = (NI - 2) * NJ;                         // MFMAs before the last two channel blocks
     static constexpr int EARLY = NJ;                                 // the MFMA that the first barrier stands behind
     static constexpr int BAR = (NI - 1 - AHEAD) * NJ + NJ;           // ... and the second
@@ -161,7 +163,7 @@ struct BigTile : BTile<WN, WM, NI, NJ, NST> {
     static constexpr int mj(int u) { return u < U0 ? u % NJ : (u - U0) / 2; }
 };
 
-// KS: k-steps per barrier.  NT: the weight loads carry the non-temporal hint.
+// KS: k-steps per barrier.
 template <int WN, int WM, int NI, int NJ, int NST, int KS_, bool NT_ = false>
 struct SmallTile : BTile<WN, WM, NI, NJ, NST> {
     using B = BTile<WN, WM, NI, NJ, NST>;
@@ -319,7 +321,9 @@ __device__ __forceinline__ BIssue bissue(const BCursor<T>& I, int nk, uint32_t s
 template <class T>
 __device__ __forceinline__ void bload(const BCursor<T>& I, const BIssue& S, int i) {
     if (i < T::WL) {
-        dma16_at(I.rw, S.w + (uint32_t)(i * 8 * ROWB), I.vw[i] | ((S.cut << (31 - i)) & OOB), S.k0);
+        const uint32_t at = S.w + (uint32_t)(i * 8 * ROWB), v = I.vw[i] | ((S.cut << (31 - i)) & OOB);
+        if (T::NT) dma16_at_nt(I.rw, at, v, S.k0);
+        else dma16_at(I.rw, at, v, S.k0);
     } else if (i < T::WL + T::AL) {
         const int j = i - T::WL;
         dma16_at(I.ra, S.a + (uint32_t)(j * 8 * ROWB), I.va[j] | ((S.cut << (15 - j)) & OOB), S.k0);
@@ -898,12 +902,14 @@ int launch_tile(const BlocksParams& p, const char* who, hipStream_t st) {
     if (p.offsets) {
         if (p.fp16) H3_B(true, false, true);
         else H3_B(false, false, true);
-    } else if (p.fp16) {
-        if (p.bias) H3_B(true, true, false);
-        else H3_B(true, false, false);
-    } else {
-        if (p.bias) H3_B(false, true, false);
-        else H3_B(false, false, false);
+    } else if constexpr (!T::NT) {                        // by expert only
+        if (p.fp16) {
+            if (p.bias) H3_B(true, true, false);
+            else H3_B(true, false, false);
+        } else {
+            if (p.bias) H3_B(false, true, false);
+            else H3_B(false, false, false);
+        }
     }
 #undef H3_B
     H3_CHECK_HIP(hipGetLastError());
@@ -990,11 +996,16 @@ int grouped_form(int64_t M, int64_t N, int64_t E, int G) {
     return large_form(M / 128 + (E + 1) / 2, M / 256 + (E + 1) / 2, N, G);
 }
 
-// The non-temporal hint on the weight loads of the forms that stream them once: for more than 64 MiB of weights, of which a next
-// call finds little in the last-level cache (256 MiB) whatever this one leaves there.  With / without it, us: 1 x 21 504 x 5376
-// 19.6 / 21.7; by expert 64 rows x 32 x 2048 x 4096 46.5 / 49.7, 256 x 32 x 4096 x 4096 106 / 116 (64 x 32); but weights that are
-// still in that cache come slower: two sets of 8 x 4096 x 4096 in turn, 20 rows, 25.9 / 21.7.
+// The non-temporal hint on the weight loads that stream them once: for more than 64 MiB of weights, of which a next call finds
+// little in the last-level cache (256 MiB) whatever this one leaves there.  With / without it, us: 1 x 21 504 x 5376 19.6 / 21.7;
+// by expert 64 rows x 32 x 2048 x 4096 46.5 / 49.7, 256 x 32 x 4096 x 4096 106 / 116 (64 x 32); but weights that are still in
+// that cache come slower: two sets of 8 x 4096 x 4096 in turn, 20 rows, 25.9 / 21.7.
 bool streams(const BlocksParams& p) { return (int64_t)p.N * p.K * std::min<int64_t>(p.E, p.M) > (64LL << 20); }
+
+// ... and of the large tiles, by expert, while one row tile holds a mean expert's rows.  16 experts of 4096 x 4096: 64 rows each 67
+// / 73, 128: 77 / 80, 256: 85 / 92; but with two row tiles that share the weights in L2, 384: 137 / 127, and 32 768 rows
+// over 32 experts 585 / 557.
+bool once(const BlocksParams& p, int64_t rows) { return p.offsets && p.M <= rows * p.E; }
 
 int form_for(int64_t M, int64_t N, int64_t E, bool grouped, int G) { return grouped ? grouped_form(M, N, E, G) : dense_form(M, N, G); }
 
@@ -1009,8 +1020,12 @@ int run(const BlocksParams& p, const char* who, hipStream_t st) {
         return launch_small<SmallTile<__VA_ARGS__>>(p, who, st);
         H3_SMALL_FORMS(X)
 #undef X
-        case F_256x128: return launch_tile<BigTile<2, 4, 8, 2, 3>>(p, who, st);
-        default: return launch_tile<BigTile<2, 4, 8, 4, 2>>(p, who, st);
+        case F_256x128:
+            if (nt && once(p, 128)) return launch_tile<BigTile<2, 4, 8, 2, 3, true>>(p, who, st);
+            return launch_tile<BigTile<2, 4, 8, 2, 3>>(p, who, st);
+        default:
+            if (nt && once(p, 256)) return launch_tile<BigTile<2, 4, 8, 4, 2, true>>(p, who, st);
+            return launch_tile<BigTile<2, 4, 8, 4, 2>>(p, who, st);
     }
 }
 

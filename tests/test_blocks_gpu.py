@@ -325,6 +325,24 @@ def test_grouped_forms(cuda, M, E, N, form, K):
     assert (out[:off[0]] == -3).all() and (out[off[-1]:] == -3).all()
 
 
+@pytest.mark.parametrize("M,form", [(1000, 7), (4000, 8)])
+def test_grouped_streaming_weights(cuda, M, form):
+    """More than 64 MiB of weights, a row tile per mean expert: the large tiles' loads with the hint give the dense bits, with an
+    expert of several row tiles, one of one row and one without rows among them."""
+    from h3_tp2_amd import ops
+    E, N, K = 18, 2064, 2048
+    assert plan(M, N, E, True)[2] == form and E * N * K > 64 << 20
+    g = gen(M)
+    a, w = codes(g, M, K), codes(g, E * N, K).view(E, N, K)
+    sa, sw = scales(g, M, K // B), scales(g, E, cdiv(N, B), K // B)
+    off = [0, M // 3, M // 3 + 1, M // 3 + 1] + [M // 3 + 1 + (M - M // 3 - 1) * i // (E - 3) for i in range(1, E - 2)]
+    assert len(off) == E + 1 and off[-1] == M
+    y = ops.grouped_gemm_blocks(a, w, sa, sw, torch.tensor(off, dtype=torch.int32, device=cuda))
+    for e, (lo, hi) in enumerate(zip(off[:-1], off[1:])):
+        if hi > lo:
+            assert torch.equal(y[lo:hi], ops.gemm_blocks(a[lo:hi], w[e], sa[lo:hi], sw[e])), e
+
+
 def test_grouped_decreasing_offsets_stay_inside(cuda):
     """Offsets that decrease are a caller's mistake: an expert whose end is before its start has no rows, and nothing outside
     the union of the others is written."""
