@@ -1070,6 +1070,7 @@ int h3fp8_grouped_gemm_blocks(const void* a, int64_t lda, const void* w, int64_t
     if (rc) return rc;
     H3_REQUIRE(idx_bytes == 4 || idx_bytes == 8, "h3fp8_grouped_gemm_blocks: offsets must be int32 or int64");
     H3_REQUIRE(M == 0 || N == 0 || E == 0 || offsets, "h3fp8_grouped_gemm_blocks: null offsets");
+    H3_REQUIRE((uintptr_t)offsets % (unsigned)idx_bytes == 0, "h3fp8_grouped_gemm_blocks: misaligned offsets");
     return run(p, "h3fp8_grouped_gemm_blocks", (hipStream_t)stream);
 }
 

@@ -8,14 +8,15 @@
 // stock kernel that rounds n to bf16 before it rotates.
 //
 // HBM-bound: every head is read and written once.  A lane holds 8 consecutive dims (16-byte loads and stores), D / 8 lanes
-// a head, so a wave holds 512 / D heads of one token at a time (a pass): the token's q heads and then its k heads, UNROLL passes'
-// loads in flight together.  The norm weights and the table entries of the lane's dims are loaded once and kept.  The sum of
-// squares goes over the head's lanes by DPP.  The half-split partner of dim d is half = R / 2 away, a multiple of 8, so it is
-// in another lane at the same place: the lanes exchange their packed inputs (4 words instead of 8 normalised values) and each
-// normalises its partner's too; the interleaved partner is in the lane.  With few tokens a token's passes are dealt over
-// several waves, until every SIMD has two.
-// 18 880 tokens x (56 + 56) heads of 128, bf16: 209 us, 5.2 TB/s (one pass's loads in flight and eight fp32 exchanges: 226); 8
-// tokens x (32 + 8) heads: 5.8 us a call, 4.1 of them on the GPU (a wave per token: 9.6 a call).
+// a head, so a wave holds 512 / D heads of one token at a time (a pass), all of them q's or all of them k's, UNROLL passes'
+// loads in flight together.  cos and sin of the lane's dims are loaded once and take up the norm weights (the partner's for sin),
+// so that a dim costs one fma and three products.  The sum of squares goes over the head's lanes by DPP.  The half-split partner
+// of dim d is half = R / 2 away, a multiple of 8, so it is in another lane at the same place: the lanes exchange their packed
+// inputs (4 words instead of 8 normalised values); the interleaved partner is in the lane.  With few tokens a token's passes
+// are dealt over several waves, until every SIMD has two.
+// 18 880 tokens x (56 + 56) heads of 128, bf16: 197 us, 5.5 TB/s (two passes in flight 200, eight 192, but 4000 tokens x (32 + 8)
+// heads 17.1 / 16.8 / 18.0; with q's and k's heads in one wave, the addresses and weights selected lane by lane, 209 and 22.1);
+// 8 tokens x (32 + 8) heads 5.8 us a call, 3.2 of them on the GPU.
 #include <algorithm>
 
 #include "h3fp8_common.h"
@@ -44,7 +45,7 @@ struct QkRopeArgs {
     float eps;
     int vec;                                    // the table entries of a lane are aligned for vector loads
     int per;                                    // passes (512 / D heads each) a wave takes
-    int chunks;                                 // waves per token
+    int q_chunks, k_chunks;                     // waves per token, for q's heads and for k's
 };
 
 template <bool FP16>
@@ -107,6 +108,15 @@ __device__ __forceinline__ float rsqrt32(float v) {
     return __builtin_amdgcn_rsqf(tiny ? v * 0x1p64f : v) * (tiny ? 0x1p32f : 1.0f);
 }
 
+// A uniform value, in a scalar register from here on.
+template <class V>
+__device__ __forceinline__ V pinned(V v) {
+    asm("" : "+s"(v));
+    return v;
+}
+
+typedef v4u __attribute__((address_space(1))) GlobalV4;
+
 constexpr int UNROLL = 4;
 
 template <int D, bool FP16, bool TF32, bool INTER>
@@ -114,37 +124,44 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkRopeArgs a) {
     constexpr int LPH = D / 8, HPW = 64 / LPH;              // lanes per head, heads per pass
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int64_t unit = (int64_t)blockIdx.x * 4 + wave;
-    const int64_t t = unit / a.chunks;
-    if (t >= a.T) return;
-    const int pass0 = (int)(unit - t * a.chunks) * a.per;
+    const uint32_t unit = blockIdx.x * 4 + wave, chunks = (uint32_t)(a.q_chunks + a.k_chunks), token = unit / chunks;
+    if (token >= a.T) return;
+    const int64_t t = token;
+    const int chunk = (int)(unit - token * chunks);
+    const bool isq = chunk < a.q_chunks;                    // the wave's heads: some of q's or some of k's
     const int j = lane % LPH, sub = lane / LPH;             // the lane's 8 dims 8j .. 8j + 7 of head `sub` of a pass
-    const int heads = a.H + a.Hk;
-    const int passes = min(pass0 + a.per, (heads + HPW - 1) / HPW);
+    const int heads = isq ? a.H : a.Hk;
+    const int pass0 = (isq ? chunk : chunk - a.q_chunks) * a.per, passes = min(pass0 + a.per, (heads + HPW - 1) / HPW);
+    // its byte strides and addresses, those of head 0 of a pass; in scalar registers, not behind a pointer that is selected
+    const int64_t ih = pinned(2 * (isq ? a.q_h : a.k_h)), oh = pinned(2 * (isq ? a.oq_h : a.ok_h));
+    const int64_t in0 = pinned((int64_t)(uintptr_t)(isq ? a.q + t * a.q_t : a.k + t * a.k_t));
+    const int64_t out0 = pinned((int64_t)(uintptr_t)(isq ? a.oq + t * a.oq_t : a.ok + t * a.ok_t));
+    const int64_t in_lane = sub * ih + 16 * j, out_lane = sub * oh + 16 * j;
     const int half = a.half;
     const bool rotated = 8 * j < 2 * half;                  // half-split: half % 8 == 0, a lane is wholly in or out
     const int pj = INTER || !rotated ? j : 8 * j < half ? j + half / 8 : j - half / 8;     // the partner lane of the head
     auto load = [&](int ps) {
-        const int h = ps * HPW + sub;
-        const bool live = ps < passes && h < heads, isq = h < a.H;
-        const uint16_t* src = isq ? a.q + t * a.q_t + (int64_t)h * a.q_h : a.k + t * a.k_t + (int64_t)(h - a.H) * a.k_h;
-        return live ? __builtin_nontemporal_load(reinterpret_cast<const v4u*>(src + 8 * j)) : v4u{0u, 0u, 0u, 0u};
+        const bool live = ps < passes && ps * HPW + sub < heads;
+        return live ? __builtin_nontemporal_load((const GlobalV4*)(in0 + ps * (HPW * ih) + in_lane)) : v4u{0u, 0u, 0u, 0u};
     };
-    v4u v[UNROLL];
-#pragma unroll
-    for (int i = 0; i < UNROLL; ++i) v[i] = load(pass0 + i);
-    // the norm weights of the lane's dims and of its partner's, for q and for k
-    const v4u none = {0u, 0u, 0u, 0u};
-    const v4u wq = a.H ? *reinterpret_cast<const v4u*>(a.wq + 8 * j) : none, wk = a.Hk ? *reinterpret_cast<const v4u*>(a.wk + 8 * j) : none;
-    const v4u pq = INTER || !a.H ? none : *reinterpret_cast<const v4u*>(a.wq + 8 * pj);
-    const v4u pk = INTER || !a.Hk ? none : *reinterpret_cast<const v4u*>(a.wk + 8 * pj);
     int64_t pos = t;
     if (a.positions)
         pos = a.pos_bytes == 8 ? reinterpret_cast<const int64_t*>(a.positions)[t * a.pos_stride]
                                : (int64_t)reinterpret_cast<const int32_t*>(a.positions)[t * a.pos_stride];
+    v4u v[UNROLL];
+#pragma unroll
+    for (int i = 0; i < UNROLL; ++i) v[i] = load(pass0 + i);
+    // out_d = n_d cos + (the partner's n) sin with a sign, n = x r w: cs and sn take the weights of the dim and of its partner
+    float cs[8], sn[8], g[8], pg[8];
+    const uint16_t* w = isq ? a.wq : a.wk;
+    widen8<FP16>(*reinterpret_cast<const v4u*>(w + 8 * j), g);
+    if (INTER) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) pg[e] = g[e ^ 1];
+    } else {
+        widen8<FP16>(*reinterpret_cast<const v4u*>(w + 8 * pj), pg);
+    }
     const bool known = pos >= 0 && pos < a.P;               // else the outputs are NaN and the table is not read
-    // cos and the signed sin of each of the lane's dims: out_d = n_d cos + partner_d sin (1 and 0 past the rotated dims)
-    float cs[8], sn[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) cs[e] = known ? 1.0f : __builtin_nanf(""), sn[e] = 0.0f;
     if (known && rotated) {
@@ -179,47 +196,34 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkRopeArgs a) {
             }
         }
     }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) cs[e] *= g[e], sn[e] = rotated ? sn[e] * pg[e] : 0.0f;
     for (int ps = pass0; ps < passes; ps += UNROLL) {
-        v4u cur[UNROLL];
-#pragma unroll
-        for (int i = 0; i < UNROLL; ++i) cur[i] = v[i];
-#pragma unroll
-        for (int i = 0; i < UNROLL; ++i) v[i] = load(ps + UNROLL + i);
 #pragma unroll
         for (int i = 0; i < UNROLL; ++i) {
             if (ps + i >= passes) break;                    // uniform
-            const int h = (ps + i) * HPW + sub;
-            const bool live = h < heads, isq = h < a.H;
-            float x[8], y[8], g[8];
-            widen8<FP16>(cur[i], x);
+            float x[8], p[8], y[8];
+            widen8<FP16>(v[i], x);
+            if (!INTER) {                                   // a lane past the rotated dims has itself as its partner, and sin 0
+                v4u o;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = (uint32_t)__shfl((int)v[i][e], lane - j + pj, 64);
+                widen8<FP16>(o, p);
+            }
+            v[i] = load(ps + UNROLL + i);
             float ss = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(x[e], x[e], ss);
             const float r = rsqrt32(__builtin_fmaf(head_sum<LPH>(ss), 1.0f / D, a.eps));
-            const v4u w = {isq ? wq[0] : wk[0], isq ? wq[1] : wk[1], isq ? wq[2] : wk[2], isq ? wq[3] : wk[3]};
-            widen8<FP16>(w, g);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = x[e] * r * g[e];
-            if (INTER) {
+            for (int e = 0; e < 8; ++e) x[e] *= r;
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    y[e] = 8 * j + e < 2 * half ? __builtin_fmaf(x[e], cs[e], x[e ^ 1] * sn[e]) : x[e] * cs[e];
-            } else {
-                v4u o;
+            for (int e = 0; e < 8; ++e)
+                p[e] = INTER ? (8 * j + e < 2 * half ? x[e ^ 1] : 0.0f) : p[e] * r;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = (uint32_t)__shfl((int)cur[i][e], lane - j + pj, 64);
-                float p[8], pg[8];
-                widen8<FP16>(o, p);
-                const v4u pw = {isq ? pq[0] : pk[0], isq ? pq[1] : pk[1], isq ? pq[2] : pk[2], isq ? pq[3] : pk[3]};
-                widen8<FP16>(pw, pg);
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    y[e] = rotated ? __builtin_fmaf(x[e], cs[e], p[e] * r * pg[e] * sn[e]) : x[e] * cs[e];
-            }
-            if (live) {
-                uint16_t* dst = isq ? a.oq + t * a.oq_t + (int64_t)h * a.oq_h : a.ok + t * a.ok_t + (int64_t)(h - a.H) * a.ok_h;
-                __builtin_nontemporal_store(narrow8<FP16>(y), reinterpret_cast<v4u*>(dst + 8 * j));
-            }
+            for (int e = 0; e < 8; ++e) y[e] = __builtin_fmaf(x[e], cs[e], p[e] * sn[e]);
+            if ((ps + i) * HPW + sub < heads)
+                __builtin_nontemporal_store(narrow8<FP16>(y), (GlobalV4*)(out0 + (ps + i) * (HPW * oh) + out_lane));
         }
     }
 }
@@ -234,12 +238,14 @@ int launch_qk(const QkRopeArgs& a, bool interleaved, dim3 grid, hipStream_t st) 
 
 template <int D>
 int launch_head(QkRopeArgs a, bool fp16, bool tf32, bool interleaved, hipStream_t st) {
-    const int passes = (a.H + a.Hk + 512 / D - 1) / (512 / D);
-    // two waves per SIMD while there are passes to deal, then whole tokens
+    constexpr int HPW = 512 / D;
+    const int pq = (a.H + HPW - 1) / HPW, pk = (a.Hk + HPW - 1) / HPW;
+    // two waves per SIMD while there are passes to deal, then all of q's or k's heads of a token
     const int64_t waves = 8LL * h3host::cu_count();
-    a.per = (int)std::max<int64_t>(1, std::min<int64_t>(passes, a.T * passes / waves));
-    a.chunks = (passes + a.per - 1) / a.per;
-    const int64_t units = a.T * a.chunks;
+    a.per = (int)std::max<int64_t>(1, std::min<int64_t>(std::max(pq, pk), a.T * (pq + pk) / waves));
+    a.q_chunks = (pq + a.per - 1) / a.per;
+    a.k_chunks = (pk + a.per - 1) / a.per;
+    const int64_t units = a.T * (a.q_chunks + a.k_chunks);
     H3_REQUIRE(units <= ((int64_t)1 << 26) - 4, "h3fp8_qk_norm_rope: too many tokens for one launch");   // 2^32 threads
     const dim3 grid((unsigned)((units + 3) / 4));
     if (fp16) return tf32 ? launch_qk<D, true, true>(a, interleaved, grid, st) : launch_qk<D, true, false>(a, interleaved, grid, st);
