@@ -90,7 +90,7 @@ __device__ __forceinline__ v2u codes8(const float f[8], float inv) {
 // as a factor 1 + d ln 2 (with g held to +-200, where the exponential is 0 or inf, d stays finite).  exp2 and the reciprocal are
 // the hardware's, 1 ulp each.  A gate so low that the exponential overflows gives -0, as the division by inf does.  Without d
 // the exponential is |g| / 2 ulp off and four times as many codes at a rounding border fall on its other side.  With it 43 to
-// 59 of 36 M codes differ from those of float64, with correctly rounded fp32 operations 41 to 52; a Newton step on the reciprocal
+// 59 of 36 M codes differ from those of float64, with a library exponential and IEEE division 41 to 52; a Newton step on the rcp
 // (36 to 63) costs 6 % of the time, the sum's lost bits on top (41 to 52) 24 %.
 __device__ __forceinline__ float swiglu(float g, float u) {
     constexpr float L = -1.44269504088896340736f, LL = -1.92596299112661746887e-8f;       // -log2(e) = L + LL
