@@ -57,7 +57,8 @@ def quant32(x, rows=1):
 
 
 def plan(M, N, E=1, grouped=False, cus=256):
-    """(channels, tokens) of the tile that a product over M rows runs in: the library's own rule (csrc/gemm_blocks.hip)."""
+    """(channels, tokens) of the tile that a product over M rows runs in and its place in the list of forms: the library's own rule
+    (csrc/gemm_blocks.hip)."""
     import ctypes
 
     from h3_tp2_amd import _lib
