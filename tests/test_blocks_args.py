@@ -128,6 +128,8 @@ def test_c_entries_refuse_without_a_gpu():
     grouped = [p, 64, p, 2048, 64, p, 1, 8, p, 2, 1, 1, p, 4, p, 32, 0, 8, 32, 64, 3, z]
     bad("h3fp8_grouped_gemm_blocks", grouped[:12] + [p, 2] + grouped[14:], "int32 or int64")
     bad("h3fp8_grouped_gemm_blocks", grouped[:12] + [z, 4] + grouped[14:], "null offsets")
+    bad("h3fp8_grouped_gemm_blocks", grouped[:12] + [ctypes.c_void_p(4098), 4] + grouped[14:], "misaligned offsets")
+    bad("h3fp8_grouped_gemm_blocks", grouped[:12] + [ctypes.c_void_p(4100), 8] + grouped[14:], "misaligned offsets")
     f = ctypes.c_float(1e-6)
     qk = [p, 512, 128, p, 256, 128, 0, 5, 4, 2, 128, p, p, p, 96, 2, 9, 96, 0, z, 0, 8, f, p, 512, 128, p, 256, 128, z]
     bad("h3fp8_qk_norm_rope", qk[:10] + [96] + qk[11:], "head size")
