@@ -150,3 +150,14 @@ def test_subnormal_mean_square(cuda):
     y64, mag = ref64(q, w, tab, False, eps=0.0)
     check(oq, y64, mag)
     assert torch.equal(oq, ok)
+
+
+def test_only_keys(cuda):
+    """No query heads at all: k alone, at head counts around a wave's pass."""
+    from h3_tp2_amd import ops
+    w, tab = torch.randn(64, generator=gen(8), device=cuda).to(BF16), table(70, 64)
+    for Hk in (1, 8, 9, 17):
+        k = torch.randn(70, Hk, 64, generator=gen(Hk), device=cuda).to(BF16)
+        oq, ok = ops.qk_norm_rope(k[:, :0], k, w, w, tab, EPS, interleaved=True)
+        assert oq.shape == (70, 0, 64)
+        check(ok, *ref64(k, w, tab, True))
