@@ -177,7 +177,7 @@ struct SmallTile : BTile<WN, WM, NI, NJ, NST> {
     static constexpr int LDS = NST * STAGE;
     static_assert(B::TW % (8 * B::WAVES) == 0 && B::TT % (8 * B::WAVES) == 0, "whole load instructions per wave");
     static_assert(128 % (16 * NI) == 0 && (B::TW % 128 == 0 || 128 % B::TW == 0), "a wave's channels in one weight block");
-    static_assert(LDS <= 160 * 1024 && LOADS * (NST - 1) <= 63 && NST >= 2 * KS, "LDS, vmcnt range, ring");
+    static_assert(LDS <= 160 * 1024 && LOADS * (NST - 1) <= 63 && KS <= 2 && NST >= 2 * KS, "LDS, vmcnt range, ring");
     static constexpr int mi(int u) { return u / NJ; }
     static constexpr int mj(int u) { return u % NJ; }
 };
