@@ -88,7 +88,9 @@ __device__ __forceinline__ v2u codes8(const float f[8], float inv) {
 
 // g / (1 + exp(-g)) * u.  exp(-g) = exp2(y + d): y = -g log2(e) rounded, d what the rounding and the constant's own lost, applied
 // as a factor 1 + d ln 2 (with g held to +-200, where the exponential is 0 or inf, d stays finite).  exp2 and the reciprocal are
-// the hardware's, 1 ulp each.  A gate so low that the exponential overflows gives -0, as the division by inf does.  Without d
+// the hardware's, 1 ulp each.  The reciprocal returns 0 where its result is subnormal, which is so from an exponential of 2^126
+// on (g < -87.3), short of its overflow at 2^128 (g < -88.7): denominator and gate are held as quarters, exactly, so that it
+// stays normal.  From the overflow on the result is -0, as the division by inf gives.  Without d
 // the exponential is |g| / 2 ulp off and four times as many codes at a rounding border fall on its other side.  With it 43 to
 // 59 of 36 M codes differ from those of float64, with a library exponential and IEEE division 41 to 52; a Newton step on the rcp
 // (36 to 63) costs 6 % of the time, the sum's lost bits on top (41 to 52) 24 %.
@@ -97,8 +99,8 @@ __device__ __forceinline__ float swiglu(float g, float u) {
     const float c = __builtin_amdgcn_fmed3f(g, -200.0f, 200.0f);
     const float y = c * L;
     const float d = __builtin_fmaf(c, LL, __builtin_fmaf(c, L, -y));
-    const float e = __builtin_amdgcn_exp2f(y) * __builtin_fmaf(d, 0.69314718055994530942f, 1.0f);
-    return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
+    const float e = __builtin_amdgcn_exp2f(y) * __builtin_fmaf(d, 0.69314718055994530942f / 4, 0.25f);        // exp(-g) / 4
+    return 0.25f * g * __builtin_amdgcn_rcpf(0.25f + e) * u;
 }
 
 struct RowsArgs {

@@ -110,6 +110,33 @@ def test_silu_mul_quant_blocks_edges(cuda):
     assert (q[0, :128].float() == 0).all()
 
 
+@pytest.mark.parametrize("dtype,gates", [(BF16, (-86.5, -87.0, -87.5, -88.0, -88.5)), (FP16, (-87.3125, -87.375, -88.0, -88.6875))])
+def test_silu_mul_quant_blocks_gates_before_the_overflow(cuda, dtype, gates):
+    """Gates whose exponential is past 2^126, so that 1 / (1 + exp(-g)) is subnormal, and still finite: the formula's value,
+    which large up projections bring back into the codes' range, and its infinity.  One value to a block, so that every code is
+    -448 and the scale shows the value.  Behind the argument, whose rounding is made good: exp2 and rcp 2^-23 each, six
+    roundings of 2^-24: 2^-20.  From the overflow on it is -0, as the division by inf gives."""
+    from h3_tp2_amd import ops
+    ups = (1e28, 1e30, 1e34, 1e36, 3e38, -1e36) if dtype == BF16 else (1.0, 6e4, -6e4)
+    cells = [(g, u) for g in gates for u in (*ups, float("inf"))]
+    F = B * len(cells)
+    x = torch.tensor([[c[i] for i in (0, 1) for c in cells for _ in range(B)]], dtype=F32, device=cuda).to(dtype)
+    q, s = ops.silu_mul_quant_blocks(x)
+    g, u = x.double().chunk(2, dim=1)
+    h = (g / (1 + torch.exp(-g)) * u)[0, ::B]
+    fin = torch.isfinite(h)
+    assert torch.isinf(s[0, ~fin]).all() and (~fin).sum() == len(gates)
+    s64 = torch.clamp_min(h[fin].abs() / 448.0, 1.0 / (448.0 * 512.0))
+    assert ((s[0, fin].double() - s64).abs() <= s64 * 2.0 ** -20).all()
+    big = fin & (h.abs() > 1.0 / 512.0)
+    assert dtype == FP16 or big.sum() >= 2 * len(gates)
+    codes8 = q.float().view(len(cells), B)
+    assert torch.equal(codes8[big], (448.0 * torch.sign(h[big]).float())[:, None].expand(-1, B))
+    over = torch.tensor([[-89.0] * B + [1e36] * B], device=cuda).to(BF16)
+    q, s = ops.silu_mul_quant_blocks(over)
+    assert (q.view(torch.uint8) == 0x80).all() and (s == 1.0 / (448.0 * 512.0)).all()
+
+
 # ---- dense product --------------------------------------------------------------------------------------------------
 
 SHAPES = [(1, 16, 16), (1, 5376, 21504), (2, 128, 128), (5, 144, 272), (16, 2064, 144), (17, 528, 720), (33, 1200, 2064),
