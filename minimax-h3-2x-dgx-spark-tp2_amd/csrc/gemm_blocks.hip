@@ -919,7 +919,7 @@ int launch_tile(const BlocksParams& p, const char* who, hipStream_t st) {
 template <class T>
 int launch_small(const BlocksParams& p, const char* who, hipStream_t st) {
     const int64_t tiles_n = (p.N + T::TW - 1) / T::TW, rt = row_tiles(p, T::TT), tiles = rt * tiles_n;
-    H3_REQUIRE(tiles < ((int64_t)1 << 31), "%s: too many tiles for one launch", who);
+    H3_REQUIRE(tiles < ((int64_t)1 << 32) / (T::WAVES * 64), "%s: too many tiles for one launch", who);      // 2^32 threads
     const dim3 grid((unsigned)tiles), block(T::WAVES * 64);
 #define H3_B(FP16, BIAS, GROUPED) \
     hipLaunchKernelGGL((gemm_blocks_small_kernel<T, FP16, BIAS, GROUPED>), grid, block, T::LDS, st, p, (int)tiles_n, (int)rt)

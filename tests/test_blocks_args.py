@@ -140,6 +140,18 @@ def test_c_entries_refuse_without_a_gpu():
     bad("h3fp8_qk_norm_rope", qk[:19] + [p, 1, 2] + qk[22:], "int32 or int64")
 
 
+def test_more_threads_than_a_launch_holds_are_refused():
+    """2^20 experts of one row by 1024 channels: 2^25 tiles of 128 threads are 2^32, past what one launch takes.  The library says
+    so itself, as the quants and the rotation do, and does not leave it to the runtime."""
+    L = _lib.load()
+    p, z = ctypes.c_void_p(4096), None
+    M = E = 1 << 20
+    for n in (1024, 2048):
+        rc = L.h3fp8_grouped_gemm_blocks(p, 16, p, 0, 16, p, 1, M, p, 0, 0, 0, p, 4, p, n, 0, M, n, 16, E, z)
+        assert rc == -22 and "too many tiles for one launch" in L.h3fp8_last_error().decode(), L.h3fp8_last_error()
+    assert L.h3fp8_quant_blocks(p, 512, 0, 1 << 27, 512, 1, p, 512, p, 1, 1 << 27, z) == -22
+
+
 def test_outputs_that_share_memory_are_refused(calls):
     """Two entries in one place, an output over the other's input, an output shifted against its own input; in place and
     views that take turns are taken."""
