@@ -54,15 +54,9 @@ __device__ __forceinline__ int wave_prefix(int v) {
     return v;
 }
 
-// Row tile t (TT rows each, no tile spans two experts, an expert without rows has none); false past the last one.  A wave
+// By expert: row tile t (TT rows each, no tile spans two experts, an expert without rows has none); false past the last one.  A wave
 // looks at 64 experts at a time.
 __device__ __forceinline__ bool locate_rows(const BlocksParams& p, int TT, int64_t t, int lane, TileRows& r) {
-    if (!p.offsets) {
-        r.e = 0;
-        r.row0 = t * TT;
-        r.rows = (int)min<int64_t>(TT, p.M - r.row0);
-        return r.row0 < p.M;
-    }
     for (int e0 = 0; e0 < p.E; e0 += 64) {
         const int e = e0 + lane;
         int64_t lo = 0, hi = 0;
@@ -893,45 +887,43 @@ int64_t row_tiles(const BlocksParams& p, int TT) {
     return p.offsets ? std::min<int64_t>(p.M, p.M / TT + p.E) : full;
 }
 
-template <class T>
+template <class T, bool GROUPED>
 int launch_tile(const BlocksParams& p, const char* who, hipStream_t st) {
     const int64_t tiles = row_tiles(p, T::TT) * ((p.N + T::TW - 1) / T::TW);
     H3_REQUIRE(tiles < ((int64_t)1 << 31), "%s: too many tiles for one launch", who);
     const dim3 grid((unsigned)std::min<int64_t>(tiles, h3host::cu_count())), block(T::WAVES * 64);
-#define H3_B(FP16, BIAS, GROUPED) hipLaunchKernelGGL((gemm_blocks_tile_kernel<T, FP16, BIAS, GROUPED>), grid, block, 0, st, p)
-    if (p.offsets) {
-        if (p.fp16) H3_B(true, false, true);
-        else H3_B(false, false, true);
-    } else if constexpr (!T::NT) {                        // by expert only
-        if (p.fp16) {
-            if (p.bias) H3_B(true, true, false);
-            else H3_B(true, false, false);
-        } else {
-            if (p.bias) H3_B(false, true, false);
-            else H3_B(false, false, false);
-        }
+#define H3_B(FP16, BIAS) hipLaunchKernelGGL((gemm_blocks_tile_kernel<T, FP16, BIAS, GROUPED>), grid, block, 0, st, p)
+    if constexpr (GROUPED) {                              // without a bias
+        if (p.fp16) H3_B(true, false);
+        else H3_B(false, false);
+    } else if (p.fp16) {
+        if (p.bias) H3_B(true, true);
+        else H3_B(true, false);
+    } else {
+        if (p.bias) H3_B(false, true);
+        else H3_B(false, false);
     }
 #undef H3_B
     H3_CHECK_HIP(hipGetLastError());
     return H3FP8_OK;
 }
 
-template <class T>
+template <class T, bool GROUPED>
 int launch_small(const BlocksParams& p, const char* who, hipStream_t st) {
     const int64_t tiles_n = (p.N + T::TW - 1) / T::TW, rt = row_tiles(p, T::TT), tiles = rt * tiles_n;
     H3_REQUIRE(tiles < ((int64_t)1 << 32) / (T::WAVES * 64), "%s: too many tiles for one launch", who);      // 2^32 threads
     const dim3 grid((unsigned)tiles), block(T::WAVES * 64);
-#define H3_B(FP16, BIAS, GROUPED) \
+#define H3_B(FP16, BIAS) \
     hipLaunchKernelGGL((gemm_blocks_small_kernel<T, FP16, BIAS, GROUPED>), grid, block, T::LDS, st, p, (int)tiles_n, (int)rt)
-    if (p.offsets) {
-        if (p.fp16) H3_B(true, false, true);
-        else H3_B(false, false, true);
+    if constexpr (GROUPED) {
+        if (p.fp16) H3_B(true, false);
+        else H3_B(false, false);
     } else if (p.fp16) {
-        if (p.bias) H3_B(true, true, false);
-        else H3_B(true, false, false);
+        if (p.bias) H3_B(true, true);
+        else H3_B(true, false);
     } else {
-        if (p.bias) H3_B(false, true, false);
-        else H3_B(false, false, false);
+        if (p.bias) H3_B(false, true);
+        else H3_B(false, false);
     }
 #undef H3_B
     H3_CHECK_HIP(hipGetLastError());
@@ -940,27 +932,29 @@ int launch_small(const BlocksParams& p, const char* who, hipStream_t st) {
 
 // ---- which form runs --------------------------------------------------------------------------------------------------
 //
-// Small tiles, channels x tokens (one-shot workgroups), in ascending order of their area, and how many of them a CU holds:
+// Small tiles, channels x tokens (one-shot workgroups), in ascending order of their area: the calls that take them (kernels are
+// compiled for those only) and how many of them a CU holds.
+constexpr int DENSE = 1, EXPERTS = 2;
 #define H3_SMALL_FORMS(X)                                                                                              \
-    X(F_32x16, 3, 2, 1, 1, 1, 6, 1)                                                                                    \
-    X(F_32x32, 2, 2, 1, 1, 2, 8, 2)                                                                                    \
-    X(F_64x32, 2, 2, 1, 2, 2, 5, 1)                                                                                    \
-    X(F_32x64, 2, 2, 2, 1, 2, 6, 2)                                                                                    \
-    X(F_64x64, 1, 2, 2, 2, 2, 4, 1)                                                                                    \
-    X(F_128x64, 1, 4, 2, 2, 2, 6, 2)                                                                                   \
-    X(F_128x64_PAIR, 2, 2, 2, 4, 2, 3, 1)
+    X(F_32x16, DENSE | EXPERTS, 3, 2, 1, 1, 1, 6, 1)                                                                   \
+    X(F_32x32, DENSE, 2, 2, 1, 1, 2, 8, 2)                                                                             \
+    X(F_64x32, EXPERTS, 2, 2, 1, 2, 2, 5, 1)                                                                           \
+    X(F_32x64, DENSE, 2, 2, 2, 1, 2, 6, 2)                                                                             \
+    X(F_64x64, EXPERTS, 1, 2, 2, 2, 2, 4, 1)                                                                           \
+    X(F_128x64, DENSE, 1, 4, 2, 2, 2, 6, 2)                                                                            \
+    X(F_128x64_PAIR, DENSE, 2, 2, 2, 4, 2, 3, 1)
 enum Form {
 #define X(id, ...) id,
     H3_SMALL_FORMS(X)
 #undef X
     F_256x128, F_256x256
 };
-struct FormDims { int per_cu, tw, tt; };
+struct FormDims { int calls, per_cu, tw, tt; };
 constexpr FormDims kForms[] = {
-#define X(id, per, WN, WM, NI, NJ, NST, KS) {per, 16 * NI * WN, 16 * NJ * WM},
+#define X(id, calls, per, WN, WM, NI, NJ, NST, KS) {calls, per, 16 * NI * WN, 16 * NJ * WM},
     H3_SMALL_FORMS(X)
 #undef X
-    {1, 256, 128}, {1, 256, 256}};
+    {DENSE | EXPERTS, 1, 256, 128}, {DENSE | EXPERTS, 1, 256, 256}};
 
 int64_t tiles_of(int form, int64_t row_tiles, int64_t N) { return row_tiles * ((N + kForms[form].tw - 1) / kForms[form].tw); }
 
@@ -980,7 +974,7 @@ int large_form(int64_t rows128, int64_t rows256, int64_t N, int G) {
 int dense_form(int64_t M, int64_t N, int G) {
     if (M <= 16) return F_32x16;
     for (int f = 0; f < F_256x128; ++f)
-        if (f != F_64x32 && f != F_64x64 && tiles_of(f, (M + kForms[f].tt - 1) / kForms[f].tt, N) <= (int64_t)kForms[f].per_cu * G) return f;
+        if ((kForms[f].calls & DENSE) && tiles_of(f, (M + kForms[f].tt - 1) / kForms[f].tt, N) <= (int64_t)kForms[f].per_cu * G) return f;
     return large_form((M + 127) / 128, (M + 255) / 256, N, G);
 }
 
@@ -1005,28 +999,37 @@ bool streams(const BlocksParams& p) { return (int64_t)p.N * p.K * std::min<int64
 // ... and of the large tiles, by expert, while one row tile holds a mean expert's rows.  16 experts of 4096 x 4096: 64 rows each 67
 // / 73, 128: 77 / 80, 256: 85 / 92; but with two row tiles that share the weights in L2, 384: 137 / 127, and 32 768 rows
 // over 32 experts 585 / 557.
-bool once(const BlocksParams& p, int64_t rows) { return p.offsets && p.M <= rows * p.E; }
+bool once(const BlocksParams& p, int64_t rows) { return p.M <= rows * p.E; }
 
 int form_for(int64_t M, int64_t N, int64_t E, bool grouped, int G) { return grouped ? grouped_form(M, N, E, G) : dense_form(M, N, G); }
 
+template <bool GROUPED>
 int run(const BlocksParams& p, const char* who, hipStream_t st) {
     if (p.M == 0 || p.N == 0 || p.E == 0) return H3FP8_OK;
-    const bool grouped = p.offsets != nullptr, nt = streams(p);
-    switch (form_for(p.M, p.N, p.E, grouped, h3host::cu_count())) {
-#define X(id, per, ...)                                                                                                \
+    const bool nt = streams(p);
+    const int form = form_for(p.M, p.N, p.E, GROUPED, h3host::cu_count());
+    switch (form) {
+#define X(id, calls, per, ...)                                                                                         \
     case id:                                                                                                           \
-        if ((id == F_32x16 || id == F_64x32 || id == F_64x64) && nt)                                                   \
-            return launch_small<SmallTile<__VA_ARGS__, id == F_32x16 || id == F_64x32 || id == F_64x64>>(p, who, st);  \
-        return launch_small<SmallTile<__VA_ARGS__>>(p, who, st);
+        if constexpr (((calls) & (GROUPED ? EXPERTS : DENSE)) != 0) {                                                  \
+            if constexpr (((calls) & EXPERTS) != 0)                                                                    \
+                if (nt) return launch_small<SmallTile<__VA_ARGS__, true>, GROUPED>(p, who, st);                        \
+            return launch_small<SmallTile<__VA_ARGS__>, GROUPED>(p, who, st);                                          \
+        }                                                                                                              \
+        break;
         H3_SMALL_FORMS(X)
 #undef X
         case F_256x128:
-            if (nt && once(p, 128)) return launch_tile<BigTile<2, 4, 8, 2, 3, true>>(p, who, st);
-            return launch_tile<BigTile<2, 4, 8, 2, 3>>(p, who, st);
-        default:
-            if (nt && once(p, 256)) return launch_tile<BigTile<2, 4, 8, 4, 2, true>>(p, who, st);
-            return launch_tile<BigTile<2, 4, 8, 4, 2>>(p, who, st);
+            if constexpr (GROUPED)
+                if (nt && once(p, 128)) return launch_tile<BigTile<2, 4, 8, 2, 3, true>, true>(p, who, st);
+            return launch_tile<BigTile<2, 4, 8, 2, 3>, GROUPED>(p, who, st);
+        case F_256x256:
+            if constexpr (GROUPED)
+                if (nt && once(p, 256)) return launch_tile<BigTile<2, 4, 8, 4, 2, true>, true>(p, who, st);
+            return launch_tile<BigTile<2, 4, 8, 4, 2>, GROUPED>(p, who, st);
     }
+    H3_REQUIRE(false, "%s: no kernel for form %d", who, form);
+    return H3FP8_OK;
 }
 
 }  // namespace
@@ -1053,7 +1056,7 @@ int h3fp8_gemm_blocks(const void* a, int64_t lda, const void* w, int64_t ldw, co
     p.sa_m = sa_m; p.sa_k = sa_k; p.sw_n = sw_n; p.sw_k = sw_k;
     p.M = M; p.N = (int)N; p.K = (int)K; p.E = 1; p.fp16 = out_dtype == H3FP8_DT_FP16;
     const int rc = check(p, "h3fp8_gemm_blocks", out_dtype, N, K, 1);
-    return rc ? rc : run(p, "h3fp8_gemm_blocks", (hipStream_t)stream);
+    return rc ? rc : run<false>(p, "h3fp8_gemm_blocks", (hipStream_t)stream);
 }
 
 int h3fp8_grouped_gemm_blocks(const void* a, int64_t lda, const void* w, int64_t w_e, int64_t ldw, const float* sa,
@@ -1071,7 +1074,7 @@ int h3fp8_grouped_gemm_blocks(const void* a, int64_t lda, const void* w, int64_t
     H3_REQUIRE(idx_bytes == 4 || idx_bytes == 8, "h3fp8_grouped_gemm_blocks: offsets must be int32 or int64");
     H3_REQUIRE(M == 0 || N == 0 || E == 0 || offsets, "h3fp8_grouped_gemm_blocks: null offsets");
     H3_REQUIRE((uintptr_t)offsets % (unsigned)idx_bytes == 0, "h3fp8_grouped_gemm_blocks: misaligned offsets");
-    return run(p, "h3fp8_grouped_gemm_blocks", (hipStream_t)stream);
+    return run<true>(p, "h3fp8_grouped_gemm_blocks", (hipStream_t)stream);
 }
 
 }  // extern "C"
