@@ -246,6 +246,47 @@ def test_gemm_blocks_forms(cuda, M, N, form, K):
         assert torch.equal(y[m:m + 1], ops.gemm_blocks(a[m:m + 1], w, sa[m:m + 1], sw)), m
 
 
+def exact_operands(g, M, N, K, E=None):
+    """Integer codes, scales of 2^-2 .. 2^1: products are multiples of 2^-4 and a block's sum at most 2^13, so that every fp32 sum over
+    K <= 640 is exact, with an integer bias too."""
+    a, w = codes(g, M, K, integers=True), codes(g, (E or 1) * N, K, integers=True)
+    pow2 = lambda *s: torch.exp2(torch.randint(-2, 2, s, generator=g, device="cuda").float())            # noqa: E731
+    sa, sw = pow2(M, cdiv(K, B)), pow2(E or 1, cdiv(N, B), cdiv(K, B))
+    return (a, w, sa, sw[0]) if E is None else (a, w.view(E, N, K), sa, sw)
+
+
+@pytest.mark.parametrize("M,N,form", FORMS)
+@pytest.mark.parametrize("dtype,biased", [(BF16, True), (FP16, False), (FP16, True)])
+def test_gemm_blocks_epilogues(cuda, M, N, form, dtype, biased):
+    """Each form's epilogue with a bias and in fp16, at ragged rows and channels: the exact value, rounded once; nothing outside the
+    output is written."""
+    from h3_tp2_amd import ops
+    assert plan(M, N)[2] == form
+    K = 272
+    g = gen(M + N)
+    a, w, sa, sw = exact_operands(g, M, N, K)
+    bias = torch.randint(-300, 301, (N,), generator=g, device=cuda).float().to(dtype) if biased else None
+    out = torch.full((M + 2, N + 16), -3.0, device=cuda, dtype=dtype)
+    y = ops.gemm_blocks(a, w, sa, sw, dtype, bias, out=out[1:M + 1, :N])
+    y64, _ = product64(a, w, sa, sw, bias)
+    assert torch.equal(y, y64.to(dtype))
+    assert (out[0] == -3).all() and (out[M + 1] == -3).all() and (out[:, N:] == -3).all()
+
+
+@pytest.mark.parametrize("M", [200, 199])
+def test_gemm_blocks_out_projection(cuda, M):
+    """The out projection of a short sequence in fp16 with a bias, random operands."""
+    from h3_tp2_amd import ops
+    g = gen(M)
+    K, N = 7168, 5376
+    a, w, sa, sw = codes(g, M, K), codes(g, N, K), scales(g, M, K // B), scales(g, N // B, K // B)
+    sa, bias = sa * 0.1, (torch.randn(N, generator=g, device=cuda) * 0.5).to(FP16)
+    y = ops.gemm_blocks(a, w, sa, sw, FP16, bias)
+    y64, mag = product64(a, w, sa, sw, bias)
+    assert y64.abs().max() < 65504
+    check_product(y, y64, mag, FP16)
+
+
 def test_gemm_blocks_streaming_weight(cuda):
     """More than 64 MiB of weights: the loads with the non-temporal hint, against the same rows of a slice without it."""
     from h3_tp2_amd import ops
@@ -350,6 +391,20 @@ def test_grouped_forms(cuda, M, E, N, form, K):
         if hi > lo:
             assert torch.equal(out[lo:hi], product64(a[lo:hi], w[e], sa[lo:hi], sw[e])[0].to(BF16)), e
     assert (out[:off[0]] == -3).all() and (out[off[-1]:] == -3).all()
+
+
+@pytest.mark.parametrize("M,E,N,form", GROUPED_FORMS)
+def test_grouped_forms_fp16(cuda, M, E, N, form):
+    """Each form's fp16 output: the exact value, rounded once."""
+    from h3_tp2_amd import ops
+    assert plan(M, N, E, True)[2] == form
+    g = gen(M + E)
+    a, w, sa, sw = exact_operands(g, M, N, 272, E)
+    off = [0] + torch.randint(0, M + 1, (E - 1,), generator=g, device=cuda).sort()[0].tolist() + [M]
+    y = ops.grouped_gemm_blocks(a, w, sa, sw, torch.tensor(off, device=cuda), FP16)
+    for e, (lo, hi) in enumerate(zip(off[:-1], off[1:])):
+        if hi > lo:
+            assert torch.equal(y[lo:hi], product64(a[lo:hi], w[e], sa[lo:hi], sw[e])[0].to(FP16)), e
 
 
 @pytest.mark.parametrize("M,form", [(1000, 7), (4000, 8)])
