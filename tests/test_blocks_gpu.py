@@ -300,6 +300,22 @@ def test_gemm_blocks_streaming_weight(cuda):
     check_product(y, y64, mag, BF16)
 
 
+@pytest.mark.parametrize("dtype,biased", [(BF16, True), (FP16, False), (FP16, True)])
+def test_gemm_blocks_streaming_weight_epilogues(cuda, dtype, biased):
+    """The streaming loads with a bias and in fp16: the exact value, rounded once."""
+    from h3_tp2_amd import ops
+    g = gen(18)
+    M, K, N = 11, 272, 249856
+    assert plan(M, N)[2] == 0 and N * K > 64 << 20
+    a, w, sa, sw = exact_operands(g, M, N, K)
+    bias = torch.randint(-300, 301, (N,), generator=g, device=cuda).float().to(dtype) if biased else None
+    y = ops.gemm_blocks(a, w, sa, sw, dtype, bias)
+    for n in range(0, N, 32768):
+        part = slice(n, min(N, n + 32768))
+        ref, _ = product64(a, w[part], sa, sw[n // B:cdiv(part.stop, B)], None if bias is None else bias[part])
+        assert torch.equal(y[:, part], ref.to(dtype)), n
+
+
 def test_gemm_blocks_extreme_scales(cuda):
     """Scales of 0, inf and NaN in the last of an odd number of blocks, and products that round to a negative zero: every form
     gives the bits of the single row."""
@@ -423,6 +439,27 @@ def test_grouped_streaming_weights(cuda, M, form):
     for e, (lo, hi) in enumerate(zip(off[:-1], off[1:])):
         if hi > lo:
             assert torch.equal(y[lo:hi], ops.gemm_blocks(a[lo:hi], w[e], sa[lo:hi], sw[e])), e
+
+
+@pytest.mark.parametrize("M,form", [(60, 0), (180, 2), (300, 4), (1000, 7), (4000, 8)])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_grouped_streaming_weights_forms(cuda, M, form, dtype):
+    """More than 64 MiB of weights in every form that takes the hint, in both output types: the dense bits, with an expert of a
+    third of the rows, one of one row and one without rows."""
+    from h3_tp2_amd import ops
+    E, N, K = 18, 2064, 2048
+    assert plan(M, N, E, True)[2] == form and E * N * K > 64 << 20
+    g = gen(M + 1)
+    a, w = codes(g, M, K), codes(g, E * N, K).view(E, N, K)
+    sa, sw = scales(g, M, K // B), scales(g, E, cdiv(N, B), K // B)
+    off = [0, M // 3, M // 3 + 1, M // 3 + 1] + [M // 3 + 1 + (M - M // 3 - 1) * i // (E - 3) for i in range(1, E - 2)]
+    assert len(off) == E + 1 and off[-1] == M
+    y = ops.grouped_gemm_blocks(a, w, sa, sw, torch.tensor(off, device=cuda), dtype)
+    for e, (lo, hi) in enumerate(zip(off[:-1], off[1:])):
+        if hi > lo:
+            assert torch.equal(y[lo:hi], ops.gemm_blocks(a[lo:hi], w[e], sa[lo:hi], sw[e], dtype)), e
+    y64, mag = grouped64(a, w, sa, sw, off)
+    check_product(y, y64, mag, dtype)
 
 
 def test_grouped_decreasing_offsets_stay_inside(cuda):
