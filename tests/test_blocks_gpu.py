@@ -582,6 +582,55 @@ def test_side_streams(cuda):
     assert all(torch.equal(y, ref) for y in got)
 
 
+def test_side_streams_with_their_own_operands(cuda):
+    """Four streams at once, each with operands and sizes of its own (other forms), written on that stream right before the calls
+    and anew in every turn: each gives what the same calls give alone.  A call on another stream, or one that keeps anything
+    of another call's, would show."""
+    from h3_tp2_amd import ops
+    K = 1536
+    tab = torch.randn(256, 96, generator=gen(40), device=cuda)
+    runs = []
+    for i, (M, N, E) in enumerate(((9, 400, 2), (90, 1552, 5), (700, 2064, 6), (2050, 1280, 3))):
+        g = gen(41 + i)
+        fresh = [torch.randn(M, K, generator=g, device=cuda).to(BF16) for _ in range(3)]
+        w, sw = ops.quant_blocks(torch.randn(E * N, K, generator=g, device=cuda) * 0.05, rows=128) if N % B == 0 else (
+            codes(g, E * N, K), scales(g, E * cdiv(N, B), K // B))
+        off = torch.randint(0, M + 1, (E + 1,), generator=g, device=cuda).sort()[0]
+        off[0], off[-1] = 0, M
+        norm = 1 + 0.1 * torch.randn(128, generator=g, device=cuda)
+        pos = torch.randint(0, 256, (M,), generator=g, device=cuda)
+        runs.append(dict(x=torch.zeros(M, K, dtype=BF16, device=cuda), fresh=fresh, w=w.view(E, N, K), sw=sw.view(E, -1, K // B), off=off,
+                         norm=norm.to(BF16), pos=pos))
+
+    def step(r, turn):
+        r["x"].copy_(r["fresh"][turn])
+        q, s = ops.quant_blocks(r["x"])
+        y = ops.gemm_blocks(q, r["w"][0], s, r["sw"][0])
+        z = ops.grouped_gemm_blocks(q, r["w"], s, r["sw"], r["off"])
+        h, hs = ops.silu_mul_quant_blocks(r["x"])
+        heads = r["x"].view(-1, 12, 128)
+        qk = ops.qk_norm_rope(heads[:, :8], heads[:, 8:], r["norm"], r["norm"], tab, 1e-6, positions=r["pos"])
+        return [t.contiguous().view(torch.uint8) for t in (q, s, y, z, h, hs, *qk)]
+
+    alone = []
+    for turn in range(3):
+        for r in runs:
+            alone.append(step(r, turn))
+            torch.cuda.synchronize()
+    busy = torch.randn(4096, 4096, device=cuda)
+    streams = [torch.cuda.Stream() for _ in runs]
+    torch.cuda.synchronize()
+    got = []
+    for turn in range(3):
+        for r, st in zip(runs, streams):
+            with torch.cuda.stream(st):
+                busy @ busy                                            # the stream is behind the host when its operands are written
+                got.append(step(r, turn))
+    torch.cuda.synchronize()
+    for i, (a, b) in enumerate(zip(got, alone)):
+        assert all(torch.equal(x, y) for x, y in zip(a, b)), i
+
+
 # ---- the native host path against the Python path ---------------------------------------------------------------------
 
 def _outcome(f):
