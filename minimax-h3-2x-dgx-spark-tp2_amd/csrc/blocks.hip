@@ -13,8 +13,9 @@
 // a tile of ROWS tokens, whose scales go through LDS so that the scale tensor, token-contiguous as the product reads it,
 // is written in pieces of ROWS consecutive entries.  ROWS = 8: quant of 42848 x 7168 bf16 141 us (6.6 TB/s), SwiGLU of 18880 x
 // 2 x 14336 204 us (6.7 TB/s), of 64 x 2 x 2048 2.8 us; with 32 rows 152, 220 and 5.3 (few and long waves), 16 rows 146
-// and 217, 4 rows 151, 230 and 2.4 (a scale line in more pieces).  128 x 128: 21504 x 5376 bf16 54 us (6.4 TB/s); with 256
-// threads of 8 loads each, behind branches, it was 64.
+// and 217, 4 rows 151, 230 and 2.4 (a scale line in more pieces).  (All in one run, in turn; a kernel trace gives the 64 tokens 3.4-3.7
+// us, and the large ones are 10 us slower on new inputs.)  From fp32 42848 x 7168 276 us (5.6 TB/s).  128 x 128: 21504 x 5376 bf16
+// 54 us (6.4 TB/s), fp32 112 us (5.2 TB/s); with 256 threads of 8 loads each, behind branches, bf16 was 64.
 #include "h3fp8_common.h"
 
 namespace {
@@ -90,7 +91,7 @@ __device__ __forceinline__ v2u codes8(const float f[8], float inv) {
 // as a factor 1 + d ln 2 (with g held to +-200, where the exponential is 0 or inf, d stays finite).  exp2 and the reciprocal are
 // the hardware's, 1 ulp each.  The reciprocal returns 0 where its result is subnormal, which is so from an exponential of 2^126
 // on (g < -87.3), short of its overflow at 2^128 (g < -88.7): denominator and gate are held as quarters, exactly, so that it
-// stays normal.  From the overflow on the result is -0, as the division by inf gives.  Without d
+// stays normal (one product more: 209 us against 206 at 18880 x 2 x 14336 timed in turn, the least of each 203.6 and 203.9).  From the overflow on the result is -0, as the division by inf gives.  Without d
 // the exponential is |g| / 2 ulp off and four times as many codes at a rounding border fall on its other side.  With it 43 to
 // 59 of 36 M codes differ from those of float64, with a library exponential and IEEE division 41 to 52; a Newton step on the rcp
 // (36 to 63) costs 6 % of the time, the sum's lost bits on top (41 to 52) 24 %.

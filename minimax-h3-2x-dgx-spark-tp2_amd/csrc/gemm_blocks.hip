@@ -109,8 +109,8 @@ __device__ __forceinline__ bool locate_rows(const BlocksParams& p, int TT, int64
 //     and nothing else is limited to 32-bit offsets.
 // What bounds it: with operands in the caches the return path from L2 to LDS (64 KiB a k-step and CU) beside the matrix pipe,
 // busy 0.54 of the time at 2.0 GHz and 0.63 at the 1.5 GHz that the power limit leaves under a lasting load: 18 880 x 21 504 x
-// 5376 in 1780-1850 us (2.4 PFLOP/s), 32 768 rows over 32 experts of 4096 x 4096 in 550 (2.0: every expert's last tile is
-// partly empty).  With few rows per expert the weights' way from memory: 4100 rows over 16 experts 111 us; 16 x 128 rows 76 us
+// 5376 in 1780-1890 us (2.3-2.45 PFLOP/s), 32 768 rows over 32 experts of 4096 x 4096 in 550-600 (2.0-1.8: every expert's last tile
+// is partly empty).  With few rows per expert the weights' way from memory: 4100 rows over 16 experts 111 us; 16 x 128 rows 76 us
 // from memory, 44 from the caches.  Fetching the weights' lines into L2 some k-steps ahead by one more load per wave (a dword
 // of each line) made every case slower (1890 -> 2244 us): the requests that are under way are the limit.
 __device__ __forceinline__ int swz_w(int r) { return ((r >> 1) & 1) | (((r >> 3) & 3) << 1); }
@@ -554,7 +554,7 @@ __global__ void __launch_bounds__(T::WAVES * 64, 2) gemm_blocks_tile_kernel(Bloc
         const BIssue S = bissue<T>(I, nk, lds0 + (uint32_t)s * T::STAGE, lds0 + T::SC_OFF + (uint32_t)s * T::SC_STAGE, wave);
 #pragma unroll
         for (int i = 0; i < T::LOADS; ++i) bload<T>(I, S, i);
-            cursor_next<T, GROUPED>(I, p, sp, nk, wave, lane);
+        cursor_next<T, GROUPED>(I, p, sp, nk, wave, lane);
     }
     const BAddr<T> A = baddr<T>(wn, wm, lane);
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(T::LOADS * (T::NST - 1)));
@@ -620,7 +620,7 @@ __global__ void __launch_bounds__(T::WAVES * 64, 2) gemm_blocks_tile_kernel(Bloc
 // barrier, fragment reads and MFMAs.  One workgroup per tile, a deep ring of stages, fragments read a whole k-step ahead (two
 // sets of registers, the loop unrolled by two) and the fmas a whole k-step behind their MFMAs.
 // 200 x 5376 x 7168 22.6 us (128 x 64 tiles on 168 CUs, 0.4 us a k-step: 225 MB from L2 at 10 TB/s); 1 x 21 504 x 5376 19.5 us
-// (5.9 TB/s of weights); 64 rows over 32 experts of 2048 x 4096 45 us (5.9 TB/s).
+// (5.9 TB/s of weights); 64 rows over 32 experts of 2048 x 4096 52 us with two rows in each (5.2 TB/s), 45 with rows in 25 of them (4.7).
 // The LDS is the launch's: a size that the compiler knew would let it give a lone workgroup 512 registers a lane and put the
 // MFMAs' results into the accumulation half, a copy away from the fmas.
 template <class T>
@@ -965,12 +965,22 @@ int large_form(int64_t rows128, int64_t rows256, int64_t N, int G) {
     return 16 * r256 < 11 * r128 ? F_256x256 : F_256x128;
 }
 
-// One problem: the smallest form whose tiles the CUs hold at once, since the launch then lasts as long as one tile; with 16
-// tokens or fewer always 32 x 16 (the weights' bytes count).  Past that the large tiles.  64 x 32 and 64 x 64 are for
-// experts (below): 64 x 64 on one per CU holds what 32 x 64 does on two.
-// Measured with the weights in turn from copies, smaller / taken / larger form, us, M x N x K: 32 x 5376 x 7168 13.5 / 12.0 (32 x
-// 32) / 14.7; 128 x 5376 x 7168 24.5 / 20.2 (32 x 64) / 21.4; 200 x 5376 x 7168 31.5 / 22.8 (128 x 64) / 26.8; 512 x 5376 x 7168
-// 42.8 / 35.1 (128 x 64 in pairs) / 49.0; 256 x 21 504 x 5376 58.8 / 48.5 (256 x 128) / 62.0.
+// One problem: the smallest form whose tiles the CUs hold at once; with 16 tokens or fewer always 32 x 16 (the weights' bytes
+// count).  Past that the large tiles.  64 x 32 and 64 x 64 are compiled for experts (below).  Measured on 256 CUs, the weights in
+// turn from copies that together exceed the last-level cache, us, [taken]; 64 x 32 and 64 x 64 from a build that had them:
+//   M x N x K           32 x 16  32 x 32  64 x 32  32 x 64  64 x 64  128 x 64  in pairs  256 x 128  256 x 256
+//   32 x 5376 x 7168     [17.3]     13.6     17.5     17.0     20.5      26.6      31.3       46.5       62.8
+//   64 x 5376 x 7168     [21.5]     21.0     17.4     18.1     21.7      30.1      32.7       49.6       63.3
+//   128 x 5376 x 7168      36.6     30.0     27.6   [27.9]     21.3      29.2      32.1       56.3       65.0
+//   200 x 5376 x 7168         -        -        -     34.3     29.3    [25.4]      31.4       52.7       75.9
+//   512 x 5376 x 7168         -        -        -     65.3     49.1      53.6    [47.0]       54.1       75.9
+//   1024 x 5376 x 7168        -        -        -        -        -      75.8      67.8     [54.3]       77.0
+//   2048 x 5376 x 7168        -        -        -        -        -     150.6     119.0      107.9     [78.9]
+//   32 x 21 504 x 5376     38.0     34.0     26.3     32.0     27.0    [26.8]      29.0       40.5       53.9
+//   128 x 21 504 x 5376    98.9     71.0     61.7     59.0     45.6      47.4    [43.7]       48.6       55.5
+//   256 x 21 504 x 5376       -        -        -     94.8     75.0      65.8      59.2     [48.1]       62.4
+// So it takes the best form or one within a few per cent of it from 200 rows on and on wide outputs, but not at 17 to 128 rows of
+// 5376 channels: workgroups that share a CU share its load path too, which this rule does not count.
 int dense_form(int64_t M, int64_t N, int G) {
     if (M <= 16) return F_32x16;
     for (int f = 0; f < F_256x128; ++f)

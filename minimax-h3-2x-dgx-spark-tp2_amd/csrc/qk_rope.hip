@@ -16,7 +16,8 @@
 // are dealt over several waves, until every SIMD has two.
 // 18 880 tokens x (56 + 56) heads of 128, bf16: 197 us, 5.5 TB/s (two passes in flight 200, eight 192, but 4000 tokens x (32 + 8)
 // heads 17.1 / 16.8 / 18.0; with q's and k's heads in one wave, the addresses and weights selected lane by lane, 209 and 22.1);
-// 8 tokens x (32 + 8) heads 5.8 us a call, 3.2 of them on the GPU.
+// 8 tokens x (32 + 8) heads 5.3-5.8 us a call, 3.3 of them on the GPU.  In one run, 18 880 tokens: (56 + 56) heads of 128 half-split
+// 202 us, interleaved 201; (56 + 56) of 64 97 either way (5.6 TB/s); (28 + 28) of 256 203 and 202.
 #include <algorithm>
 
 #include "h3fp8_common.h"
