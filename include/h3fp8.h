@@ -313,6 +313,53 @@ int h3fp8_qk_norm_rope(const void* q, int64_t q_t, int64_t q_h, const void* k, i
                        int64_t ok_h, void* stream);
 
 /*
+ * The block-scaled product with an epilogue: y = round(residual + act(the sum of h3fp8_gemm_blocks + bias)), fp32 up to the
+ * one rounding.  Operands, scales, strides and sizes as h3fp8_gemm_blocks; act one of H3FP8_ACT_*; residual [M, N] in y's
+ * type, row stride ldr (a multiple of 8; 0: one row for all), or NULL; bias and residual 16-byte aligned; y may be the residual itself.
+ */
+#define H3FP8_ACT_NONE 0
+#define H3FP8_ACT_SILU 1         /* v / (1 + exp(-v)) */
+#define H3FP8_ACT_GELU 2         /* v (1 + erf(v / sqrt 2)) / 2 */
+#define H3FP8_ACT_GELU_TANH 3    /* v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) / 2 */
+#define H3FP8_ACT_RELU 4
+int h3fp8_gemm_blocks_act(const void* a, int64_t lda, const void* w, int64_t ldw, const float* sa, int64_t sa_m, int64_t sa_k,
+                          const float* sw, int64_t sw_n, int64_t sw_k, const void* bias, int act, const void* residual,
+                          int64_t ldr, void* y, int64_t ldy, int out_dtype, int64_t M, int64_t N, int64_t K, void* stream);
+
+/*
+ * The router of an expert layer: every token's k best of E experts from logits [T, E] (bf16 / fp16 / fp32: dtype; row stride ld).
+ *   score = softmax over the experts (scoring 0) or 1 / (1 + exp(-x)) (1); chosen in descending order of the logit, with bias
+ *   ([E], or NULL) of score + bias in 64 bits, the lower index first among equals; a -inf (of the logit or the sum) and a NaN are
+ *   never chosen.
+ *   weights [T, k] = the chosen scores (renorm: over their sum, 0 where that is 0) * scale; experts [T, k]; choices for which
+ *   no expert is left: expert -1, weight 0.  A NaN among a token's logits makes its weights NaN.
+ *   order [T k]: the pairs p = t k + j sorted by expert, ascending within one, those without an expert last; offsets [E + 1]: expert
+ *   e has the places offsets[e] .. offsets[e + 1] - 1 (the rows of h3fp8_grouped_gemm_blocks); place [T k]: where p went.
+ * E at most 512, k at most 16.  workspace: h3fp8_moe_route_workspace(T, E) bytes of device memory (0 up to 128 tokens).
+ */
+int64_t h3fp8_moe_route_workspace(int64_t T, int64_t E);
+int h3fp8_moe_route(const void* logits, int64_t ld, int dtype, int64_t T, int64_t E, int k, int scoring, int renorm,
+                    float scale, const float* bias, float* weights, int32_t* experts, int32_t* offsets, int32_t* order,
+                    int32_t* place, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * A whole layer of block-scaled experts for at most 128 tokens, two launches:
+ *   y[t] = residual[t] + sum_j weights[t, j] * W2[e] (silu(g) * u),  g | u = W1[e] x[t],  e = experts[t, j]
+ * x, residual (or NULL), y [T, H] bf16 or fp16 (dtype), not quantised; w1 [E, 2F, H] (gate rows, then up rows) and w2 [E, H, F]
+ * e4m3 with expert strides and row strides, scales [E, ceil(2F / 128), ceil(H / 128)] and [E, ceil(H / 128), ceil(F / 128)] in
+ * any strides; weights, experts, offsets, order: those of h3fp8_moe_route.  fp32 throughout, the inner values h carried in 16
+ * bits of mantissa, one rounding of y.  An expert's NaN or infinity reaches its own tokens only.  y may be the residual itself.
+ * H, F multiples of 16; x and weights 16-byte aligned, row strides of x multiples of 8, of the weights of 16, of y and the
+ * residual of 4 (8-byte aligned).  workspace: h3fp8_moe_blocks_workspace bytes of device memory, 16-byte aligned.
+ */
+int64_t h3fp8_moe_blocks_workspace(int64_t T, int64_t k, int64_t F);
+int h3fp8_moe_blocks(const void* x, int64_t ldx, int dtype, int64_t T, int64_t H, int64_t F, int64_t E, int k, const void* w1,
+                     int64_t w1_e, int64_t ld1, const float* s1, int64_t s1_e, int64_t s1_n, int64_t s1_k, const void* w2,
+                     int64_t w2_e, int64_t ld2, const float* s2, int64_t s2_e, int64_t s2_n, int64_t s2_k, const float* weights,
+                     const int32_t* experts, const int32_t* offsets, const int32_t* order, const void* residual, int64_t ldr,
+                     void* y, int64_t ldy, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * Self-checks used by the install probe and the tests (no reference counterpart beyond its install probes,
  * h3_tp2/fp8_cutlass.py:196-249):
  *   h3fp8_selfcheck_e4m3   converts every fp32 bit pattern with |x| <= 448 (and the NaNs) with the hardware cvt used

@@ -1,7 +1,8 @@
 // The host path of the common calls, natively: the argument checks, the output allocations and the C-ABI call of
 // ops.quant_rows, ops.gemm, the dispatcher's scaled product, ops.gemm_quant, ops.gemm_swiglu_quant, ops.silu_mul_quant,
 // ops.rms_quant and ops.gate_rms_quant (h3_tp2_amd/ops.py, fp8_gemm.py), and of the block-scaled calls ops.quant_blocks,
-// ops.silu_mul_quant_blocks, ops.gemm_blocks, ops.grouped_gemm_blocks and ops.qk_norm_rope.
+// ops.silu_mul_quant_blocks, ops.gemm_blocks, ops.gemm_blocks_act, ops.grouped_gemm_blocks and ops.qk_norm_rope, and of the
+// expert layer's ops.moe_route and ops.moe_blocks.
 //
 // Every function takes the call only in its plain form -- exact torch tensors on one GPU, the dtypes, shapes and strides
 // that the kernels read in place, no caller-supplied outputs -- and returns None for any other, which the Python path then
@@ -499,6 +500,156 @@ PyObject* grouped_gemm_blocks(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// A residual of y's shape and type that is y itself or whose extent is apart from y's: its pointer and row stride (0: none).
+bool residual_of(PyObject* arg, const at::Tensor& y, int64_t ldy, const void** p, int64_t* ld) {
+    *p = nullptr;
+    *ld = 0;
+    if (arg == Py_None) return true;
+    const at::Tensor* t = plain(arg);
+    if (!t || t->scalar_type() != y.scalar_type() || t->device() != y.device() || t->dim() != 2 || t->sizes() != y.sizes()) return false;
+    *ld = row_stride(*t);
+    if (*ld < 0) return false;
+    *p = t->data_ptr();
+    const char *a = static_cast<const char*>(*p), *b = static_cast<const char*>(y.data_ptr());
+    const int64_t span_a = ((t->size(0) - 1) * *ld + t->size(1)) * 2, span_b = ((y.size(0) - 1) * ldy + y.size(1)) * 2;
+    return a + span_a <= b || b + span_b <= a || (a == b && (*ld == ldy || t->size(0) == 1));
+}
+
+// gemm_blocks_act(a, w, scale_a, scale_b, out_dtype, bias, act, residual, out)
+PyObject* gemm_blocks_act(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 9 || !THPDtype_Check(args[4]) || !PyLong_CheckExact(args[6])) DECLINE;
+    const at::ScalarType dt = reinterpret_cast<THPDtype*>(args[4])->scalar_type;
+    const at::Tensor* t[4];
+    for (int i = 0; i < 4; ++i) {
+        t[i] = plain(args[i]);
+        if (!t[i] || t[i]->device() != t[0]->device() || t[i]->dim() != 2) DECLINE;
+    }
+    const at::Tensor &a = *t[0], &w = *t[1], &sa = *t[2], &sw = *t[3];
+    const int64_t lda = row_stride(a), ldw = row_stride(w);
+    const void* bias;
+    if (!on_current(a) || a.scalar_type() != at::kFloat8_e4m3fn || w.scalar_type() != at::kFloat8_e4m3fn || lda < 0 || ldw < 0 ||
+        a.size(1) != w.size(1) || (dt != at::kBFloat16 && dt != at::kHalf) || sa.scalar_type() != at::kFloat ||
+        sw.scalar_type() != at::kFloat)
+        DECLINE;
+    const int64_t M = a.size(0), K = a.size(1), N = w.size(0), KB = (K + 127) / 128;
+    if (sa.size(0) != M || sa.size(1) != KB || sw.size(0) != (N + 127) / 128 || sw.size(1) != KB ||
+        !bias_of(args[5], N, dt, a.device(), &bias))
+        DECLINE;
+    at::Tensor y;
+    int64_t ldy, ldr;
+    const void* residual;
+    if (!output_of(args[8], M, N, dt, a.device(), &y, &ldy) || !residual_of(args[7], y, ldy, &residual, &ldr)) DECLINE;
+    const int act = (int)PyLong_AsLong(args[6]);
+    int rc;
+    {
+        pybind11::gil_scoped_release nogil;
+        rc = h3fp8_gemm_blocks_act(a.data_ptr(), lda, w.data_ptr(), ldw, static_cast<const float*>(sa.data_ptr()), axis(sa, 0),
+                                   axis(sa, 1), static_cast<const float*>(sw.data_ptr()), axis(sw, 0), axis(sw, 1), bias, act,
+                                   residual, ldr, y.data_ptr(), ldy, dtype_code(dt), M, N, K, stream_of(a.device()));
+    }
+    if (rc) return failed("h3fp8_gemm_blocks_act", rc);
+    return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
+// ---- a layer of experts ------------------------------------------------------------------------------------------------
+
+// moe_route(logits, k, scoring, renormalize, scale, bias)
+PyObject* moe_route(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 6 || !PyLong_CheckExact(args[1]) || !PyUnicode_CheckExact(args[2]) || !PyBool_Check(args[3]) || !PyFloat_CheckExact(args[4]))
+        DECLINE;
+    const at::Tensor* x = plain(args[0]);
+    if (!x || !on_current(*x)) DECLINE;
+    const int dt = dtype_code(x->scalar_type());
+    const int64_t ld = row_stride(*x);
+    const long k = PyLong_AsLong(args[1]);
+    if (k == -1 && PyErr_Occurred()) PyErr_Clear();
+    const bool sigmoid = PyUnicode_CompareWithASCIIString(args[2], "sigmoid") == 0;
+    if (dt < 0 || ld < 0 || k < 1 || k > 16 || k > x->size(1) || x->size(1) > 512 ||
+        (!sigmoid && PyUnicode_CompareWithASCIIString(args[2], "softmax") != 0))
+        DECLINE;
+    const int64_t T = x->size(0), E = x->size(1);
+    const at::Device dev = x->device();
+    const float* bias = nullptr;
+    if (args[5] != Py_None) {
+        const at::Tensor* b = plain(args[5]);
+        if (!b || !vector_of(*b, E, at::kFloat, dev)) DECLINE;
+        bias = static_cast<const float*>(b->data_ptr());
+    }
+    at::Tensor weights, experts, offsets, order, place, ws;
+    int rc;
+    {
+        pybind11::gil_scoped_release nogil;
+        const at::TensorOptions opt = at::TensorOptions().dtype(at::kInt).device(dev);
+        weights = empty(T, k, at::kFloat, dev);
+        experts = at::empty({T, k}, opt);
+        offsets = at::empty({E + 1}, opt);
+        order = at::empty({T * k}, opt);
+        place = at::empty({T, k}, opt);
+        const int64_t bytes = h3fp8_moe_route_workspace(T, E);
+        if (bytes) ws = at::empty({bytes / 4}, opt);
+        rc = h3fp8_moe_route(x->data_ptr(), ld, dt, T, E, (int)k, sigmoid, args[3] == Py_True, (float)PyFloat_AS_DOUBLE(args[4]), bias,
+                             static_cast<float*>(weights.data_ptr()), static_cast<int32_t*>(experts.data_ptr()),
+                             static_cast<int32_t*>(offsets.data_ptr()), static_cast<int32_t*>(order.data_ptr()),
+                             static_cast<int32_t*>(place.data_ptr()), bytes ? ws.data_ptr() : nullptr, bytes, stream_of(dev));
+    }
+    if (rc) return failed("h3fp8_moe_route", rc);
+    return tuple_of(std::move(weights), std::move(experts), std::move(offsets), std::move(order), std::move(place));
+    END_HANDLE_TH_ERRORS
+}
+
+// e4m3 weights [E, N, K] with contiguous rows, and their scales [E, ceil(N / 128), ceil(K / 128)].
+bool experts_of(PyObject* wa, PyObject* sa, const at::Device& dev, const at::Tensor** w, const at::Tensor** s) {
+    *w = plain(wa);
+    *s = plain(sa);
+    return *w && *s && (*w)->device() == dev && (*s)->device() == dev && (*w)->scalar_type() == at::kFloat8_e4m3fn &&
+           (*s)->scalar_type() == at::kFloat && (*w)->dim() == 3 && (*s)->dim() == 3 && (*w)->stride(2) == 1 &&
+           (*s)->size(0) == (*w)->size(0) && (*s)->size(1) == ((*w)->size(1) + 127) / 128 && (*s)->size(2) == ((*w)->size(2) + 127) / 128;
+}
+
+// moe_blocks(x, w_gate_up, scale_gate_up, w_down, scale_down, routing, residual, out)
+PyObject* moe_blocks(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 8 || !PyTuple_Check(args[5]) || PyTuple_GET_SIZE(args[5]) < 4) DECLINE;
+    const at::Tensor* x = plain(args[0]);
+    if (!x || !on_current(*x) || (x->scalar_type() != at::kBFloat16 && x->scalar_type() != at::kHalf)) DECLINE;
+    const int64_t ldx = row_stride(*x);
+    const at::Device dev = x->device();
+    const at::Tensor *w1, *s1, *w2, *s2, *r[4];
+    if (ldx < 0 || !experts_of(args[1], args[2], dev, &w1, &s1) || !experts_of(args[3], args[4], dev, &w2, &s2)) DECLINE;
+    const int64_t T = x->size(0), H = x->size(1), E = w2->size(0), F = w2->size(2);
+    if (w1->size(0) != E || w1->size(1) != 2 * F || w1->size(2) != H || w2->size(1) != H || T > 128 || E < 1 || H < 16 || F < 16) DECLINE;
+    for (int i = 0; i < 4; ++i) {
+        r[i] = plain(PyTuple_GET_ITEM(args[5], i));
+        if (!r[i] || r[i]->device() != dev || !r[i]->is_contiguous() || r[i]->scalar_type() != (i ? at::kInt : at::kFloat)) DECLINE;
+    }
+    if (r[0]->dim() != 2 || r[0]->size(0) != T) DECLINE;
+    const int64_t k = r[0]->size(1);
+    if (r[1]->sizes() != r[0]->sizes() || r[2]->dim() != 1 || r[2]->size(0) != E + 1 || r[3]->dim() != 1 || r[3]->size(0) != T * k) DECLINE;
+    at::Tensor y, ws;
+    int64_t ldy, ldr;
+    const void* residual;
+    if (!output_of(args[7], T, H, x->scalar_type(), dev, &y, &ldy) || !residual_of(args[6], y, ldy, &residual, &ldr)) DECLINE;
+    int rc;
+    {
+        pybind11::gil_scoped_release nogil;
+        const int64_t bytes = h3fp8_moe_blocks_workspace(T, k, F);
+        ws = at::empty({bytes}, at::TensorOptions().dtype(at::kByte).device(dev));
+        rc = h3fp8_moe_blocks(x->data_ptr(), ldx, dtype_code(x->scalar_type()), T, H, F, E, (int)k, w1->data_ptr(), axis(*w1, 0),
+                              w1->stride(1), static_cast<const float*>(s1->data_ptr()), axis(*s1, 0), axis(*s1, 1), axis(*s1, 2),
+                              w2->data_ptr(), axis(*w2, 0), w2->stride(1), static_cast<const float*>(s2->data_ptr()), axis(*s2, 0),
+                              axis(*s2, 1), axis(*s2, 2), static_cast<const float*>(r[0]->data_ptr()),
+                              static_cast<const int32_t*>(r[1]->data_ptr()), static_cast<const int32_t*>(r[2]->data_ptr()),
+                              static_cast<const int32_t*>(r[3]->data_ptr()), residual, ldr, y.data_ptr(), ldy, ws.data_ptr(), bytes,
+                              stream_of(dev));
+    }
+    if (rc) return failed("h3fp8_moe_blocks", rc);
+    return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
 // qk_norm_rope(q, k, q_weight, k_weight, rope_table, eps, positions, interleaved)
 PyObject* qk_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -552,6 +703,7 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyMethodDef kMethods[] = {METHOD(quant_rows), METHOD(scaled_mm), METHOD(gemm), METHOD(gemm_quant),
                           METHOD(gemm_swiglu_quant), METHOD(silu_mul_quant), METHOD(rms_quant), METHOD(gate_rms_quant), METHOD(quant_blocks),
                           METHOD(silu_mul_quant_blocks), METHOD(gemm_blocks), METHOD(grouped_gemm_blocks), METHOD(qk_norm_rope),
+                          METHOD(gemm_blocks_act), METHOD(moe_route), METHOD(moe_blocks),
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", "the common calls' host path", -1, kMethods,
                        nullptr, nullptr, nullptr, nullptr};

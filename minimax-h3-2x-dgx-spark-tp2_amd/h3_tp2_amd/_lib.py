@@ -73,6 +73,12 @@ _SIGS = {
                                    I64, P], I),
     "h3fp8_qk_norm_rope": ([P, I64, I64, P, I64, I64, I, I64, I, I, I, P, P, P, I64, I, I64, I, I, P, I64, I,
                             ctypes.c_float, P, I64, I64, P, I64, I64, P], I),
+    "h3fp8_gemm_blocks_act": ([P, I64, P, I64, P, I64, I64, P, I64, I64, P, I, P, I64, P, I64, I, I64, I64, I64, P], I),
+    "h3fp8_moe_route_workspace": ([I64, I64], I64),
+    "h3fp8_moe_route": ([P, I64, I, I64, I64, I, I, I, ctypes.c_float, P, P, P, P, P, P, P, I64, P], I),
+    "h3fp8_moe_blocks_workspace": ([I64, I64, I64], I64),
+    "h3fp8_moe_blocks": ([P, I64, I, I64, I64, I64, I64, I, P, I64, I64, P, I64, I64, I64, P, I64, I64, P, I64, I64, I64, P, P, P, P,
+                          P, I64, P, I64, P, I64, P], I),
     "h3fp8_selfcheck_e4m3": ([ctypes.POINTER(ctypes.c_uint64), ctypes.POINTER(ctypes.c_uint64)], I),
     "h3fp8_selfcheck_bf16": ([ctypes.POINTER(ctypes.c_uint64), ctypes.POINTER(ctypes.c_uint64)], I),
     "h3fp8_copy_silu_table": ([P, P], I),

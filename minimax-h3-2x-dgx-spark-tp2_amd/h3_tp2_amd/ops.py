@@ -10,6 +10,7 @@ row-major; weights as vLLM's ``b`` [K, N] whose transpose ``w = b.t()`` is a row
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple
 
 import torch
 
@@ -842,6 +843,165 @@ def grouped_gemm_blocks(a: torch.Tensor, w: torch.Tensor, scale_a: torch.Tensor,
     _call_on(a, "h3fp8_grouped_gemm_blocks", a.data_ptr(), lda, w.data_ptr(), w.stride(0) if E > 1 else 0, ldw,
              scale_a.data_ptr(), *_axes(scale_a), scale_b.data_ptr(), *_axes(scale_b), offsets.data_ptr(),
              offsets.element_size(), y.data_ptr(), _rows(y, "out"), _DT[out_dtype], M, N, K, E)
+    return y
+
+
+# ---- the block-scaled linear with an epilogue ------------------------------------------------------------------------
+
+ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "relu": 4}         # H3FP8_ACT_*
+
+
+def _residual(name: str, residual: torch.Tensor | None, shape: tuple, dtype: torch.dtype, out: torch.Tensor) -> int:
+    """The row stride of a residual that is ``out`` itself or lies apart from it (0: one row for all, or none)."""
+    if residual is None:
+        return 0
+    if not isinstance(residual, torch.Tensor) or residual.dtype != dtype or tuple(residual.shape) != shape:
+        raise ValueError(f"{name}: residual must be {dtype} {shape}, got {getattr(residual, 'dtype', type(residual).__name__)} "
+                         f"{tuple(getattr(residual, 'shape', ()))}")
+    if shape[1] > 1 and residual.stride(1) != 1:
+        raise ValueError(f"{name}: the rows of residual must be contiguous")
+    same = residual.data_ptr() == out.data_ptr() and _axes(residual) == _axes(out)
+    if not same and not _apart(residual.unsqueeze(1), out.unsqueeze(1)):
+        raise ValueError(f"{name}: out must be the residual itself or lie apart from it")
+    return residual.stride(0) if shape[0] > 1 else shape[1]
+
+
+def gemm_blocks_act(a: torch.Tensor, w: torch.Tensor, scale_a: torch.Tensor, scale_b: torch.Tensor,
+                    out_dtype: torch.dtype = torch.bfloat16, bias: torch.Tensor | None = None, activation: str | None = None,
+                    residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``gemm_blocks`` with an epilogue: y [M, N] = round(residual + act(the block-scaled product + bias)) in fp32, rounded once.
+    ``activation``: None, "silu", "gelu" (by erf), "gelu_tanh" or "relu"; ``residual`` [M, N] in the output's type (any row
+    stride, 0 too); ``out`` may be the residual itself and otherwise lies apart from it.  bias and residual 16-byte aligned."""
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"gemm_blocks_act: activation must be one of {tuple(ACTIVATIONS)}, got {activation!r}")
+    act = ACTIVATIONS[activation]
+    if _host is not None:
+        y = _host.gemm_blocks_act(a, w, scale_a, scale_b, out_dtype, bias, act, residual, out)
+        if y is not None:
+            return y
+    if a.dtype != E4M3 or w.dtype != E4M3:
+        raise ValueError("gemm_blocks_act: a and w must be float8_e4m3fn")
+    if a.dim() != 2 or w.dim() != 2 or a.shape[1] != w.shape[1]:
+        raise ValueError(f"gemm_blocks_act: shape mismatch: a {tuple(a.shape)}, w {tuple(w.shape)} (w is [N, K])")
+    (M, K), N = a.shape, w.shape[0]
+    _block_scale(scale_a, "scale_a", (M, _blocks(K)))
+    _block_scale(scale_b, "scale_b", (_blocks(N), _blocks(K)))
+    if bias is not None and (bias.dim() != 1 or bias.numel() != N or bias.dtype != out_dtype or not bias.is_contiguous()):
+        raise ValueError("gemm_blocks_act: bias must be a contiguous [N] vector in the output dtype")
+    lda, ldw = _rows(a, "a"), _rows(w, "w")
+    _same_device("gemm_blocks_act", a, w, scale_a, scale_b, bias, residual)
+    y = _block_out("gemm_blocks_act", a, M, N, out_dtype, out)
+    ldr = _residual("gemm_blocks_act", residual, (M, N), out_dtype, y)
+    _call_on(a, "h3fp8_gemm_blocks_act", a.data_ptr(), lda, w.data_ptr(), ldw, scale_a.data_ptr(), *_axes(scale_a),
+             scale_b.data_ptr(), *_axes(scale_b), bias.data_ptr() if bias is not None else None, act,
+             residual.data_ptr() if residual is not None else None, ldr, y.data_ptr(), _rows(y, "out"), _DT[out_dtype], M, N, K)
+    return y
+
+
+# ---- a layer of experts ---------------------------------------------------------------------------------------------
+
+MOE_MAX_TOKENS = 128            # of moe_blocks
+MOE_MAX_EXPERTS = 512
+MOE_MAX_CHOICES = 16
+
+
+class Routing(NamedTuple):
+    """The tokens' experts (``moe_route``).  A pair is (token, choice), number token * k + choice."""
+    weights: torch.Tensor       # [T, k] fp32
+    experts: torch.Tensor       # [T, k] int32, best first; -1 (weight 0) where no expert is left
+    offsets: torch.Tensor       # [E + 1] int32: expert e has the sorted rows offsets[e] .. offsets[e + 1] - 1
+    order: torch.Tensor         # [T k] int32: the pair of each sorted row; pairs without an expert last
+    place: torch.Tensor         # [T, k] int32: the sorted row of each pair
+
+
+def moe_route(logits: torch.Tensor, k: int, scoring: str = "softmax", renormalize: bool = True, scale: float = 1.0,
+              bias: torch.Tensor | None = None) -> Routing:
+    """The router of an expert layer: the ``k`` best experts of every row of ``logits`` [T, E] (bf16 / fp16 / fp32) and the order
+    of the (token, choice) pairs by expert, all on the GPU (no synchronisation, capturable).  The weights are the chosen experts'
+    scores ("softmax" over the experts, or "sigmoid"), over their sum with ``renormalize``, times ``scale``.  Experts are chosen
+    by their logits, the lower index first among equals, or with ``bias`` ([E] fp32) by score + bias in 64 bits.  An expert at -inf
+    or NaN is never chosen; a NaN among a token's logits makes its weights NaN.  ``offsets`` are what ``grouped_gemm_blocks`` takes
+    for the rows ``order // k``; y[place] are the pairs' results again.  At most 512 experts, 16 choices."""
+    if _host is not None and (r := _host.moe_route(logits, k, scoring, renormalize, scale, bias)) is not None:
+        return Routing(*r)
+    if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.dtype not in _DT:
+        raise ValueError("moe_route takes bf16, fp16 or fp32 logits [T, E]")
+    T, E = logits.shape
+    if not 1 <= E <= MOE_MAX_EXPERTS or not 1 <= k <= min(E, MOE_MAX_CHOICES):
+        raise ValueError(f"moe_route: k = {k} of {E} experts (1 to {MOE_MAX_CHOICES} of 1 to {MOE_MAX_EXPERTS})")
+    if scoring not in ("softmax", "sigmoid"):
+        raise ValueError(f'moe_route: scoring must be "softmax" or "sigmoid", got {scoring!r}')
+    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (E,) or not bias.is_contiguous()):
+        raise ValueError(f"moe_route: bias must be a contiguous float32 [{E}] vector")
+    ld = _rows(logits, "logits")
+    _same_device("moe_route", logits, bias)
+
+    def new(*shape, dtype=torch.int32):  # noqa: ANN002,ANN202
+        return torch.empty(shape, device=logits.device, dtype=dtype)
+    r = Routing(new(T, k, dtype=torch.float32), new(T, k), new(E + 1), new(T * k), new(T, k))
+    ws_bytes = _lib.load().h3fp8_moe_route_workspace(T, E)
+    ws = new(ws_bytes // 4)
+    _call_on(logits, "h3fp8_moe_route", logits.data_ptr(), ld, _DT[logits.dtype], T, E, k, int(scoring == "sigmoid"),
+             int(bool(renormalize)), float(scale), bias.data_ptr() if bias is not None else None, r.weights.data_ptr(),
+             r.experts.data_ptr(), r.offsets.data_ptr(), r.order.data_ptr(), r.place.data_ptr(), ws.data_ptr(), ws_bytes)
+    return r
+
+
+def _expert_weight(name: str, w: torch.Tensor, shape: tuple) -> int:
+    """The row stride of e4m3 expert weights [E, N, K] whose rows are contiguous."""
+    if not isinstance(w, torch.Tensor) or w.dtype != E4M3 or w.dim() != 3 or tuple(w.shape) != shape:
+        raise ValueError(f"{name} must be float8_e4m3fn {shape}, got {getattr(w, 'dtype', type(w).__name__)} "
+                         f"{tuple(getattr(w, 'shape', ()))}")
+    if w.stride(2) != 1:
+        raise ValueError(f"{name}: its rows must be contiguous")
+    return w.stride(1)
+
+
+def moe_blocks(x: torch.Tensor, w_gate_up: torch.Tensor, scale_gate_up: torch.Tensor, w_down: torch.Tensor,
+               scale_down: torch.Tensor, routing: Routing, residual: torch.Tensor | None = None,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """A whole layer of block-scaled experts for a few tokens (at most 128), in two launches: y [T, H] = residual + the sum over a
+    token's choices of weight * w_down[e] (silu(gate) * up), gate | up = w_gate_up[e] x.  ``x`` bf16 / fp16 [T, H], not
+    quantised; ``w_gate_up`` e4m3 [E, 2F, H] and ``w_down`` [E, H, F] with one scale per 128 x 128 (``quant_blocks(rows=128)``; any
+    strides); ``routing`` as ``moe_route`` returns it.  fp32 throughout, rounded once.  ``out`` may be the residual itself and
+    otherwise lies apart from it.  More tokens: ``quant_blocks``, ``grouped_gemm_blocks`` and ``silu_mul_quant_blocks``."""
+    if _host is not None:
+        y = _host.moe_blocks(x, w_gate_up, scale_gate_up, w_down, scale_down, routing, residual, out)
+        if y is not None:
+            return y
+    if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("moe_blocks takes a bf16 or fp16 [T, H] tensor")
+    T, H = x.shape
+    if T > MOE_MAX_TOKENS:
+        raise ValueError(f"moe_blocks takes at most {MOE_MAX_TOKENS} tokens, got {T}: more go by quant_blocks and grouped_gemm_blocks")
+    if not isinstance(w_down, torch.Tensor) or w_down.dim() != 3:
+        raise ValueError("w_down must be float8_e4m3fn [E, H, F]")
+    E, _, F = w_down.shape
+    if H % 16 or F % 16 or H == 0 or F == 0:
+        raise ValueError(f"moe_blocks: H = {H} and F = {F} must be positive multiples of 16")
+    ld1 = _expert_weight("w_gate_up", w_gate_up, (E, 2 * F, H))
+    ld2 = _expert_weight("w_down", w_down, (E, H, F))
+    _block_scale(scale_gate_up, "scale_gate_up", (E, _blocks(2 * F), _blocks(H)))
+    _block_scale(scale_down, "scale_down", (E, _blocks(H), _blocks(F)))
+    weights, experts, offsets, order = routing[:4]
+    if weights.dim() != 2 or not 1 <= weights.shape[1] <= min(E, MOE_MAX_CHOICES) or not 1 <= E <= MOE_MAX_EXPERTS:
+        raise ValueError(f"moe_blocks: routing weights {tuple(weights.shape)} of {E} experts (1 to {MOE_MAX_CHOICES} choices of 1 to "
+                         f"{MOE_MAX_EXPERTS})")
+    k = weights.shape[1]
+    for t, n, shape, dt in ((weights, "weights", (T, k), torch.float32), (experts, "experts", (T, k), torch.int32),
+                            (offsets, "offsets", (E + 1,), torch.int32), (order, "order", (T * k,), torch.int32)):
+        check_buffer(t, f"routing.{n}", shape, dt, x.device, contiguous=True)
+    ldx = _rows(x, "x")
+    _same_device("moe_blocks", x, w_gate_up, scale_gate_up, w_down, scale_down, residual)
+    y = _block_out("moe_blocks", x, T, H, x.dtype, out)
+    ldr = _residual("moe_blocks", residual, (T, H), x.dtype, y)
+    ws_bytes = _lib.load().h3fp8_moe_blocks_workspace(T, k, F)
+    ws = torch.empty(ws_bytes, device=x.device, dtype=torch.uint8)
+    _call_on(x, "h3fp8_moe_blocks", x.data_ptr(), ldx, _DT[x.dtype], T, H, F, E, k, w_gate_up.data_ptr(),
+             w_gate_up.stride(0) if E > 1 else 0, ld1, scale_gate_up.data_ptr(), *_axes(scale_gate_up), w_down.data_ptr(),
+             w_down.stride(0) if E > 1 else 0, ld2, scale_down.data_ptr(), *_axes(scale_down), weights.data_ptr(),
+             experts.data_ptr(), offsets.data_ptr(), order.data_ptr(), residual.data_ptr() if residual is not None else None, ldr,
+             y.data_ptr(), _rows(y, "out"), ws.data_ptr(), ws_bytes)
     return y
 
 
