@@ -352,7 +352,7 @@ int h3fp8_moe_route(const void* logits, int64_t ld, int dtype, int64_t T, int64_
  * H, F multiples of 16; x and weights 16-byte aligned, row strides of x multiples of 8, of the weights of 16, of y and the
  * residual of 4 (8-byte aligned).  workspace: h3fp8_moe_blocks_workspace bytes of device memory, 16-byte aligned.
  */
-int64_t h3fp8_moe_blocks_workspace(int64_t T, int64_t k, int64_t F);
+int64_t h3fp8_moe_blocks_workspace(int64_t T, int64_t k, int64_t H, int64_t F, int64_t E);
 int h3fp8_moe_blocks(const void* x, int64_t ldx, int dtype, int64_t T, int64_t H, int64_t F, int64_t E, int k, const void* w1,
                      int64_t w1_e, int64_t ld1, const float* s1, int64_t s1_e, int64_t s1_n, int64_t s1_k, const void* w2,
                      int64_t w2_e, int64_t ld2, const float* s2, int64_t s2_e, int64_t s2_n, int64_t s2_k, const float* weights,

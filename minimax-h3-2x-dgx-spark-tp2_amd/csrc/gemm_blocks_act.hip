@@ -8,9 +8,8 @@
 // in the same piece, so that the output may be the residual itself.
 //
 // The activations take the hardware's exponential and reciprocal (1 ulp each; the exponent's argument, up to 64 in size where
-// the result counts, is rounded to 2^-18): relative errors below 2^-17, a 64th of the smallest rounding behind them.
-//   sigmoid(z): t = 2^(64 - |z| log2 e), r = 1 / (1 + 2^-64 t); r, or r t 2^-64 for z < 0, so that nothing is
-//     subnormal before the last product (the hardware's exponential and reciprocal return 0 for a subnormal result)
+// the result counts, is rounded to 2^-18): relative errors below 2^-17, a 64th of the smallest rounding behind them.  sigmoid:
+// gemm_core.h.
 //   silu y sigmoid(y); gelu_tanh 0.5 y (1 + tanh u) = y sigmoid(2u), u = sqrt(2 / pi) (y + 0.044715 y^3)
 //   gelu y Phi(y): with a = |y|, Q(a) = erfc(a / sqrt 2) / 2 = 2^(-a^2 log2 e / 2) p(1 / (1 + 0.36 a)), p of degree 7 without
 //     a constant, fitted to Q's other factor by least squares with weights moved towards the largest relative error (1e-6 on
@@ -26,15 +25,6 @@ struct ActParams {
     int64_t ldr;
     int act;                    // H3FP8_ACT_*
 };
-
-constexpr float LOG2E = 1.4426950408889634f;
-
-// y sigmoid(z)
-__device__ __forceinline__ float times_sigmoid(float y, float z) {
-    const float t = __builtin_amdgcn_exp2f(__builtin_fmaf(-__builtin_fabsf(z), LOG2E, 64.0f));
-    const float yr = y * __builtin_amdgcn_rcpf(__builtin_fmaf(t, 0x1p-64f, 1.0f));
-    return z < 0.0f ? yr * t * 0x1p-64f : yr;
-}
 
 __device__ __forceinline__ float gelu_tanh(float y) {
     const float u = y * __builtin_fmaf(0.044715f * y, y, 1.0f);

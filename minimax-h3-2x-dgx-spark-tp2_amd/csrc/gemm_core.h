@@ -202,6 +202,15 @@ __device__ __forceinline__ void accumulators_ready(v16f (&acc)[NI][NJ]) {
         }
 }
 
+// y sigmoid(z) by the hardware's exponential and reciprocal: with t = 2^(64 - |z| log2 e) and r = 1 / (1 + 2^-64 t), y r, or
+// y r t 2^-64 for z < 0, so that nothing is subnormal before the last product (both instructions return 0 for a subnormal result).
+constexpr float LOG2E = 1.4426950408889634f;
+__device__ __forceinline__ float times_sigmoid(float y, float z) {
+    const float t = __builtin_amdgcn_exp2f(__builtin_fmaf(-__builtin_fabsf(z), LOG2E, 64.0f));
+    const float yr = y * __builtin_amdgcn_rcpf(__builtin_fmaf(t, 0x1p-64f, 1.0f));
+    return z < 0.0f ? yr * t * 0x1p-64f : yr;
+}
+
 // A +0 the compiler cannot see through, made once per epilogue: x + z turns -0 into +0 (round to nearest) and leaves
 // every other value (NaN included) unchanged, and the add is not folded away.
 __device__ __forceinline__ float opaque_zero() {

@@ -635,7 +635,7 @@ PyObject* moe_blocks(PyObject*, PyObject* const* args, Py_ssize_t n) {
     int rc;
     {
         pybind11::gil_scoped_release nogil;
-        const int64_t bytes = h3fp8_moe_blocks_workspace(T, k, F);
+        const int64_t bytes = h3fp8_moe_blocks_workspace(T, k, H, F, E);
         ws = at::empty({bytes}, at::TensorOptions().dtype(at::kByte).device(dev));
         rc = h3fp8_moe_blocks(x->data_ptr(), ldx, dtype_code(x->scalar_type()), T, H, F, E, (int)k, w1->data_ptr(), axis(*w1, 0),
                               w1->stride(1), static_cast<const float*>(s1->data_ptr()), axis(*s1, 0), axis(*s1, 1), axis(*s1, 2),

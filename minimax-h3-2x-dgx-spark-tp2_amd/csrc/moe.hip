@@ -47,6 +47,7 @@ struct MoeParams {
     uint16_t* y;                // [T, H]
     int64_t ldy;
     char* h;                    // [T k, F] pairs of bf16: 16 values, then what they leave
+    float* z;                   // [T k, H]: the pairs' results (more rows per expert)
     int T, E, k, H, F;
     int fp16;
 };
@@ -108,178 +109,254 @@ __device__ __forceinline__ void sums_ready(v4f (&b)[A][B]) {
         for (int j = 0; j < B; ++j) asm volatile("" : "+v"(b[i][j]));
 }
 
-// The slot-th expert that has pairs, and its pairs' places.
-__device__ __forceinline__ bool find_expert(const MoeParams& p, int slot, int lane, int& e, int& r0, int& r1) {
-    for (int e0 = 0; e0 < p.E; e0 += 64) {
-        int lo = 0, hi = 0;
-        if (e0 + lane < p.E) lo = offset_at(p, e0 + lane), hi = offset_at(p, e0 + lane + 1);
-        const uint64_t has = __ballot(hi > lo);
-        const int n = __popcll(has);
-        if (slot < n) {
-            const uint64_t at = __ballot(hi > lo && __popcll(has & ((1ull << lane) - 1)) == slot);
-            const int f = __builtin_ctzll(at);
-            e = e0 + f;
-            r0 = __builtin_amdgcn_readlane(lo, f);
-            r1 = __builtin_amdgcn_readlane(hi, f);
-            return true;
-        }
-        slot -= n;
+__device__ __forceinline__ int wave_prefix(int v) {       // inclusive
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+    return v;
+}
+
+// ---- the routing, in LDS ------------------------------------------------------------------------------------------------
+//
+// All that a workgroup needs of the routing is loaded at once, and looked up from then on: one trip to memory before the first
+// weights can be asked for instead of one per step (offsets, order, experts).
+
+struct Block { int e, r0, n; };                           // n sorted rows from r0 on, of expert e
+
+struct Routed {
+    int* count;                                           // of blocks
+    int* pair;                                            // [P] of a sorted row
+    float* weight;                                        // [P] of a sorted row: of all its token's choices of its expert (the
+                                                          // second of two equal ones has the same, and is not read)
+    Block* blocks;                                        // the experts' rows in blocks of at most ROWS
+    int* experts;                                         // [P] of a pair
+    float* weights;                                       // [P]
+};
+
+template <int ROWS>
+constexpr int max_blocks(int E, int P) { return (E < P ? E : P) + P / ROWS; }
+
+template <int ROWS>
+constexpr size_t routed_bytes(int E, int P) { return (size_t)P * 16 + (size_t)max_blocks<ROWS>(E, P) * sizeof(Block) + 16; }
+
+// By all threads, with barriers.
+template <int ROWS>
+__device__ __forceinline__ Routed load_routing(const MoeParams& p, char* lds, int threads) {
+    const int P = p.T * p.k, lane = threadIdx.x & 63, cap = max_blocks<ROWS>(p.E, P);
+    Routed r;
+    r.count = reinterpret_cast<int*>(lds);
+    r.pair = r.count + 4;
+    r.weight = reinterpret_cast<float*>(r.pair + P);
+    r.experts = reinterpret_cast<int*>(r.weight + P);
+    r.weights = reinterpret_cast<float*>(r.experts + P);
+    r.blocks = reinterpret_cast<Block*>(r.weights + P);
+    for (int i = threadIdx.x; i < P; i += threads) {
+        const int o = p.order[i], e = p.experts[i];
+        const float w = p.weights[i];
+        r.pair[i] = min(max(o, 0), P - 1);                // whatever it holds, no row outside the tokens is read
+        r.experts[i] = e;
+        r.weights[i] = w;
     }
-    return false;
+    if (threadIdx.x < 64) {
+        int blocks = 0;
+        for (int e0 = 0; e0 < p.E; e0 += 64) {
+            int lo = 0, hi = 0;
+            if (e0 + lane < p.E) lo = offset_at(p, e0 + lane), hi = offset_at(p, e0 + lane + 1);
+            const int n = max(hi - lo, 0), nb = (n + ROWS - 1) / ROWS, at = blocks + wave_prefix(nb) - nb;
+            for (int i = 0; i < nb; ++i)                  // (offsets that are not ascending may name more blocks than there are pairs)
+                if (at + i < cap) r.blocks[at + i] = Block{e0 + lane, lo + i * ROWS, min(ROWS, n - i * ROWS)};
+            blocks = __builtin_amdgcn_readlane(at + nb, 63);
+        }
+        if (lane == 0) *r.count = min(blocks, cap);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < P; i += threads) {
+        const int e = r.experts[r.pair[i]];
+        float w = 0.0f;
+        for (int j = 0, q = r.pair[i] / p.k * p.k; j < p.k; ++j) w += r.experts[q + j] == e ? r.weights[q + j] : 0.0f;
+        r.weight[i] = w;
+    }
+    __syncthreads();
+    return r;
+}
+
+// An item of a persistent workgroup: a block of rows and a tile of output channels.
+struct Item {
+    int blk, tile;
+
+    __device__ __forceinline__ void next(int step_blk, int step_tile, int tiles) {
+        blk += step_blk;
+        tile += step_tile;
+        if (tile >= tiles) tile -= tiles, ++blk;
+    }
+};
+
+// silu(g) u w of 4 consecutive channels f .. f + 3 of a pair, as two bf16 numbers each.
+__device__ __forceinline__ void store_h(const MoeParams& p, int pair, int f, float weight, const v4f& gate, const v4f& up) {
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const float h = times_sigmoid(gate[r], gate[r]) * up[r] * weight;
+        hi[r] = bf16_rne(h);
+        const float rest = h - bf16_to_f32(hi[r]);
+        lo[r] = (hi[r] & 0x7f80u) == 0x7f80u ? 0u : bf16_rne(rest);       // infinite or NaN: nothing is left
+    }
+    char* at = p.h + (int64_t)pair * p.F * 4 + f / 16 * 64 + f % 16 * 2;
+    *reinterpret_cast<uint2*>(at) = uint2{hi[0] | (hi[1] << 16), hi[2] | (hi[3] << 16)};
+    *reinterpret_cast<uint2*>(at + 32) = uint2{lo[0] | (lo[1] << 16), lo[2] | (lo[3] << 16)};
+}
+
+// 4 consecutive channels n .. n + 3 of a token, with the residual.
+__device__ __forceinline__ void store_y(const MoeParams& p, int t, int n, v4f v) {
+    if (p.residual) {
+        const uint2 r = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p.residual) + t * p.ldr + n);
+        const uint32_t b[4] = {r.x & 0xffffu, r.x >> 16, r.y & 0xffffu, r.y >> 16};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] += p.fp16 ? fp16_to_f32(b[q]) : bf16_to_f32(b[q]);
+    }
+    const uint2 o = p.fp16 ? uint2{fp16_rne(v[0]) | (fp16_rne(v[1]) << 16), fp16_rne(v[2]) | (fp16_rne(v[3]) << 16)}
+                           : uint2{cvt_bf16x2(v[0], v[1]), cvt_bf16x2(v[2], v[3])};
+    *reinterpret_cast<uint2*>(p.y + t * p.ldy + n) = o;
 }
 
 // ---- kernel 1 ---------------------------------------------------------------------------------------------------------
+//
+// An item is a block of up to 16 rows of one expert and 16 gate rows; the workgroup's 8 waves share out the blocks of K.  Two
+// workgroups per CU, persistent: a wave's loads run D of its units (blocks of K) ahead, across items.
 
-// NI: blocks of 16 gate rows; NT: blocks of 16 tokens; D: k-blocks in flight per wave.
-template <bool FP16, int NI, int NT, int D>
-__global__ void __launch_bounds__(WAVES * 64) moe_up_kernel(MoeParams p, int tiles) {
-    constexpr int ITEMS = NI * NT * 64;                   // results of 4 channels x 1 token
-    __shared__ v4f part[WAVES][2 * NI * NT][64];
-    __shared__ int s_pair[16 * NT];
-    __shared__ float s_weight[16 * NT];
+template <bool FP16, int D>
+__global__ void __launch_bounds__(WAVES * 64, 4) moe_up_kernel(MoeParams p, int tiles, int step_blk, int step_tile) {
+    extern __shared__ __attribute__((aligned(16))) char up_lds[];
+    __shared__ v4f part[2][WAVES][2][64];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int slot = (int)blockIdx.x / tiles, f0 = ((int)blockIdx.x - slot * tiles) * 16 * NI;
-    int e, r0, r1;
-    if (!find_expert(p, slot, lane, e, r0, r1)) return;
     const int c = lane & 15, g = lane >> 4;
-    const int kb = (p.H + BK - 1) / BK, frows = min(16 * NI, p.F - f0);
-    const uint32_t wbytes = (uint32_t)((frows - 1) * p.ld1 + p.H);
-    const uint8_t* wg = p.w1 + e * p.w1_e + (int64_t)f0 * p.ld1;
-    const __amdgpu_buffer_rsrc_t rg = make_rsrc(wg, wbytes), ru = make_rsrc(wg + (int64_t)p.F * p.ld1, wbytes);
-    // in the vector memory's order of loads: a scalar load's wait is for all that are under way
-    const __amdgpu_buffer_rsrc_t rs = make_rsrc(p.s1 + e * p.s1_e, 0x7fffffffu);
+    const Routed R = load_routing<16>(p, up_lds, WAVES * 64);
+    const int blocks = __builtin_amdgcn_readfirstlane(*R.count);
+    const int kb = (p.H + BK - 1) / BK, rounds = (kb + D * WAVES - 1) / (D * WAVES);
     const __amdgpu_buffer_rsrc_t rx = make_rsrc(p.x, (uint32_t)(((p.T - 1) * p.ldx + p.H) * 2));
-    uint32_t vw[NI];
+    const __amdgpu_buffer_rsrc_t rs = make_rsrc(p.s1, 0x7fffffffu);
+    // what the next loads need: buffers, lane offsets of the weight row and the token, offsets of the scales, the block
+    __amdgpu_buffer_rsrc_t rg, ru;
+    uint32_t vw, vx, sg, su;
+    int lb, lend;                                         // (past the last item no block is there)
+    auto aim = [&](const Item& it) {
+        const bool live = it.blk < blocks;
+        const Block& B = R.blocks[live ? it.blk : 0];
+        const int e = __builtin_amdgcn_readfirstlane(B.e), r0 = __builtin_amdgcn_readfirstlane(B.r0), n = __builtin_amdgcn_readfirstlane(B.n);
+        const int f0 = it.tile * 16;
+        const uint32_t bytes = live ? (uint32_t)(15 * p.ld1 + p.H) : 0u;
+        const uint8_t* w = p.w1 + e * p.w1_e + f0 * p.ld1;
+        rg = make_rsrc(w, bytes);
+        ru = make_rsrc(w + p.F * p.ld1, bytes);
+        vx = live && c < n ? (uint32_t)(R.pair[r0 + min(c, n - 1)] / p.k) * (uint32_t)(p.ldx * 2) + 32u * g : OOB;
+        sg = (uint32_t)(e * p.s1_e + f0 / BK * p.s1_n) * 4u;
+        su = (uint32_t)(e * p.s1_e + (p.F + f0) / BK * p.s1_n) * 4u;
+        lb = wave;
+        lend = live ? kb : 0;
+    };
+    vw = (uint32_t)(c * p.ld1) + 16u * g;
+    v4u w[D][2][2], x[D][2][2];
+    float sc[D][2];
+    // always the same loads, past the last block of nothing, so that the count of those under way is known
+    auto load = [&](int d) {
+        const int b = lb + d * WAVES, at = b < lend ? b * BK : 0, left = b < lend ? p.H - at : 0;
 #pragma unroll
-    for (int i = 0; i < NI; ++i) vw[i] = 16 * i + c < frows ? (uint32_t)((16 * i + c) * p.ld1) + 16u * g : OOB;
-    for (int rt = r0; rt < r1; rt += 16 * NT) {
-        uint32_t vx[NT];
+        for (int s = 0; s < 2; ++s) {
+            const bool in = 64 * s + 16 * g < left;
+            w[d][0][s] = load16<true>(rg, (in ? vw : OOB) + 64 * s, at);
+            w[d][1][s] = load16<true>(ru, (in ? vw : OOB) + 64 * s, at);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            const int r = rt + 16 * j + c;
-            const int pair = r < r1 ? p.order[r] : -1;
-            vx[j] = pair >= 0 && pair < p.T * p.k ? (uint32_t)(pair / p.k * p.ldx * 2) + 32u * g : OOB;
+            for (int q = 0; q < 2; ++q) x[d][s][q] = load16<false>(rx, (in ? vx : OOB) + 128 * s + 16 * q, 2 * at);
         }
-        if (threadIdx.x < 16 * NT) {                      // the pair of each column and its weight (of every choice of this expert)
-            const int r = rt + (int)threadIdx.x;
-            int pair = r < r1 ? p.order[r] : -1;
-            float w = 0.0f;
-            if (pair < 0 || pair >= p.T * p.k) pair = -1;
-            else
-                for (int j = 0, q = pair / p.k * p.k; j < p.k; ++j) w += p.experts[q + j] == e ? p.weights[q + j] : 0.0f;
-            s_pair[threadIdx.x] = pair;
-            s_weight[threadIdx.x] = w;
-        }
-        v4u w[D][2 * NI][2], x[D][NT][2][2];
-        float sc[D][2][NI];
-        // always the same loads, past the last block of nothing, so that the count of those under way is known
-        auto load = [&](int d, int b) {
-            const int at = b < kb ? b * BK : 0;
+        const uint32_t sb = (uint32_t)(min(b, kb - 1) * p.s1_k) * 4u;
+        sc[d][0] = load4(rs, sg + sb);
+        sc[d][1] = load4(rs, su + sb);
+        __builtin_amdgcn_sched_barrier(0);                // in this order: the waits count them
+    };
+    Item it{(int)blockIdx.x / tiles, (int)blockIdx.x % tiles}, nx = it;
+    if (it.blk >= blocks) return;
+    aim(it);
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const bool in = b * BK + 64 * s + 16 * g < p.H;
-#pragma unroll
-                for (int i = 0; i < NI; ++i) {
-                    w[d][i][s] = load16<true>(rg, (in ? vw[i] : OOB) + 64 * s, at);
-                    w[d][NI + i][s] = load16<true>(ru, (in ? vw[i] : OOB) + 64 * s, at);
-                }
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) x[d][j][s][q] = load16<false>(rx, (in ? vx[j] : OOB) + 128 * s + 16 * q, 2 * at);
-            }
-#pragma unroll
-            for (int i = 0; i < NI; ++i) {
-                const int n = f0 + 16 * i < p.F ? f0 + 16 * i : f0;
-                const int bb = min(b, kb - 1);
-                sc[d][0][i] = load4(rs, (uint32_t)(n / BK * p.s1_n + bb * p.s1_k) * 4u);
-                sc[d][1][i] = load4(rs, (uint32_t)((p.F + n) / BK * p.s1_n + bb * p.s1_k) * 4u);
-            }
-            __builtin_amdgcn_sched_barrier(0);            // in this order: the waits count them
-        };
-        v4f acc[2 * NI][NT];
-#pragma unroll
-        for (int i = 0; i < 2 * NI; ++i)
-#pragma unroll
-            for (int j = 0; j < NT; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int d = 0; d < D; ++d) load(d, wave + d * WAVES);
-        for (int b0 = wave; b0 < kb; b0 += D * WAVES) {
+    for (int d = 0; d < D; ++d) load(d);
+    for (int buf = 0;; buf ^= 1) {
+        v4f acc[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
+        for (int r = 0; r < rounds; ++r) {
+            if (r + 1 < rounds) lb += D * WAVES;
+            else nx.next(step_blk, step_tile, tiles), aim(nx);
 #pragma unroll
             for (int d = 0; d < D; ++d) {
-                const int b = b0 + d * WAVES;
-                if (b < kb) {
-                    v4f sum[2 * NI][NT];
+                v4f sum[2][1];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q)           // 32 of the block's k each
+                for (int q = 0; q < 4; ++q)               // 32 of the block's k each
 #pragma unroll
-                        for (int i = 0; i < 2 * NI; ++i)
+                    for (int i = 0; i < 2; ++i) {
+                        const v4u& a = w[d][i][q >> 1];
+                        if (q == 0) mfma<FP16, true>(sum[i][0], a[0], a[1], x[d][0][0]);
+                        else mfma<FP16, false>(sum[i][0], a[2 * (q & 1)], a[2 * (q & 1) + 1], x[d][q >> 1][q & 1]);
+                    }
+                sums_ready(sum);
 #pragma unroll
-                            for (int j = 0; j < NT; ++j) {
-                                const v4u& a = w[d][i][q >> 1];
-                                if (q == 0) mfma<FP16, true>(sum[i][j], a[0], a[1], x[d][j][0][0]);
-                                else mfma<FP16, false>(sum[i][j], a[2 * (q & 1)], a[2 * (q & 1) + 1], x[d][j][q >> 1][q & 1]);
-                            }
-                    sums_ready(sum);
+                for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int i = 0; i < 2 * NI; ++i)
-#pragma unroll
-                        for (int j = 0; j < NT; ++j)
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(sum[i][j][r], sc[d][i / NI][i % NI], acc[i][j][r]);
-                }
-                load(d, b + D * WAVES);
+                    for (int k = 0; k < 4; ++k) acc[i][k] = __builtin_fmaf(sum[i][0][k], sc[d][i], acc[i][k]);
+                __builtin_amdgcn_sched_barrier(0);
+                load(d);
             }
         }
+        // join the waves' sums; the other buffer is the next item's
 #pragma unroll
-        for (int i = 0; i < 2 * NI; ++i)
-#pragma unroll
-            for (int j = 0; j < NT; ++j) part[wave][i * NT + j][lane] = acc[i][j];
-        __syncthreads();
-        for (int it = threadIdx.x; it < ITEMS; it += WAVES * 64) {
-            const int l = it & 63, ij = it >> 6, col = ij % NT * 16 + (l & 15), f = f0 + ij / NT * 16 + 4 * (l >> 4);
-            v4f gate = part[0][ij][l], up = part[0][NI * NT + ij][l];
+        for (int i = 0; i < 2; ++i) part[buf][wave][i][lane] = acc[i];
+        wait_lgkm0();
+        barrier_nofence();
+        if (wave == (it.tile & (WAVES - 1))) {
+            v4f gate = part[buf][0][0][lane], up = part[buf][0][1][lane];
 #pragma unroll
             for (int v = 1; v < WAVES; ++v) {
-                gate += part[v][ij][l];
-                up += part[v][NI * NT + ij][l];
+                gate += part[buf][v][0][lane];
+                up += part[buf][v][1][lane];
+                asm volatile("" : "+v"(gate), "+v"(up)::"memory");        // not all of them in registers at once
             }
-            const int pair = s_pair[col];
-            if (pair >= 0 && f < p.F) {
-                uint32_t hi[4], lo[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float h = gate[r] / (1.0f + expf(-gate[r])) * up[r] * s_weight[col];
-                    hi[r] = bf16_rne(h);
-                    const float rest = h - bf16_to_f32(hi[r]);
-                    lo[r] = (hi[r] & 0x7f80u) == 0x7f80u ? 0u : bf16_rne(rest);     // infinite or NaN: nothing is left
-                }
-                char* at = p.h + (int64_t)pair * p.F * 4 + f / 16 * 64 + f % 16 * 2;
-                *reinterpret_cast<uint2*>(at) = uint2{hi[0] | (hi[1] << 16), hi[2] | (hi[3] << 16)};
-                *reinterpret_cast<uint2*>(at + 32) = uint2{lo[0] | (lo[1] << 16), lo[2] | (lo[3] << 16)};
-            }
+            const Block& B = R.blocks[it.blk];
+            if (c < B.n) store_h(p, R.pair[B.r0 + c], it.tile * 16 + 4 * g, R.weight[B.r0 + c], gate, up);
         }
-        __syncthreads();
+        it.next(step_blk, step_tile, tiles);
+        if (it.blk >= blocks) return;
     }
 }
 
-// ---- kernel 2 ---------------------------------------------------------------------------------------------------------
+// ---- kernel 2, few rows per expert --------------------------------------------------------------------------------------
+//
+// A workgroup takes 16 channels for all experts; its 16 waves share out the units, the blocks of F of every expert that has rows.
+// Column c of the MFMAs is token 16 j + c, zero where it is not the expert's, so that the accumulators run over all experts.
 
-// CT: blocks of 16 channels; NT: blocks of 16 tokens (all of them); D: units in flight per wave.
-template <int CT, int NT, int D>
-__global__ void __launch_bounds__(WAVES * 64) moe_down_kernel(MoeParams p) {
+constexpr int DOWN_WAVES = 16;
+
+// NT: blocks of 16 tokens (all of them); D: units in flight per wave.
+template <int NT, int D>
+__global__ void __launch_bounds__(DOWN_WAVES * 64) moe_down_kernel(MoeParams p) {
+    constexpr int THREADS = DOWN_WAVES * 64;
     extern __shared__ __attribute__((aligned(16))) char down_lds[];
-    v4f(*part)[CT * NT][64] = reinterpret_cast<v4f(*)[CT * NT][64]>(down_lds);                // [WAVES]
-    int* s_expert = reinterpret_cast<int*>(down_lds + sizeof(v4f) * WAVES * CT * NT * 64);      // the experts that have pairs
+    v4f(*part)[NT][64] = reinterpret_cast<v4f(*)[NT][64]>(down_lds);                            // [DOWN_WAVES]
+    int* s_expert = reinterpret_cast<int*>(down_lds + sizeof(v4f) * DOWN_WAVES * NT * 64);      // the experts that have pairs
     uint16_t* s_slot = reinterpret_cast<uint16_t*>(s_expert + MAX_E);                           // ... and where an expert is among them
     uint8_t* s_map = reinterpret_cast<uint8_t*>(s_slot + MAX_E);                                // [slots][16 NT]: 1 + the token's choice, or 0
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4;
-    const int n0 = (int)blockIdx.x * 16 * CT, rows = min(16 * CT, p.H - n0), P = p.T * p.k;
-    const int cap = min(p.E, P);
-    for (int i = threadIdx.x; i < cap * 16 * NT / 4; i += WAVES * 64) reinterpret_cast<uint32_t*>(s_map)[i] = 0;
+    const int n0 = (int)blockIdx.x * 16, P = p.T * p.k, cap = min(p.E, P);
+    // the pairs' experts, under way together with the offsets
+    constexpr int MINE = (16 * NT * MAX_K + THREADS - 1) / THREADS;
+    int experts[MINE];
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+        const int q = threadIdx.x + i * THREADS;
+        experts[i] = q < P ? p.experts[q] : -1;
+    }
+    for (int i = threadIdx.x; i < cap * 4 * NT; i += THREADS) reinterpret_cast<uint32_t*>(s_map)[i] = 0;
     int active = 0;
     for (int e0 = 0; e0 < p.E; e0 += 64) {                // every wave counts, the first one writes
         const int e = e0 + lane;
@@ -294,145 +371,360 @@ __global__ void __launch_bounds__(WAVES * 64) moe_down_kernel(MoeParams p) {
     }
     active = min(active, cap);
     __syncthreads();
-    for (int q = threadIdx.x; q < P; q += WAVES * 64) {
-        const int e = p.experts[q], t = q / p.k;
-        if (e >= 0 && e < p.E && s_slot[e] != 0xffff) s_map[s_slot[e] * 16 * NT + t] = (uint8_t)(1 + q - t * p.k);
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+        const int q = threadIdx.x + i * THREADS, e = experts[i];
+        if (e >= 0 && e < p.E && s_slot[e] != 0xffff) s_map[s_slot[e] * 16 * NT + q / p.k] = (uint8_t)(1 + q % p.k);
     }
     __syncthreads();
     const int fb = (p.F + BK - 1) / BK, units = active * fb;
-    const __amdgpu_buffer_rsrc_t rh = make_rsrc(p.h, (uint32_t)P * (uint32_t)p.F * 4u);
-    uint32_t vw[CT];
-#pragma unroll
-    for (int i = 0; i < CT; ++i) vw[i] = 16 * i + c < rows ? (uint32_t)((16 * i + c) * p.ld2) + 16u * g : OOB;
-    constexpr bool AHEAD = NT <= 2;                       // the tokens' values are loaded with the weights, else when they are needed
-    v4u w[D][CT][2], h[AHEAD ? D : 1][AHEAD ? NT : 1][2][4];          // h: 16 values, what they leave
+    const __amdgpu_buffer_rsrc_t rh = make_rsrc(p.h, (uint32_t)P * (uint32_t)p.F * 4u), rs = make_rsrc(p.s2, 0x7fffffffu);
+    const uint32_t vw = (uint32_t)(c * p.ld2) + 16u * g, wbytes = (uint32_t)(15 * p.ld2 + p.F);
+    const uint8_t* w0 = p.w2 + n0 * p.ld2;
+    const uint32_t s0 = (uint32_t)(n0 / BK * p.s2_n) * 4u;
+    v4u w[D][2], h[D][NT][2][4];                          // h: 16 values, what they leave
     float sc[D];
-    auto load_h = [&](int d, int j, int m, int b, int width) {
-        const uint32_t vh = (uint32_t)((16 * j + c) * p.k + m - 1) * (uint32_t)p.F * 4u + 64u * g;
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const uint32_t v = m && b * BK + 64 * s + 16 * g < width ? vh : OOB;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) h[d][AHEAD ? j : 0][s][q] = load16<false>(rh, v + 256 * s + 16 * q, 4 * b * BK);
-        }
-    };
+    int ls = 0, lb = wave;                                // the next unit's expert and block
+    while (lb >= fb && ls < active) lb -= fb, ++ls;
     // always the same loads, past the last unit of nothing, so that the count of those under way is known
-    auto load = [&](int d, int u) {
-        int width = u < units ? p.F : 0;
-        asm("" : "+v"(width));                            // a value, so that it selects offsets and does not branch around loads
-        const int v = min(u, units - 1), slot = v / fb, b = v - slot * fb, e = __builtin_amdgcn_readfirstlane(s_expert[slot]);
-        const __amdgpu_buffer_rsrc_t rw = make_rsrc(p.w2 + e * p.w2_e + (int64_t)n0 * p.ld2, (uint32_t)((rows - 1) * p.ld2 + p.F));
+    auto load = [&](int d) {
+        const bool live = ls < active;
+        const int slot = live ? ls : 0, b = live ? lb : 0, e = __builtin_amdgcn_readfirstlane(s_expert[slot]);
+        const int left = live ? p.F - b * BK : 0;
+        const __amdgpu_buffer_rsrc_t rw = make_rsrc(w0 + e * p.w2_e, live ? wbytes : 0u);
+        uint32_t vh[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int m = s_map[slot * 16 * NT + 16 * j + c];
+            vh[j] = m ? (uint32_t)((16 * j + c) * p.k + m - 1) * (uint32_t)p.F * 4u + 64u * g : OOB;
+        }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const bool in = b * BK + 64 * s + 16 * g < width;
+            const bool in = 64 * s + 16 * g < left;
+            w[d][s] = load16<true>(rw, (in ? vw : OOB) + 64 * s, b * BK);
 #pragma unroll
-            for (int i = 0; i < CT; ++i) w[d][i][s] = load16<true>(rw, (in ? vw[i] : OOB) + 64 * s, b * BK);
-        }
-        if constexpr (AHEAD) {
+            for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) load_h(d, j, s_map[slot * 16 * NT + 16 * j + c], b, width);
+                for (int q = 0; q < 4; ++q) h[d][j][s][q] = load16<false>(rh, (in ? vh[j] : OOB) + 256 * s + 16 * q, 4 * b * BK);
         }
-        sc[d] = load4(make_rsrc(p.s2 + e * p.s2_e, 0x7fffffffu), (uint32_t)(n0 / BK * p.s2_n + b * p.s2_k) * 4u);
+        sc[d] = load4(rs, (uint32_t)(e * p.s2_e + b * p.s2_k) * 4u + s0);
+        lb += DOWN_WAVES;
+        while (lb >= fb && ls < active) lb -= fb, ++ls;
         __builtin_amdgcn_sched_barrier(0);                // in this order: the waits count them
     };
-    v4f acc[CT][NT];
+    v4f acc[NT];
 #pragma unroll
-    for (int i = 0; i < CT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < NT; ++j) acc[j] = v4f{0.f, 0.f, 0.f, 0.f};
     if (units > 0) {
 #pragma unroll
-        for (int d = 0; d < D; ++d) load(d, wave + d * WAVES);
+        for (int d = 0; d < D; ++d) load(d);
     }
-    for (int u0 = wave; u0 < units; u0 += D * WAVES) {
+    int slot = 0, b = wave;                               // of the unit at hand
+    while (b >= fb && slot < active) b -= fb, ++slot;
+    for (int u0 = wave; u0 < units; u0 += D * DOWN_WAVES) {
 #pragma unroll
         for (int d = 0; d < D; ++d) {
-            const int u = u0 + d * WAVES;
-            if (u < units) {
-                const int slot = u / fb;
+            v4f sum[1][NT];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
-                    const int m = s_map[slot * 16 * NT + 16 * j + c];
-                    if (__ballot(m != 0) == 0) continue;  // none of these tokens is the expert's
-                    const int hd = AHEAD ? d : 0, hj = AHEAD ? j : 0;
-                    if constexpr (!AHEAD) load_h(0, j, m, u - slot * fb, p.F);
-                    v4f sum[CT][1];
+                    const uint32_t lo = w[d][q >> 1][2 * (q & 1)], hi = w[d][q >> 1][2 * (q & 1) + 1];
+                    if (q == 0) mfma<false, true>(sum[0][j], lo, hi, h[d][j][0][0]);
+                    else mfma<false, false>(sum[0][j], lo, hi, h[d][j][q >> 1][q & 1]);
+                    mfma<false, false>(sum[0][j], lo, hi, h[d][j][q >> 1][2 + (q & 1)]);
+                }
+            sums_ready(sum);
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+                if (slot < active && s_map[slot * 16 * NT + 16 * j + c] != 0) {       // an expert's NaN is not another token's
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[j][r] = __builtin_fmaf(sum[0][j][r], sc[d], acc[j][r]);
+                }
+            __builtin_amdgcn_sched_barrier(0);
+            load(d);
+            b += DOWN_WAVES;
+            while (b >= fb && slot < active) b -= fb, ++slot;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) part[wave][j][lane] = acc[j];
+    __syncthreads();
+    if (threadIdx.x < NT * 64) {
+        const int j = threadIdx.x >> 6, t = 16 * j + c, n = n0 + 4 * g;
+        v4f v = part[0][j][lane];
+#pragma unroll
+        for (int q = 1; q < DOWN_WAVES; ++q) v += part[q][j][lane];
+        if (t < p.T) store_y(p, t, n, v);
+    }
+}
+
+// ---- more rows per expert -----------------------------------------------------------------------------------------------
+//
+// With many rows the tokens' values, read again for every 16 weight rows, are more than the weights.  So the 8 waves of a workgroup
+// take 8 neighbouring tiles of weight rows, the whole of K each (no join), and share the tokens' values through LDS: an item is a
+// block of up to 16 NT rows and 8 tiles.  A unit is 256 (NT = 1) or 128 of K in kernel 1, 128 of F (both numbers) in kernel 2.  It comes by LDS-DMA, two units ahead of its use in a ring of three, one barrier per unit; the weights come two units
+// ahead into registers.  Kernel 2 leaves the pairs' results in fp32, and a third kernel adds up the choices of each token, in their
+// order.
+
+template <bool UP, int NT, int CT>
+struct Rows {
+    static constexpr int RT = UP ? 2 : CT;                // tiles of 16 weight rows of a wave: gate and up; channels
+    static constexpr int KB = UP && NT == 1 ? 2 : 1;      // blocks of 128 of a unit
+    static constexpr int ROW = UP ? 256 * KB : 512;       // bytes of a row's unit
+    static constexpr int STAGE = 16 * NT * ROW, DX = STAGE / 1024 / WAVES;    // LDS-DMA instructions of a wave, 1 KiB each
+    static constexpr int SC = UP ? 2 : 1;                 // scales of a block
+    static constexpr int OUT = UP ? 16 : 16 * CT;         // output channels of a wave
+    static constexpr int LOADS = KB * (2 * RT + SC);      // of a unit, per wave
+};
+
+// LDS place of 16-byte chunk i of row r: the 16 lanes that are served together (0-3, 12-15 and 20-27; 4-11, 16-19 and 28-31) meet 16
+// places.  Kernel 1: lane group g reads chunks 2 g + ..; kernel 2: 4 g + ..
+template <bool UP>
+__device__ __forceinline__ int chunk_at(int r, int i) {
+    const int c = r & 15;
+    return i ^ (UP ? c : (((c >> 2) ^ (c >> 3)) & 1) | ((c & 3) << 1) | (c & 8));
+}
+
+constexpr int STAGES = 3, AHEAD = 2;
+
+template <bool UP, bool FP16, int NT, int CT>
+__global__ void __launch_bounds__(WAVES * 64, NT <= 2 ? 4 : 2) moe_rows_kernel(MoeParams p, int tiles, int step_blk, int step_tile, int cap) {
+    using C = Rows<UP, NT, CT>;
+    constexpr int STAGE = C::STAGE, DX = C::DX, LPR = C::ROW / 16, RPI = 64 / LPR;     // lanes of a row, rows of an instruction
+    extern __shared__ __attribute__((aligned(1024))) uint8_t rows_lds[];
+    uint8_t* lds = rows_lds;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int c = lane & 15, g = lane >> 4;
+    const uint32_t lds0 = lds_addr(lds);
+    const Routed R = load_routing<16 * NT>(p, reinterpret_cast<char*>(lds + STAGES * STAGE), WAVES * 64);
+    const int blocks = __builtin_amdgcn_readfirstlane(*R.count);
+    const int K = UP ? p.H : p.F, N = UP ? p.F : p.H, kb = (K + BK - 1) / BK, units = (kb + AHEAD * C::KB - 1) / (AHEAD * C::KB) * AHEAD;
+    const int64_t ld = UP ? p.ld1 : p.ld2;
+    const v4u rx = buffer_desc(UP ? p.x : p.h, UP ? (uint32_t)(((p.T - 1) * p.ldx + p.H) * 2) : (uint32_t)(p.T * p.k) * (uint32_t)p.F * 4u);
+    const __amdgpu_buffer_rsrc_t rs = make_rsrc(UP ? p.s1 : p.s2, 0x7fffffffu);
+    const uint32_t row_bytes = UP ? (uint32_t)p.H * 2u : (uint32_t)p.F * 4u;
+    // what the next loads need: buffers, lane offsets of the tokens' chunks, offsets of the scales, the unit
+    __amdgpu_buffer_rsrc_t rw, ru;
+    uint32_t vx[DX], vc[DX], s_at, s_up;
+    int lu = 0;
+    bool alive;
+    const uint32_t vw = (uint32_t)(c * ld) + 16u * g;
+#pragma unroll
+    for (int i = 0; i < DX; ++i)                          // the chunk that the lane's 16 bytes of its row are
+        vc[i] = 16u * (uint32_t)chunk_at<UP>(RPI * (wave * DX + i) + lane / LPR, lane % LPR);
+    auto aim = [&](const Item& it) {
+        const bool live = it.blk < blocks;
+        const Block& B = R.blocks[live ? it.blk : 0];
+        const int e = __builtin_amdgcn_readfirstlane(B.e), r0 = __builtin_amdgcn_readfirstlane(B.r0), n = __builtin_amdgcn_readfirstlane(B.n);
+        const int n0 = (it.tile * WAVES + wave) * C::OUT, rows = min(C::OUT, N - n0);
+        alive = live && rows > 0;
+        const uint32_t bytes = alive ? (uint32_t)((rows - 1) * ld + K) : 0u;
+        const int at = alive ? n0 : 0;
+        const uint8_t* w = (UP ? p.w1 + e * p.w1_e : p.w2 + e * p.w2_e) + at * ld;
+        rw = make_rsrc(w, bytes);
+        if (UP) ru = make_rsrc(w + p.F * ld, bytes);
+        s_at = (uint32_t)(UP ? e * p.s1_e + at / BK * p.s1_n : e * p.s2_e + at / BK * p.s2_n) * 4u;
+        s_up = UP ? (uint32_t)(e * p.s1_e + (p.F + at) / BK * p.s1_n) * 4u : 0u;
+#pragma unroll
+        for (int i = 0; i < DX; ++i) {
+            const int row = RPI * (wave * DX + i) + lane / LPR;
+            uint32_t v = OOB;
+            if (live && row < n) v = UP ? (uint32_t)(R.pair[r0 + row] / p.k) * (uint32_t)(p.ldx * 2) : (uint32_t)R.pair[r0 + row] * row_bytes;
+            vx[i] = v;
+        }
+        lu = 0;
+    };
+    v4u w[AHEAD][C::KB][C::RT][2];
+    float sc[AHEAD][C::KB][C::SC];
+    // the tokens' values of the unit into a stage, the weights of the unit: always the same loads, past the last of nothing
+    auto fetch = [&](int stage, int u) {
+        const uint32_t at = lds0 + (uint32_t)(stage * STAGE + wave * DX * 1024), k0 = (uint32_t)(u * C::ROW);
+#pragma unroll
+        for (int i = 0; i < DX; ++i) dma16(rx, __builtin_amdgcn_readfirstlane(at + 1024u * i), vx[i] != OOB && k0 + vc[i] < row_bytes ? vx[i] + k0 + vc[i] : OOB);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto load = [&](int d, int u) {
+#pragma unroll
+        for (int b = 0; b < C::KB; ++b) {
+            const int blk = u * C::KB + b, k0 = alive && blk < kb ? blk * BK : 0, left = alive && blk < kb ? K - k0 : 0;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const bool in = 64 * s + 16 * g < left;
+#pragma unroll
+                for (int i = 0; i < C::RT; ++i)
+                    w[d][b][i][s] = load16<true>(UP && i ? ru : rw, (in ? vw + (UP ? 0u : (uint32_t)(16 * i * ld)) : OOB) + 64 * s, k0);
+            }
+            const uint32_t sb = (uint32_t)(min(blk, kb - 1) * (UP ? p.s1_k : p.s2_k)) * 4u;
+            sc[d][b][0] = load4(rs, s_at + sb);
+            if (UP) sc[d][b][C::SC - 1] = load4(rs, s_up + sb);
+        }
+        __builtin_amdgcn_sched_barrier(0);                // in this order: the waits count them
+    };
+    Item it{(int)blockIdx.x / tiles, (int)blockIdx.x % tiles}, nx = it;
+    if (it.blk >= blocks) return;
+    aim(it);
+#pragma unroll
+    for (int d = 0; d < AHEAD; ++d) {
+        fetch(d, d);
+        load(d, d);
+    }
+    for (int stage = 0;;) {
+        const Block B = R.blocks[it.blk];
+        const int n = __builtin_amdgcn_readfirstlane(B.n);
+        v4f acc[C::RT][NT];
+#pragma unroll
+        for (int i = 0; i < C::RT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+        for (int u = 0; u < units; u += AHEAD) {
+            if (u + AHEAD < units) lu += AHEAD;
+            else nx.next(step_blk, step_tile, tiles), aim(nx);
+#pragma unroll
+            for (int d = 0; d < AHEAD; ++d) {
+                // this wave's share of the unit has landed (behind it: its weights, the next unit's both), and its reads of the last one
+                __builtin_amdgcn_s_waitcnt(vmcnt_imm(AHEAD * C::LOADS + (AHEAD - 1) * DX));
+                wait_lgkm0();
+                barrier_nofence();
+                const int free = stage == 0 ? STAGES - 1 : stage - 1;             // the last one's place
+                fetch(free, lu + d);
+                const uint8_t* st = lds + stage * STAGE;
+#pragma unroll
+                for (int b = 0; b < C::KB; ++b) {
+                    v4f sum[C::RT][NT];
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
 #pragma unroll
-                        for (int i = 0; i < CT; ++i) {
-                            const uint32_t lo = w[d][i][q >> 1][2 * (q & 1)], hi = w[d][i][q >> 1][2 * (q & 1) + 1];
-                            if (q == 0) mfma<false, true>(sum[i][0], lo, hi, h[hd][hj][0][0]);
-                            else mfma<false, false>(sum[i][0], lo, hi, h[hd][hj][q >> 1][q & 1]);
-                            mfma<false, false>(sum[i][0], lo, hi, h[hd][hj][q >> 1][2 + (q & 1)]);
+                        for (int j = 0; j < NT; ++j) {
+                            if (j && 16 * j >= n) continue;   // uniform
+                            const int chunk = UP ? 16 * b + 8 * (q >> 1) + 2 * g + (q & 1) : 4 * (4 * (q >> 1) + g) + (q & 1);
+                            const uint8_t* row = st + (16 * j + c) * C::ROW;
+                            const v4u t = *reinterpret_cast<const v4u*>(row + 16 * chunk_at<UP>(c, chunk));
+#pragma unroll
+                            for (int i = 0; i < C::RT; ++i) {
+                                const uint32_t lo = w[d][b][i][q >> 1][2 * (q & 1)], hi = w[d][b][i][q >> 1][2 * (q & 1) + 1];
+                                if (q == 0) mfma<UP && FP16, true>(sum[i][j], lo, hi, t);
+                                else mfma<UP && FP16, false>(sum[i][j], lo, hi, t);
+                            }
+                            if (!UP) {
+                                const v4u t2 = *reinterpret_cast<const v4u*>(row + 16 * chunk_at<UP>(c, chunk + 2));
+#pragma unroll
+                                for (int i = 0; i < C::RT; ++i)
+                                    mfma<false, false>(sum[i][j], w[d][b][i][q >> 1][2 * (q & 1)], w[d][b][i][q >> 1][2 * (q & 1) + 1], t2);
+                            }
                         }
                     sums_ready(sum);
-                    if (m) {                              // an expert's NaN is not another token's
 #pragma unroll
-                        for (int i = 0; i < CT; ++i)
+                    for (int j = 0; j < NT; ++j) {
+                        if (j && 16 * j >= n) continue;
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(sum[i][0][r], sc[d], acc[i][j][r]);
+                        for (int i = 0; i < C::RT; ++i)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) acc[i][j][k] = __builtin_fmaf(sum[i][j][k], sc[d][b][UP ? i : 0], acc[i][j][k]);
                     }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                load(d, lu + d);
+                stage = stage == STAGES - 1 ? 0 : stage + 1;
+            }
+        }
+        const int n0 = (it.tile * WAVES + wave) * C::OUT + 4 * g;
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+            if (16 * j + c < n) {
+                const int pair = R.pair[B.r0 + 16 * j + c];
+                if constexpr (UP) {
+                    if (n0 < N) store_h(p, pair, n0, R.weight[B.r0 + 16 * j + c], acc[0][j], acc[1][j]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < C::RT; ++i)
+                        if (n0 + 16 * i < N) *reinterpret_cast<v4f*>(p.z + (int64_t)pair * p.H + n0 + 16 * i) = acc[i][j];
                 }
             }
-            load(d, u + D * WAVES);
-        }
+        it.next(step_blk, step_tile, tiles);
+        if (it.blk >= blocks) break;
     }
-#pragma unroll
-    for (int i = 0; i < CT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) part[wave][i * NT + j][lane] = acc[i][j];
-    __syncthreads();
-    for (int it = threadIdx.x; it < CT * NT * 64; it += WAVES * 64) {
-        const int l = it & 63, ij = it >> 6, t = ij % NT * 16 + (l & 15), n = n0 + ij / NT * 16 + 4 * (l >> 4);
-        v4f v = part[0][ij][l];
-#pragma unroll
-        for (int q = 1; q < WAVES; ++q) v += part[q][ij][l];
-        if (t >= p.T || n >= p.H) continue;
-        if (p.residual) {
-            const uint2 r = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p.residual) + t * p.ldr + n);
-            const uint32_t b[4] = {r.x & 0xffffu, r.x >> 16, r.y & 0xffffu, r.y >> 16};
-#pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] += p.fp16 ? fp16_to_f32(b[q]) : bf16_to_f32(b[q]);
-        }
-        const uint2 o = p.fp16 ? uint2{fp16_rne(v[0]) | (fp16_rne(v[1]) << 16), fp16_rne(v[2]) | (fp16_rne(v[3]) << 16)}
-                               : uint2{cvt_bf16x2(v[0], v[1]), cvt_bf16x2(v[2], v[3])};
-        *reinterpret_cast<uint2*>(p.y + t * p.ldy + n) = o;
-    }
+    wait_vm0();                                           // the loads behind the last unit have landed before the exit
 }
 
-template <bool FP16, int NI, int NT, int D>
+// y: the sum over a token's choices, in their order; of equal experts the first counts (it has both weights).
+__global__ void __launch_bounds__(256) moe_combine_kernel(MoeParams p) {
+    const int t = blockIdx.y, n = 4 * (int)(blockIdx.x * 256 + threadIdx.x);
+    if (n >= p.H) return;
+    v4f v = {0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < p.k; ++j) {
+        const int q = t * p.k + j, e = p.experts[q];
+        bool count = e >= 0 && e < p.E;
+        for (int i = 0; i < j; ++i) count = count && p.experts[t * p.k + i] != e;
+        if (count) v += *reinterpret_cast<const v4f*>(p.z + (int64_t)q * p.H + n);
+    }
+    store_y(p, t, n, v);
+}
+
+template <bool UP, bool FP16, int NT, int CT>
+int launch_rows(const MoeParams& p, hipStream_t st) {
+    const int out = WAVES * Rows<UP, NT, CT>::OUT, tiles = ((UP ? p.F : p.H) + out - 1) / out, P = p.T * p.k, cap = max_blocks<16 * NT>(p.E, P);
+    const size_t lds = STAGES * Rows<UP, NT, CT>::STAGE + routed_bytes<16 * NT>(p.E, P);
+    const int grid = (int)std::min<int64_t>((int64_t)tiles * cap, (NT <= 2 ? 2 : 1) * h3host::cu_count());
+    hipLaunchKernelGGL((moe_rows_kernel<UP, FP16, NT, CT>), dim3(grid), dim3(WAVES * 64), lds, st, p, tiles, grid / tiles, grid % tiles, cap);
+    H3_CHECK_HIP(hipGetLastError());
+    return H3FP8_OK;
+}
+
+int launch_combine(const MoeParams& p, hipStream_t st) {
+    hipLaunchKernelGGL(moe_combine_kernel, dim3((unsigned)((p.H + 1023) / 1024), (unsigned)p.T), dim3(256), 0, st, p);
+    H3_CHECK_HIP(hipGetLastError());
+    return H3FP8_OK;
+}
+
+template <bool FP16, int D>
 int launch_up(const MoeParams& p, hipStream_t st) {
-    const int tiles = (p.F + 16 * NI - 1) / (16 * NI);
-    const int64_t blocks = (int64_t)tiles * std::min(p.E, p.T * p.k);
-    hipLaunchKernelGGL((moe_up_kernel<FP16, NI, NT, D>), dim3((unsigned)blocks), dim3(WAVES * 64), 0, st, p, tiles);
+    const int tiles = p.F / 16, P = p.T * p.k;
+    const int grid = (int)std::min<int64_t>((int64_t)tiles * max_blocks<16>(p.E, P), 2 * h3host::cu_count());
+    hipLaunchKernelGGL((moe_up_kernel<FP16, D>), dim3(grid), dim3(WAVES * 64), routed_bytes<16>(p.E, P), st, p, tiles, grid / tiles,
+                       grid % tiles);
     H3_CHECK_HIP(hipGetLastError());
     return H3FP8_OK;
 }
 
-template <int CT, int NT, int D>
+template <int NT, int D>
 int launch_down(const MoeParams& p, hipStream_t st) {
-    const size_t lds = sizeof(v4f) * WAVES * CT * NT * 64 + 6 * MAX_E + (size_t)std::min(p.E, p.T * p.k) * 16 * NT;
-    hipLaunchKernelGGL((moe_down_kernel<CT, NT, D>), dim3((unsigned)((p.H + 16 * CT - 1) / (16 * CT))), dim3(WAVES * 64), lds, st, p);
+    const size_t lds = sizeof(v4f) * DOWN_WAVES * NT * 64 + 6 * MAX_E + (size_t)std::min(p.E, p.T * p.k) * 16 * NT;
+    hipLaunchKernelGGL((moe_down_kernel<NT, D>), dim3((unsigned)(p.H / 16)), dim3(DOWN_WAVES * 64), lds, st, p);
     H3_CHECK_HIP(hipGetLastError());
     return H3FP8_OK;
+}
+
+// Which kernels run (host only; for the workspace too).
+bool by_rows(int64_t T, int64_t k, int64_t E) { return T > 16 || T * k > 4 * E; }
+
+template <bool FP16, int NT>
+int run_rows(const MoeParams& p, hipStream_t st) {
+    int rc = launch_rows<true, FP16, NT, 1>(p, st);
+    if (!rc) rc = launch_rows<false, false, NT, 2>(p, st);
+    return rc ? rc : launch_combine(p, st);
 }
 
 template <bool FP16>
 int run(const MoeParams& p, hipStream_t st) {
-    const int rc = p.T <= 16 ? launch_up<FP16, 1, 1, 4>(p, st) : launch_up<FP16, 1, 2, 2>(p, st);
-    if (rc) return rc;
-    if (p.T <= 16) return launch_down<1, 1, 3>(p, st);
-    if (p.T <= 32) return launch_down<1, 2, 2>(p, st);
-    if (p.T <= 64) return launch_down<1, 4, 4>(p, st);
-    return launch_down<1, 8, 4>(p, st);
+    if (by_rows(p.T, p.k, p.E)) {
+        const int mean = (p.T * p.k + p.E - 1) / p.E;
+        if (mean <= 8) return run_rows<FP16, 1>(p, st);
+        if (mean <= 24) return run_rows<FP16, 2>(p, st);
+        return run_rows<FP16, 4>(p, st);
+    }
+    const int rc = launch_up<FP16, 2>(p, st);
+    return rc ? rc : launch_down<1, 2>(p, st);
 }
 
 constexpr int64_t kMaxSpan = 0x7fff0000LL;
 
 }  // namespace
 
-extern "C" int64_t h3fp8_moe_blocks_workspace(int64_t T, int64_t k, int64_t F) { return T < 0 || k < 0 || F < 0 ? 0 : T * k * F * 4; }
+extern "C" int64_t h3fp8_moe_blocks_workspace(int64_t T, int64_t k, int64_t H, int64_t F, int64_t E) {
+    return T < 0 || k < 0 || H < 0 || F < 0 ? 0 : T * k * 4 * (by_rows(T, k, E) ? F + H : F);
+}
 
 extern "C" int h3fp8_moe_blocks(const void* x, int64_t ldx, int dtype, int64_t T, int64_t H, int64_t F, int64_t E, int k,
                                 const void* w1, int64_t w1_e, int64_t ld1, const float* s1, int64_t s1_e, int64_t s1_n, int64_t s1_k,
@@ -461,17 +753,17 @@ extern "C" int h3fp8_moe_blocks(const void* x, int64_t ldx, int dtype, int64_t T
     H3_REQUIRE(128 * ldx * 2 + 2 * H <= kMaxSpan && 64 * ld1 + H <= kMaxSpan && 64 * ld2 + F <= kMaxSpan && T * k * F * 4 <= kMaxSpan,
                "%s: a stride or size is too large", who);
     const int64_t hb = (H + 127) / 128, fb = (F + 127) / 128, f2 = (2 * F + 127) / 128;
-    H3_REQUIRE(f2 * s1_n * 4 <= kMaxSpan / 2 && hb * s1_k * 4 <= kMaxSpan / 2 && hb * s2_n * 4 <= kMaxSpan / 2 && fb * s2_k * 4 <= kMaxSpan / 2,
+    H3_REQUIRE((E * s1_e + f2 * s1_n) * 4 <= kMaxSpan / 2 && hb * s1_k * 4 <= kMaxSpan / 2 && hb * s2_n * 4 <= kMaxSpan / 2 && fb * s2_k * 4 <= kMaxSpan / 2,
                "%s: a scale stride is too large", who);
-    H3_REQUIRE(workspace_bytes >= h3fp8_moe_blocks_workspace(T, k, F), "%s: the workspace needs %lld bytes", who,
-               (long long)h3fp8_moe_blocks_workspace(T, k, F));
+    const int64_t need = h3fp8_moe_blocks_workspace(T, k, H, F, E);
+    H3_REQUIRE(workspace_bytes >= need, "%s: the workspace needs %lld bytes", who, (long long)need);
     MoeParams p{};
     p.x = x; p.ldx = ldx;
     p.w1 = (const uint8_t*)w1; p.s1 = s1; p.w2 = (const uint8_t*)w2; p.s2 = s2;
     p.w1_e = w1_e; p.ld1 = ld1; p.w2_e = w2_e; p.ld2 = ld2;
     p.s1_e = s1_e; p.s1_n = s1_n; p.s1_k = s1_k; p.s2_e = s2_e; p.s2_n = s2_n; p.s2_k = s2_k;
     p.weights = weights; p.experts = experts; p.offsets = offsets; p.order = order;
-    p.residual = residual; p.ldr = ldr; p.y = (uint16_t*)y; p.ldy = ldy; p.h = (char*)workspace;
+    p.residual = residual; p.ldr = ldr; p.y = (uint16_t*)y; p.ldy = ldy; p.h = (char*)workspace; p.z = (float*)(p.h + T * k * F * 4);
     p.T = (int)T; p.E = (int)E; p.k = k; p.H = (int)H; p.F = (int)F; p.fp16 = dtype == H3FP8_DT_FP16;
     return p.fp16 ? run<true>(p, (hipStream_t)stream) : run<false>(p, (hipStream_t)stream);
 }

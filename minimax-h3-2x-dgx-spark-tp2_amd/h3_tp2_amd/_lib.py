@@ -76,7 +76,7 @@ _SIGS = {
     "h3fp8_gemm_blocks_act": ([P, I64, P, I64, P, I64, I64, P, I64, I64, P, I, P, I64, P, I64, I, I64, I64, I64, P], I),
     "h3fp8_moe_route_workspace": ([I64, I64], I64),
     "h3fp8_moe_route": ([P, I64, I, I64, I64, I, I, I, ctypes.c_float, P, P, P, P, P, P, P, I64, P], I),
-    "h3fp8_moe_blocks_workspace": ([I64, I64, I64], I64),
+    "h3fp8_moe_blocks_workspace": ([I64, I64, I64, I64, I64], I64),
     "h3fp8_moe_blocks": ([P, I64, I, I64, I64, I64, I64, I, P, I64, I64, P, I64, I64, I64, P, I64, I64, P, I64, I64, I64, P, P, P, P,
                           P, I64, P, I64, P, I64, P], I),
     "h3fp8_selfcheck_e4m3": ([ctypes.POINTER(ctypes.c_uint64), ctypes.POINTER(ctypes.c_uint64)], I),

@@ -995,7 +995,7 @@ def moe_blocks(x: torch.Tensor, w_gate_up: torch.Tensor, scale_gate_up: torch.Te
     _same_device("moe_blocks", x, w_gate_up, scale_gate_up, w_down, scale_down, residual)
     y = _block_out("moe_blocks", x, T, H, x.dtype, out)
     ldr = _residual("moe_blocks", residual, (T, H), x.dtype, y)
-    ws_bytes = _lib.load().h3fp8_moe_blocks_workspace(T, k, F)
+    ws_bytes = _lib.load().h3fp8_moe_blocks_workspace(T, k, H, F, E)
     ws = torch.empty(ws_bytes, device=x.device, dtype=torch.uint8)
     _call_on(x, "h3fp8_moe_blocks", x.data_ptr(), ldx, _DT[x.dtype], T, H, F, E, k, w_gate_up.data_ptr(),
              w_gate_up.stride(0) if E > 1 else 0, ld1, scale_gate_up.data_ptr(), *_axes(scale_gate_up), w_down.data_ptr(),
