@@ -110,13 +110,6 @@ __device__ __forceinline__ bool locate_rows(const BlocksParams& p, int TT, int64
 // of each line) made every case slower (1890 -> 2244 us): the requests that are under way are the limit.
 __device__ __forceinline__ int swz_w(int r) { return ((r >> 1) & 1) | (((r >> 3) & 3) << 1); }
 
-__device__ __forceinline__ void dma4_at(v4u desc, uint32_t lds_base, uint32_t voff, uint32_t soff) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"
-                 :
-                 : "s"(lds_base), "v"(voff), "s"(desc), "s"(soff)
-                 : "memory", "m0");
-}
-
 constexpr int LAG = 5;
 constexpr int AHEAD = 3;                                  // channel blocks read ahead of their MFMAs
 

@@ -145,6 +145,14 @@ __device__ __forceinline__ void dma4(v4u desc, uint32_t lds_base, uint32_t voff)
                  : "memory", "m0");
 }
 
+// ... at a further uniform byte offset.
+__device__ __forceinline__ void dma4_at(v4u desc, uint32_t lds_base, uint32_t voff, uint32_t soff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"
+                 :
+                 : "s"(lds_base), "v"(voff), "s"(desc), "s"(soff)
+                 : "memory", "m0");
+}
+
 // Orders one wave's LDS accesses across its lanes: a lane's staging writes become visible to the other lanes' reads
 // that follow.  The wave's LDS accesses already complete in order, so this emits no wait; it is there for the compiler,
 // which under per-lane semantics may otherwise reorder or tail-duplicate lane-divergent writes past other lanes' reads

@@ -16,6 +16,7 @@
 // MFMA's 16 columns are tokens by their own number, zero where a token is not the expert's, so that the sums over experts
 // stay in the accumulators and no order of workgroups shows in the result.
 #include <algorithm>
+#include <type_traits>
 
 #include "gemm_core.h"
 
@@ -26,7 +27,6 @@ using namespace h3g;
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8hf __attribute__((ext_vector_type(8)));
 
-constexpr int WAVES = 8;
 constexpr int MAX_T = 128, MAX_K = 16, MAX_E = 512;
 
 struct MoeParams {
@@ -58,9 +58,8 @@ __device__ __forceinline__ int offset_at(const MoeParams& p, int e) {
 
 // 16 bytes per lane; OOB (and up to 64 KiB past it) and what lies past the buffer read as zeros.  The hardware checks the lane's
 // offset against the buffer's size less the uniform offset: that one is the start of a block that there is.
-template <bool NT>
 __device__ __forceinline__ v4u load16(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff) {
-    return __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(r, (int)voff, (int)soff, NT ? 2 : 0));
+    return __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(r, (int)voff, (int)soff, 0));
 }
 
 // One number for all lanes.
@@ -119,80 +118,103 @@ __device__ __forceinline__ int wave_prefix(int v) {       // inclusive
     return v;
 }
 
+
 // ---- the routing, in LDS ------------------------------------------------------------------------------------------------
 //
 // All that a workgroup needs of the routing is loaded at once, and looked up from then on: one trip to memory before the first
 // weights can be asked for instead of one per step (offsets, order, experts).
 
-struct Block { int e, r0, n; };                           // n sorted rows from r0 on, of expert e
+// An expert that has pairs: sorted rows r0 .. r0 + rows - 1, in blocks; `start`: its first item (see Item).
+struct Expert { uint16_t e, r0, rows, none; int start; };
 
 struct Routed {
-    int* count;                                           // of blocks
-    int* pair;                                            // [P] of a sorted row
+    int* count;                                           // of experts that have pairs, of the workgroup's XCD's items
+    Expert* list;
     float* weight;                                        // [P] of a sorted row: of all its token's choices of its expert (the
                                                           // second of two equal ones has the same, and is not read)
-    Block* blocks;                                        // the experts' rows in blocks of at most ROWS
-    int* experts;                                         // [P] of a pair
-    float* weights;                                       // [P]
+    uint16_t* pair;                                       // [P] of a sorted row
 };
 
-template <int ROWS>
-constexpr int max_blocks(int E, int P) { return (E < P ? E : P) + P / ROWS; }
+constexpr size_t routed_bytes(int E, int P, bool weights) {
+    return 16 + (size_t)(E < P ? E : P) * sizeof(Expert) + (size_t)P * (weights ? 6 : 2);
+}
+constexpr int TEMP_BYTES = 8 * MAX_T * MAX_K;             // what load_routing needs besides, before the first stage is loaded
 
-template <int ROWS>
-constexpr size_t routed_bytes(int E, int P) { return (size_t)P * 16 + (size_t)max_blocks<ROWS>(E, P) * sizeof(Block) + 16; }
+// The items of a launch are a block of up to ROWS rows of an expert and a tile of its output channels.  Blocks of one expert read
+// the same weights, so they run at the same time on the same XCD, whose L2 then has them: tile t of the s-th expert is XCD
+// (s tiles + t) % 8's (workgroups are dealt over the XCDs in turn), and a XCD's items are ordered by expert, tile, block.
+struct Item {
+    int e, r0, n, tile;                                   // n = 0: past the last one
+};
 
-// By all threads, with barriers.
-template <int ROWS>
-__device__ __forceinline__ Routed load_routing(const MoeParams& p, char* lds, int threads) {
-    const int P = p.T * p.k, lane = threadIdx.x & 63, cap = max_blocks<ROWS>(p.E, P);
+constexpr int XCDS = 8;
+
+// By all threads, with barriers.  temp: experts and weights of the pairs, while the weights are added up.
+template <int ROWS, bool WEIGHTS>
+__device__ __forceinline__ Routed load_routing(const MoeParams& p, char* lds, char* temp, int threads, int tiles) {
+    const int P = p.T * p.k, lane = threadIdx.x & 63, cap = min(p.E, P), xcd = (int)blockIdx.x % XCDS;
     Routed r;
     r.count = reinterpret_cast<int*>(lds);
-    r.pair = r.count + 4;
-    r.weight = reinterpret_cast<float*>(r.pair + P);
-    r.experts = reinterpret_cast<int*>(r.weight + P);
-    r.weights = reinterpret_cast<float*>(r.experts + P);
-    r.blocks = reinterpret_cast<Block*>(r.weights + P);
+    r.list = reinterpret_cast<Expert*>(r.count + 4);
+    r.weight = reinterpret_cast<float*>(r.list + cap);
+    r.pair = reinterpret_cast<uint16_t*>(r.weight + (WEIGHTS ? P : 0));
+    int* experts_of = reinterpret_cast<int*>(temp);
+    float* weights_of = reinterpret_cast<float*>(experts_of + P);
     for (int i = threadIdx.x; i < P; i += threads) {
-        const int o = p.order[i], e = p.experts[i];
-        const float w = p.weights[i];
-        r.pair[i] = min(max(o, 0), P - 1);                // whatever it holds, no row outside the tokens is read
-        r.experts[i] = e;
-        r.weights[i] = w;
+        const int o = p.order[i];
+        if (WEIGHTS) {
+            const int e = p.experts[i];
+            const float w = p.weights[i];
+            experts_of[i] = e;
+            weights_of[i] = w;
+        }
+        r.pair[i] = (uint16_t)min(max(o, 0), P - 1);      // whatever it holds, no row outside the tokens is read
     }
     if (threadIdx.x < 64) {
-        int blocks = 0;
+        int experts = 0, items = 0;
         for (int e0 = 0; e0 < p.E; e0 += 64) {
             int lo = 0, hi = 0;
             if (e0 + lane < p.E) lo = offset_at(p, e0 + lane), hi = offset_at(p, e0 + lane + 1);
-            const int n = max(hi - lo, 0), nb = (n + ROWS - 1) / ROWS, at = blocks + wave_prefix(nb) - nb;
-            for (int i = 0; i < nb; ++i)                  // (offsets that are not ascending may name more blocks than there are pairs)
-                if (at + i < cap) r.blocks[at + i] = Block{e0 + lane, lo + i * ROWS, min(ROWS, n - i * ROWS)};
-            blocks = __builtin_amdgcn_readlane(at + nb, 63);
+            const int n = max(hi - lo, 0);
+            const uint64_t has = __ballot(n > 0);
+            const int s = experts + __popcll(has & ((1ull << lane) - 1));
+            const int t0 = (xcd + XCDS - s * tiles % XCDS) % XCDS, mine = n > 0 && t0 < tiles ? (tiles - t0 + XCDS - 1) / XCDS : 0;
+            const int m = mine * ((n + ROWS - 1) / ROWS), at = items + wave_prefix(m) - m;
+            // (offsets that are not ascending may name more experts than there are pairs)
+            if (n > 0 && s < cap) r.list[s] = Expert{(uint16_t)(e0 + lane), (uint16_t)lo, (uint16_t)n, 0, at};
+            experts += __popcll(has);
+            items = __builtin_amdgcn_readlane(at + m, 63);
         }
-        if (lane == 0) *r.count = min(blocks, cap);
+        if (lane == 0) r.count[0] = min(experts, cap), r.count[1] = items;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < P; i += threads) {
-        const int e = r.experts[r.pair[i]];
-        float w = 0.0f;
-        for (int j = 0, q = r.pair[i] / p.k * p.k; j < p.k; ++j) w += r.experts[q + j] == e ? r.weights[q + j] : 0.0f;
-        r.weight[i] = w;
+    if (WEIGHTS) {
+        for (int i = threadIdx.x; i < P; i += threads) {
+            const int pair = r.pair[i], e = experts_of[pair];
+            float w = 0.0f;
+            for (int j = 0, q = pair / p.k * p.k; j < p.k; ++j) w += experts_of[q + j] == e ? weights_of[q + j] : 0.0f;
+            r.weight[i] = w;
+        }
+        __syncthreads();
     }
-    __syncthreads();
     return r;
 }
 
-// An item of a persistent workgroup: a block of rows and a tile of output channels.
-struct Item {
-    int blk, tile;
-
-    __device__ __forceinline__ void next(int step_blk, int step_tile, int tiles) {
-        blk += step_blk;
-        tile += step_tile;
-        if (tile >= tiles) tile -= tiles, ++blk;
-    }
-};
+// Item i of the workgroup's XCD, by a wave; all scalars.
+template <int ROWS>
+__device__ __forceinline__ Item item_at(const Routed& r, int experts, int items, int i, int tiles, int lane) {
+    if (i >= items) return Item{0, 0, 0, 0};
+    int s = -1;
+    for (int s0 = 0; s0 < experts; s0 += 64)              // the last expert that starts no later
+        s += __popcll(__ballot(s0 + lane < experts && r.list[min(s0 + lane, experts - 1)].start <= i));
+    // experts without a tile here start where the next one does, and are not the last
+    const Expert& x = r.list[s];
+    const int e = __builtin_amdgcn_readfirstlane(x.e), r0 = __builtin_amdgcn_readfirstlane(x.r0);
+    const int rows = __builtin_amdgcn_readfirstlane(x.rows), k = i - __builtin_amdgcn_readfirstlane(x.start);
+    const int nb = (rows + ROWS - 1) / ROWS, t = k / nb, b = k - t * nb;
+    const int t0 = ((int)blockIdx.x % XCDS + XCDS - s * tiles % XCDS) % XCDS;
+    return Item{e, r0 + b * ROWS, min(ROWS, rows - b * ROWS), t0 + XCDS * t};
+}
 
 // silu(g) u w of 4 consecutive channels f .. f + 3 of a pair, as two bf16 numbers each.
 __device__ __forceinline__ void store_h(const MoeParams& p, int pair, int f, float weight, const v4f& gate, const v4f& up) {
@@ -220,112 +242,6 @@ __device__ __forceinline__ void store_y(const MoeParams& p, int t, int n, v4f v)
     const uint2 o = p.fp16 ? uint2{fp16_rne(v[0]) | (fp16_rne(v[1]) << 16), fp16_rne(v[2]) | (fp16_rne(v[3]) << 16)}
                            : uint2{cvt_bf16x2(v[0], v[1]), cvt_bf16x2(v[2], v[3])};
     *reinterpret_cast<uint2*>(p.y + t * p.ldy + n) = o;
-}
-
-// ---- kernel 1 ---------------------------------------------------------------------------------------------------------
-//
-// An item is a block of up to 16 rows of one expert and 16 gate rows; the workgroup's 8 waves share out the blocks of K.  Two
-// workgroups per CU, persistent: a wave's loads run D of its units (blocks of K) ahead, across items.
-
-template <bool FP16, int D>
-__global__ void __launch_bounds__(WAVES * 64, 4) moe_up_kernel(MoeParams p, int tiles, int step_blk, int step_tile) {
-    extern __shared__ __attribute__((aligned(16))) char up_lds[];
-    __shared__ v4f part[2][WAVES][2][64];
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int c = lane & 15, g = lane >> 4;
-    const Routed R = load_routing<16>(p, up_lds, WAVES * 64);
-    const int blocks = __builtin_amdgcn_readfirstlane(*R.count);
-    const int kb = (p.H + BK - 1) / BK, rounds = (kb + D * WAVES - 1) / (D * WAVES);
-    const __amdgpu_buffer_rsrc_t rx = make_rsrc(p.x, (uint32_t)(((p.T - 1) * p.ldx + p.H) * 2));
-    const __amdgpu_buffer_rsrc_t rs = make_rsrc(p.s1, 0x7fffffffu);
-    // what the next loads need: buffers, lane offsets of the weight row and the token, offsets of the scales, the block
-    __amdgpu_buffer_rsrc_t rg, ru;
-    uint32_t vw, vx, sg, su;
-    int lb, lend;                                         // (past the last item no block is there)
-    auto aim = [&](const Item& it) {
-        const bool live = it.blk < blocks;
-        const Block& B = R.blocks[live ? it.blk : 0];
-        const int e = __builtin_amdgcn_readfirstlane(B.e), r0 = __builtin_amdgcn_readfirstlane(B.r0), n = __builtin_amdgcn_readfirstlane(B.n);
-        const int f0 = it.tile * 16;
-        const uint32_t bytes = live ? (uint32_t)(15 * p.ld1 + p.H) : 0u;
-        const uint8_t* w = p.w1 + e * p.w1_e + f0 * p.ld1;
-        rg = make_rsrc(w, bytes);
-        ru = make_rsrc(w + p.F * p.ld1, bytes);
-        vx = live && c < n ? (uint32_t)(R.pair[r0 + min(c, n - 1)] / p.k) * (uint32_t)(p.ldx * 2) + 32u * g : OOB;
-        sg = (uint32_t)(e * p.s1_e + f0 / BK * p.s1_n) * 4u;
-        su = (uint32_t)(e * p.s1_e + (p.F + f0) / BK * p.s1_n) * 4u;
-        lb = wave;
-        lend = live ? kb : 0;
-    };
-    vw = (uint32_t)(c * p.ld1) + 16u * g;
-    v4u w[D][2][2], x[D][2][2];
-    float sc[D][2];
-    // always the same loads, past the last block of nothing, so that the count of those under way is known
-    auto load = [&](int d) {
-        const int b = lb + d * WAVES, at = b < lend ? b * BK : 0, left = b < lend ? p.H - at : 0;
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const bool in = 64 * s + 16 * g < left;
-            w[d][0][s] = load16<true>(rg, (in ? vw : OOB) + 64 * s, at);
-            w[d][1][s] = load16<true>(ru, (in ? vw : OOB) + 64 * s, at);
-#pragma unroll
-            for (int q = 0; q < 2; ++q) x[d][s][q] = load16<false>(rx, (in ? vx : OOB) + 128 * s + 16 * q, 2 * at);
-        }
-        const uint32_t sb = (uint32_t)(min(b, kb - 1) * p.s1_k) * 4u;
-        sc[d][0] = load4(rs, sg + sb);
-        sc[d][1] = load4(rs, su + sb);
-        __builtin_amdgcn_sched_barrier(0);                // in this order: the waits count them
-    };
-    Item it{(int)blockIdx.x / tiles, (int)blockIdx.x % tiles}, nx = it;
-    if (it.blk >= blocks) return;
-    aim(it);
-#pragma unroll
-    for (int d = 0; d < D; ++d) load(d);
-    for (int buf = 0;; buf ^= 1) {
-        v4f acc[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
-        for (int r = 0; r < rounds; ++r) {
-            if (r + 1 < rounds) lb += D * WAVES;
-            else nx.next(step_blk, step_tile, tiles), aim(nx);
-#pragma unroll
-            for (int d = 0; d < D; ++d) {
-                v4f sum[2][1];
-#pragma unroll
-                for (int q = 0; q < 4; ++q)               // 32 of the block's k each
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const v4u& a = w[d][i][q >> 1];
-                        if (q == 0) mfma<FP16, true>(sum[i][0], a[0], a[1], x[d][0][0]);
-                        else mfma<FP16, false>(sum[i][0], a[2 * (q & 1)], a[2 * (q & 1) + 1], x[d][q >> 1][q & 1]);
-                    }
-                sums_ready(sum);
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) acc[i][k] = __builtin_fmaf(sum[i][0][k], sc[d][i], acc[i][k]);
-                __builtin_amdgcn_sched_barrier(0);
-                load(d);
-            }
-        }
-        // join the waves' sums; the other buffer is the next item's
-#pragma unroll
-        for (int i = 0; i < 2; ++i) part[buf][wave][i][lane] = acc[i];
-        wait_lgkm0();
-        barrier_nofence();
-        if (wave == (it.tile & (WAVES - 1))) {
-            v4f gate = part[buf][0][0][lane], up = part[buf][0][1][lane];
-#pragma unroll
-            for (int v = 1; v < WAVES; ++v) {
-                gate += part[buf][v][0][lane];
-                up += part[buf][v][1][lane];
-                asm volatile("" : "+v"(gate), "+v"(up)::"memory");        // not all of them in registers at once
-            }
-            const Block& B = R.blocks[it.blk];
-            if (c < B.n) store_h(p, R.pair[B.r0 + c], it.tile * 16 + 4 * g, R.weight[B.r0 + c], gate, up);
-        }
-        it.next(step_blk, step_tile, tiles);
-        if (it.blk >= blocks) return;
-    }
 }
 
 // ---- kernel 2, few rows per expert --------------------------------------------------------------------------------------
@@ -401,11 +317,11 @@ __global__ void __launch_bounds__(DOWN_WAVES * 64) moe_down_kernel(MoeParams p) 
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             const bool in = 64 * s + 16 * g < left;
-            w[d][s] = load16<true>(rw, (in ? vw : OOB) + 64 * s, b * BK);
+            w[d][s] = load16(rw, (in ? vw : OOB) + 64 * s, b * BK);
 #pragma unroll
             for (int j = 0; j < NT; ++j)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) h[d][j][s][q] = load16<false>(rh, (in ? vh[j] : OOB) + 256 * s + 16 * q, 4 * b * BK);
+                for (int q = 0; q < 4; ++q) h[d][j][s][q] = load16(rh, (in ? vh[j] : OOB) + 256 * s + 16 * q, 4 * b * BK);
         }
         sc[d] = load4(rs, (uint32_t)(e * p.s2_e + b * p.s2_k) * 4u + s0);
         lb += DOWN_WAVES;
@@ -467,15 +383,23 @@ __global__ void __launch_bounds__(DOWN_WAVES * 64) moe_down_kernel(MoeParams p) 
 // ahead into registers.  Kernel 2 leaves the pairs' results in fp32, and a third kernel adds up the choices of each token, in their
 // order.
 
-template <bool UP, int NT, int CT>
+// LDS place of 16-byte chunk i of weight row r (128 bytes): i ^ this.
+__device__ __forceinline__ int weight_swz(int r) { return (r & 2) | ((r >> 1) & 4); }
+
+// WV: waves of a workgroup; AH: units under way.
+template <bool UP, int NT, int CT, int WV, int AH>
 struct Rows {
     static constexpr int RT = UP ? 2 : CT;                // tiles of 16 weight rows of a wave: gate and up; channels
-    static constexpr int KB = UP && NT == 1 ? 2 : 1;      // blocks of 128 of a unit
-    static constexpr int ROW = UP ? 256 * KB : 512;       // bytes of a row's unit
-    static constexpr int STAGE = 16 * NT * ROW, DX = STAGE / 1024 / WAVES;    // LDS-DMA instructions of a wave, 1 KiB each
-    static constexpr int SC = UP ? 2 : 1;                 // scales of a block
+    static constexpr int SC = UP ? 2 : 1;                 // scales of a block, per wave
     static constexpr int OUT = UP ? 16 : 16 * CT;         // output channels of a wave
-    static constexpr int LOADS = KB * (2 * RT + SC);      // of a unit, per wave
+    static constexpr int ROW = UP ? 256 : 512;            // bytes of a token's block
+    static constexpr int STAGES = AH + 1;
+    static constexpr int XSTAGE = 16 * NT * ROW, DX = XSTAGE / 1024 / WV;             // of the tokens: bytes, load instructions of a wave
+    static constexpr int WSTAGE = RT * 16 * 128, DW = WSTAGE / 1024;                  // of a wave's weights
+    static constexpr int W_OFF = STAGES * XSTAGE, S_OFF = W_OFF + STAGES * WV * WSTAGE;      // behind them the waves' scales, 256 bytes a stage
+    static constexpr int USED = S_OFF + STAGES * 256, LDS = !UP || USED > TEMP_BYTES ? USED : TEMP_BYTES;
+    static constexpr int LOADS = DX + DW + 1;
+    static_assert(DX >= 1 && (AH - 1) * LOADS <= 63, "vmcnt range");
 };
 
 // LDS place of 16-byte chunk i of row r: the 16 lanes that are served together (0-3, 12-15 and 20-27; 4-11, 16-19 and 28-31) meet 16
@@ -486,164 +410,177 @@ __device__ __forceinline__ int chunk_at(int r, int i) {
     return i ^ (UP ? c : (((c >> 2) ^ (c >> 3)) & 1) | ((c & 3) << 1) | (c & 8));
 }
 
-constexpr int STAGES = 3, AHEAD = 2;
-
-template <bool UP, bool FP16, int NT, int CT>
-__global__ void __launch_bounds__(WAVES * 64, NT <= 2 ? 4 : 2) moe_rows_kernel(MoeParams p, int tiles, int step_blk, int step_tile, int cap) {
-    using C = Rows<UP, NT, CT>;
-    constexpr int STAGE = C::STAGE, DX = C::DX, LPR = C::ROW / 16, RPI = 64 / LPR;     // lanes of a row, rows of an instruction
+#ifndef ROT_E
+#define ROT_E 0
+#define ROT_T 0
+#endif
+template <bool UP, bool FP16, int NT, int CT, int WV, int AH>
+__global__ void __launch_bounds__(WV * 64) moe_rows_kernel(MoeParams p, int tiles) {
+    using C = Rows<UP, NT, CT, WV, AH>;
+    constexpr int BLOCK = 16 * NT, DX = C::DX, DW = C::DW, LPR = C::ROW / 16, RPI = 64 / LPR;       // lanes of a token, tokens of an instruction
     extern __shared__ __attribute__((aligned(1024))) uint8_t rows_lds[];
-    uint8_t* lds = rows_lds;
+    const uint8_t* lds = rows_lds;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4;
     const uint32_t lds0 = lds_addr(lds);
-    const Routed R = load_routing<16 * NT>(p, reinterpret_cast<char*>(lds + STAGES * STAGE), WAVES * 64);
-    const int blocks = __builtin_amdgcn_readfirstlane(*R.count);
-    const int K = UP ? p.H : p.F, N = UP ? p.F : p.H, kb = (K + BK - 1) / BK, units = (kb + AHEAD * C::KB - 1) / (AHEAD * C::KB) * AHEAD;
+    const Routed R = load_routing<BLOCK, UP>(p, reinterpret_cast<char*>(rows_lds + C::LDS), reinterpret_cast<char*>(rows_lds), WV * 64, tiles);
+    const int experts = __builtin_amdgcn_readfirstlane(R.count[0]), items = __builtin_amdgcn_readfirstlane(R.count[1]);
+    const int K = UP ? p.H : p.F, N = UP ? p.F : p.H, kb = (K + BK - 1) / BK, units = (kb + AH - 1) / AH * AH;
     const int64_t ld = UP ? p.ld1 : p.ld2;
-    const v4u rx = buffer_desc(UP ? p.x : p.h, UP ? (uint32_t)(((p.T - 1) * p.ldx + p.H) * 2) : (uint32_t)(p.T * p.k) * (uint32_t)p.F * 4u);
-    const __amdgpu_buffer_rsrc_t rs = make_rsrc(UP ? p.s1 : p.s2, 0x7fffffffu);
     const uint32_t row_bytes = UP ? (uint32_t)p.H * 2u : (uint32_t)p.F * 4u;
-    // what the next loads need: buffers, lane offsets of the tokens' chunks, offsets of the scales, the unit
-    __amdgpu_buffer_rsrc_t rw, ru;
-    uint32_t vx[DX], vc[DX], s_at, s_up;
-    int lu = 0;
-    bool alive;
-    const uint32_t vw = (uint32_t)(c * ld) + 16u * g;
+    const v4u qx = buffer_desc(UP ? p.x : p.h, UP ? (uint32_t)(((p.T - 1) * p.ldx + p.H) * 2) : (uint32_t)(p.T * p.k) * (uint32_t)p.F * 4u);
+    const v4u qs = buffer_desc(UP ? p.s1 : p.s2, 0x7fffffffu);
+    // what the next loads need: the weights' buffers, lane offsets of the tokens' and of the weights' chunks (OOB: nothing), offsets
+    // of the scales, the unit
+    v4u qw, qu;
+    uint32_t vx[DX], vw[UP ? 2 : DW], s_at, s_up;
+    int lu = 0, first = 0, blocks = 0;
+    // the chunk that a lane's 16 bytes of its token are; of its weight row (8 rows an instruction)
+    uint32_t cx[DX], cw[2];
 #pragma unroll
-    for (int i = 0; i < DX; ++i)                          // the chunk that the lane's 16 bytes of its row are
-        vc[i] = 16u * (uint32_t)chunk_at<UP>(RPI * (wave * DX + i) + lane / LPR, lane % LPR);
+    for (int i = 0; i < DX; ++i) cx[i] = 16u * (uint32_t)chunk_at<UP>(RPI * (wave * DX + i) + lane / LPR, lane % LPR);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) cw[i] = 16u * (uint32_t)((lane & 7) ^ weight_swz(8 * i + (lane >> 3)));
     auto aim = [&](const Item& it) {
-        const bool live = it.blk < blocks;
-        const Block& B = R.blocks[live ? it.blk : 0];
-        const int e = __builtin_amdgcn_readfirstlane(B.e), r0 = __builtin_amdgcn_readfirstlane(B.r0), n = __builtin_amdgcn_readfirstlane(B.n);
-        const int n0 = (it.tile * WAVES + wave) * C::OUT, rows = min(C::OUT, N - n0);
-        alive = live && rows > 0;
-        const uint32_t bytes = alive ? (uint32_t)((rows - 1) * ld + K) : 0u;
+        const int n0 = (it.tile * WV + wave) * C::OUT, rows = min(C::OUT, N - n0);
+        const bool alive = it.n > 0 && rows > 0;
         const int at = alive ? n0 : 0;
-        const uint8_t* w = (UP ? p.w1 + e * p.w1_e : p.w2 + e * p.w2_e) + at * ld;
-        rw = make_rsrc(w, bytes);
-        if (UP) ru = make_rsrc(w + p.F * ld, bytes);
-        s_at = (uint32_t)(UP ? e * p.s1_e + at / BK * p.s1_n : e * p.s2_e + at / BK * p.s2_n) * 4u;
-        s_up = UP ? (uint32_t)(e * p.s1_e + (p.F + at) / BK * p.s1_n) * 4u : 0u;
+        const uint32_t bytes = alive ? (uint32_t)((rows - 1) * ld + K) : 0u;
+        const uint8_t* w = (UP ? p.w1 + it.e * p.w1_e : p.w2 + it.e * p.w2_e) + at * ld;
+        qw = buffer_desc(w, bytes);
+        if (UP) qu = buffer_desc(w + p.F * ld, bytes);
+        blocks = alive ? kb : 0;
+#pragma unroll
+        for (int i = 0; i < (UP ? 2 : DW); ++i) {
+            const int row = 8 * i + (lane >> 3);
+            vw[i] = row < rows ? (uint32_t)(row * ld) + cw[i & 1] : OOB;
+        }
+        s_at = (uint32_t)(UP ? it.e * p.s1_e + at / BK * p.s1_n : it.e * p.s2_e + at / BK * p.s2_n) * 4u;
+        s_up = UP ? (uint32_t)(it.e * p.s1_e + (p.F + at) / BK * p.s1_n) * 4u : 0u;
 #pragma unroll
         for (int i = 0; i < DX; ++i) {
             const int row = RPI * (wave * DX + i) + lane / LPR;
             uint32_t v = OOB;
-            if (live && row < n) v = UP ? (uint32_t)(R.pair[r0 + row] / p.k) * (uint32_t)(p.ldx * 2) : (uint32_t)R.pair[r0 + row] * row_bytes;
+            if (row < it.n) v = UP ? (uint32_t)(R.pair[it.r0 + row] / p.k) * (uint32_t)(p.ldx * 2) : (uint32_t)R.pair[it.r0 + row] * row_bytes;
             vx[i] = v;
         }
         lu = 0;
+        first = (3 * it.e + 5 * it.tile) % units;
     };
-    v4u w[AHEAD][C::KB][C::RT][2];
-    float sc[AHEAD][C::KB][C::SC];
-    // the tokens' values of the unit into a stage, the weights of the unit: always the same loads, past the last of nothing
-    auto fetch = [&](int stage, int u) {
-        const uint32_t at = lds0 + (uint32_t)(stage * STAGE + wave * DX * 1024), k0 = (uint32_t)(u * C::ROW);
+    // a unit of the next loads into a stage: always the same instructions, past the last block or item of nothing
+    auto load = [&](int stage, int u) {
+        const int blk = u + first >= units ? u + first - units : u + first;
+        const uint32_t x0 = (uint32_t)(blk * C::ROW), xs = lds0 + (uint32_t)(stage * C::XSTAGE + wave * DX * 1024);
 #pragma unroll
-        for (int i = 0; i < DX; ++i) dma16(rx, __builtin_amdgcn_readfirstlane(at + 1024u * i), vx[i] != OOB && k0 + vc[i] < row_bytes ? vx[i] + k0 + vc[i] : OOB);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int i = 0; i < DX; ++i)
+            dma16(qx, __builtin_amdgcn_readfirstlane(xs + 1024u * i), vx[i] != OOB && x0 + cx[i] < row_bytes ? vx[i] + x0 + cx[i] : OOB);
+        const uint32_t k0 = blk < blocks ? (uint32_t)(blk * BK) : 0u, left = blk < blocks ? (uint32_t)K - k0 : 0u;
+        const uint32_t ws = lds0 + (uint32_t)(C::W_OFF + (stage * WV + wave) * C::WSTAGE);
+#pragma unroll
+        for (int i = 0; i < DW; ++i)
+            dma16_at(UP && i >= 2 ? qu : qw, __builtin_amdgcn_readfirstlane(ws + 1024u * i), cw[i & 1] < left ? vw[UP ? i & 1 : i] : OOB,
+                     __builtin_amdgcn_readfirstlane(k0));
+        // the wave's scales (of the gate rows, of the up rows), by lanes of its own
+        const uint32_t sb = (uint32_t)(min(blk, kb - 1) * (UP ? p.s1_k : p.s2_k)) * 4u;
+        if (lane / C::SC == wave)
+            dma4(qs, __builtin_amdgcn_readfirstlane(lds0 + (uint32_t)(C::S_OFF + stage * 256)), (UP && (lane & 1) ? s_up : s_at) + sb);
     };
-    auto load = [&](int d, int u) {
+    v4f acc[C::RT][NT];
+    // a block of K on the first J blocks of 16 tokens
+    auto block_sums = [&](auto blocks_of_16, int stage) {
+        constexpr int J = decltype(blocks_of_16)::value, PARTS = UP ? 1 : 2;
+        const uint8_t *xs = lds + stage * C::XSTAGE + c * C::ROW, *ws = lds + C::W_OFF + (stage * WV + wave) * C::WSTAGE + c * 128;
+        v4f sum[C::RT][J];
+        v4u w[C::RT][2];
+        float scale[C::SC];
 #pragma unroll
-        for (int b = 0; b < C::KB; ++b) {
-            const int blk = u * C::KB + b, k0 = alive && blk < kb ? blk * BK : 0, left = alive && blk < kb ? K - k0 : 0;
+        for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const bool in = 64 * s + 16 * g < left;
+            for (int i = 0; i < C::RT; ++i)
+                w[i][s] = *reinterpret_cast<const v4u*>(ws + 2048 * i + 16 * ((4 * s + g) ^ weight_swz(c)));
 #pragma unroll
-                for (int i = 0; i < C::RT; ++i)
-                    w[d][b][i][s] = load16<true>(UP && i ? ru : rw, (in ? vw + (UP ? 0u : (uint32_t)(16 * i * ld)) : OOB) + 64 * s, k0);
-            }
-            const uint32_t sb = (uint32_t)(min(blk, kb - 1) * (UP ? p.s1_k : p.s2_k)) * 4u;
-            sc[d][b][0] = load4(rs, s_at + sb);
-            if (UP) sc[d][b][C::SC - 1] = load4(rs, s_up + sb);
+        for (int i = 0; i < C::SC; ++i) scale[i] = *reinterpret_cast<const float*>(lds + C::S_OFF + stage * 256 + 4 * (wave * C::SC + i));
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {                     // half a block's values first, then its products
+            v4u t[2][J][PARTS];
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+                for (int j = 0; j < J; ++j)
+#pragma unroll
+                    for (int h = 0; h < PARTS; ++h)
+                        t[q][j][h] = *reinterpret_cast<const v4u*>(
+                            xs + 16 * j * C::ROW + 16 * chunk_at<UP>(c, UP ? 8 * s + 2 * g + q : 4 * (4 * s + g) + q + 2 * h));
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+                for (int h = 0; h < PARTS; ++h)
+#pragma unroll
+                    for (int j = 0; j < J; ++j)
+#pragma unroll
+                        for (int i = 0; i < C::RT; ++i) {
+                            const uint32_t lo = w[i][s][2 * q], hi = w[i][s][2 * q + 1];
+                            if (s + q + h == 0) mfma<UP && FP16, true>(sum[i][j], lo, hi, t[q][j][h]);
+                            else mfma<UP && FP16, false>(sum[i][j], lo, hi, t[q][j][h]);
+                        }
         }
-        __builtin_amdgcn_sched_barrier(0);                // in this order: the waits count them
+        sums_ready(sum);
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+            for (int i = 0; i < C::RT; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[i][j][k] = __builtin_fmaf(sum[i][j][k], scale[UP ? i : 0], acc[i][j][k]);
     };
-    Item it{(int)blockIdx.x / tiles, (int)blockIdx.x % tiles}, nx = it;
-    if (it.blk >= blocks) return;
+    const int step = (int)gridDim.x / XCDS;
+    int next = (int)blockIdx.x / XCDS;
+    Item it = item_at<BLOCK>(R, experts, items, next, tiles, lane);
+    if (it.n == 0) return;
     aim(it);
 #pragma unroll
-    for (int d = 0; d < AHEAD; ++d) {
-        fetch(d, d);
-        load(d, d);
-    }
+    for (int d = 0; d < AH; ++d) load(d, d);
     for (int stage = 0;;) {
-        const Block B = R.blocks[it.blk];
-        const int n = __builtin_amdgcn_readfirstlane(B.n);
-        v4f acc[C::RT][NT];
 #pragma unroll
         for (int i = 0; i < C::RT; ++i)
 #pragma unroll
             for (int j = 0; j < NT; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
-        for (int u = 0; u < units; u += AHEAD) {
-            if (u + AHEAD < units) lu += AHEAD;
-            else nx.next(step_blk, step_tile, tiles), aim(nx);
+        Item nx = it;
+        for (int u = 0; u < units; u += AH) {
+            if (u + AH < units) {
+                lu += AH;
+            } else {
+                next += step;
+                nx = item_at<BLOCK>(R, experts, items, next, tiles, lane);
+                aim(nx);
+            }
 #pragma unroll
-            for (int d = 0; d < AHEAD; ++d) {
-                // this wave's share of the unit has landed (behind it: its weights, the next unit's both), and its reads of the last one
-                __builtin_amdgcn_s_waitcnt(vmcnt_imm(AHEAD * C::LOADS + (AHEAD - 1) * DX));
+            for (int d = 0; d < AH; ++d) {
+                // this wave's share of the unit has landed, its reads of the last one have returned, and so have all waves'
+                __builtin_amdgcn_s_waitcnt(vmcnt_imm((AH - 1) * C::LOADS));
                 wait_lgkm0();
                 barrier_nofence();
-                const int free = stage == 0 ? STAGES - 1 : stage - 1;             // the last one's place
-                fetch(free, lu + d);
-                const uint8_t* st = lds + stage * STAGE;
-#pragma unroll
-                for (int b = 0; b < C::KB; ++b) {
-                    v4f sum[C::RT][NT];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-#pragma unroll
-                        for (int j = 0; j < NT; ++j) {
-                            if (j && 16 * j >= n) continue;   // uniform
-                            const int chunk = UP ? 16 * b + 8 * (q >> 1) + 2 * g + (q & 1) : 4 * (4 * (q >> 1) + g) + (q & 1);
-                            const uint8_t* row = st + (16 * j + c) * C::ROW;
-                            const v4u t = *reinterpret_cast<const v4u*>(row + 16 * chunk_at<UP>(c, chunk));
-#pragma unroll
-                            for (int i = 0; i < C::RT; ++i) {
-                                const uint32_t lo = w[d][b][i][q >> 1][2 * (q & 1)], hi = w[d][b][i][q >> 1][2 * (q & 1) + 1];
-                                if (q == 0) mfma<UP && FP16, true>(sum[i][j], lo, hi, t);
-                                else mfma<UP && FP16, false>(sum[i][j], lo, hi, t);
-                            }
-                            if (!UP) {
-                                const v4u t2 = *reinterpret_cast<const v4u*>(row + 16 * chunk_at<UP>(c, chunk + 2));
-#pragma unroll
-                                for (int i = 0; i < C::RT; ++i)
-                                    mfma<false, false>(sum[i][j], w[d][b][i][q >> 1][2 * (q & 1)], w[d][b][i][q >> 1][2 * (q & 1) + 1], t2);
-                            }
-                        }
-                    sums_ready(sum);
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        if (j && 16 * j >= n) continue;
-#pragma unroll
-                        for (int i = 0; i < C::RT; ++i)
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) acc[i][j][k] = __builtin_fmaf(sum[i][j][k], sc[d][b][UP ? i : 0], acc[i][j][k]);
-                    }
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-                load(d, lu + d);
-                stage = stage == STAGES - 1 ? 0 : stage + 1;
+                load(stage == 0 ? C::STAGES - 1 : stage - 1, lu + d);         // in the last one's place
+                if (NT == 1 || it.n <= 16) block_sums(std::integral_constant<int, 1>(), stage);
+                else block_sums(std::integral_constant<int, NT>(), stage);
+                stage = stage == C::STAGES - 1 ? 0 : stage + 1;
             }
         }
-        const int n0 = (it.tile * WAVES + wave) * C::OUT + 4 * g;
+        const int n0 = (it.tile * WV + wave) * C::OUT + 4 * g;
 #pragma unroll
         for (int j = 0; j < NT; ++j)
-            if (16 * j + c < n) {
-                const int pair = R.pair[B.r0 + 16 * j + c];
+            if (16 * j + c < it.n) {
+                const int pair = R.pair[it.r0 + 16 * j + c];
                 if constexpr (UP) {
-                    if (n0 < N) store_h(p, pair, n0, R.weight[B.r0 + 16 * j + c], acc[0][j], acc[1][j]);
+                    if (n0 < N) store_h(p, pair, n0, R.weight[it.r0 + 16 * j + c], acc[0][j], acc[1][j]);
                 } else {
 #pragma unroll
                     for (int i = 0; i < C::RT; ++i)
                         if (n0 + 16 * i < N) *reinterpret_cast<v4f*>(p.z + (int64_t)pair * p.H + n0 + 16 * i) = acc[i][j];
                 }
             }
-        it.next(step_blk, step_tile, tiles);
-        if (it.blk >= blocks) break;
+        it = nx;
+        if (it.n == 0) break;
     }
     wait_vm0();                                           // the loads behind the last unit have landed before the exit
 }
@@ -662,28 +599,21 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(MoeParams p) {
     store_y(p, t, n, v);
 }
 
-template <bool UP, bool FP16, int NT, int CT>
+template <bool UP, bool FP16, int NT, int WV>
 int launch_rows(const MoeParams& p, hipStream_t st) {
-    const int out = WAVES * Rows<UP, NT, CT>::OUT, tiles = ((UP ? p.F : p.H) + out - 1) / out, P = p.T * p.k, cap = max_blocks<16 * NT>(p.E, P);
-    const size_t lds = STAGES * Rows<UP, NT, CT>::STAGE + routed_bytes<16 * NT>(p.E, P);
-    const int grid = (int)std::min<int64_t>((int64_t)tiles * cap, (NT <= 2 ? 2 : 1) * h3host::cu_count());
-    hipLaunchKernelGGL((moe_rows_kernel<UP, FP16, NT, CT>), dim3(grid), dim3(WAVES * 64), lds, st, p, tiles, grid / tiles, grid % tiles, cap);
+    constexpr int CT = 2, AH = 2;
+    using C = Rows<UP, NT, CT, WV, AH>;
+    const int out = WV * C::OUT, tiles = ((UP ? p.F : p.H) + out - 1) / out, P = p.T * p.k, most = std::min(p.E, P) + P / (16 * NT);
+    const size_t lds = C::LDS + routed_bytes(p.E, P, UP);
+    // 8 waves per CU
+    const int64_t grid = std::min<int64_t>(((int64_t)tiles * most + XCDS - 1) / XCDS * XCDS, std::max(XCDS, 8 / WV * h3host::cu_count() / XCDS * XCDS));
+    hipLaunchKernelGGL((moe_rows_kernel<UP, FP16, NT, CT, WV, AH>), dim3((unsigned)grid), dim3(WV * 64), lds, st, p, tiles);
     H3_CHECK_HIP(hipGetLastError());
     return H3FP8_OK;
 }
 
 int launch_combine(const MoeParams& p, hipStream_t st) {
     hipLaunchKernelGGL(moe_combine_kernel, dim3((unsigned)((p.H + 1023) / 1024), (unsigned)p.T), dim3(256), 0, st, p);
-    H3_CHECK_HIP(hipGetLastError());
-    return H3FP8_OK;
-}
-
-template <bool FP16, int D>
-int launch_up(const MoeParams& p, hipStream_t st) {
-    const int tiles = p.F / 16, P = p.T * p.k;
-    const int grid = (int)std::min<int64_t>((int64_t)tiles * max_blocks<16>(p.E, P), 2 * h3host::cu_count());
-    hipLaunchKernelGGL((moe_up_kernel<FP16, D>), dim3(grid), dim3(WAVES * 64), routed_bytes<16>(p.E, P), st, p, tiles, grid / tiles,
-                       grid % tiles);
     H3_CHECK_HIP(hipGetLastError());
     return H3FP8_OK;
 }
@@ -697,25 +627,19 @@ int launch_down(const MoeParams& p, hipStream_t st) {
 }
 
 // Which kernels run (host only; for the workspace too).
-bool by_rows(int64_t T, int64_t k, int64_t E) { return T > 16 || T * k > 4 * E; }
-
-template <bool FP16, int NT>
-int run_rows(const MoeParams& p, hipStream_t st) {
-    int rc = launch_rows<true, FP16, NT, 1>(p, st);
-    if (!rc) rc = launch_rows<false, false, NT, 2>(p, st);
-    return rc ? rc : launch_combine(p, st);
-}
+bool by_rows(int64_t T, int64_t k, int64_t E) { return T > 16 || T * k > 16; }
 
 template <bool FP16>
 int run(const MoeParams& p, hipStream_t st) {
-    if (by_rows(p.T, p.k, p.E)) {
-        const int mean = (p.T * p.k + p.E - 1) / p.E;
-        if (mean <= 8) return run_rows<FP16, 1>(p, st);
-        if (mean <= 24) return run_rows<FP16, 2>(p, st);
-        return run_rows<FP16, 4>(p, st);
+    if (!by_rows(p.T, p.k, p.E)) {
+        const int rc = launch_rows<true, FP16, 1, 4>(p, st);
+        return rc ? rc : launch_down<1, 2>(p, st);
     }
-    const int rc = launch_up<FP16, 2>(p, st);
-    return rc ? rc : launch_down<1, 2>(p, st);
+    const bool many = p.T * p.k > 20 * p.E;
+    int rc = many ? launch_rows<true, FP16, 2, 8>(p, st) : launch_rows<true, FP16, 1, 4>(p, st);
+    if (rc) return rc;
+    rc = many && (int64_t)p.H * p.E >= 256 * h3host::cu_count() ? launch_rows<false, false, 2, 8>(p, st) : launch_rows<false, false, 1, 4>(p, st);
+    return rc ? rc : launch_combine(p, st);
 }
 
 constexpr int64_t kMaxSpan = 0x7fff0000LL;
