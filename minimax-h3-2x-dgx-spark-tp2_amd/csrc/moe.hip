@@ -244,135 +244,199 @@ __device__ __forceinline__ void store_y(const MoeParams& p, int t, int n, v4f v)
     *reinterpret_cast<uint2*>(p.y + t * p.ldy + n) = o;
 }
 
-// ---- kernel 2, few rows per expert --------------------------------------------------------------------------------------
+// ---- a token or a few -----------------------------------------------------------------------------------------------------
 //
-// A workgroup takes 16 channels for all experts; its 16 waves share out the units, the blocks of F of every expert that has rows.
-// Column c of the MFMAs is token 16 j + c, zero where it is not the expert's, so that the accumulators run over all experts.
+// What counts is how soon the weights' bytes are asked for.  The pairs, at most 64, are a lane each: the experts that have
+// pairs, the pairs of one and their tokens come out of ballots on one load of `experts`, by every wave for itself.
 
-constexpr int DOWN_WAVES = 16;
+constexpr int FEW = 64;                                   // pairs
+constexpr int UP_WAVES = 8, DOWN_WAVES = 16;
 
-// NT: blocks of 16 tokens (all of them); D: units in flight per wave.
-template <int NT, int D>
-__global__ void __launch_bounds__(DOWN_WAVES * 64) moe_down_kernel(MoeParams p) {
-    constexpr int THREADS = DOWN_WAVES * 64;
-    extern __shared__ __attribute__((aligned(16))) char down_lds[];
-    v4f(*part)[NT][64] = reinterpret_cast<v4f(*)[NT][64]>(down_lds);                            // [DOWN_WAVES]
-    int* s_expert = reinterpret_cast<int*>(down_lds + sizeof(v4f) * DOWN_WAVES * NT * 64);      // the experts that have pairs
-    uint16_t* s_slot = reinterpret_cast<uint16_t*>(s_expert + MAX_E);                           // ... and where an expert is among them
-    uint8_t* s_map = reinterpret_cast<uint8_t*>(s_slot + MAX_E);                                // [slots][16 NT]: 1 + the token's choice, or 0
+// Each token's first pair among the pairs `same` (of one expert): the second of two equal choices is not a row of its own.
+__device__ __forceinline__ uint64_t first_pairs(uint64_t same, int lane, int k) {
+    const int t = lane / k;
+    return same & __ballot(((same >> (t * k)) & ((1ull << (lane - t * k)) - 1)) == 0);
+}
+
+// Kernel 1: a workgroup takes 16 gate rows and the up rows that belong to them, of one expert; its 8 waves share out the blocks of K,
+// D each under way, and join through LDS.
+template <bool FP16, int D>
+__global__ void __launch_bounds__(UP_WAVES * 64, 4) moe_few_up_kernel(MoeParams p, int tiles) {
+    __shared__ v4f part[UP_WAVES][2][64];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int c = lane & 15, g = lane >> 4;
-    const int n0 = (int)blockIdx.x * 16, P = p.T * p.k, cap = min(p.E, P);
-    // the pairs' experts, under way together with the offsets
-    constexpr int MINE = (16 * NT * MAX_K + THREADS - 1) / THREADS;
-    int experts[MINE];
-#pragma unroll
-    for (int i = 0; i < MINE; ++i) {
-        const int q = threadIdx.x + i * THREADS;
-        experts[i] = q < P ? p.experts[q] : -1;
+    const int c = lane & 15, g = lane >> 4, P = p.T * p.k;
+    const int mine = lane < P ? p.experts[lane] : -1;
+    const float weight = lane < P ? p.weights[lane] : 0.0f;
+    int slot = (int)blockIdx.x / tiles;
+    const int f0 = ((int)blockIdx.x - slot * tiles) * 16;
+    uint64_t left = __ballot(mine >= 0 && mine < p.E), same = 0;
+    int e = 0;
+    for (; left; --slot) {
+        e = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
+        same = __ballot(mine == e);
+        if (slot == 0) break;
+        left &= ~same;
     }
-    for (int i = threadIdx.x; i < cap * 4 * NT; i += THREADS) reinterpret_cast<uint32_t*>(s_map)[i] = 0;
-    int active = 0;
-    for (int e0 = 0; e0 < p.E; e0 += 64) {                // every wave counts, the first one writes
-        const int e = e0 + lane;
-        const bool in = e < p.E && offset_at(p, e + 1) > offset_at(p, e);
-        const uint64_t has = __ballot(in);
-        const int at = active + __popcll(has & ((1ull << lane) - 1));
-        if (wave == 0 && e < p.E) {
-            s_slot[e] = in && at < cap ? (uint16_t)at : (uint16_t)0xffff;
-            if (in && at < cap) s_expert[at] = e;
+    if (!left) return;
+    const uint64_t rows = first_pairs(same, lane, p.k);
+    const int n = __popcll(rows);
+    // column c: the c-th of the rows
+    const int at = (rows >> lane) & 1 ? __popcll(rows & ((1ull << lane) - 1)) : 63;
+    const int pair = __builtin_amdgcn_ds_permute(4 * at, lane), col = __shfl(pair, c, 64);
+    const int kb = (p.H + BK - 1) / BK;
+    const uint8_t* w0 = p.w1 + e * p.w1_e + f0 * p.ld1;
+    const uint32_t bytes = (uint32_t)(15 * p.ld1 + p.H);
+    const __amdgpu_buffer_rsrc_t rg = make_rsrc(w0, bytes), ru = make_rsrc(w0 + p.F * p.ld1, bytes), rs = make_rsrc(p.s1, 0x7fffffffu);
+    const __amdgpu_buffer_rsrc_t rx = make_rsrc(p.x, (uint32_t)(((p.T - 1) * p.ldx + p.H) * 2));
+    const uint32_t vw = (uint32_t)(c * p.ld1) + 16u * g, vx = c < n ? (uint32_t)(col / p.k) * (uint32_t)(p.ldx * 2) + 32u * g : OOB;
+    const uint32_t sg = (uint32_t)(e * p.s1_e + f0 / BK * p.s1_n) * 4u, su = (uint32_t)(e * p.s1_e + (p.F + f0) / BK * p.s1_n) * 4u;
+    v4u w[D][2][2], x[D][2][2];
+    float sc[D][2];
+    // always the same loads, past the last block of nothing, so that the count of those under way is known
+    auto load = [&](int d, int b) {
+        const int k0 = b < kb ? b * BK : 0, rest = b < kb ? p.H - k0 : 0;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const bool in = 64 * s + 16 * g < rest;
+            w[d][0][s] = load16(rg, (in ? vw : OOB) + 64 * s, k0);
+            w[d][1][s] = load16(ru, (in ? vw : OOB) + 64 * s, k0);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) x[d][s][q] = load16(rx, (in ? vx : OOB) + 128 * s + 16 * q, 2 * k0);
         }
-        active += __popcll(has);
-    }
-    active = min(active, cap);
-    __syncthreads();
+        const uint32_t sb = (uint32_t)(min(b, kb - 1) * p.s1_k) * 4u;
+        sc[d][0] = load4(rs, sg + sb);
+        sc[d][1] = load4(rs, su + sb);
+        __builtin_amdgcn_sched_barrier(0);                // in this order: the waits count them
+    };
 #pragma unroll
-    for (int i = 0; i < MINE; ++i) {
-        const int q = threadIdx.x + i * THREADS, e = experts[i];
-        if (e >= 0 && e < p.E && s_slot[e] != 0xffff) s_map[s_slot[e] * 16 * NT + q / p.k] = (uint8_t)(1 + q % p.k);
+    for (int d = 0; d < D; ++d) load(d, wave + d * UP_WAVES);
+    v4f acc[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
+    for (int b = wave; b < kb; b += D * UP_WAVES) {
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            v4f sum[2][1];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)                   // 32 of the block's k each
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const v4u& a = w[d][i][q >> 1];
+                    if (q == 0) mfma<FP16, true>(sum[i][0], a[0], a[1], x[d][0][0]);
+                    else mfma<FP16, false>(sum[i][0], a[2 * (q & 1)], a[2 * (q & 1) + 1], x[d][q >> 1][q & 1]);
+                }
+            sums_ready(sum);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[i][k] = __builtin_fmaf(sum[i][0][k], sc[d][i], acc[i][k]);
+            __builtin_amdgcn_sched_barrier(0);
+            load(d, b + (d + D) * UP_WAVES);
+        }
     }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) part[wave][i][lane] = acc[i];
     __syncthreads();
-    const int fb = (p.F + BK - 1) / BK, units = active * fb;
+    if (wave != 0) return;
+    v4f gate = part[0][0][lane], up = part[0][1][lane];
+#pragma unroll
+    for (int v = 1; v < UP_WAVES; ++v) {
+        gate += part[v][0][lane];
+        up += part[v][1][lane];
+    }
+    float sum = 0.0f;                                     // of all the token's choices of this expert
+    for (uint64_t m = same; m; m &= m - 1) {
+        const int q = __builtin_ctzll(m);
+        const float wq = u2f(__builtin_amdgcn_readlane((int)f2u(weight), q));
+        sum += q / p.k == col / p.k ? wq : 0.0f;
+    }
+    if (c < n) store_h(p, col, f0 + 4 * g, sum, gate, up);
+}
+
+// Kernel 2: a workgroup takes 16 channels for all experts; its 16 waves share out the units, the blocks of F of every expert that has
+// pairs.  Column c of the MFMAs is token c, zero where it is not the expert's, so that the accumulators run over all experts.
+template <int D>
+__global__ void __launch_bounds__(DOWN_WAVES * 64) moe_few_down_kernel(MoeParams p) {
+    __shared__ v4f part[DOWN_WAVES][64];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int c = lane & 15, g = lane >> 4, P = p.T * p.k, n0 = (int)blockIdx.x * 16;
+    const int mine = lane < P ? p.experts[lane] : -1;
+    const uint64_t all = __ballot(mine >= 0 && mine < p.E);
+    const int fb = (p.F + BK - 1) / BK;
     const __amdgpu_buffer_rsrc_t rh = make_rsrc(p.h, (uint32_t)P * (uint32_t)p.F * 4u), rs = make_rsrc(p.s2, 0x7fffffffu);
     const uint32_t vw = (uint32_t)(c * p.ld2) + 16u * g, wbytes = (uint32_t)(15 * p.ld2 + p.F);
     const uint8_t* w0 = p.w2 + n0 * p.ld2;
     const uint32_t s0 = (uint32_t)(n0 / BK * p.s2_n) * 4u;
-    v4u w[D][2], h[D][NT][2][4];                          // h: 16 values, what they leave
+    // the units of a wave: block b of the expert at hand, whose pairs are the first of `left`
+    struct Unit { uint64_t left, same; int e, b; };
+    auto settle = [&](Unit& u) {                          // ... to where b is one of the expert's blocks, or nothing is left
+        for (;;) {
+            if (u.left) {
+                u.e = __builtin_amdgcn_readlane(mine, __builtin_ctzll(u.left));
+                u.same = __ballot(mine == u.e);
+            }
+            if (!u.left || u.b < fb) return;
+            u.b -= fb;
+            u.left &= ~u.same;
+        }
+    };
+    v4u w[D][2], h[D][2][4];                              // h: 16 values, what they leave
     float sc[D];
-    int ls = 0, lb = wave;                                // the next unit's expert and block
-    while (lb >= fb && ls < active) lb -= fb, ++ls;
+    bool has[D];                                          // token c is the expert's
+    Unit next{all, 0, 0, wave};
+    settle(next);
     // always the same loads, past the last unit of nothing, so that the count of those under way is known
     auto load = [&](int d) {
-        const bool live = ls < active;
-        const int slot = live ? ls : 0, b = live ? lb : 0, e = __builtin_amdgcn_readfirstlane(s_expert[slot]);
-        const int left = live ? p.F - b * BK : 0;
+        const bool live = next.left != 0;
+        const int b = live ? next.b : 0, e = live ? next.e : 0, rest = live ? p.F - b * BK : 0;
+        const uint64_t pairs = live && c < p.T ? (next.same >> (c * p.k)) & ((1ull << p.k) - 1) : 0;
+        has[d] = pairs != 0;
+        const uint32_t vh = pairs ? (uint32_t)(c * p.k + __builtin_ctzll(pairs)) * (uint32_t)p.F * 4u + 64u * g : OOB;
         const __amdgpu_buffer_rsrc_t rw = make_rsrc(w0 + e * p.w2_e, live ? wbytes : 0u);
-        uint32_t vh[NT];
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            const int m = s_map[slot * 16 * NT + 16 * j + c];
-            vh[j] = m ? (uint32_t)((16 * j + c) * p.k + m - 1) * (uint32_t)p.F * 4u + 64u * g : OOB;
-        }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const bool in = 64 * s + 16 * g < left;
+            const bool in = 64 * s + 16 * g < rest;
             w[d][s] = load16(rw, (in ? vw : OOB) + 64 * s, b * BK);
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) h[d][j][s][q] = load16(rh, (in ? vh[j] : OOB) + 256 * s + 16 * q, 4 * b * BK);
+            for (int q = 0; q < 4; ++q) h[d][s][q] = load16(rh, (in ? vh : OOB) + 256 * s + 16 * q, 4 * b * BK);
         }
         sc[d] = load4(rs, (uint32_t)(e * p.s2_e + b * p.s2_k) * 4u + s0);
-        lb += DOWN_WAVES;
-        while (lb >= fb && ls < active) lb -= fb, ++ls;
+        next.b += DOWN_WAVES;
+        settle(next);
         __builtin_amdgcn_sched_barrier(0);                // in this order: the waits count them
     };
-    v4f acc[NT];
+    v4f acc = v4f{0.f, 0.f, 0.f, 0.f};
+    bool more = next.left != 0;
 #pragma unroll
-    for (int j = 0; j < NT; ++j) acc[j] = v4f{0.f, 0.f, 0.f, 0.f};
-    if (units > 0) {
-#pragma unroll
-        for (int d = 0; d < D; ++d) load(d);
-    }
-    int slot = 0, b = wave;                               // of the unit at hand
-    while (b >= fb && slot < active) b -= fb, ++slot;
-    for (int u0 = wave; u0 < units; u0 += D * DOWN_WAVES) {
+    for (int d = 0; d < D; ++d) load(d);
+    while (more) {
+        more = next.left != 0;                            // units of the round behind the loads under way
 #pragma unroll
         for (int d = 0; d < D; ++d) {
-            v4f sum[1][NT];
+            v4f sum[1][1];
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    const uint32_t lo = w[d][q >> 1][2 * (q & 1)], hi = w[d][q >> 1][2 * (q & 1) + 1];
-                    if (q == 0) mfma<false, true>(sum[0][j], lo, hi, h[d][j][0][0]);
-                    else mfma<false, false>(sum[0][j], lo, hi, h[d][j][q >> 1][q & 1]);
-                    mfma<false, false>(sum[0][j], lo, hi, h[d][j][q >> 1][2 + (q & 1)]);
-                }
+            for (int q = 0; q < 4; ++q) {
+                const uint32_t lo = w[d][q >> 1][2 * (q & 1)], hi = w[d][q >> 1][2 * (q & 1) + 1];
+                if (q == 0) mfma<false, true>(sum[0][0], lo, hi, h[d][0][0]);
+                else mfma<false, false>(sum[0][0], lo, hi, h[d][q >> 1][q & 1]);
+                mfma<false, false>(sum[0][0], lo, hi, h[d][q >> 1][2 + (q & 1)]);
+            }
             sums_ready(sum);
+            if (has[d]) {                                 // an expert's NaN is not another token's
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
-                if (slot < active && s_map[slot * 16 * NT + 16 * j + c] != 0) {       // an expert's NaN is not another token's
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[j][r] = __builtin_fmaf(sum[0][j][r], sc[d], acc[j][r]);
-                }
+                for (int r = 0; r < 4; ++r) acc[r] = __builtin_fmaf(sum[0][0][r], sc[d], acc[r]);
+            }
             __builtin_amdgcn_sched_barrier(0);
-            load(d);
-            b += DOWN_WAVES;
-            while (b >= fb && slot < active) b -= fb, ++slot;
+            if (more) load(d);
         }
     }
-#pragma unroll
-    for (int j = 0; j < NT; ++j) part[wave][j][lane] = acc[j];
+    part[wave][lane] = acc;
     __syncthreads();
-    if (threadIdx.x < NT * 64) {
-        const int j = threadIdx.x >> 6, t = 16 * j + c, n = n0 + 4 * g;
-        v4f v = part[0][j][lane];
+    if (wave != 0) return;
+    v4f v = part[0][lane];
 #pragma unroll
-        for (int q = 1; q < DOWN_WAVES; ++q) v += part[q][j][lane];
-        if (t < p.T) store_y(p, t, n, v);
-    }
+    for (int q = 1; q < DOWN_WAVES; ++q) v += part[q][lane];
+    if (c < p.T) store_y(p, c, n0 + 4 * g, v);
 }
 
 // ---- more rows per expert -----------------------------------------------------------------------------------------------
@@ -618,23 +682,32 @@ int launch_combine(const MoeParams& p, hipStream_t st) {
     return H3FP8_OK;
 }
 
-template <int NT, int D>
-int launch_down(const MoeParams& p, hipStream_t st) {
-    const size_t lds = sizeof(v4f) * DOWN_WAVES * NT * 64 + 6 * MAX_E + (size_t)std::min(p.E, p.T * p.k) * 16 * NT;
-    hipLaunchKernelGGL((moe_down_kernel<NT, D>), dim3((unsigned)(p.H / 16)), dim3(DOWN_WAVES * 64), lds, st, p);
+template <bool FP16>
+int launch_few(const MoeParams& p, hipStream_t st) {
+    const int tiles = p.F / 16;
+    hipLaunchKernelGGL((moe_few_up_kernel<FP16, 2>), dim3((unsigned)(tiles * std::min(p.E, p.T * p.k))), dim3(UP_WAVES * 64), 0, st, p, tiles);
+    H3_CHECK_HIP(hipGetLastError());
+    hipLaunchKernelGGL((moe_few_down_kernel<2>), dim3((unsigned)(p.H / 16)), dim3(DOWN_WAVES * 64), 0, st, p);
     H3_CHECK_HIP(hipGetLastError());
     return H3FP8_OK;
 }
 
-// Which kernels run (host only; for the workspace too).
-bool by_rows(int64_t T, int64_t k, int64_t E) { return T > 16 || T * k > 16; }
+// ---- which kernels run --------------------------------------------------------------------------------------------------
+//
+// A token or a few, while launches and first loads count (up to 8 pairs, 128 MiB of their experts' weights); then by rows.  us of
+// the kernels, few / by rows, 32 experts of 4096 x 2048: 4 pairs 26 / 40, 8 53 / 47, 16 88 / 73; 8 of 2048 x 2048: 4 pairs 22 / 32,
+// 8 30 / 32, 16 38 / 32; 16 of 1200 x 1040: 4 pairs 14 / 26, 8 23 / 27, 16 28 / 27.
+bool few(int64_t T, int64_t k, int64_t H, int64_t F, int64_t E) {
+    return T * k <= 8 && 3 * H * F * std::min(T * k, E) <= (128LL << 20);
+}
 
 template <bool FP16>
 int run(const MoeParams& p, hipStream_t st) {
-    if (!by_rows(p.T, p.k, p.E)) {
-        const int rc = launch_rows<true, FP16, 1, 4>(p, st);
-        return rc ? rc : launch_down<1, 2>(p, st);
-    }
+    if (few(p.T, p.k, p.H, p.F, p.E)) return launch_few<FP16>(p, st);
+    // Blocks of 32 rows and 8 waves past 20 rows per expert, in kernel 2 while they are items enough for the CUs (one of 256
+    // channels and all rows of an expert at least); else blocks of 16 and 4 waves.  us, 16 rows and 4 waves / 32 and 8, kernel 1 and
+    // kernel 2: 32 experts of 4096 x 2048, 12 rows each 104 / 98 and 58 / 58, 16 110 / 122 and 64 / 71, 24 132 / 117 and 77 / 75,
+    // 32 150 / 115 and 110 / 79; 8 experts of 2048 x 2048, 32 rows 27 / 22 and 19 / 25; 16 of 1200 x 1040, 32 rows 21 / 17 and 15 / 19.
     const bool many = p.T * p.k > 20 * p.E;
     int rc = many ? launch_rows<true, FP16, 2, 8>(p, st) : launch_rows<true, FP16, 1, 4>(p, st);
     if (rc) return rc;
@@ -647,7 +720,7 @@ constexpr int64_t kMaxSpan = 0x7fff0000LL;
 }  // namespace
 
 extern "C" int64_t h3fp8_moe_blocks_workspace(int64_t T, int64_t k, int64_t H, int64_t F, int64_t E) {
-    return T < 0 || k < 0 || H < 0 || F < 0 ? 0 : T * k * 4 * (by_rows(T, k, E) ? F + H : F);
+    return T < 0 || k < 0 || H < 0 || F < 0 || E < 0 ? 0 : T * k * 4 * (few(T, k, H, F, E) ? F : F + H);
 }
 
 extern "C" int h3fp8_moe_blocks(const void* x, int64_t ldx, int dtype, int64_t T, int64_t H, int64_t F, int64_t E, int k,
