@@ -9,11 +9,14 @@
 // Pair p = t k + j; order = the pairs by expert, each expert's in ascending p, then those without an expert; place[p] = where p
 // went; offsets[e] = the first place of expert e.
 //
-// A wave takes one token: lane l holds the logits V l .. V l + V - 1 as unsigned keys of the same order, so that a round is a
-// maximum over the lanes (DPP) and the lowest lane that has it; a workgroup of 16 waves takes 128 tokens at a time, and
-// ranks their pairs in LDS: the lanes of 64 consecutive pairs with the same expert by one ballot per bit of its number,
-// then the 64s in turn.  Up to 128 tokens one workgroup does it all; past that a second launch adds up the counts of the
-// workgroups before its own (at most 512) and moves the ranks to their places.
+// 16 lanes take a token, a wave four; a lane holds V = E / 16 of its logits as unsigned keys of the same order, so that a round
+// is a maximum over the lane's keys and over the 16 lanes (DPP).  With a bias the rounds run on
+// fp32 scores, and what could be among the k best by their error, at most 16 experts a token, is scored and ranked again in 64
+// bits, a lane each (the 64-bit exponentials and divisions of all scores were most of the time: 64 tokens x 256 experts, sigmoid,
+// 32 us); only where more are within that error, all are.
+// A workgroup of 16 waves takes 64 tokens at a time, and ranks the pairs of 128 in LDS: the lanes of 64 consecutive pairs with the
+// same expert by one ballot per bit of its number, then the 64s in turn.  Up to 128 tokens one workgroup does it all; past that
+// a second launch adds up the counts of the workgroups before its own (at most 512) and moves the ranks to their places.
 #include <algorithm>
 
 #include "h3fp8_common.h"
@@ -22,8 +25,8 @@ namespace {
 
 using namespace h3;
 
-constexpr int TB = 128;                                   // tokens of a batch
-constexpr int WAVES = 16;
+constexpr int TB = 128;                                   // tokens of a batch; what one workgroup takes without a second launch
+constexpr int WAVES = 16;                                 // of a workgroup; 8 where a lane holds 32 logits and 64-bit scores
 constexpr int MAX_BLOCKS = 512;
 constexpr int MAX_E = 512, MAX_K = 16;
 constexpr int CHUNKS = TB * MAX_K / 64;                   // of 64 pairs, in a batch
@@ -41,8 +44,10 @@ struct RouteArgs {
     int* offsets;
     int* order;
     int* place;
-    int* counts;                                          // [blocks, E + 1]: pairs per expert (E: without one)
-    int per;                                              // tokens per workgroup, a multiple of TB
+    int* counts;                                          // [blocks, row]: pairs per expert (E: without one)
+    int row;                                              // E + 1 rounded up to 4
+    int vec;                                              // the logits' rows take 16-byte loads
+    int per;                                              // tokens per workgroup
 };
 
 // fp32 as an unsigned number of the same order, 0 for what is never chosen (-inf, NaN); +0 and -0 alike.
@@ -58,32 +63,48 @@ __device__ __forceinline__ uint64_t key_of(double x) {
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp(uint32_t v) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true); }
 
-// The maximum over the wave, in a scalar.
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-    v = max(v, dpp<0xb1>(v));                             // lane ^ 1, lane ^ 2, the other four, the other eight of 16
+// Over the 16 lanes of a token, in all of them: lane ^ 1, lane ^ 2, the other four of eight, the other eight.
+__device__ __forceinline__ uint32_t max16(uint32_t v) {
+    v = max(v, dpp<0xb1>(v));
     v = max(v, dpp<0x4e>(v));
     v = max(v, dpp<0x141>(v));
-    v = max(v, dpp<0x140>(v));
-    const uint32_t a = max((uint32_t)__builtin_amdgcn_readlane((int)v, 0), (uint32_t)__builtin_amdgcn_readlane((int)v, 16));
-    const uint32_t b = max((uint32_t)__builtin_amdgcn_readlane((int)v, 32), (uint32_t)__builtin_amdgcn_readlane((int)v, 48));
-    return max(a, b);
+    return max(v, dpp<0x140>(v));
 }
-
-// Sums over the wave in one fixed order.
-__device__ __forceinline__ float wave_sum(float v) {
+__device__ __forceinline__ uint32_t min16(uint32_t v) {
+    v = min(v, dpp<0xb1>(v));
+    v = min(v, dpp<0x4e>(v));
+    v = min(v, dpp<0x141>(v));
+    return min(v, dpp<0x140>(v));
+}
+__device__ __forceinline__ float sum16(float v) {
     v += u2f(dpp<0xb1>(f2u(v)));
     v += u2f(dpp<0x4e>(f2u(v)));
     v += u2f(dpp<0x141>(f2u(v)));
-    v += u2f(dpp<0x140>(f2u(v)));
-    const float a = u2f(__builtin_amdgcn_readlane((int)f2u(v), 0)) + u2f(__builtin_amdgcn_readlane((int)f2u(v), 16));
-    const float b = u2f(__builtin_amdgcn_readlane((int)f2u(v), 32)) + u2f(__builtin_amdgcn_readlane((int)f2u(v), 48));
-    return a + b;
+    return v + u2f(dpp<0x140>(f2u(v)));
 }
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
-    return v;
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double v) {
+    const uint64_t u = (uint64_t)__double_as_longlong(v);
+    return __longlong_as_double((long long)((uint64_t)dpp<CTRL>((uint32_t)(u >> 32)) << 32 | dpp<CTRL>((uint32_t)u)));
 }
+__device__ __forceinline__ double sum16(double v) {
+    v += dpp64<0xb1>(v);
+    v += dpp64<0x4e>(v);
+    v += dpp64<0x141>(v);
+    return v + dpp64<0x140>(v);
+}
+// Exclusive prefix sums over the 16 lanes.
+__device__ __forceinline__ int prefix16(int n) {
+    int v = n;
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    return v - n;
+}
+// Lane `at` of each 16.
+__device__ __forceinline__ int lane16(int v, int at, int lane) { return __shfl(v, (lane & ~15) + at, 64); }
+__device__ __forceinline__ double lane16(double v, int at, int lane) { return __shfl(v, (lane & ~15) + at, 64); }
 
 __device__ __forceinline__ int wave_prefix(int v) {       // inclusive
     v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
@@ -95,6 +116,13 @@ __device__ __forceinline__ int wave_prefix(int v) {       // inclusive
     return v;
 }
 
+// A lane's logits: element v is expert at(v) + W l16, so that 16 lanes read 16 W consecutive ones at once (W of them 16 bytes).
+template <int DT, int V>
+struct Lay {
+    static constexpr int FULL = DT == H3FP8_DT_F32 ? 4 : 8, W = V < FULL ? V : FULL;
+    __host__ __device__ static constexpr int at(int v) { return v / W * 16 * W + v % W; }
+};
+
 template <int DT>
 __device__ __forceinline__ float load_logit(const void* row, int i) {
     if (DT == H3FP8_DT_F32) return reinterpret_cast<const float*>(row)[i];
@@ -102,17 +130,90 @@ __device__ __forceinline__ float load_logit(const void* row, int i) {
     return DT == H3FP8_DT_FP16 ? fp16_to_f32(h) : bf16_to_f32(h);
 }
 
-// The logits of lane l, V l on; past E: -inf.
 template <int DT, int V>
-__device__ __forceinline__ void load_token(const RouteArgs& a, int64_t t, int lane, float (&x)[V]) {
-    const char* row = reinterpret_cast<const char*>(a.logits) + t * a.ld * (DT == H3FP8_DT_F32 ? 4 : 2);
+__device__ __forceinline__ void load_token(const RouteArgs& a, const char* row, bool live, int l16, float (&x)[V]) {
+    using L = Lay<DT, V>;
+    constexpr int SIZE = DT == H3FP8_DT_F32 ? 4 : 2;
+    if (L::W == L::FULL && a.vec) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) x[v] = V * lane + v < a.E ? load_logit<DT>(row, V * lane + v) : -__builtin_inff();
+        for (int v = 0; v < V; v += L::W) {
+            const int e = L::at(v) + L::W * l16;
+            const v4u u = live && e < a.E ? *reinterpret_cast<const v4u*>(row + e * SIZE) : v4u{0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int i = 0; i < L::W; ++i) {
+                const uint32_t h = SIZE == 4 ? u[i & 3] : (u[(i >> 1) & 3] >> (16 * (i & 1))) & 0xffffu;
+                const float f = SIZE == 4 ? u2f(h) : DT == H3FP8_DT_FP16 ? fp16_to_f32(h) : bf16_to_f32(h);
+                x[v + i] = live && e < a.E ? f : -__builtin_inff();
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int e = L::at(v) + L::W * l16;
+        x[v] = live && e < a.E ? load_logit<DT>(row, e) : -__builtin_inff();
+    }
 }
 
-// One token by one wave: lane j < k returns choice j (expert or -1, weight).
-template <int V, bool BIAS>
-__device__ __forceinline__ void pick(const RouteArgs& a, const float (&x)[V], int lane, int& expert, float& weight) {
+__device__ __forceinline__ float value_of(uint32_t key) { return u2f((key >> 31) ? key ^ 0x80000000u : ~key); }
+
+// The largest of the lane's keys, over the 16 lanes; 0: none is left.
+template <int V>
+__device__ __forceinline__ uint32_t best16(const uint32_t (&key)[V]) {
+    uint32_t m = key[0];
+#pragma unroll
+    for (int v = 1; v < V; ++v) m = max(m, key[v]);
+    return max16(m);
+}
+
+// The lowest index whose key is m, which is taken out.
+template <int DT, int V>
+__device__ __forceinline__ int take16(uint32_t (&key)[V], uint32_t m, int l16) {
+    using L = Lay<DT, V>;
+    uint32_t c = 0xffff0000u;
+#pragma unroll
+    for (int v = V - 1; v >= 0; --v) c = key[v] == m ? (uint32_t)L::at(v) : c;
+    const uint32_t e = min16(c + (uint32_t)(L::W * l16)), mine = e - (uint32_t)(L::W * l16);
+#pragma unroll
+    for (int v = 0; v < V; ++v) key[v] = mine == (uint32_t)L::at(v) ? 0u : key[v];
+    return (int)e;
+}
+
+__device__ __forceinline__ double score64(const RouteArgs& a, double x, double top, double sum) {
+    return a.sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - top) / sum;
+}
+
+// Whether lane `other` (rotated in) comes before this one: by key, then by index.
+template <class K, int N>
+__device__ __forceinline__ int rank_step(K key, int e) {
+    constexpr int ROR = 0x120 + N;
+    uint64_t o = dpp<ROR>((uint32_t)key);
+    if constexpr (sizeof(K) == 8) o |= (uint64_t)dpp<ROR>((uint32_t)(key >> 32)) << 32;
+    const int oe = (int)dpp<ROR>((uint32_t)e);
+    return o > key || (o == key && oe < e) ? 1 : 0;
+}
+template <class K>
+__device__ __forceinline__ int rank16(K key, int e) {
+    return rank_step<K, 1>(key, e) + rank_step<K, 2>(key, e) + rank_step<K, 3>(key, e) + rank_step<K, 4>(key, e) + rank_step<K, 5>(key, e) +
+           rank_step<K, 6>(key, e) + rank_step<K, 7>(key, e) + rank_step<K, 8>(key, e) + rank_step<K, 9>(key, e) + rank_step<K, 10>(key, e) +
+           rank_step<K, 11>(key, e) + rank_step<K, 12>(key, e) + rank_step<K, 13>(key, e) + rank_step<K, 14>(key, e) + rank_step<K, 15>(key, e);
+}
+
+// A wave's LDS accesses in order, for the compiler.
+__device__ __forceinline__ void wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Four tokens by a wave: lane j < k of each token's 16 returns choice j (expert or -1, weight).  token: the lane's row of logits.
+//
+// k rounds, each the largest key and all that equal it taken out, leave the key that the k best reach at least; the experts that
+// reach it (with a bias: but for the error of the fp32 scores), k of them unless some are equal, get a lane each and are ranked.
+template <int DT, int V, bool BIAS>
+__device__ __forceinline__ void pick(const RouteArgs& a, const void* token, const float (&x)[V], int lane, int* scratch, int& expert, float& weight) {
+    using L = Lay<DT, V>;
+    const int l16 = lane & 15;
     float top = x[0];
     bool nan = false;
 #pragma unroll
@@ -120,84 +221,140 @@ __device__ __forceinline__ void pick(const RouteArgs& a, const float (&x)[V], in
         top = fmaxf(top, x[v]);
         nan = nan || x[v] != x[v];
     }
-    const bool any_nan = __ballot(nan) != 0;
-    const uint32_t top_key = wave_max(key_of(top));       // 0: every logit is masked
-    const float xmax = top_key == 0 ? 0.0f : u2f((top_key >> 31) ? top_key ^ 0x80000000u : ~top_key);
+    const bool any_nan = max16(nan ? 1u : 0u) != 0;
+    const uint32_t top_key = max16(key_of(top));          // 0: every logit is masked
+    const float xmax = top_key == 0 ? 0.0f : value_of(top_key);
+    // the softmax's sum: terms by the hardware's exponential; those that count have small exponents
+    float sum = 0.0f;
+    if (!a.sigmoid && (BIAS || !a.renorm)) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) sum += __builtin_amdgcn_exp2f((x[v] - xmax) * 1.4426950408889634f);
+        sum = sum16(sum);
+    }
+    // what the rounds go by: the logit, or score + bias in fp32, the score off by at most 2^-20 (hardware exponential and
+    // reciprocal), the sum by 2^-24 of it
+    auto rough = [&](int v) {
+        if (!BIAS) return x[v];
+        const int e = L::at(v) + L::W * l16;
+        const float b = e < a.E ? a.bias[e] : -__builtin_inff();
+        const float t = __builtin_amdgcn_exp2f((a.sigmoid ? -x[v] : x[v] - xmax) * 1.4426950408889634f);
+        const float s = __builtin_amdgcn_rcpf(a.sigmoid ? 1.0f + t : sum) * (a.sigmoid ? 1.0f : t);
+        // beside an infinite logit there are no scores: those experts go by the bias
+        return x[v] > -__builtin_inff() ? (s == s ? s : 0.0f) + b : -__builtin_inff();
+    };
+    uint32_t key[V], least = 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v) key[v] = key_of(rough(v));
+    for (int j = 0; j < a.k; ++j) {
+        const uint32_t m = best16(key);
+        least = m != 0 ? m : least;
+#pragma unroll
+        for (int v = 0; v < V; ++v) key[v] = key[v] < m ? key[v] : 0u;
+    }
+    const float edge = value_of(least);
+    const float floor = !BIAS ? edge : edge - 0x1p-18f * (1.0f + fabsf(edge));
+    const bool some = least != 0, flat = BIAS && !(fabsf(edge) < __builtin_inff());
+    uint32_t in = 0;                                      // bit v: element v can be among the best
+#pragma unroll
+    for (int v = V - 1; v >= 0; --v) {
+        const float r = rough(v);
+        in = 2 * in + (some && r > -__builtin_inff() && r >= floor ? 1u : 0u);
+    }
+    const int n = __popc(in);
+    int at = prefix16(n);
+    const int total = lane16(at + n, 15, lane);
+    double sum64 = 1.0;
+    if (BIAS && !a.sigmoid) {
+        sum64 = 0.0;
+#pragma unroll 1
+        for (int v = 0; v < V; ++v) {
+            const int e = L::at(v) + L::W * l16;
+            const double t = e < a.E ? exp((double)load_logit<DT>(token, e) - (double)xmax) : 0.0;
+            sum64 += t == t ? t : 0.0;                    // a NaN is not among those to choose from
+        }
+        sum64 = sum16(sum64);
+    }
     expert = -1;
-    float mine = 0.0f, score = 0.0f;                      // lane j: the logit of choice j, its score
-    double score64 = 0.0;
-    if constexpr (BIAS) {
-        double s[V], sum = 0.0;
-        uint64_t key[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            s[v] = a.sigmoid ? 1.0 / (1.0 + exp(-(double)x[v])) : exp((double)x[v] - (double)xmax);
-            sum += s[v] == s[v] ? s[v] : 0.0;             // a NaN is not among those to choose from
+    float mine = 0.0f;                                    // lane j: the logit of choice j, or
+    double mine64 = 0.0;                                  // ... its score
+    if (__ballot(some && (total > 16 || flat)) == 0) {
+        int* list = scratch + (lane & ~15);
+        while (__ballot(in != 0)) {
+            if (in != 0) {
+                const int v = __ffs((int)in) - 1;
+                list[at++] = L::at(v) + L::W * l16;
+                in &= in - 1;
+            }
         }
-        if (!a.sigmoid) {
-            sum = wave_sum(sum);
-#pragma unroll
-            for (int v = 0; v < V; ++v) s[v] = s[v] / sum;
+        wave_order();
+        const bool has = l16 < total;
+        const int e = has ? list[l16] : 0xffff;
+        const float f = has ? load_logit<DT>(token, e) : 0.0f;
+        int rank;
+        double s = 0.0;
+        if constexpr (BIAS) {
+            s = has ? score64(a, (double)f, (double)xmax, sum64) : 0.0;
+            const uint64_t k64 = has ? key_of((s == s ? s : 0.0) + (double)a.bias[e]) : 0ull;
+            rank = rank16(k64, e);
+        } else {
+            rank = rank16(has ? key_of(f) : 0u, e);
         }
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int e = V * lane + v;
-            // beside an infinite logit there are no scores: such a token's experts go by the bias
-            const double base = s[v] == s[v] ? s[v] : 0.0;
-            key[v] = e < a.E && x[v] > -__builtin_inff() ? key_of(base + (double)a.bias[e]) : 0ull;
-        }
+        wave_order();
+        if (has && rank < a.k) list[rank] = e | (l16 << 16);
+        wave_order();
+        const int got = l16 < min(total, a.k) ? list[l16] : l16 << 16, from = got >> 16;
+        if (l16 < min(total, a.k)) expert = got & 0xffff;
+        if constexpr (BIAS) mine64 = lane16(s, from, lane);
+        else mine = u2f((uint32_t)lane16((int)f2u(f), from, lane));
+    } else if constexpr (BIAS) {
+        // all of them again in every round, from memory: few registers, and rarely
+        uint64_t taken = 0;
+#pragma unroll 1
         for (int j = 0; j < a.k; ++j) {
-            uint64_t best = key[0];
-            double bs = s[0];
+            uint64_t best = 0;
+            double bs = 0.0;
             int bv = 0;
-#pragma unroll
-            for (int v = 1; v < V; ++v)
-                if (key[v] > best) best = key[v], bs = s[v], bv = v;
-            const uint32_t hi = wave_max((uint32_t)(best >> 32));
-            const uint32_t lo = wave_max((uint32_t)(best >> 32) == hi ? (uint32_t)best : 0u);
-            if ((hi | lo) == 0) break;
-            const int win = __builtin_ctzll(__ballot(best == (((uint64_t)hi << 32) | lo)));
-            const int e = __builtin_amdgcn_readlane(V * lane + bv, win);
-            const double es = __shfl(bs, win, 64);
-            if (lane == j) expert = e, score64 = es;
-#pragma unroll
-            for (int v = 0; v < V; ++v)
-                if (V * lane + v == e) key[v] = 0ull;
+#pragma unroll 1
+            for (int v = 0; v < V; ++v) {
+                const int e = L::at(v) + L::W * l16;
+                if (e >= a.E || ((taken >> v) & 1)) continue;
+                const float f = load_logit<DT>(token, e);
+                const double s = score64(a, (double)f, (double)xmax, sum64);
+                const uint64_t o = f > -__builtin_inff() ? key_of((s == s ? s : 0.0) + (double)a.bias[e]) : 0ull;
+                if (o > best) best = o, bs = s, bv = v;
+            }
+            const uint32_t hi = max16((uint32_t)(best >> 32)), lo = max16((uint32_t)(best >> 32) == hi ? (uint32_t)best : 0u);
+            const bool at_best = best != 0 && best == ((uint64_t)hi << 32 | lo);
+            const uint32_t own = at_best ? (uint32_t)(L::at(bv) + L::W * l16) : 0xffff0000u, e = min16(own);
+            const int by = (int)max16(own == e && at_best ? (uint32_t)l16 : 0u);
+            const double s = lane16(bs, by, lane);
+            if (own == e && at_best) taken |= 1ull << bv;
+            if (l16 == j && e < 0xffff0000u) expert = (int)e, mine64 = s;
         }
-        if (a.renorm) {
-            const double total = wave_sum(lane < a.k ? score64 : 0.0);
-            score64 = total == 0.0 ? 0.0 : score64 / total;
-        }
-        weight = (float)(score64 * (double)a.scale);
     } else {
-        uint32_t key[V];
-        float sum = 0.0f;
+        // more than 16 reach it: equal ones, taken one by one, the lowest index first
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            key[v] = key_of(x[v]);
-            if (!a.sigmoid && !a.renorm) sum += expf(x[v] - xmax);
-        }
-        if (!a.sigmoid && !a.renorm) sum = wave_sum(sum);
+        for (int v = 0; v < V; ++v) key[v] = key_of(x[v]);
         for (int j = 0; j < a.k; ++j) {
-            uint32_t best = key[0];
-            int bv = 0;
-#pragma unroll
-            for (int v = 1; v < V; ++v)
-                if (key[v] > best) best = key[v], bv = v;
-            const uint32_t m = wave_max(best);
-            if (m == 0) break;
-            const int win = __builtin_ctzll(__ballot(best == m));
-            const int e = __builtin_amdgcn_readlane(V * lane + bv, win);
-            if (lane == j) expert = e, mine = u2f((m >> 31) ? m ^ 0x80000000u : ~m);
-#pragma unroll
-            for (int v = 0; v < V; ++v)
-                if (V * lane + v == e) key[v] = 0u;
+            const uint32_t m = best16(key);
+            const int e = take16<DT, V>(key, m, l16);
+            if (l16 == j && m != 0) expert = e, mine = value_of(m);
         }
+    }
+    if constexpr (BIAS) {
+        if (expert < 0) mine64 = 0.0;
+        if (a.renorm) {
+            const double all = sum16(mine64);
+            mine64 = all == 0.0 ? 0.0 : mine64 / all;
+        }
+        weight = (float)(mine64 * (double)a.scale);
+    } else {
+        float score = 0.0f;
         if (expert >= 0) {
             const float t = expf(a.sigmoid ? -fabsf(mine) : mine - xmax);
             score = a.sigmoid ? (mine >= 0.0f ? 1.0f : t) / (1.0f + t) : t;
         }
-        if (a.renorm) sum = wave_sum(score);
+        if (a.renorm) sum = sum16(score);
         else if (a.sigmoid) sum = 1.0f;
         weight = sum == 0.0f ? 0.0f : score / sum * a.scale;
     }
@@ -205,9 +362,12 @@ __device__ __forceinline__ void pick(const RouteArgs& a, const float (&x)[V], in
     if (expert < 0) weight = 0.0f;
 }
 
+constexpr int pick_waves(int V, bool bias) { return V > 16 && bias ? WAVES / 2 : WAVES; }
+
 struct RouteLds {
     int expert[TB * MAX_K];                               // of the batch's pairs; E: none
     uint16_t count[CHUNKS * (MAX_E + 2)];                 // per 64 pairs and expert (rows of E + 1 rounded up to even), then what comes before them
+    int scratch[WAVES * 64];
     int run[MAX_E + 1];                                   // of the batches before
     int base[MAX_E + 1];
 };
@@ -223,7 +383,8 @@ __device__ __forceinline__ void scan(const int* total, int* base, int E, int lan
 }
 
 template <int DT, int V, bool BIAS>
-__global__ void __launch_bounds__(WAVES * 64) moe_route_pick_kernel(RouteArgs a) {
+__global__ void __launch_bounds__(pick_waves(V, BIAS) * 64) moe_route_pick_kernel(RouteArgs a) {
+    constexpr int WAVES = pick_waves(V, BIAS);
     extern __shared__ __attribute__((aligned(16))) char route_lds[];
     RouteLds& s = *reinterpret_cast<RouteLds*>(route_lds);
     const int lane = threadIdx.x & 63;
@@ -235,21 +396,21 @@ __global__ void __launch_bounds__(WAVES * 64) moe_route_pick_kernel(RouteArgs a)
     for (int64_t t0 = first; t0 < last; t0 += TB) {
         const int n = (int)min<int64_t>(TB, last - t0), pairs = n * k, chunks = (pairs + 63) / 64;
         for (int i = threadIdx.x; i < chunks * row / 2; i += WAVES * 64) reinterpret_cast<uint32_t*>(s.count)[i] = 0;
-        float x[V], next[V];
-        if (wave < n) load_token<DT, V>(a, t0 + wave, lane, x);
-        for (int i = wave; i < n; i += WAVES) {
-            if (i + WAVES < n) load_token<DT, V>(a, t0 + i + WAVES, lane, next);
+        const int l16 = lane & 15;
+        for (int i0 = 4 * wave; i0 < n; i0 += 4 * WAVES) {
+            const int i = i0 + (lane >> 4);
+            const char* token = reinterpret_cast<const char*>(a.logits) + (t0 + min(i, n - 1)) * a.ld * (DT == H3FP8_DT_F32 ? 4 : 2);
+            float x[V];
+            load_token<DT, V>(a, token, i < n, l16, x);
             int expert;
             float weight;
-            pick<V, BIAS>(a, x, lane, expert, weight);
-            if (lane < k) {
-                const int64_t p = (t0 + i) * k + lane;
+            pick<DT, V, BIAS>(a, token, x, lane, s.scratch + wave * 64, expert, weight);
+            if (i < n && l16 < k) {
+                const int64_t p = (t0 + i) * k + l16;
                 a.weights[p] = weight;
                 a.experts[p] = expert;
-                s.expert[i * k + lane] = expert < 0 ? E : expert;
+                s.expert[i * k + l16] = expert < 0 ? E : expert;
             }
-#pragma unroll
-            for (int v = 0; v < V; ++v) x[v] = next[v];
         }
         __syncthreads();
         // ranks within 64 pairs
@@ -302,29 +463,41 @@ __global__ void __launch_bounds__(WAVES * 64) moe_route_pick_kernel(RouteArgs a)
             for (int e = threadIdx.x; e <= E; e += WAVES * 64) a.offsets[e] = s.base[e];
         }
     } else {
-        for (int e = threadIdx.x; e <= E; e += WAVES * 64) a.counts[(int64_t)blockIdx.x * (E + 1) + e] = s.run[e];
+        for (int e = threadIdx.x; e <= E; e += WAVES * 64) a.counts[(int64_t)blockIdx.x * a.row + e] = s.run[e];
     }
 }
 
 // The pairs of workgroup b of the first launch to their places: counts of the workgroups before it, and offsets.
 __global__ void __launch_bounds__(WAVES * 64) moe_route_place_kernel(RouteArgs a, int blocks) {
-    __shared__ int before[MAX_E + 1], total[MAX_E + 1], base[MAX_E + 1];
+    __shared__ int before[MAX_E + 4], total[MAX_E + 4], base[MAX_E + 1];
     const int lane = threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-    const int n = a.E + 1;
-    for (int e = threadIdx.x; e < n; e += WAVES * 64) before[e] = total[e] = 0;
+    const int n = a.E + 1, quads = a.row / 4;
+    for (int e = threadIdx.x; e < a.row; e += WAVES * 64) before[e] = total[e] = 0;
     __syncthreads();
-    // a thread sums one expert's counts of every parts-th workgroup; LDS adds of whole numbers, in any order
-    const int parts = max(1, WAVES * 64 / n);
-    for (int i = threadIdx.x; i < n * parts; i += WAVES * 64) {
-        const int e = i % n;
-        int lo = 0, all = 0;
-        for (int b = i / n; b < blocks; b += parts) {
-            const int c = a.counts[(int64_t)b * n + e];
-            all += c;
-            lo += b < (int)blockIdx.x ? c : 0;
+    // a thread sums four experts' counts of every parts-th workgroup, eight loads under way; LDS adds of whole numbers, in any order
+    typedef int v4i __attribute__((ext_vector_type(4)));
+    const int parts = WAVES * 64 / quads, q = threadIdx.x % quads, part = threadIdx.x / quads;
+    if (part < parts) {
+        v4i lo = {0, 0, 0, 0}, all = {0, 0, 0, 0};
+        for (int b0 = part; b0 < blocks; b0 += 8 * parts) {
+            v4i c[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int b = b0 + u * parts;
+                c[u] = b < blocks ? *reinterpret_cast<const v4i*>(a.counts + (int64_t)b * a.row + 4 * q) : v4i{0, 0, 0, 0};
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                all += c[u];
+                if (b0 + u * parts < (int)blockIdx.x) lo += c[u];
+            }
         }
-        atomicAdd(&before[e], lo);
-        atomicAdd(&total[e], all);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (4 * q + u < n) {                          // the rows' last places hold nothing
+                atomicAdd(&before[4 * q + u], lo[u]);
+                atomicAdd(&total[4 * q + u], all[u]);
+            }
     }
     __syncthreads();
     if (wave == 0) scan(total, base, a.E, lane);
@@ -339,30 +512,35 @@ __global__ void __launch_bounds__(WAVES * 64) moe_route_place_kernel(RouteArgs a
     }
 }
 
-// Tokens per workgroup of the first launch.
-int64_t per_block(int64_t T) { return TB * std::max<int64_t>(1, (T + (int64_t)TB * MAX_BLOCKS - 1) / ((int64_t)TB * MAX_BLOCKS)); }
+// Tokens per workgroup of the first launch: one batch each until every CU has one, then as many as keep them within 256, or 512.
+int64_t per_block(int64_t T) {
+    if (T <= TB) return TB;
+    const int64_t most = T > 128LL * MAX_BLOCKS ? MAX_BLOCKS : MAX_BLOCKS / 2;
+    return 64 * ((T + 64 * most - 1) / (64 * most));
+}
 
 template <int DT, int V>
 int launch_pick(const RouteArgs& a, unsigned blocks, hipStream_t st) {
-    if (a.bias) hipLaunchKernelGGL((moe_route_pick_kernel<DT, V, true>), dim3(blocks), dim3(WAVES * 64), sizeof(RouteLds), st, a);
-    else hipLaunchKernelGGL((moe_route_pick_kernel<DT, V, false>), dim3(blocks), dim3(WAVES * 64), sizeof(RouteLds), st, a);
+    if (a.bias) hipLaunchKernelGGL((moe_route_pick_kernel<DT, V, true>), dim3(blocks), dim3(pick_waves(V, true) * 64), sizeof(RouteLds), st, a);
+    else hipLaunchKernelGGL((moe_route_pick_kernel<DT, V, false>), dim3(blocks), dim3(pick_waves(V, false) * 64), sizeof(RouteLds), st, a);
     H3_CHECK_HIP(hipGetLastError());
     return H3FP8_OK;
 }
 
 template <int DT>
 int launch_width(const RouteArgs& a, unsigned blocks, hipStream_t st) {
-    if (a.E <= 64) return launch_pick<DT, 1>(a, blocks, st);
-    if (a.E <= 128) return launch_pick<DT, 2>(a, blocks, st);
-    if (a.E <= 256) return launch_pick<DT, 4>(a, blocks, st);
-    return launch_pick<DT, 8>(a, blocks, st);
+    if (a.E <= 32) return launch_pick<DT, 2>(a, blocks, st);
+    if (a.E <= 64) return launch_pick<DT, 4>(a, blocks, st);
+    if (a.E <= 128) return launch_pick<DT, 8>(a, blocks, st);
+    if (a.E <= 256) return launch_pick<DT, 16>(a, blocks, st);
+    return launch_pick<DT, 32>(a, blocks, st);
 }
 
 }  // namespace
 
 extern "C" int64_t h3fp8_moe_route_workspace(int64_t T, int64_t E) {
     if (T <= TB || E < 0) return 0;
-    return (T + per_block(T) - 1) / per_block(T) * (E + 1) * 4;
+    return (T + per_block(T) - 1) / per_block(T) * ((E + 4) / 4 * 4) * 4;
 }
 
 extern "C" int h3fp8_moe_route(const void* logits, int64_t ld, int dtype, int64_t T, int64_t E, int k, int scoring, int renorm,
@@ -377,7 +555,7 @@ extern "C" int h3fp8_moe_route(const void* logits, int64_t ld, int dtype, int64_
     H3_REQUIRE(T <= 1 || ld >= 0, "h3fp8_moe_route: negative stride");
     const unsigned elem = dtype == H3FP8_DT_F32 ? 4 : 2;
     H3_REQUIRE((((uintptr_t)logits & (elem - 1)) | (((uintptr_t)bias | (uintptr_t)weights | (uintptr_t)experts | (uintptr_t)offsets |
-                (uintptr_t)order | (uintptr_t)place | (uintptr_t)workspace) & 3)) == 0, "h3fp8_moe_route: misaligned pointer");
+                (uintptr_t)order | (uintptr_t)place) & 3) | ((uintptr_t)workspace & 15)) == 0, "h3fp8_moe_route: misaligned pointer");
     const int64_t need = h3fp8_moe_route_workspace(T, E);
     H3_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "h3fp8_moe_route: the workspace needs %lld bytes", (long long)need);
     RouteArgs a{};
@@ -385,6 +563,8 @@ extern "C" int h3fp8_moe_route(const void* logits, int64_t ld, int dtype, int64_
     a.bias = bias; a.weights = weights; a.experts = experts; a.offsets = offsets; a.order = order; a.place = place;
     a.counts = need ? (int*)workspace : nullptr;
     a.per = (int)per_block(T);
+    a.row = (int)(E + 4) / 4 * 4;
+    a.vec = ((uintptr_t)logits & 15) == 0 && ld * elem % 16 == 0 && E * elem % 16 == 0;
     const unsigned blocks = (unsigned)std::max<int64_t>(1, (T + a.per - 1) / a.per);
     hipStream_t st = (hipStream_t)stream;
     const int rc = dtype == H3FP8_DT_F32 ? launch_width<H3FP8_DT_F32>(a, blocks, st)

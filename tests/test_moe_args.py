@@ -96,11 +96,11 @@ def test_c_entries():
     def route(logits=p, ld=64, dtype=2, T=4, E=64, k=2, scoring=0, out=p, offsets=p, ws=None, ws_bytes=0, bias=None):
         return L.h3fp8_moe_route(logits, ld, dtype, T, E, k, scoring, 1, 1.0, bias, out, out, offsets, out, out, ws, ws_bytes, None)
     for kw in (dict(T=-1), dict(E=0), dict(E=513), dict(k=0), dict(k=17), dict(E=4, k=5), dict(dtype=3), dict(scoring=2), dict(logits=None),
-               dict(out=None), dict(offsets=None), dict(T=129), dict(T=129, ws=p, ws_bytes=2 * 65 * 4 - 1), dict(logits=ctypes.c_void_p(4098)),
+               dict(out=None), dict(offsets=None), dict(T=129), dict(T=129, ws=p, ws_bytes=3 * 68 * 4 - 1), dict(logits=ctypes.c_void_p(4098)),
                dict(bias=ctypes.c_void_p(4098)), dict(T=1 << 31), dict(ld=-1)):
         assert route(**kw) == -22, kw
-    assert L.h3fp8_moe_route_workspace(128, 64) == 0 and L.h3fp8_moe_route_workspace(129, 64) == 2 * 65 * 4
-    assert L.h3fp8_moe_route_workspace(1 << 24, 8) <= 512 * 9 * 4
+    assert L.h3fp8_moe_route_workspace(128, 64) == 0 and L.h3fp8_moe_route_workspace(129, 64) == 3 * 68 * 4
+    assert L.h3fp8_moe_route_workspace(1 << 24, 8) <= 512 * 12 * 4
 
     def layer(x=p, ldx=256, dtype=0, T=4, H=256, F=128, E=8, k=2, w=p, we=1 << 16, ld1=256, ld2=128, s=p, sn=2, sk=1, r=p, res=None, ldr=256, y=p,
               ldy=256, ws=p, ws_bytes=4 * 2 * 128 * 4):
