@@ -47,6 +47,7 @@ struct RouteArgs {
     int* counts;                                          // [blocks, row]: pairs per expert (E: without one)
     int row;                                              // E + 1 rounded up to 4
     int vec;                                              // the logits' rows take 16-byte loads
+    int vec_bias;                                         // so do four biases
     int per;                                              // tokens per workgroup
 };
 
@@ -166,6 +167,17 @@ __device__ __forceinline__ uint32_t best16(const uint32_t (&key)[V]) {
     return max16(m);
 }
 
+// The largest key below m != 0, over the 16 lanes; 0: none.  m - 1 - key, as an unsigned number, is smallest for it: keys from m on
+// wrap to 2^32 - 1 - (key - m), which is more than m - 1 - other for any other key, two keys being less than 2^32 apart.
+template <int V>
+__device__ __forceinline__ uint32_t next16(const uint32_t (&key)[V], uint32_t m) {
+    uint32_t d = m - 1 - key[0];
+#pragma unroll
+    for (int v = 1; v < V; ++v) d = min(d, m - 1 - key[v]);
+    const uint32_t next = m - 1 - min16(d);
+    return next < m ? next : 0u;
+}
+
 // The lowest index whose key is m, which is taken out.
 template <int DT, int V>
 __device__ __forceinline__ int take16(uint32_t (&key)[V], uint32_t m, int l16) {
@@ -181,6 +193,28 @@ __device__ __forceinline__ int take16(uint32_t (&key)[V], uint32_t m, int l16) {
 
 __device__ __forceinline__ double score64(const RouteArgs& a, double x, double top, double sum) {
     return a.sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - top) / sum;
+}
+
+// The biases of a lane's experts, -inf past the last.
+template <int DT, int V>
+__device__ __forceinline__ void load_bias(const RouteArgs& a, int l16, float (&b)[V]) {
+    using L = Lay<DT, V>;
+    typedef float v4f __attribute__((ext_vector_type(4)));
+    if (L::W >= 4 && a.vec_bias) {
+#pragma unroll
+        for (int v = 0; v < V; v += 4) {
+            const int e = L::at(v) + L::W * l16;
+            const v4f q = e < a.E ? *reinterpret_cast<const v4f*>(a.bias + e) : v4f{} - __builtin_inff();
+#pragma unroll
+            for (int u = 0; u < 4; ++u) b[(v + u) % V] = q[u];
+        }
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int e = L::at(v) + L::W * l16;
+            b[v] = e < a.E ? a.bias[e] : -__builtin_inff();
+        }
+    }
 }
 
 // Whether lane `other` (rotated in) comes before this one: by key, then by index.
@@ -208,10 +242,10 @@ __device__ __forceinline__ void wave_order() {
 
 // Four tokens by a wave: lane j < k of each token's 16 returns choice j (expert or -1, weight).  token: the lane's row of logits.
 //
-// k rounds, each the largest key and all that equal it taken out, leave the key that the k best reach at least; the experts that
-// reach it (with a bias: but for the error of the fp32 scores), k of them unless some are equal, get a lane each and are ranked.
+// k rounds, each the largest key below the last, leave the key that the k best reach at least; the experts that reach it (with a
+// bias: but for the error of the fp32 scores), k of them unless some are equal, get a lane each and are ranked.
 template <int DT, int V, bool BIAS>
-__device__ __forceinline__ void pick(const RouteArgs& a, const void* token, const float (&x)[V], int lane, int* scratch, int& expert, float& weight) {
+__device__ __forceinline__ void pick(const RouteArgs& a, const void* token, float (&x)[V], int lane, int* scratch, int& expert, float& weight) {
     using L = Lay<DT, V>;
     const int l16 = lane & 15;
     float top = x[0];
@@ -232,34 +266,33 @@ __device__ __forceinline__ void pick(const RouteArgs& a, const void* token, cons
         sum = sum16(sum);
     }
     // what the rounds go by: the logit, or score + bias in fp32, the score off by at most 2^-20 (hardware exponential and
-    // reciprocal), the sum by 2^-24 of it
-    auto rough = [&](int v) {
-        if (!BIAS) return x[v];
-        const int e = L::at(v) + L::W * l16;
-        const float b = e < a.E ? a.bias[e] : -__builtin_inff();
-        const float t = __builtin_amdgcn_exp2f((a.sigmoid ? -x[v] : x[v] - xmax) * 1.4426950408889634f);
-        const float s = __builtin_amdgcn_rcpf(a.sigmoid ? 1.0f + t : sum) * (a.sigmoid ? 1.0f : t);
-        // beside an infinite logit there are no scores: those experts go by the bias
-        return x[v] > -__builtin_inff() ? (s == s ? s : 0.0f) + b : -__builtin_inff();
-    };
-    uint32_t key[V], least = 0;
+    // reciprocal), the sum by 2^-24 of it; beside an infinite logit there are no scores: those experts go by the bias
+    if constexpr (BIAS) {
+        float b[V];
+        load_bias<DT, V>(a, l16, b);
 #pragma unroll
-    for (int v = 0; v < V; ++v) key[v] = key_of(rough(v));
-    for (int j = 0; j < a.k; ++j) {
-        const uint32_t m = best16(key);
+        for (int v = 0; v < V; ++v) {
+            const float t = __builtin_amdgcn_exp2f((a.sigmoid ? -x[v] : x[v] - xmax) * 1.4426950408889634f);
+            const float s = __builtin_amdgcn_rcpf(a.sigmoid ? 1.0f + t : sum) * (a.sigmoid ? 1.0f : t);
+            x[v] = x[v] > -__builtin_inff() ? (s == s ? s : 0.0f) + b[v] : -__builtin_inff();
+        }
+    }
+    uint32_t key[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) key[v] = key_of(x[v]);
+    uint32_t least = best16(key);
+    for (int j = 1; j < a.k; ++j) {
+        const uint32_t m = next16(key, least);
+        if (__ballot(m != 0) == 0) break;
         least = m != 0 ? m : least;
-#pragma unroll
-        for (int v = 0; v < V; ++v) key[v] = key[v] < m ? key[v] : 0u;
     }
     const float edge = value_of(least);
     const float floor = !BIAS ? edge : edge - 0x1p-18f * (1.0f + fabsf(edge));
-    const bool some = least != 0, flat = BIAS && !(fabsf(edge) < __builtin_inff());
+    const bool some = least != 0, flat = BIAS && (any_nan || !(fabsf(edge) < __builtin_inff()));
+    const uint32_t least_key = !some ? 0xffffffffu : BIAS ? max(key_of(floor), 1u) : least;
     uint32_t in = 0;                                      // bit v: element v can be among the best
 #pragma unroll
-    for (int v = V - 1; v >= 0; --v) {
-        const float r = rough(v);
-        in = 2 * in + (some && r > -__builtin_inff() && r >= floor ? 1u : 0u);
-    }
+    for (int v = V - 1; v >= 0; --v) in = 2 * in + (key[v] >= least_key ? 1u : 0u);
     const int n = __popc(in);
     int at = prefix16(n);
     const int total = lane16(at + n, 15, lane);
@@ -333,8 +366,6 @@ __device__ __forceinline__ void pick(const RouteArgs& a, const void* token, cons
         }
     } else {
         // more than 16 reach it: equal ones, taken one by one, the lowest index first
-#pragma unroll
-        for (int v = 0; v < V; ++v) key[v] = key_of(x[v]);
         for (int j = 0; j < a.k; ++j) {
             const uint32_t m = best16(key);
             const int e = take16<DT, V>(key, m, l16);
@@ -565,6 +596,7 @@ extern "C" int h3fp8_moe_route(const void* logits, int64_t ld, int dtype, int64_
     a.per = (int)per_block(T);
     a.row = (int)(E + 4) / 4 * 4;
     a.vec = ((uintptr_t)logits & 15) == 0 && ld * elem % 16 == 0 && E * elem % 16 == 0;
+    a.vec_bias = ((uintptr_t)bias & 15) == 0 && E % 4 == 0;
     const unsigned blocks = (unsigned)std::max<int64_t>(1, (T + a.per - 1) / a.per);
     hipStream_t st = (hipStream_t)stream;
     const int rc = dtype == H3FP8_DT_F32 ? launch_width<H3FP8_DT_F32>(a, blocks, st)
