@@ -474,10 +474,6 @@ __device__ __forceinline__ int chunk_at(int r, int i) {
     return i ^ (UP ? c : (((c >> 2) ^ (c >> 3)) & 1) | ((c & 3) << 1) | (c & 8));
 }
 
-#ifndef ROT_E
-#define ROT_E 0
-#define ROT_T 0
-#endif
 template <bool UP, bool FP16, int NT, int CT, int WV, int AH>
 __global__ void __launch_bounds__(WV * 64) moe_rows_kernel(MoeParams p, int tiles) {
     using C = Rows<UP, NT, CT, WV, AH>;
@@ -747,11 +743,14 @@ extern "C" int h3fp8_moe_blocks(const void* x, int64_t ldx, int dtype, int64_t T
     H3_REQUIRE(ld1 >= H && ld2 >= F && ld1 % 16 == 0 && ld2 % 16 == 0 && w1_e >= 0 && w2_e >= 0 && w1_e % 16 == 0 && w2_e % 16 == 0,
                "%s: the weights' row strides must cover their rows, theirs and the expert strides be multiples of 16", who);
     H3_REQUIRE(s1_e >= 0 && s1_n >= 0 && s1_k >= 0 && s2_e >= 0 && s2_n >= 0 && s2_k >= 0, "%s: negative stride", who);
-    H3_REQUIRE(128 * ldx * 2 + 2 * H <= kMaxSpan && 64 * ld1 + H <= kMaxSpan && 64 * ld2 + F <= kMaxSpan && T * k * F * 4 <= kMaxSpan,
-               "%s: a stride or size is too large", who);
+    const int64_t span = kMaxSpan;
+    H3_REQUIRE(ldx <= span / 512 && ld1 <= span / 128 && ld2 <= span / 128 && T * k * F * 4 <= span, "%s: a stride or size is too large", who);
+    // the scales' offsets are 32 bits of bytes
+    const auto bounded = [&](int64_t n, int64_t kb, int64_t se, int64_t sn, int64_t sk) {
+        return se <= span / 4 && sn <= span / 4 && sk <= span / 4 && ((E - 1) * se + (n - 1) * sn + (kb - 1) * sk) * 4 <= span / 2;
+    };
     const int64_t hb = (H + 127) / 128, fb = (F + 127) / 128, f2 = (2 * F + 127) / 128;
-    H3_REQUIRE((E * s1_e + f2 * s1_n) * 4 <= kMaxSpan / 2 && hb * s1_k * 4 <= kMaxSpan / 2 && hb * s2_n * 4 <= kMaxSpan / 2 && fb * s2_k * 4 <= kMaxSpan / 2,
-               "%s: a scale stride is too large", who);
+    H3_REQUIRE(bounded(f2, hb, s1_e, s1_n, s1_k) && bounded(hb, fb, s2_e, s2_n, s2_k), "%s: a scale stride is too large", who);
     const int64_t need = h3fp8_moe_blocks_workspace(T, k, H, F, E);
     H3_REQUIRE(workspace_bytes >= need, "%s: the workspace needs %lld bytes", who, (long long)need);
     MoeParams p{};

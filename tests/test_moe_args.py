@@ -88,6 +88,19 @@ def test_product_with_an_epilogue(calls):
     assert len(calls) == n
 
 
+def test_c_entry_bounds_every_stride():
+    """The experts' offsets, and strides whose products would pass 64 bits."""
+    L = _lib.load()
+    p = ctypes.c_void_p(4096)
+
+    def layer(ldx=256, ld1=256, ld2=128, s1=(4, 2, 1), s2=(4, 2, 1)):
+        return L.h3fp8_moe_blocks(p, ldx, 0, 4, 256, 128, 8, 2, p, 1 << 16, ld1, p, *s1, p, 1 << 16, ld2, p, *s2, p, p, p, p, None, 0, p, 256, p, 0, None)
+    big = 1 << 28
+    for kw in (dict(s1=(big, 2, 1)), dict(s2=(big, 2, 1)), dict(s1=(4, big, 1)), dict(s2=(4, big, 1)), dict(s1=(4, 2, big)), dict(s1=(1 << 62, 2, 1)),
+               dict(s2=(1 << 62, 2, 1)), dict(s2=(4, 1 << 62, 1)), dict(s2=(4, 2, 1 << 62)), dict(ldx=1 << 62), dict(ld1=1 << 62), dict(ld2=1 << 62)):
+        assert layer(**kw) == -22 and b"too large" in _lib.load().h3fp8_last_error(), kw
+
+
 def test_c_entries():
     """The C side checks again, before any HIP call."""
     L = _lib.load()
