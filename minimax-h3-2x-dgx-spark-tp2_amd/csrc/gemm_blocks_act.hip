@@ -41,8 +41,8 @@ __device__ __forceinline__ float gelu_erf(float y) {
     p = __builtin_fmaf(p, t, 0.14182958544f);
     p = __builtin_fmaf(p, t, 0.14370902344f);
     const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(a * -0.5f * LOG2E, a, 64.0f));
-    p *= t;
-    return y < 0.0f ? y * p * e * 0x1p-64f : y * __builtin_fmaf(p * e, -0x1p-64f, 1.0f);
+    const bool neg = y < 0.0f;
+    return y * __builtin_fmaf(p * t * e, neg ? 0x1p-64f : -0x1p-64f, neg ? 0.0f : 1.0f);
 }
 
 template <int N>

@@ -171,7 +171,6 @@ struct BCursor {
     uint32_t vw[T::WL], va[T::AL];  // lane offsets of the wave's 8-row groups
     uint32_t cut;               // bit i (weights) / 16 + j (tokens): the lane's chunk lies at or past K in the last k-step
     uint32_t vs;                // lane offset of the scale load
-    uint32_t s_step;            // bytes between two k-blocks' scales
     uint32_t k0, s0;            // byte offsets of the k-step: operands, scales
     int ks, c;
     bool valid;
@@ -252,7 +251,6 @@ __device__ __forceinline__ void cursor_tile(BCursor<T>& I, const BlocksParams& p
     I.valid = tile_at<T, GROUPED>(p, sp, (int)blockIdx.x + c * (int)gridDim.x, lane, r, tn);
     if (!I.valid) {                                       // the loads still run, read nothing and fill the stage with zeros
         I.rw[2] = I.ra[2] = I.rs[2] = 0;
-        I.s_step = 0;
         return;
     }
     const int n0 = tn * T::TW, nrows = min(T::TW, p.N - n0);
@@ -266,7 +264,6 @@ __device__ __forceinline__ void cursor_tile(BCursor<T>& I, const BlocksParams& p
     const int entries = tok ? r.rows : nb, first = tok ? 64 * wave : 64 * (wave - T::SC_A);
     I.rs = buffer_desc(base, (uint32_t)(((entries - 1) * st + (kb - 1) * sk) * 4 + 4));
     I.vs = first + lane < entries ? (uint32_t)((first + lane) * st * 4) : OOB;
-    I.s_step = (uint32_t)(sk * 4);
 }
 
 template <class T, bool GROUPED>
@@ -274,7 +271,7 @@ __device__ __forceinline__ void cursor_next(BCursor<T>& I, const BlocksParams& p
     if (!I.valid) return;                                 // empty descriptors: offset 0
     ++I.ks;
     I.k0 += BK;
-    I.s0 += I.s_step;
+    I.s0 += (uint32_t)__builtin_amdgcn_readfirstlane((int)((wave < T::SC_A ? p.sa_k : p.sw_k) * 4));
     if (__builtin_expect(I.ks == nk, 0)) cursor_tile<T, GROUPED>(I, p, sp, I.c + 1, wave, lane);
 }
 
