@@ -645,16 +645,25 @@ __global__ void __launch_bounds__(WV * 64) moe_rows_kernel(MoeParams p, int tile
     wait_vm0();                                           // the loads behind the last unit have landed before the exit
 }
 
-// y: the sum over a token's choices, in their order; of equal experts the first counts (it has both weights).
+// y: the sum over a token's choices, in their order; of equal experts the first counts (it has both weights).  What bounds it is the
+// trip to memory: eight choices are asked for at once, those that do not count too, and left out of the sum.
 __global__ void __launch_bounds__(256) moe_combine_kernel(MoeParams p) {
-    const int t = blockIdx.y, n = 4 * (int)(blockIdx.x * 256 + threadIdx.x);
+    constexpr int AT_ONCE = 8;
+    const int t = blockIdx.y, n = 4 * (int)(blockIdx.x * 256 + threadIdx.x), lane = threadIdx.x & 63;
+    const int e = lane < p.k ? p.experts[t * p.k + lane] : -1;
+    bool first = true;
+    for (int i = 0; i < p.k; ++i) first = first && (i >= lane || __builtin_amdgcn_readlane(e, i) != e);
+    const uint64_t count = __ballot(first && e >= 0 && e < p.E);
     if (n >= p.H) return;
+    const float* z = p.z + (int64_t)t * p.k * p.H + n;
     v4f v = {0.f, 0.f, 0.f, 0.f};
-    for (int j = 0; j < p.k; ++j) {
-        const int q = t * p.k + j, e = p.experts[q];
-        bool count = e >= 0 && e < p.E;
-        for (int i = 0; i < j; ++i) count = count && p.experts[t * p.k + i] != e;
-        if (count) v += *reinterpret_cast<const v4f*>(p.z + (int64_t)q * p.H + n);
+    for (int j0 = 0; j0 < p.k; j0 += AT_ONCE) {
+        v4f c[AT_ONCE];
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) c[j] = *reinterpret_cast<const v4f*>(z + (int64_t)min(j0 + j, p.k - 1) * p.H);
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j)
+            if ((count >> (j0 + j)) & 1) v += c[j];
     }
     store_y(p, t, n, v);
 }
