@@ -77,6 +77,73 @@ def test_route_ties_masks_and_nan(cuda, E, bias):
         assert r.experts[9, 0] == 2 and bool(torch.isnan(r.weights[9]).any())
 
 
+@pytest.mark.parametrize("E", [12, 16, 17, 40, 300])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_route_with_bias_near_ties(cuda, E, scoring):
+    """Scores that the bias makes equal but for its own rounding: 64 bits tell them apart, whether up to 16 experts are that near
+    or more."""
+    g = torch.Generator(device=cuda).manual_seed(E)
+    x = torch.randn(1, E, generator=g, device=cuda)
+    score = torch.softmax(x.double(), 1) if scoring == "softmax" else torch.sigmoid(x.double())
+    bias = (0.75 - score[0]).float()
+    near = torch.arange(E, device=cuda) % 3 == 0
+    for b in (bias, torch.where(near, bias, bias - 1.0)):
+        kw = dict(scoring=scoring, bias=b)
+        same_route(ops.moe_route(x, 4, **kw), route64(x, 4, **kw), x)
+        two = torch.cat([x, x + 0.5, x])
+        same_route(ops.moe_route(two, 4, **kw), route64(two, 4, **kw), two)
+
+
+@pytest.mark.parametrize("E", [9, 100])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_route_with_bias_infinities(cuda, E, scoring):
+    g = torch.Generator(device=cuda).manual_seed(E)
+    x = torch.randn(12, E, generator=g, device=cuda)
+    x[3, 4] = INF
+    x[4, 2] = float("nan")
+    x[5] *= 1e30
+    x[6] = 1e38
+    bias = 0.2 * torch.randn(E, generator=g, device=cuda)
+    for at, v in ((0, INF), (1, -INF), (5, float("nan")), (7, 1e38)):
+        b = bias.clone()
+        b[at] = v
+        b[at + 1] = v
+        for b in (b, torch.full_like(b, v)):
+            kw = dict(scoring=scoring, bias=b)
+            same_route(ops.moe_route(x, 3, **kw), route64(x, 3, **kw), x)
+
+
+def test_route_largest(cuda):
+    """512 experts, 16 choices, both kinds of bias vectors and rows: those of 16 bytes and others."""
+    g = torch.Generator(device=cuda).manual_seed(11)
+    wide = torch.randn(150, 513, generator=g, device=cuda)
+    wb = 0.1 * torch.randn(513, generator=g, device=cuda)
+    for x, b in ((wide[:, :512].contiguous(), wb[:512].clone()), (wide[:, 1:], wb[1:]), (wide[:, :511].to(BF16), wb[:511])):
+        for T in (120, 150):
+            for scoring in ("softmax", "sigmoid"):
+                for bias in (None, b):
+                    kw = dict(scoring=scoring, renormalize=False, bias=bias)
+                    same_route(ops.moe_route(x[:T], 16, **kw), route64(x[:T], 16, **kw), x)
+
+
+def test_route_in_two_launches_captured(cuda):
+    """Its counts live in a workspace that every replay fills anew."""
+    x = torch.empty(3000, 40, device=cuda)
+    x.normal_()
+    ops.moe_route(x, 4)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a, b = ops.moe_route(x, 4), ops.moe_route(x[:700], 3, "sigmoid")
+    for seed in range(4):
+        x.normal_(generator=torch.Generator(device=cuda).manual_seed(seed))
+        if seed == 2:
+            x[:, :35] = -INF
+        ea, eb = ops.moe_route(x, 4), ops.moe_route(x[:700], 3, "sigmoid")
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip((*a, *b), (*ea, *eb)))
+
+
 def test_route_strides_and_no_tokens(cuda):
     g = torch.Generator(device=cuda).manual_seed(5)
     wide = torch.randn(40, 77, generator=g, device=cuda).to(BF16)
@@ -150,6 +217,32 @@ def test_layer_masks_and_uneven_experts(cuda):
             y = ops.moe_blocks(x, w1, s1, w2, s2, r)
             check(y, *moe64(x, w1, s1, w2, s2, weights, r.experts), BF16)
         assert bool((ops.moe_blocks(x, w1, s1, w2, s2, routing_of(ops, none, weights, E)) == 0).all())
+
+
+@pytest.mark.parametrize("T,E,k,H,F", [(128, 512, 16, 256, 128), (128, 102, 16, 672, 144), (128, 101, 16, 656, 144), (128, 32, 16, 2064, 272),
+                                       (128, 16, 16, 144, 16), (8, 3, 1, 272, 144), (1, 12, 8, 272, 144), (2, 7, 4, 272, 144)])
+def test_layer_at_its_limits(cuda, T, E, k, H, F):
+    """Most tokens, choices and experts; around the rules; a few pairs with equal choices and without one."""
+    g = torch.Generator(device=cuda).manual_seed(E)
+    w1, s1, w2, s2 = layer(g, E, H, F, cuda)
+    x = torch.randn(T, H, generator=g, device=cuda).to(BF16)
+    r = ops.moe_route(torch.randn(T, E, generator=g, device=cuda) + torch.randn(E, generator=g, device=cuda), k)
+    check(ops.moe_blocks(x, w1, s1, w2, s2, r), *moe64(x, w1, s1, w2, s2, r.weights, r.experts), BF16)
+    q = torch.Generator().manual_seed(E)
+    experts = torch.randint(-1, min(E, 3), (T, k), dtype=torch.int32, generator=q)
+    r = routing_of(ops, experts, torch.randn(T, k, generator=g, device=cuda), E)
+    check(ops.moe_blocks(x, w1, s1, w2, s2, r), *moe64(x, w1, s1, w2, s2, r.weights, r.experts), BF16)
+
+
+def test_layer_without_tokens(cuda):
+    g = torch.Generator(device=cuda).manual_seed(1)
+    w = layer(g, 3, 144, 80, cuda)
+    x = torch.empty(0, 144, device=cuda, dtype=BF16)
+    r = ops.moe_route(torch.empty(0, 3, device=cuda), 2)
+    for host in (ops._host, None):
+        with pytest.MonkeyPatch.context() as m:
+            m.setattr(ops, "_host", host)
+            assert ops.moe_blocks(x, *w, r).shape == (0, 144) and ops.moe_blocks(x, *w, r, residual=x).shape == (0, 144)
 
 
 def test_layer_strides(cuda):
