@@ -242,8 +242,10 @@ __device__ __forceinline__ void wave_order() {
 
 // Four tokens by a wave: lane j < k of each token's 16 returns choice j (expert or -1, weight).  token: the lane's row of logits.
 //
-// k rounds, each the largest key below the last, leave the key that the k best reach at least; the experts that reach it (with a
-// bias: but for the error of the fp32 scores), k of them unless some are equal, get a lane each and are ranked.
+// The k-th largest of the 16 lanes' own largest keys is one that the k best reach.  Where up to 16 experts reach it, as mostly with
+// up to 8 choices (it takes 10.6 draws to meet 8 of 16 lanes), they get a lane each and are ranked.  Else k rounds, each the
+// largest key below the last, leave the key of the k-th best, unless some are equal a later one.  With a bias both keys are lowered
+// by what the fp32 scores may be off by.
 template <int DT, int V, bool BIAS>
 __device__ __forceinline__ void pick(const RouteArgs& a, const void* token, float (&x)[V], int lane, int* scratch, int& expert, float& weight) {
     using L = Lay<DT, V>;
@@ -280,22 +282,40 @@ __device__ __forceinline__ void pick(const RouteArgs& a, const void* token, floa
     uint32_t key[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) key[v] = key_of(x[v]);
-    uint32_t least = best16(key);
-    for (int j = 1; j < a.k; ++j) {
-        const uint32_t m = next16(key, least);
-        if (__ballot(m != 0) == 0) break;
-        least = m != 0 ? m : least;
-    }
-    const float edge = value_of(least);
-    const float floor = !BIAS ? edge : edge - 0x1p-18f * (1.0f + fabsf(edge));
-    const bool some = least != 0, flat = BIAS && (any_nan || !(fabsf(edge) < __builtin_inff()));
-    const uint32_t least_key = !some ? 0xffffffffu : BIAS ? max(key_of(floor), 1u) : least;
-    uint32_t in = 0;                                      // bit v: element v can be among the best
+    // those from `least` on (with a bias: less what the fp32 scores may be off by), the lane's place among them and their number
+    uint32_t in = 0;                                      // bit v: element v is one
+    int at = 0, total = 0;
+    bool flat = false;
+    auto choose = [&](uint32_t least) {
+        const float edge = value_of(least);
+        flat = BIAS && (any_nan || !(fabsf(edge) < __builtin_inff()));
+        const uint32_t from = least == 0 ? 0xffffffffu : BIAS ? max(key_of(edge - 0x1p-18f * (1.0f + fabsf(edge))), 1u) : least;
+        in = 0;
 #pragma unroll
-    for (int v = V - 1; v >= 0; --v) in = 2 * in + (key[v] >= least_key ? 1u : 0u);
-    const int n = __popc(in);
-    int at = prefix16(n);
-    const int total = lane16(at + n, 15, lane);
+        for (int v = V - 1; v >= 0; --v) in = 2 * in + (key[v] >= from ? 1u : 0u);
+        const int n = __popc(in);
+        at = prefix16(n);
+        total = lane16(at + n, 15, lane);
+    };
+    const bool some = top_key != 0;
+    bool done = false;
+    if (a.k <= 8) {
+        uint32_t m = key[0];
+#pragma unroll
+        for (int v = 1; v < V; ++v) m = max(m, key[v]);
+        const uint32_t least = max16(rank16(m, l16) == a.k - 1 ? m : 0u);
+        choose(least);
+        done = __ballot(some && (least == 0 || total > 16)) == 0;
+    }
+    if (!done) {
+        uint32_t least = best16(key);
+        for (int j = 1; j < a.k; ++j) {
+            const uint32_t m = next16(key, least);
+            if (__ballot(m != 0) == 0) break;
+            least = m != 0 ? m : least;
+        }
+        choose(least);
+    }
     double sum64 = 1.0;
     if (BIAS && !a.sigmoid) {
         sum64 = 0.0;
