@@ -16,7 +16,7 @@
 // 32 us); only where more are within that error, all are.
 // A workgroup of 16 waves takes 64 tokens at a time, and ranks the pairs of 128 in LDS: the lanes of 64 consecutive pairs with the
 // same expert by one ballot per bit of its number, then the 64s in turn.  Up to 128 tokens one workgroup does it all; past that
-// a second launch adds up the counts of the workgroups before its own (at most 512) and moves the ranks to their places.
+// a second launch adds up the counts of the workgroups before its own (at most 256) and moves the ranks to their places.
 #include <algorithm>
 
 #include "h3fp8_common.h"
@@ -27,7 +27,7 @@ using namespace h3;
 
 constexpr int TB = 128;                                   // tokens of a batch; what one workgroup takes without a second launch
 constexpr int WAVES = 16;                                 // of a workgroup; 8 where a lane holds 32 logits and 64-bit scores
-constexpr int MAX_BLOCKS = 512;
+constexpr int MAX_BLOCKS = 256;
 constexpr int MAX_E = 512, MAX_K = 16;
 constexpr int CHUNKS = TB * MAX_K / 64;                   // of 64 pairs, in a batch
 
@@ -233,6 +233,14 @@ __device__ __forceinline__ int rank16(K key, int e) {
            rank_step<K, 11>(key, e) + rank_step<K, 12>(key, e) + rank_step<K, 13>(key, e) + rank_step<K, 14>(key, e) + rank_step<K, 15>(key, e);
 }
 
+// How many of the other 15 lanes have a larger key.
+template <int N = 1>
+__device__ __forceinline__ int above16(uint32_t key) {
+    const int more = dpp<0x120 + N>(key) > key ? 1 : 0;
+    if constexpr (N < 15) return more + above16<N + 1>(key);
+    return more;
+}
+
 // A wave's LDS accesses in order, for the compiler.
 __device__ __forceinline__ void wave_order() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -253,9 +261,9 @@ __device__ __forceinline__ void pick(const RouteArgs& a, const void* token, floa
     float top = x[0];
     bool nan = false;
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        top = fmaxf(top, x[v]);
-        nan = nan || x[v] != x[v];
+    for (int v = 0; v < V; v += 2) {
+        top = fmaxf(fmaxf(top, x[v]), x[v + 1]);
+        nan = nan || __builtin_isunordered(x[v], x[v + 1]);
     }
     const bool any_nan = max16(nan ? 1u : 0u) != 0;
     const uint32_t top_key = max16(key_of(top));          // 0: every logit is masked
@@ -279,20 +287,19 @@ __device__ __forceinline__ void pick(const RouteArgs& a, const void* token, floa
             x[v] = x[v] > -__builtin_inff() ? (s == s ? s : 0.0f) + b[v] : -__builtin_inff();
         }
     }
-    uint32_t key[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) key[v] = key_of(x[v]);
-    // those from `least` on (with a bias: less what the fp32 scores may be off by), the lane's place among them and their number
+    // those from the value of `least` on (with a bias: less what the fp32 scores may be off by), the lane's place among them and
+    // their number
     uint32_t in = 0;                                      // bit v: element v is one
     int at = 0, total = 0;
     bool flat = false;
     auto choose = [&](uint32_t least) {
         const float edge = value_of(least);
         flat = BIAS && (any_nan || !(fabsf(edge) < __builtin_inff()));
-        const uint32_t from = least == 0 ? 0xffffffffu : BIAS ? max(key_of(edge - 0x1p-18f * (1.0f + fabsf(edge))), 1u) : least;
+        const float lowest = -0x1.fffffep127f;
+        const float from = least == 0 ? __builtin_nanf("") : BIAS ? fmaxf(edge - 0x1p-18f * (1.0f + fabsf(edge)), lowest) : edge;
         in = 0;
 #pragma unroll
-        for (int v = V - 1; v >= 0; --v) in = 2 * in + (key[v] >= from ? 1u : 0u);
+        for (int v = V - 1; v >= 0; --v) in = 2 * in + (x[v] >= from ? 1u : 0u);
         const int n = __popc(in);
         at = prefix16(n);
         total = lane16(at + n, 15, lane);
@@ -300,14 +307,19 @@ __device__ __forceinline__ void pick(const RouteArgs& a, const void* token, floa
     const bool some = top_key != 0;
     bool done = false;
     if (a.k <= 8) {
-        uint32_t m = key[0];
+        if (BIAS) {
+            top = x[0];
 #pragma unroll
-        for (int v = 1; v < V; ++v) m = max(m, key[v]);
-        const uint32_t least = max16(rank16(m, l16) == a.k - 1 ? m : 0u);
+            for (int v = 1; v < V; ++v) top = fmaxf(top, x[v]);
+        }
+        const uint32_t m = key_of(top), least = min16(above16(m) < a.k ? m : 0xffffffffu);
         choose(least);
         done = __ballot(some && (least == 0 || total > 16)) == 0;
     }
     if (!done) {
+        uint32_t key[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) key[v] = key_of(x[v]);
         uint32_t least = best16(key);
         for (int j = 1; j < a.k; ++j) {
             const uint32_t m = next16(key, least);
@@ -386,6 +398,9 @@ __device__ __forceinline__ void pick(const RouteArgs& a, const void* token, floa
         }
     } else {
         // more than 16 reach it: equal ones, taken one by one, the lowest index first
+        uint32_t key[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) key[v] = key_of(x[v]);
         for (int j = 0; j < a.k; ++j) {
             const uint32_t m = best16(key);
             const int e = take16<DT, V>(key, m, l16);
@@ -563,11 +578,10 @@ __global__ void __launch_bounds__(WAVES * 64) moe_route_place_kernel(RouteArgs a
     }
 }
 
-// Tokens per workgroup of the first launch: one batch each until every CU has one, then as many as keep them within 256, or 512.
+// Tokens per workgroup of the first launch: as few 64s as keep the workgroups at 256, one per CU.  The second launch reads all their
+// counts in each: 131072 tokens x 256 experts 70 us with 512 workgroups.
 int64_t per_block(int64_t T) {
-    if (T <= TB) return TB;
-    const int64_t most = T > 128LL * MAX_BLOCKS ? MAX_BLOCKS : MAX_BLOCKS / 2;
-    return 64 * ((T + 64 * most - 1) / (64 * most));
+    return T <= TB ? TB : 64 * ((T + 64 * MAX_BLOCKS - 1) / (64 * MAX_BLOCKS));
 }
 
 template <int DT, int V>
