@@ -335,7 +335,8 @@ int h3fp8_gemm_blocks_act(const void* a, int64_t lda, const void* w, int64_t ldw
  *   no expert is left: expert -1, weight 0.  A NaN among a token's logits makes its weights NaN.
  *   order [T k]: the pairs p = t k + j sorted by expert, ascending within one, those without an expert last; offsets [E + 1]: expert
  *   e has the places offsets[e] .. offsets[e + 1] - 1 (the rows of h3fp8_grouped_gemm_blocks); place [T k]: where p went.
- * E at most 512, k at most 16.  workspace: h3fp8_moe_route_workspace(T, E) bytes of device memory (0 up to 128 tokens).
+ * E at most 512, k at most 16.  workspace: h3fp8_moe_route_workspace(T, E) bytes of device memory, 16-byte aligned (0 up to 128
+ * tokens).
  */
 int64_t h3fp8_moe_route_workspace(int64_t T, int64_t E);
 int h3fp8_moe_route(const void* logits, int64_t ld, int dtype, int64_t T, int64_t E, int k, int scoring, int renorm,
@@ -343,14 +344,15 @@ int h3fp8_moe_route(const void* logits, int64_t ld, int dtype, int64_t T, int64_
                     int32_t* place, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
- * A whole layer of block-scaled experts for at most 128 tokens, two launches:
+ * A whole layer of block-scaled experts for at most 128 tokens, two launches (up to 8 pairs) or three:
  *   y[t] = residual[t] + sum_j weights[t, j] * W2[e] (silu(g) * u),  g | u = W1[e] x[t],  e = experts[t, j]
  * x, residual (or NULL), y [T, H] bf16 or fp16 (dtype), not quantised; w1 [E, 2F, H] (gate rows, then up rows) and w2 [E, H, F]
  * e4m3 with expert strides and row strides, scales [E, ceil(2F / 128), ceil(H / 128)] and [E, ceil(H / 128), ceil(F / 128)] in
  * any strides; weights, experts, offsets, order: those of h3fp8_moe_route.  fp32 throughout, the inner values h carried in 16
  * bits of mantissa, one rounding of y.  An expert's NaN or infinity reaches its own tokens only.  y may be the residual itself.
  * H, F multiples of 16; x and weights 16-byte aligned, row strides of x multiples of 8, of the weights of 16, of y and the
- * residual of 4 (8-byte aligned).  workspace: h3fp8_moe_blocks_workspace bytes of device memory, 16-byte aligned.
+ * residual of 4 (8-byte aligned); 256 rows of x and 128 of a weight within 2 GiB, all scales of a layer within 1.  workspace:
+ * h3fp8_moe_blocks_workspace bytes of device memory, 16-byte aligned.
  */
 int64_t h3fp8_moe_blocks_workspace(int64_t T, int64_t k, int64_t H, int64_t F, int64_t E);
 int h3fp8_moe_blocks(const void* x, int64_t ldx, int dtype, int64_t T, int64_t H, int64_t F, int64_t E, int k, const void* w1,

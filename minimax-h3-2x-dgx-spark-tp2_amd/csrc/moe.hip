@@ -1,20 +1,20 @@
-// A whole layer of block-scaled FP8 experts for a few tokens (gfx950), in two kernels.
+// A whole layer of block-scaled FP8 experts for a few tokens (gfx950), in two or three kernels.
 //
 //   y[t] = residual[t] + sum_j weight[t, j] * W2[e] h,  h = silu(g) * u,  g | u = W1[e] x[t],  e = experts[t, j]
 //
-// Every weight is read once, the tokens of an expert together, and the time is that of the weights' bytes.  The tokens stay as
+// Every weight is read once, the tokens of an expert together, and the floor is the weights' bytes.  The tokens stay as
 // they are (bf16 / fp16), unlike in the path of many tokens, whose products quantise them: the weights' e4m3 codes are
 // widened in registers (bf16 and fp16 hold them exactly), MFMAs 16x16x32 make the sum of one block of 128 from a zero
 // accumulator, the weight rows as the A operand and the tokens as B, and one fma per element adds it with the block's
-// scale in fp32.
+// scale in fp32.  Kernel 1 leaves h times the pair's weight as two bf16 numbers, the value and what its rounding left (16 bits
+// in all), so that the layer has one rounding to the output's type and none that counts before.
 //
-// Kernel 1: a workgroup takes 16 NI gate rows and the up rows that belong to them, of one expert that has tokens, and all of
-// that expert's tokens; its 8 waves share out the blocks of K and join through LDS.  h times the pair's weight leaves as two
-// bf16 numbers, the value and what its rounding left (16 bits in all, so that the layer has one rounding to the output's
-// type and none that counts before).
-// Kernel 2: a workgroup takes 16 CT rows of W2 for all experts, and its waves share out the (expert, block of F) units; the
-// MFMA's 16 columns are tokens by their own number, zero where a token is not the expert's, so that the sums over experts
-// stay in the accumulators and no order of workgroups shows in the result.
+// Up to 8 pairs (a token or a few) what counts is the latency up to the first bytes: kernels that find their rows by ballots.
+// Past that a workgroup's waves share the tokens' values through LDS, and its items follow each other without a pause.
+//
+// us of the kernels together, and the weights' bytes over that: 4 experts of 4096 x 2048 (1 token) 29, 3.5 TB/s; 12 of 1200 x
+// 1040 (37 tokens, fp16) 24, 1.9; 28 to 32 of 4096 x 2048 (16 tokens) 116 to 128, 6.1; 32 of 4096 x 2048 (128 tokens, 1024 pairs)
+// 186 to 200, 4.2.  A copy of 2 GiB runs at 5.0 TB/s, read and written together.
 #include <algorithm>
 #include <type_traits>
 
@@ -441,11 +441,21 @@ __global__ void __launch_bounds__(DOWN_WAVES * 64) moe_few_down_kernel(MoeParams
 
 // ---- more rows per expert -----------------------------------------------------------------------------------------------
 //
-// With many rows the tokens' values, read again for every 16 weight rows, are more than the weights.  So the 8 waves of a workgroup
-// take 8 neighbouring tiles of weight rows, the whole of K each (no join), and share the tokens' values through LDS: an item is a
-// block of up to 16 NT rows and 8 tiles.  A unit is 256 (NT = 1) or 128 of K in kernel 1, 128 of F (both numbers) in kernel 2.  It comes by LDS-DMA, two units ahead of its use in a ring of three, one barrier per unit; the weights come two units
-// ahead into registers.  Kernel 2 leaves the pairs' results in fp32, and a third kernel adds up the choices of each token, in their
-// order.
+// With many rows the tokens' values, read again for every 16 weight rows, are more than the weights.  So the waves of a workgroup
+// (4 or 8) take neighbouring tiles of weight rows, the whole of K each (no join), and share the tokens' values through LDS: an item
+// is a block of up to 16 NT rows of an expert and a tile of 16 output channels (kernel 1, gate and up rows) or 32 (kernel 2) per
+// wave.  A unit is a block of 128 of K.  Tokens, weights and scales come by LDS-DMA, two units ahead of their use in a ring of
+// three, one barrier per unit; the loads of the next item follow those of the last without a pause.
+//
+// What bounded the steps before, us of the layer at 32 experts of 4096 x 2048, 64 / 1024 pairs: a workgroup per item, the weights
+// straight into registers, 216 / 709; items one behind the other, the tokens shared through LDS, 145 / 330 (a lane had 16 bytes of its
+// row, which the memory pipe takes one by one); weights in whole lines of 128 bytes through LDS, blocks of one expert at the same
+// time on one XCD, so that its L2 has the weights, and each item's K from a start of its own, (3 e + 5 tile) units in (rows a
+// power of two apart meet the same channels: 7 to 8 %), 115 / 200.  What bounds it now: up to 20 rows per expert the weights' bytes
+// (6.1 TB/s); past that the largest XCD's items, whole rounds of blocks over its 32 CUs.  Blocks of 64 rows make those rounds
+// coarser: 110 to 140 us in kernel 1 against 114, 83 to 105 in kernel 2 against 78.
+
+// Kernel 2 leaves the pairs' results in fp32, and a third kernel adds up the choices of each token, in their order.
 
 // LDS place of 16-byte chunk i of weight row r (128 bytes): i ^ this.
 __device__ __forceinline__ int weight_swz(int r) { return (r & 2) | ((r >> 1) & 4); }

@@ -927,7 +927,7 @@ def moe_route(logits: torch.Tensor, k: int, scoring: str = "softmax", renormaliz
     if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.dtype not in _DT:
         raise ValueError("moe_route takes bf16, fp16 or fp32 logits [T, E]")
     T, E = logits.shape
-    if not 1 <= E <= MOE_MAX_EXPERTS or not 1 <= k <= min(E, MOE_MAX_CHOICES):
+    if not isinstance(k, int) or not 1 <= E <= MOE_MAX_EXPERTS or not 1 <= k <= min(E, MOE_MAX_CHOICES):
         raise ValueError(f"moe_route: k = {k} of {E} experts (1 to {MOE_MAX_CHOICES} of 1 to {MOE_MAX_EXPERTS})")
     if scoring not in ("softmax", "sigmoid"):
         raise ValueError(f'moe_route: scoring must be "softmax" or "sigmoid", got {scoring!r}')
@@ -960,7 +960,7 @@ def _expert_weight(name: str, w: torch.Tensor, shape: tuple) -> int:
 def moe_blocks(x: torch.Tensor, w_gate_up: torch.Tensor, scale_gate_up: torch.Tensor, w_down: torch.Tensor,
                scale_down: torch.Tensor, routing: Routing, residual: torch.Tensor | None = None,
                out: torch.Tensor | None = None) -> torch.Tensor:
-    """A whole layer of block-scaled experts for a few tokens (at most 128), in two launches: y [T, H] = residual + the sum over a
+    """A whole layer of block-scaled experts for a few tokens (at most 128), in two launches or three: y [T, H] = residual + the sum over a
     token's choices of weight * w_down[e] (silu(gate) * up), gate | up = w_gate_up[e] x.  ``x`` bf16 / fp16 [T, H], not
     quantised; ``w_gate_up`` e4m3 [E, 2F, H] and ``w_down`` [E, H, F] with one scale per 128 x 128 (``quant_blocks(rows=128)``; any
     strides); ``routing`` as ``moe_route`` returns it.  fp32 throughout, rounded once.  ``out`` may be the residual itself and

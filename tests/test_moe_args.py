@@ -36,7 +36,7 @@ def test_route(calls):
     assert [t.dtype for t in r] == [F32] + 4 * [torch.int32]
     ops.moe_route(x.to(BF16), 1, "sigmoid", False, 2.5, torch.zeros(24))
     n = len(calls)
-    refused(lambda **kw: ops.moe_route(**{"logits": x, "k": 3, **kw}), dict(k=0), dict(k=25), dict(k=17), dict(logits=x[0]), dict(logits=x.t()),
+    refused(lambda **kw: ops.moe_route(**{"logits": x, "k": 3, **kw}), dict(k=0), dict(k=25), dict(k=17), dict(k=2.0), dict(logits=x[0]), dict(logits=x.t()),
             dict(logits=x.double()), dict(logits=torch.zeros(2, 513)), dict(logits=torch.zeros(2, 0)), dict(scoring="relu"),
             dict(bias=torch.zeros(23)), dict(bias=torch.zeros(24, dtype=BF16)), dict(bias=torch.zeros(48)[::2]))
     assert len(calls) == n
