@@ -56,17 +56,6 @@ __device__ __forceinline__ int offset_at(const MoeParams& p, int e) {
     return min(max(p.offsets[e], 0), p.T * p.k);          // whatever the offsets hold, no pair outside [0, T k) is read
 }
 
-// 16 bytes per lane; OOB (and up to 64 KiB past it) and what lies past the buffer read as zeros.  The hardware checks the lane's
-// offset against the buffer's size less the uniform offset: that one is the start of a block that there is.
-__device__ __forceinline__ v4u load16(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff) {
-    return __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(r, (int)voff, (int)soff, 0));
-}
-
-// One number for all lanes.
-__device__ __forceinline__ float load4(__amdgpu_buffer_rsrc_t r, uint32_t off) {
-    return u2f(__builtin_amdgcn_raw_buffer_load_b32(r, (int)off, 0, 0));
-}
-
 // Eight e4m3 codes as an MFMA operand.
 __device__ __forceinline__ v8bf widen_bf16(uint32_t lo, uint32_t hi) {
     typedef __bf16 v2 __attribute__((ext_vector_type(2)));
@@ -231,10 +220,14 @@ __device__ __forceinline__ void store_h(const MoeParams& p, int pair, int f, flo
     *reinterpret_cast<uint2*>(at + 32) = uint2{lo[0] | (lo[1] << 16), lo[2] | (lo[3] << 16)};
 }
 
-// 4 consecutive channels n .. n + 3 of a token, with the residual.
-__device__ __forceinline__ void store_y(const MoeParams& p, int t, int n, v4f v) {
+// The residual's 4 channels n .. n + 3 of a token; zeros without one.
+__device__ __forceinline__ uint2 residual_at(const MoeParams& p, int t, int n) {
+    return p.residual ? *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p.residual) + t * p.ldr + n) : uint2{0u, 0u};
+}
+
+// 4 consecutive channels of a token, with the residual.
+__device__ __forceinline__ void store_y(const MoeParams& p, int t, int n, v4f v, uint2 r) {
     if (p.residual) {
-        const uint2 r = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p.residual) + t * p.ldr + n);
         const uint32_t b[4] = {r.x & 0xffffu, r.x >> 16, r.y & 0xffffu, r.y >> 16};
 #pragma unroll
         for (int q = 0; q < 4; ++q) v[q] += p.fp16 ? fp16_to_f32(b[q]) : bf16_to_f32(b[q]);
@@ -249,8 +242,16 @@ __device__ __forceinline__ void store_y(const MoeParams& p, int t, int n, v4f v)
 // What counts is how soon the weights' bytes are asked for.  The pairs, at most 64, are a lane each: the experts that have
 // pairs, the pairs of one and their tokens come out of ballots on one load of `experts`, by every wave for itself.
 
-constexpr int FEW = 64;                                   // pairs
-constexpr int UP_WAVES = 8, DOWN_WAVES = 16;
+// LDS place of 16-byte chunk i of weight row r (128 bytes): i ^ this.
+__device__ __forceinline__ int weight_swz(int r) { return (r & 2) | ((r >> 1) & 4); }
+
+// LDS place of 16-byte chunk i of row r: the 16 lanes that are served together (0-3, 12-15 and 20-27; 4-11, 16-19 and 28-31) meet 16
+// places.  Kernel 1: lane group g reads chunks 2 g + ..; kernel 2: 4 g + ..
+template <bool UP>
+__device__ __forceinline__ int chunk_at(int r, int i) {
+    const int c = r & 15;
+    return i ^ (UP ? c : (((c >> 2) ^ (c >> 3)) & 1) | ((c & 3) << 1) | (c & 8));
+}
 
 // Each token's first pair among the pairs `same` (of one expert): the second of two equal choices is not a row of its own.
 __device__ __forceinline__ uint64_t first_pairs(uint64_t same, int lane, int k) {
@@ -258,18 +259,38 @@ __device__ __forceinline__ uint64_t first_pairs(uint64_t same, int lane, int k) 
     return same & __ballot(((same >> (t * k)) & ((1ull << (lane - t * k)) - 1)) == 0);
 }
 
-// Kernel 1: a workgroup takes 16 gate rows and the up rows that belong to them, of one expert; its 8 waves share out the blocks of K,
-// D each under way, and join through LDS.
-template <bool FP16, int D>
-__global__ void __launch_bounds__(UP_WAVES * 64, 4) moe_few_up_kernel(MoeParams p, int tiles) {
-    __shared__ v4f part[UP_WAVES][2][64];
+// A wave has two units under way, in LDS of its own: weights in whole lines, the values of up to TOKENS tokens (more columns of the
+// MFMAs repeat them), scales.
+template <bool UP, int TOKENS>
+struct Few {
+    static constexpr int WAVES = UP ? 8 : TOKENS > 2 ? 8 : 16;
+    static constexpr int ROW = UP ? 256 : 512, LPR = ROW / 16, RPI = 64 / LPR;        // bytes of a token's block; lanes; tokens of an instruction
+    static constexpr int DW = UP ? 4 : 2, DX = TOKENS > RPI ? TOKENS / RPI : 1;
+    static constexpr int X = DW * 1024, S = X + TOKENS * ROW, STAGE = S + 16, LDS = 2 * STAGE * WAVES;
+    static constexpr int LOADS = DW + DX + 1;
+    static_assert(LDS >= WAVES * 64 * 16 * (UP ? 2 : 1), "the waves' sums take the place of the stages");
+};
+
+// All but the last N loads have landed; LDS is read behind this.
+template <int N>
+__device__ __forceinline__ void stage_landed() {
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(N));
+    asm volatile("" ::: "memory");
+}
+
+// Kernel 1: a workgroup takes 16 gate rows and the up rows that belong to them, of one expert; its 8 waves share out the blocks of K
+// and join through LDS.
+template <bool FP16, int TOKENS>
+__global__ void __launch_bounds__((Few<true, TOKENS>::WAVES * 64)) moe_few_up_kernel(MoeParams p, int tiles) {
+    using C = Few<true, TOKENS>;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[C::LDS];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4, P = p.T * p.k;
     const int mine = lane < P ? p.experts[lane] : -1;
     const float weight = lane < P ? p.weights[lane] : 0.0f;
     int slot = (int)blockIdx.x / tiles;
-    const int f0 = ((int)blockIdx.x - slot * tiles) * 16;
+    const int tile = (int)blockIdx.x - slot * tiles, f0 = tile * 16;
     uint64_t left = __ballot(mine >= 0 && mine < p.E), same = 0;
     int e = 0;
     for (; left; --slot) {
@@ -286,62 +307,87 @@ __global__ void __launch_bounds__(UP_WAVES * 64, 4) moe_few_up_kernel(MoeParams 
     const int pair = __builtin_amdgcn_ds_permute(4 * at, lane), col = __shfl(pair, c, 64);
     const int kb = (p.H + BK - 1) / BK;
     const uint8_t* w0 = p.w1 + e * p.w1_e + f0 * p.ld1;
-    const uint32_t bytes = (uint32_t)(15 * p.ld1 + p.H);
-    const __amdgpu_buffer_rsrc_t rg = make_rsrc(w0, bytes), ru = make_rsrc(w0 + p.F * p.ld1, bytes), rs = make_rsrc(p.s1, 0x7fffffffu);
-    const __amdgpu_buffer_rsrc_t rx = make_rsrc(p.x, (uint32_t)(((p.T - 1) * p.ldx + p.H) * 2));
-    const uint32_t vw = (uint32_t)(c * p.ld1) + 16u * g, vx = c < n ? (uint32_t)(col / p.k) * (uint32_t)(p.ldx * 2) + 32u * g : OOB;
-    const uint32_t sg = (uint32_t)(e * p.s1_e + f0 / BK * p.s1_n) * 4u, su = (uint32_t)(e * p.s1_e + (p.F + f0) / BK * p.s1_n) * 4u;
-    v4u w[D][2][2], x[D][2][2];
-    float sc[D][2];
-    // always the same loads, past the last block of nothing, so that the count of those under way is known
-    auto load = [&](int d, int b) {
-        const int k0 = b < kb ? b * BK : 0, rest = b < kb ? p.H - k0 : 0;
+    const uint32_t bytes = (uint32_t)(15 * p.ld1 + p.H), row_bytes = (uint32_t)p.H * 2u;
+    const v4u qg = buffer_desc(w0, bytes), qu = buffer_desc(w0 + p.F * p.ld1, bytes), qs = buffer_desc(p.s1, 0x7fffffffu);
+    const v4u qx = buffer_desc(p.x, (uint32_t)(((p.T - 1) * p.ldx + p.H) * 2));
+    uint32_t cw[2], vw[2], cx[C::DX], vx[C::DX];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const bool in = 64 * s + 16 * g < rest;
-            w[d][0][s] = load16(rg, (in ? vw : OOB) + 64 * s, k0);
-            w[d][1][s] = load16(ru, (in ? vw : OOB) + 64 * s, k0);
-#pragma unroll
-            for (int q = 0; q < 2; ++q) x[d][s][q] = load16(rx, (in ? vx : OOB) + 128 * s + 16 * q, 2 * k0);
-        }
-        const uint32_t sb = (uint32_t)(min(b, kb - 1) * p.s1_k) * 4u;
-        sc[d][0] = load4(rs, sg + sb);
-        sc[d][1] = load4(rs, su + sb);
-        __builtin_amdgcn_sched_barrier(0);                // in this order: the waits count them
-    };
-#pragma unroll
-    for (int d = 0; d < D; ++d) load(d, wave + d * UP_WAVES);
-    v4f acc[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
-    for (int b = wave; b < kb; b += D * UP_WAVES) {
-#pragma unroll
-        for (int d = 0; d < D; ++d) {
-            v4f sum[2][1];
-#pragma unroll
-            for (int q = 0; q < 4; ++q)                   // 32 of the block's k each
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const v4u& a = w[d][i][q >> 1];
-                    if (q == 0) mfma<FP16, true>(sum[i][0], a[0], a[1], x[d][0][0]);
-                    else mfma<FP16, false>(sum[i][0], a[2 * (q & 1)], a[2 * (q & 1) + 1], x[d][q >> 1][q & 1]);
-                }
-            sums_ready(sum);
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) acc[i][k] = __builtin_fmaf(sum[i][0][k], sc[d][i], acc[i][k]);
-            __builtin_amdgcn_sched_barrier(0);
-            load(d, b + (d + D) * UP_WAVES);
-        }
+    for (int i = 0; i < 2; ++i) {
+        const int r = 8 * i + (lane >> 3);
+        cw[i] = 16u * (uint32_t)((lane & 7) ^ weight_swz(r));
+        vw[i] = (uint32_t)(r * p.ld1) + cw[i];
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) part[wave][i][lane] = acc[i];
+    for (int i = 0; i < C::DX; ++i) {
+        const int r = C::RPI * i + lane / C::LPR, token = __shfl(pair, r, 64) / p.k;
+        cx[i] = 16u * (uint32_t)chunk_at<true>(r, lane % C::LPR);
+        vx[i] = r < n ? (uint32_t)token * (uint32_t)(p.ldx * 2) + cx[i] : OOB;
+    }
+    const uint32_t sv = (uint32_t)(e * p.s1_e + (lane & 1 ? p.F + f0 : f0) / BK * p.s1_n) * 4u;
+    const uint8_t* own = lds + wave * 2 * C::STAGE;
+    const uint32_t own0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds_addr(own));
+    const int turn = (3 * e + 5 * tile) % kb;
+    // always the same loads, past the last block of nothing, so that the count of those under way is known
+    auto load = [&](int d, int b) {
+        const int blk = b < kb ? (b + turn < kb ? b + turn : b + turn - kb) : 0;
+        const uint32_t k0 = (uint32_t)(blk * BK), left = b < kb ? (uint32_t)p.H - k0 : 0u, at0 = own0 + (uint32_t)(d * C::STAGE);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            dma16_at(i < 2 ? qg : qu, __builtin_amdgcn_readfirstlane(at0 + 1024u * i), cw[i & 1] < left ? vw[i & 1] : OOB, __builtin_amdgcn_readfirstlane(k0));
+#pragma unroll
+        for (int i = 0; i < C::DX; ++i)
+            if (C::RPI * (i + 1) <= TOKENS || lane < TOKENS * C::LPR)
+                dma16(qx, __builtin_amdgcn_readfirstlane(at0 + C::X + 1024u * i),
+                      b < kb && vx[i] != OOB && 2 * k0 + cx[i] < row_bytes ? vx[i] + 2 * k0 : OOB);
+        if (lane < 2) dma4(qs, __builtin_amdgcn_readfirstlane(at0 + C::S), sv + (uint32_t)(blk * p.s1_k) * 4u);
+    };
+#pragma unroll
+    for (int d = 0; d < 2; ++d) load(d, wave + d * C::WAVES);
+    v4f acc[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
+    int d = 0;
+    for (int b = wave; b < kb; b += C::WAVES, d ^= 1) {
+        stage_landed<C::LOADS>();
+        const uint8_t *ws = own + d * C::STAGE + c * 128, *xs = own + d * C::STAGE + C::X + (c & (TOKENS - 1)) * C::ROW;
+        v4u w[2][2], x[2][2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) w[i][s] = *reinterpret_cast<const v4u*>(ws + 2048 * i + 16 * ((4 * s + g) ^ weight_swz(c)));
+#pragma unroll
+            for (int q = 0; q < 2; ++q) x[s][q] = *reinterpret_cast<const v4u*>(xs + 16 * chunk_at<true>(c & (TOKENS - 1), 8 * s + 2 * g + q));
+        }
+        const float sg = *reinterpret_cast<const float*>(own + d * C::STAGE + C::S), su = *reinterpret_cast<const float*>(own + d * C::STAGE + C::S + 4);
+        wait_lgkm0();
+        __builtin_amdgcn_sched_barrier(0);
+        load(d, b + 2 * C::WAVES);
+        v4f sum[2][1];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)                       // 32 of the block's k each
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const v4u& a = w[i][q >> 1];
+                if (q == 0) mfma<FP16, true>(sum[i][0], a[0], a[1], x[0][0]);
+                else mfma<FP16, false>(sum[i][0], a[2 * (q & 1)], a[2 * (q & 1) + 1], x[q >> 1][q & 1]);
+            }
+        sums_ready(sum);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            acc[0][r] = __builtin_fmaf(sum[0][0][r], sg, acc[0][r]);
+            acc[1][r] = __builtin_fmaf(sum[1][0][r], su, acc[1][r]);
+        }
+    }
+    wait_vm0();                                           // the loads behind the last unit
+    __syncthreads();
+    v4f* part = reinterpret_cast<v4f*>(lds);              // [wave][gate, up][lane]
+#pragma unroll
+    for (int i = 0; i < 2; ++i) part[(wave * 2 + i) * 64 + lane] = acc[i];
     __syncthreads();
     if (wave != 0) return;
-    v4f gate = part[0][0][lane], up = part[0][1][lane];
+    v4f gate = part[lane], up = part[64 + lane];
 #pragma unroll
-    for (int v = 1; v < UP_WAVES; ++v) {
-        gate += part[v][0][lane];
-        up += part[v][1][lane];
+    for (int v = 1; v < C::WAVES; ++v) {
+        gate += part[2 * v * 64 + lane];
+        up += part[(2 * v + 1) * 64 + lane];
     }
     float sum = 0.0f;                                     // of all the token's choices of this expert
     for (uint64_t m = same; m; m &= m - 1) {
@@ -352,21 +398,35 @@ __global__ void __launch_bounds__(UP_WAVES * 64, 4) moe_few_up_kernel(MoeParams 
     if (c < n) store_h(p, col, f0 + 4 * g, sum, gate, up);
 }
 
-// Kernel 2: a workgroup takes 16 channels for all experts; its 16 waves share out the units, the blocks of F of every expert that has
+// Kernel 2: a workgroup takes 16 channels for all experts; its waves share out the units, the blocks of F of every expert that has
 // pairs.  Column c of the MFMAs is token c, zero where it is not the expert's, so that the accumulators run over all experts.
-template <int D>
-__global__ void __launch_bounds__(DOWN_WAVES * 64) moe_few_down_kernel(MoeParams p) {
-    __shared__ v4f part[DOWN_WAVES][64];
+template <int TOKENS>
+__global__ void __launch_bounds__((Few<false, TOKENS>::WAVES * 64)) moe_few_down_kernel(MoeParams p) {
+    using C = Few<false, TOKENS>;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[C::LDS];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4, P = p.T * p.k, n0 = (int)blockIdx.x * 16;
     const int mine = lane < P ? p.experts[lane] : -1;
-    const uint64_t all = __ballot(mine >= 0 && mine < p.E);
+    const uint2 residual = wave == 0 && c < p.T ? residual_at(p, c, n0 + 4 * g) : uint2{0u, 0u};      // on its way from here on
+    const uint64_t all = __ballot(mine >= 0 && mine < p.E), choices = (1ull << p.k) - 1;
     const int fb = (p.F + BK - 1) / BK;
-    const __amdgpu_buffer_rsrc_t rh = make_rsrc(p.h, (uint32_t)P * (uint32_t)p.F * 4u), rs = make_rsrc(p.s2, 0x7fffffffu);
-    const uint32_t vw = (uint32_t)(c * p.ld2) + 16u * g, wbytes = (uint32_t)(15 * p.ld2 + p.F);
+    const uint32_t row_bytes = (uint32_t)p.F * 4u;
+    const v4u qh = buffer_desc(p.h, (uint32_t)P * row_bytes), qs = buffer_desc(p.s2, 0x7fffffffu);
+    const uint32_t wbytes = (uint32_t)(15 * p.ld2 + p.F);
     const uint8_t* w0 = p.w2 + n0 * p.ld2;
     const uint32_t s0 = (uint32_t)(n0 / BK * p.s2_n) * 4u;
+    uint32_t cw[2], vw[2], cx[C::DX];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = 8 * i + (lane >> 3);
+        cw[i] = 16u * (uint32_t)((lane & 7) ^ weight_swz(r));
+        vw[i] = (uint32_t)(r * p.ld2) + cw[i];
+    }
+#pragma unroll
+    for (int i = 0; i < C::DX; ++i) cx[i] = 16u * (uint32_t)chunk_at<false>(C::RPI * i + lane / C::LPR, lane % C::LPR);
+    const uint8_t* own = lds + wave * 2 * C::STAGE;
+    const uint32_t own0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds_addr(own));
     // the units of a wave: block b of the expert at hand, whose pairs are the first of `left`
     struct Unit { uint64_t left, same; int e, b; };
     auto settle = [&](Unit& u) {                          // ... to where b is one of the expert's blocks, or nothing is left
@@ -380,63 +440,71 @@ __global__ void __launch_bounds__(DOWN_WAVES * 64) moe_few_down_kernel(MoeParams
             u.left &= ~u.same;
         }
     };
-    v4u w[D][2], h[D][2][4];                              // h: 16 values, what they leave
-    float sc[D];
-    bool has[D];                                          // token c is the expert's
-    Unit next{all, 0, 0, wave};
+    Unit next{all, 0, 0, wave}, now = next;
     settle(next);
+    now = next;
+    auto step = [&](Unit& u) { u.b += C::WAVES; settle(u); };
     // always the same loads, past the last unit of nothing, so that the count of those under way is known
     auto load = [&](int d) {
         const bool live = next.left != 0;
-        const int b = live ? next.b : 0, e = live ? next.e : 0, rest = live ? p.F - b * BK : 0;
-        const uint64_t pairs = live && c < p.T ? (next.same >> (c * p.k)) & ((1ull << p.k) - 1) : 0;
-        has[d] = pairs != 0;
-        const uint32_t vh = pairs ? (uint32_t)(c * p.k + __builtin_ctzll(pairs)) * (uint32_t)p.F * 4u + 64u * g : OOB;
-        const __amdgpu_buffer_rsrc_t rw = make_rsrc(w0 + e * p.w2_e, live ? wbytes : 0u);
+        const int b = live ? next.b : 0, e = live ? next.e : 0;
+        const uint32_t k0 = (uint32_t)(b * BK), left = live ? (uint32_t)p.F - k0 : 0u, at0 = own0 + (uint32_t)(d * C::STAGE);
+        const v4u qw = buffer_desc(w0 + e * p.w2_e, live ? wbytes : 0u);
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const bool in = 64 * s + 16 * g < rest;
-            w[d][s] = load16(rw, (in ? vw : OOB) + 64 * s, b * BK);
+        for (int i = 0; i < 2; ++i)
+            dma16_at(qw, __builtin_amdgcn_readfirstlane(at0 + 1024u * i), cw[i] < left ? vw[i] : OOB, __builtin_amdgcn_readfirstlane(k0));
 #pragma unroll
-            for (int q = 0; q < 4; ++q) h[d][s][q] = load16(rh, (in ? vh : OOB) + 256 * s + 16 * q, 4 * b * BK);
+        for (int i = 0; i < C::DX; ++i) {
+            const int t = C::RPI * i + lane / C::LPR;
+            const uint64_t pairs = live && t < p.T ? (next.same >> (t * p.k)) & choices : 0;
+            dma16(qh, __builtin_amdgcn_readfirstlane(at0 + C::X + 1024u * i),
+                  pairs && 4 * k0 + cx[i] < row_bytes ? (uint32_t)(t * p.k + __builtin_ctzll(pairs)) * row_bytes + 4 * k0 + cx[i] : OOB);
         }
-        sc[d] = load4(rs, (uint32_t)(e * p.s2_e + b * p.s2_k) * 4u + s0);
-        next.b += DOWN_WAVES;
-        settle(next);
-        __builtin_amdgcn_sched_barrier(0);                // in this order: the waits count them
+        if (lane == 0) dma4(qs, __builtin_amdgcn_readfirstlane(at0 + C::S), (uint32_t)(e * p.s2_e + b * p.s2_k) * 4u + s0);
+        step(next);
     };
     v4f acc = v4f{0.f, 0.f, 0.f, 0.f};
-    bool more = next.left != 0;
 #pragma unroll
-    for (int d = 0; d < D; ++d) load(d);
-    while (more) {
-        more = next.left != 0;                            // units of the round behind the loads under way
+    for (int d = 0; d < 2; ++d) load(d);
+    for (int d = 0; now.left; step(now), d ^= 1) {
+        stage_landed<C::LOADS>();
+        const uint8_t *ws = own + d * C::STAGE + c * 128, *xs = own + d * C::STAGE + C::X + (c & (TOKENS - 1)) * C::ROW;
+        v4u w[2], h[2][4];                                // h: 16 values, what they leave
 #pragma unroll
-        for (int d = 0; d < D; ++d) {
-            v4f sum[1][1];
+        for (int s = 0; s < 2; ++s) {
+            w[s] = *reinterpret_cast<const v4u*>(ws + 16 * ((4 * s + g) ^ weight_swz(c)));
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const uint32_t lo = w[d][q >> 1][2 * (q & 1)], hi = w[d][q >> 1][2 * (q & 1) + 1];
-                if (q == 0) mfma<false, true>(sum[0][0], lo, hi, h[d][0][0]);
-                else mfma<false, false>(sum[0][0], lo, hi, h[d][q >> 1][q & 1]);
-                mfma<false, false>(sum[0][0], lo, hi, h[d][q >> 1][2 + (q & 1)]);
-            }
-            sums_ready(sum);
-            if (has[d]) {                                 // an expert's NaN is not another token's
+            for (int q = 0; q < 4; ++q) h[s][q] = *reinterpret_cast<const v4u*>(xs + 16 * chunk_at<false>(c & (TOKENS - 1), 4 * (4 * s + g) + q));
+        }
+        const float scale = *reinterpret_cast<const float*>(own + d * C::STAGE + C::S);
+        const bool has = c < p.T && ((now.same >> (c * p.k)) & choices) != 0;
+        wait_lgkm0();
+        __builtin_amdgcn_sched_barrier(0);
+        load(d);
+        v4f sum[1][1];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) acc[r] = __builtin_fmaf(sum[0][0][r], sc[d], acc[r]);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            if (more) load(d);
+        for (int q = 0; q < 4; ++q) {
+            const uint32_t lo = w[q >> 1][2 * (q & 1)], hi = w[q >> 1][2 * (q & 1) + 1];
+            if (q == 0) mfma<false, true>(sum[0][0], lo, hi, h[0][0]);
+            else mfma<false, false>(sum[0][0], lo, hi, h[q >> 1][q & 1]);
+            mfma<false, false>(sum[0][0], lo, hi, h[q >> 1][2 + (q & 1)]);
+        }
+        sums_ready(sum);
+        if (has) {                                        // an expert's NaN is not another token's
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[r] = __builtin_fmaf(sum[0][0][r], scale, acc[r]);
         }
     }
-    part[wave][lane] = acc;
+    wait_vm0();                                           // the loads behind the last unit
+    __syncthreads();
+    v4f* part = reinterpret_cast<v4f*>(lds);              // [wave][lane]
+    part[wave * 64 + lane] = acc;
     __syncthreads();
     if (wave != 0) return;
-    v4f v = part[0][lane];
+    v4f v = part[lane];
 #pragma unroll
-    for (int q = 1; q < DOWN_WAVES; ++q) v += part[q][lane];
-    if (c < p.T) store_y(p, c, n0 + 4 * g, v);
+    for (int q = 1; q < C::WAVES; ++q) v += part[q * 64 + lane];
+    if (c < p.T) store_y(p, c, n0 + 4 * g, v, residual);
 }
 
 // ---- more rows per expert -----------------------------------------------------------------------------------------------
@@ -457,9 +525,6 @@ __global__ void __launch_bounds__(DOWN_WAVES * 64) moe_few_down_kernel(MoeParams
 
 // Kernel 2 leaves the pairs' results in fp32, and a third kernel adds up the choices of each token, in their order.
 
-// LDS place of 16-byte chunk i of weight row r (128 bytes): i ^ this.
-__device__ __forceinline__ int weight_swz(int r) { return (r & 2) | ((r >> 1) & 4); }
-
 // WV: waves of a workgroup; AH: units under way.
 template <bool UP, int NT, int CT, int WV, int AH>
 struct Rows {
@@ -475,14 +540,6 @@ struct Rows {
     static constexpr int LOADS = DX + DW + 1;
     static_assert(DX >= 1 && (AH - 1) * LOADS <= 63, "vmcnt range");
 };
-
-// LDS place of 16-byte chunk i of row r: the 16 lanes that are served together (0-3, 12-15 and 20-27; 4-11, 16-19 and 28-31) meet 16
-// places.  Kernel 1: lane group g reads chunks 2 g + ..; kernel 2: 4 g + ..
-template <bool UP>
-__device__ __forceinline__ int chunk_at(int r, int i) {
-    const int c = r & 15;
-    return i ^ (UP ? c : (((c >> 2) ^ (c >> 3)) & 1) | ((c & 3) << 1) | (c & 8));
-}
 
 template <bool UP, bool FP16, int NT, int CT, int WV, int AH>
 __global__ void __launch_bounds__(WV * 64) moe_rows_kernel(MoeParams p, int tiles) {
@@ -665,6 +722,7 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(MoeParams p) {
     for (int i = 0; i < p.k; ++i) first = first && (i >= lane || __builtin_amdgcn_readlane(e, i) != e);
     const uint64_t count = __ballot(first && e >= 0 && e < p.E);
     if (n >= p.H) return;
+    const uint2 residual = residual_at(p, t, n);
     const float* z = p.z + (int64_t)t * p.k * p.H + n;
     v4f v = {0.f, 0.f, 0.f, 0.f};
     for (int j0 = 0; j0 < p.k; j0 += AT_ONCE) {
@@ -675,7 +733,7 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(MoeParams p) {
         for (int j = 0; j < AT_ONCE; ++j)
             if ((count >> (j0 + j)) & 1) v += c[j];
     }
-    store_y(p, t, n, v);
+    store_y(p, t, n, v, residual);
 }
 
 template <bool UP, bool FP16, int NT, int WV>
@@ -697,12 +755,13 @@ int launch_combine(const MoeParams& p, hipStream_t st) {
     return H3FP8_OK;
 }
 
-template <bool FP16>
+template <bool FP16, int TOKENS>
 int launch_few(const MoeParams& p, hipStream_t st) {
     const int tiles = p.F / 16;
-    hipLaunchKernelGGL((moe_few_up_kernel<FP16, 2>), dim3((unsigned)(tiles * std::min(p.E, p.T * p.k))), dim3(UP_WAVES * 64), 0, st, p, tiles);
+    hipLaunchKernelGGL((moe_few_up_kernel<FP16, TOKENS>), dim3((unsigned)(tiles * std::min(p.E, p.T * p.k))), dim3(Few<true, TOKENS>::WAVES * 64), 0, st,
+                       p, tiles);
     H3_CHECK_HIP(hipGetLastError());
-    hipLaunchKernelGGL((moe_few_down_kernel<2>), dim3((unsigned)(p.H / 16)), dim3(DOWN_WAVES * 64), 0, st, p);
+    hipLaunchKernelGGL((moe_few_down_kernel<TOKENS>), dim3((unsigned)(p.H / 16)), dim3(Few<false, TOKENS>::WAVES * 64), 0, st, p);
     H3_CHECK_HIP(hipGetLastError());
     return H3FP8_OK;
 }
@@ -718,7 +777,7 @@ bool few(int64_t T, int64_t k, int64_t H, int64_t F, int64_t E) {
 
 template <bool FP16>
 int run(const MoeParams& p, hipStream_t st) {
-    if (few(p.T, p.k, p.H, p.F, p.E)) return launch_few<FP16>(p, st);
+    if (few(p.T, p.k, p.H, p.F, p.E)) return p.T <= 2 ? launch_few<FP16, 2>(p, st) : launch_few<FP16, 8>(p, st);
     // Blocks of 32 rows and 8 waves past 20 rows per expert, in kernel 2 while they are items enough for the CUs (one of 256
     // channels and all rows of an expert at least); else blocks of 16 and 4 waves.  us, 16 rows and 4 waves / 32 and 8, kernel 1 and
     // kernel 2: 32 experts of 4096 x 2048, 12 rows each 104 / 98 and 58 / 58, 16 110 / 122 and 64 / 71, 24 132 / 117 and 77 / 75,
