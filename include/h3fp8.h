@@ -344,13 +344,13 @@ int h3fp8_moe_route(const void* logits, int64_t ld, int dtype, int64_t T, int64_
                     int32_t* place, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
- * A whole layer of block-scaled experts for at most 128 tokens, two launches (up to 8 pairs) or three:
+ * A whole layer of block-scaled experts for at most 128 tokens, two launches (up to 8 or 16 pairs) or three:
  *   y[t] = residual[t] + sum_j weights[t, j] * W2[e] (silu(g) * u),  g | u = W1[e] x[t],  e = experts[t, j]
  * x, residual (or NULL), y [T, H] bf16 or fp16 (dtype), not quantised; w1 [E, 2F, H] (gate rows, then up rows) and w2 [E, H, F]
  * e4m3 with expert strides and row strides, scales [E, ceil(2F / 128), ceil(H / 128)] and [E, ceil(H / 128), ceil(F / 128)] in
  * any strides; weights, experts, offsets, order: those of h3fp8_moe_route.  fp32 throughout, the inner values h carried in 16
  * bits of mantissa, one rounding of y.  An expert's NaN or infinity reaches its own tokens only.  y may be the residual itself.
- * H, F multiples of 16; x and weights 16-byte aligned, row strides of x multiples of 8, of the weights of 16, of y and the
+ * H, F multiples of 16 up to 2^22; x and weights 16-byte aligned, row strides of x multiples of 8, of the weights of 16, of y and the
  * residual of 4 (8-byte aligned); 256 rows of x and 128 of a weight within 2 GiB, all scales of a layer within 1.  workspace:
  * h3fp8_moe_blocks_workspace bytes of device memory, 16-byte aligned.
  */

@@ -9,10 +9,10 @@
 // scale in fp32.  Kernel 1 leaves h times the pair's weight as two bf16 numbers, the value and what its rounding left (16 bits
 // in all), so that the layer has one rounding to the output's type and none that counts before.
 //
-// Up to 8 pairs (a token or a few) what counts is the latency up to the first bytes: kernels that find their rows by ballots.
+// Up to 8 or 16 pairs (a token or a few) what counts is the latency up to the first bytes: kernels that find their rows by ballots.
 // Past that a workgroup's waves share the tokens' values through LDS, and its items follow each other without a pause.
 //
-// us of the kernels together, and the weights' bytes over that: 4 experts of 4096 x 2048 (1 token) 29, 3.5 TB/s; 12 of 1200 x
+// us of the kernels together, and the weights' bytes over that: 4 experts of 4096 x 2048 (1 token) 24, 4.3 TB/s; 12 of 1200 x
 // 1040 (37 tokens, fp16) 24, 1.9; 28 to 32 of 4096 x 2048 (16 tokens) 116 to 128, 6.1; 32 of 4096 x 2048 (128 tokens, 1024 pairs)
 // 186 to 200, 4.2.  A copy of 2 GiB runs at 5.0 TB/s, read and written together.
 #include <algorithm>
@@ -239,7 +239,7 @@ __device__ __forceinline__ void store_y(const MoeParams& p, int t, int n, v4f v,
 
 // ---- a token or a few -----------------------------------------------------------------------------------------------------
 //
-// What counts is how soon the weights' bytes are asked for.  The pairs, at most 64, are a lane each: the experts that have
+// What counts is how soon the weights' bytes are asked for.  The pairs, at most 16, are a lane each: the experts that have
 // pairs, the pairs of one and their tokens come out of ballots on one load of `experts`, by every wave for itself.
 
 // LDS place of 16-byte chunk i of weight row r (128 bytes): i ^ this.
@@ -260,7 +260,8 @@ __device__ __forceinline__ uint64_t first_pairs(uint64_t same, int lane, int k) 
 }
 
 // A wave has two units under way, in LDS of its own: weights in whole lines, the values of up to TOKENS tokens (more columns of the
-// MFMAs repeat them), scales.
+// MFMAs repeat them), scales.  (Straight into registers, a lane 16 bytes of its row, the memory pipe took a clock per lane: 1 token,
+// 4 experts of 4096 x 2048 29 us in place of 24, 8 of 1536 x 2304 42 in place of 28.)
 template <bool UP, int TOKENS>
 struct Few {
     static constexpr int WAVES = UP ? 8 : TOKENS > 2 ? 8 : 16;
@@ -768,11 +769,13 @@ int launch_few(const MoeParams& p, hipStream_t st) {
 
 // ---- which kernels run --------------------------------------------------------------------------------------------------
 //
-// A token or a few, while launches and first loads count (up to 8 pairs, 128 MiB of their experts' weights); then by rows.  us of
-// the kernels, few / by rows, 32 experts of 4096 x 2048: 4 pairs 26 / 40, 8 53 / 47, 16 88 / 73; 8 of 2048 x 2048: 4 pairs 22 / 32,
-// 8 30 / 32, 16 38 / 32; 16 of 1200 x 1040: 4 pairs 14 / 26, 8 23 / 27, 16 28 / 27.
+// A token or a few, while launches and first loads count: one or two tokens up to 16 pairs, up to 8 tokens at 8 pairs and 128 MiB of
+// their experts' weights; then by rows.  us of the kernels, few / by rows, for 1 x 4 (token x choices), 2 x 4, 2 x 8, 8 x 1, 4 x 4:
+// 32 experts of 4096 x 2048 24 / 40, 41 / 47, 74 / 79, 47 / 42, 87 / 73; 8 of 2048 x 2048 18 / 33, 24 / 33, 29 / 33, 31 / 32,
+// 39 / 33; 16 of 1200 x 1040 13 / 23, 20 / 25, 26 / 26, 20 / 25, 33 / 26; 128 of 2048 x 1024 14 / 28, 18 / 29, 29 / 30, 23 / 28,
+// 40 / 30.
 bool few(int64_t T, int64_t k, int64_t H, int64_t F, int64_t E) {
-    return T * k <= 8 && 3 * H * F * std::min(T * k, E) <= (128LL << 20);
+    return T <= 2 ? T * k <= 16 : T * k <= 8 && 3 * H * F * std::min(T * k, E) <= (128LL << 20);
 }
 
 template <bool FP16>
@@ -808,8 +811,8 @@ extern "C" int h3fp8_moe_blocks(const void* x, int64_t ldx, int dtype, int64_t T
     H3_REQUIRE(E >= 1 && E <= MAX_E && k >= 1 && k <= MAX_K && k <= E, "%s: k = %d of %lld experts (at most %d of %d)", who, k,
                (long long)E, MAX_K, MAX_E);
     H3_REQUIRE(dtype == H3FP8_DT_BF16 || dtype == H3FP8_DT_FP16, "%s: bad dtype %d", who, dtype);
-    H3_REQUIRE(H >= 16 && F >= 16 && H % 16 == 0 && F % 16 == 0 && H <= (1 << 24) && F <= (1 << 24),
-               "%s: H=%lld and F=%lld must be positive multiples of 16", who, (long long)H, (long long)F);
+    H3_REQUIRE(H >= 16 && F >= 16 && H % 16 == 0 && F % 16 == 0 && H <= (1 << 22) && F <= (1 << 22),
+               "%s: H=%lld and F=%lld must be positive multiples of 16, at most 2^22", who, (long long)H, (long long)F);
     if (T == 0) return H3FP8_OK;
     H3_REQUIRE(x && w1 && s1 && w2 && s2 && weights && experts && offsets && order && y && workspace, "%s: null pointer", who);
     H3_REQUIRE(((((uintptr_t)x | (uintptr_t)w1 | (uintptr_t)w2 | (uintptr_t)workspace) & 15) | (((uintptr_t)y | (uintptr_t)residual) & 7)) == 0,

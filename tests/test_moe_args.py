@@ -119,13 +119,17 @@ def test_c_entries():
               ldy=256, ws=p, ws_bytes=4 * 2 * 128 * 4):
         return L.h3fp8_moe_blocks(x, ldx, dtype, T, H, F, E, k, w, we, ld1, s, 4, sn, sk, w, we, ld2, s, 4, sn, sk, r, r, r, r, res, ldr, y, ldy, ws,
                                   ws_bytes, None)
-    for kw in (dict(T=-1), dict(T=129), dict(E=0), dict(E=513), dict(k=0), dict(k=9), dict(k=17, E=32), dict(dtype=2), dict(H=0), dict(H=248), dict(F=120),
+    for kw in (dict(T=-1), dict(T=129), dict(E=0), dict(E=513), dict(k=0), dict(k=9), dict(k=17, E=32), dict(dtype=2), dict(H=0), dict(H=248), dict(F=120), dict(F=(1 << 22) + 16),
                dict(x=None), dict(w=None), dict(s=None), dict(r=None), dict(y=None), dict(ws=None), dict(ws_bytes=4095), dict(ldx=255), dict(ldx=252),
                dict(ldy=254), dict(ld1=240), dict(ld1=264), dict(ld2=120), dict(we=8), dict(we=-16), dict(sn=-1), dict(x=ctypes.c_void_p(4104)),
                dict(y=ctypes.c_void_p(4100)), dict(res=ctypes.c_void_p(4100)), dict(res=p, ldr=-4), dict(res=p, ldr=2), dict(s=ctypes.c_void_p(4098)),
                dict(r=ctypes.c_void_p(4098)), dict(ldx=1 << 24), dict(ld1=1 << 26), dict(sn=1 << 30)):
         assert layer(**kw) == -22, kw
     assert layer(T=0) == 0
+    # h alone for a token or a few, else the pairs' results too
+    ws = L.h3fp8_moe_blocks_workspace
+    assert ws(1, 16, 256, 128, 32) == 16 * 4 * 128 and ws(2, 9, 256, 128, 32) == 18 * 4 * (128 + 256)
+    assert ws(8, 1, 256, 128, 32) == 8 * 4 * 128 and ws(8, 1, 4096, 2048, 32) == 8 * 4 * (2048 + 4096) and ws(9, 1, 256, 128, 32) == 9 * 4 * (128 + 256)
 
     def act(bias=None, act=0, res=None, ldr=64, ldy=64, out_dtype=0, M=4, N=64, K=64):
         return L.h3fp8_gemm_blocks_act(p, 64, p, 64, p, 1, 1, p, 1, 1, bias, act, res, ldr, p, ldy, out_dtype, M, N, K, None)
