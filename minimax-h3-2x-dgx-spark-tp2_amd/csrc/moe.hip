@@ -12,9 +12,9 @@
 // Up to 8 or 16 pairs (a token or a few) what counts is the latency up to the first bytes: kernels that find their rows by ballots.
 // Past that a workgroup's waves share the tokens' values through LDS, and its items follow each other without a pause.
 //
-// us of the kernels together, and the weights' bytes over that: 4 experts of 4096 x 2048 (1 token) 24, 4.3 TB/s; 12 of 1200 x
-// 1040 (37 tokens, fp16) 24, 1.9; 28 to 32 of 4096 x 2048 (16 tokens) 116 to 128, 6.1; 32 of 4096 x 2048 (128 tokens, 1024 pairs)
-// 186 to 200, 4.2.  A copy of 2 GiB runs at 5.0 TB/s, read and written together.
+// us of a layer, and the weights' bytes over that: 4 experts of 4096 x 2048 (1 token) 24, 4.3 TB/s; 2 of 1536 x 2304 (1 token)
+// 13.5, 1.6; 12 of 1200 x 1040 (37 tokens, fp16) 24, 1.9; 23 to 28 of 4096 x 2048 (16 tokens) 113 to 134, 5.2; 32 of them (128
+// tokens, 1024 pairs) 186 to 206, 4.1.  A copy of 2 GiB runs at 5.0 TB/s, read and written together.
 #include <algorithm>
 #include <type_traits>
 
@@ -521,8 +521,9 @@ __global__ void __launch_bounds__((Few<false, TOKENS>::WAVES * 64)) moe_few_down
 // row, which the memory pipe takes one by one); weights in whole lines of 128 bytes through LDS, blocks of one expert at the same
 // time on one XCD, so that its L2 has the weights, and each item's K from a start of its own, (3 e + 5 tile) units in (rows a
 // power of two apart meet the same channels: 7 to 8 %), 115 / 200.  What bounds it now: up to 20 rows per expert the weights' bytes
-// (6.1 TB/s); past that the largest XCD's items, whole rounds of blocks over its 32 CUs.  Blocks of 64 rows make those rounds
-// coarser: 110 to 140 us in kernel 1 against 114, 83 to 105 in kernel 2 against 78.
+// (5.2 TB/s; kernel 1 5.8); past that the largest XCD's items, whole rounds of blocks over its 32 CUs.  Blocks of 64 rows make those rounds
+// coarser: 110 to 140 us in kernel 1 against 114, 83 to 105 in kernel 2 against 78; two waves to a block of K in kernel 2, so that
+// each reads half the tokens' values from LDS, take 79.
 
 // Kernel 2 leaves the pairs' results in fp32, and a third kernel adds up the choices of each token, in their order.
 
