@@ -97,6 +97,19 @@ def test_strides(cuda):
         assert torch.equal(ops.gemm_blocks_act(a, w, sa, sw, BF16, None, "relu", one), ops.gemm_blocks_act(a, w, sa, sw, BF16, None, "relu", one.contiguous()))
 
 
+def test_offsets_past_32_bits(cuda):
+    g = torch.Generator(device=cuda).manual_seed(10)
+    M, N, K = 2200, 5376, 128
+    a, w = codes(g, M, K), codes(g, N, K)
+    sa, sw = scales(g, M, 1), scales(g, N // 128, 1)
+    res = torch.empty(M, 1 << 20, dtype=BF16, device=cuda)[:, :N]
+    res.copy_(torch.randn(M, N, generator=g, device=cuda))
+    for m in (M, 300):
+        want = ops.gemm_blocks_act(a[:m], w, sa[:m], sw, BF16, None, "silu", res[:m].contiguous())
+        out = torch.empty(m, 1 << 20, dtype=BF16, device=cuda)[:, :N]
+        assert torch.equal(ops.gemm_blocks_act(a[:m], w, sa[:m], sw, BF16, None, "silu", res[:m], out=out), want)
+
+
 def test_captured_on_streams_and_natively(cuda, monkeypatch):
     g = torch.Generator(device=cuda).manual_seed(9)
     shapes = [(1, 1040, 272), (60, 1040, 400), (300, 5376, 256), (2100, 5376, 144)]

@@ -235,6 +235,30 @@ def test_layer_at_its_limits(cuda, T, E, k, H, F):
     check(ops.moe_blocks(x, w1, s1, w2, s2, r), *moe64(x, w1, s1, w2, s2, r.weights, r.experts), BF16)
 
 
+def test_offsets_past_32_bits(cuda):
+    """Rows of logits, experts' weights and outputs more than 4 GiB apart."""
+    g = torch.Generator(device=cuda).manual_seed(12)
+    far = torch.empty(600, 1 << 21, device=cuda)[:, :40]
+    far.copy_(torch.randn(600, 40, generator=g, device=cuda))
+    same_route(ops.moe_route(far, 4), route64(far, 4), far)
+    E, H, F = 3, 272, 144
+    w1, s1, w2, s2 = layer(g, E, H, F, cuda)
+    apart = torch.empty(E, (9 << 28) // 16, 16, dtype=torch.uint8, device=cuda)
+
+    def spaced(w, at):
+        v = apart[:, at:at + w.shape[1] * w.shape[2] // 16].view(E, w.shape[1], w.shape[2]).view(w.dtype)
+        v.view(torch.uint8).copy_(w.view(torch.uint8))
+        return v
+    v1, v2 = spaced(w1, 0), spaced(w2, 1 << 20)
+    assert v1.stride(0) * 2 > 1 << 32
+    for T, k in ((1, 3), (40, 2)):
+        x = torch.randn(T, H, generator=g, device=cuda).to(BF16)
+        r = ops.moe_route(torch.randn(T, E, generator=g, device=cuda), k)
+        out = torch.empty(T, 1 << 26, dtype=BF16, device=cuda)[:, :H]
+        y = ops.moe_blocks(x, w1, s1, w2, s2, r, residual=x)
+        assert torch.equal(ops.moe_blocks(x, v1, s1, v2, s2, r, residual=x, out=out), y)
+
+
 def test_layer_without_tokens(cuda):
     g = torch.Generator(device=cuda).manual_seed(1)
     w = layer(g, 3, 144, 80, cuda)
