@@ -315,7 +315,8 @@ int h3fp8_qk_norm_rope(const void* q, int64_t q_t, int64_t q_h, const void* k, i
 /*
  * The block-scaled product with an epilogue: y = round(residual + act(the sum of h3fp8_gemm_blocks + bias)), fp32 up to the
  * one rounding.  Operands, scales, strides and sizes as h3fp8_gemm_blocks; act one of H3FP8_ACT_*; residual [M, N] in y's
- * type, row stride ldr (a multiple of 8; 0: one row for all), or NULL; bias and residual 16-byte aligned; y may be the residual itself.
+ * type, row stride ldr (a multiple of 8; 0: one row for all), or NULL; bias and residual 16-byte aligned; y may be the residual
+ * itself.  One launch, or two: the rows that fill whole rounds of large tiles, and the rest.
  */
 #define H3FP8_ACT_NONE 0
 #define H3FP8_ACT_SILU 1         /* v / (1 + exp(-v)) */

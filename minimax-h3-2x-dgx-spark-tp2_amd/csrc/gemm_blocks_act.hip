@@ -8,8 +8,8 @@
 // in the same piece, so that the output may be the residual itself.
 //
 // us, here / the product alone with a bias: 1 x 5376 -> 21 504, gelu_tanh 20 / 20.4; 200 x 7168 -> 5376 fp16 onto a residual 20.4
-// (weights from HBM 25 / 25); 4100 x 5376 -> 14 336, gelu 309 to 318 / 292 to 309; 18 880 x 14 336 -> 5376 onto a residual 1300 to
-// 1330 / 1217 to 1290.  What bounds it is the product (gemm_blocks_core.h); the epilogue of the 256 x 256 tiles stands between two
+// (weights from HBM 25 / 25); 4100 x 5376 -> 14 336, gelu 309 to 318 / 292 to 309; 18 880 x 14 336 -> 5376 onto a residual 1255 to
+// 1316 (in one launch 1300 to 1359) / 1217 to 1290.  What bounds it is the product (gemm_blocks_core.h); the epilogue of the 256 x 256 tiles stands between two
 // tiles of its workgroup: the residual's 203 MB 35 us, gelu's 15 instructions an element 45 (silu and gelu_tanh 25, relu none).
 // Its registers are the k-steps' own: a value that only they used, kept in memory during them, was loaded again in every k-step
 // and waited for all the loads under way (1400 us in place of 1295 with a bias alone).  The activation's
@@ -171,10 +171,17 @@ int launch_small(const BlocksParams& p, const ActParams& a, const char* who, hip
     return H3FP8_OK;
 }
 
-int run(const BlocksParams& p, const ActParams& a, const char* who, hipStream_t st) {
-    if (p.M == 0 || p.N == 0) return H3FP8_OK;
+// The rows that fill whole rounds of 256 x 256 tiles on G CUs, where what is left is up to half a round: a launch of smaller tiles
+// (the same sums) takes it in less than the round that it would cost.  us, in one launch / split, tiles left of 256 in brackets:
+// 6200 x 5376 x 7168 277 / 220 (21), 12 500 x 5376 x 5376 387 / 354 (21), 18 880 x 5376 x 14 336 1359 / 1306 (21), 18 880 x 14 336
+// x 5376 1381 / 1342 (56), 3800 x 5376 x 7168 183 / 148 (63), 16 740 x 9216 x 3328 545 / 540 (72), 4200 x 5376 x 7168 184 / 166 (105).
+int64_t whole_rounds(int64_t M, int64_t N, int G) {
+    const int64_t cols = (N + 255) / 256, tiles = (M + 255) / 256 * cols, rt = tiles / G * G / cols;
+    return rt > 0 && 2 * (tiles - rt * cols) <= G ? rt * 256 : M;
+}
+
+int run_form(const BlocksParams& p, const ActParams& a, int form, const char* who, hipStream_t st) {
     const bool nt = streams(p);
-    const int form = dense_form(p.M, p.N, h3host::cu_count());
     switch (form) {
 #define X(id, calls, per, ...)                                                                                         \
     case id:                                                                                                           \
@@ -191,6 +198,23 @@ int run(const BlocksParams& p, const ActParams& a, const char* who, hipStream_t 
     }
     H3_REQUIRE(false, "%s: no kernel for form %d", who, form);
     return H3FP8_OK;
+}
+
+int run(const BlocksParams& p, const ActParams& a, const char* who, hipStream_t st) {
+    if (p.M == 0 || p.N == 0) return H3FP8_OK;
+    const int G = h3host::cu_count(), form = dense_form(p.M, p.N, G);
+    const int64_t rows = form == F_256x256 ? whole_rounds(p.M, p.N, G) : p.M;
+    if (rows == p.M) return run_form(p, a, form, who, st);
+    BlocksParams head = p, rest = p;
+    ActParams b = a;
+    head.M = rows;
+    rest.M = p.M - rows;
+    rest.a += rows * p.lda;
+    rest.sa += rows * p.sa_m;
+    rest.y += rows * p.ldy;
+    if (a.residual) b.residual += rows * a.ldr;
+    const int rc = run_form(head, a, form, who, st);
+    return rc ? rc : run_form(rest, b, dense_form(rest.M, p.N, G), who, st);
 }
 
 }  // namespace

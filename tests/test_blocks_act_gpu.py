@@ -8,9 +8,9 @@ from h3_tp2_amd import ops
 pytestmark = pytest.mark.gpu
 E4M3, BF16, FP16 = torch.float8_e4m3fn, torch.bfloat16, torch.float16
 ACTS = (None, "silu", "gelu", "gelu_tanh", "relu")
-# every form of the dense rule on 256 CUs, with edges in rows, channels and K
+# every form of the dense rule on 256 CUs, with edges in rows, channels and K; the last two in whole rounds and a rest
 SHAPES = [(1, 400, 272), (16, 1040, 400), (30, 13008, 144), (40, 1296, 528), (100, 5376, 256), (200, 5376, 272), (256, 8208, 144), (500, 5376, 400),
-          (1000, 5376, 272), (2100, 5376, 144), (4100, 5376, 128)]
+          (1000, 5376, 272), (2100, 5376, 144), (4100, 5376, 128), (6200, 5376, 272)]
 
 
 def act64(v, act):
@@ -83,7 +83,7 @@ def test_activation_values(cuda, dtype, act):
 
 def test_strides(cuda):
     g = torch.Generator(device=cuda).manual_seed(8)
-    for M, N, K in ((5, 272, 144), (300, 1040, 272), (2100, 5376, 144)):
+    for M, N, K in ((5, 272, 144), (300, 1040, 272), (2100, 5376, 144), (6200, 5376, 144)):
         a, w = codes(g, M, K), codes(g, N, K)
         sa, sw = scales(g, M, -(-K // 128)), scales(g, -(-N // 128), -(-K // 128))
         wide = torch.randn(M, 2 * N + 16, generator=g, device=cuda).to(BF16)
@@ -112,7 +112,7 @@ def test_offsets_past_32_bits(cuda):
 
 def test_captured_on_streams_and_natively(cuda, monkeypatch):
     g = torch.Generator(device=cuda).manual_seed(9)
-    shapes = [(1, 1040, 272), (60, 1040, 400), (300, 5376, 256), (2100, 5376, 144)]
+    shapes = [(1, 1040, 272), (60, 1040, 400), (300, 5376, 256), (2100, 5376, 144), (6200, 5376, 144)]
     calls = []
     for M, N, K in shapes:
         a, w = codes(g, M, K), codes(g, N, K)
