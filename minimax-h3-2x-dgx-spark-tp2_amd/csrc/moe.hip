@@ -513,8 +513,9 @@ __global__ void __launch_bounds__((Few<false, TOKENS>::WAVES * 64)) moe_few_down
 // With many rows the tokens' values, read again for every 16 weight rows, are more than the weights.  So the waves of a workgroup
 // (4 or 8) take neighbouring tiles of weight rows, the whole of K each (no join), and share the tokens' values through LDS: an item
 // is a block of up to 16 NT rows of an expert and a tile of 16 output channels (kernel 1, gate and up rows) or 32 (kernel 2) per
-// wave.  A unit is a block of 128 of K.  Tokens, weights and scales come by LDS-DMA, two units ahead of their use in a ring of
-// three, one barrier per unit; the loads of the next item follow those of the last without a pause.
+// wave; of a few items two groups of 4 waves take alternate units each.  A unit is a block of 128 of K.  Tokens, weights and scales
+// come by LDS-DMA, two units ahead of their use in a ring of three, one barrier per unit; the loads of the next item follow those
+// of the last without a pause.
 //
 // What bounded the steps before, us of the layer at 32 experts of 4096 x 2048, 64 / 1024 pairs: a workgroup per item, the weights
 // straight into registers, 216 / 709; items one behind the other, the tokens shared through LDS, 145 / 330 (a lane had 16 bytes of its
@@ -527,8 +528,8 @@ __global__ void __launch_bounds__((Few<false, TOKENS>::WAVES * 64)) moe_few_down
 
 // Kernel 2 leaves the pairs' results in fp32, and a third kernel adds up the choices of each token, in their order.
 
-// WV: waves of a workgroup; AH: units under way.
-template <bool UP, int NT, int CT, int WV, int AH>
+// KS groups of WV waves share out the units of an item; AH: units under way, of each.
+template <bool UP, int NT, int CT, int WV, int KS, int AH>
 struct Rows {
     static constexpr int RT = UP ? 2 : CT;                // tiles of 16 weight rows of a wave: gate and up; channels
     static constexpr int SC = UP ? 2 : 1;                 // scales of a block, per wave
@@ -538,24 +539,25 @@ struct Rows {
     static constexpr int XSTAGE = 16 * NT * ROW, DX = XSTAGE / 1024 / WV;             // of the tokens: bytes, load instructions of a wave
     static constexpr int WSTAGE = RT * 16 * 128, DW = WSTAGE / 1024;                  // of a wave's weights
     static constexpr int W_OFF = STAGES * XSTAGE, S_OFF = W_OFF + STAGES * WV * WSTAGE;      // behind them the waves' scales, 256 bytes a stage
-    static constexpr int USED = S_OFF + STAGES * 256, LDS = !UP || USED > TEMP_BYTES ? USED : TEMP_BYTES;
+    static constexpr int RING = S_OFF + STAGES * 256, USED = KS * RING, LDS = !UP || USED > TEMP_BYTES ? USED : TEMP_BYTES;
     static constexpr int LOADS = DX + DW + 1;
     static_assert(DX >= 1 && (AH - 1) * LOADS <= 63, "vmcnt range");
+    static_assert(RT * NT * 1024 <= WSTAGE, "a wave's sums take the place of a unit's weights");
 };
 
-template <bool UP, bool FP16, int NT, int CT, int WV, int AH>
-__global__ void __launch_bounds__(WV * 64) moe_rows_kernel(MoeParams p, int tiles) {
-    using C = Rows<UP, NT, CT, WV, AH>;
+template <bool UP, bool FP16, int NT, int CT, int WV, int KS, int AH>
+__global__ void __launch_bounds__(WV * KS * 64) moe_rows_kernel(MoeParams p, int tiles) {
+    using C = Rows<UP, NT, CT, WV, KS, AH>;
     constexpr int BLOCK = 16 * NT, DX = C::DX, DW = C::DW, LPR = C::ROW / 16, RPI = 64 / LPR;       // lanes of a token, tokens of an instruction
     extern __shared__ __attribute__((aligned(1024))) uint8_t rows_lds[];
-    const uint8_t* lds = rows_lds;
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int all = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wave = all % WV, part = all / WV;      // in its group; the group
+    const uint8_t* lds = rows_lds + part * C::RING;
     const int c = lane & 15, g = lane >> 4;
-    const uint32_t lds0 = lds_addr(lds);
-    const Routed R = load_routing<BLOCK, UP>(p, reinterpret_cast<char*>(rows_lds + C::LDS), reinterpret_cast<char*>(rows_lds), WV * 64, tiles);
+    const uint32_t lds0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds_addr(lds));
+    const Routed R = load_routing<BLOCK, UP>(p, reinterpret_cast<char*>(rows_lds + C::LDS), reinterpret_cast<char*>(rows_lds), WV * KS * 64, tiles);
     const int experts = __builtin_amdgcn_readfirstlane(R.count[0]), items = __builtin_amdgcn_readfirstlane(R.count[1]);
-    const int K = UP ? p.H : p.F, N = UP ? p.F : p.H, kb = (K + BK - 1) / BK, units = (kb + AH - 1) / AH * AH;
+    const int K = UP ? p.H : p.F, N = UP ? p.F : p.H, kb = (K + BK - 1) / BK, units = ((kb + KS - 1) / KS + AH - 1) / AH * AH;
     const int64_t ld = UP ? p.ld1 : p.ld2;
     const uint32_t row_bytes = UP ? (uint32_t)p.H * 2u : (uint32_t)p.F * 4u;
     const v4u qx = buffer_desc(UP ? p.x : p.h, UP ? (uint32_t)(((p.T - 1) * p.ldx + p.H) * 2) : (uint32_t)(p.T * p.k) * (uint32_t)p.F * 4u);
@@ -595,11 +597,11 @@ __global__ void __launch_bounds__(WV * 64) moe_rows_kernel(MoeParams p, int tile
             vx[i] = v;
         }
         lu = 0;
-        first = (3 * it.e + 5 * it.tile) % units;
+        first = (3 * it.e + 5 * it.tile) % (units * KS);
     };
     // a unit of the next loads into a stage: always the same instructions, past the last block or item of nothing
     auto load = [&](int stage, int u) {
-        const int blk = u + first >= units ? u + first - units : u + first;
+        const int at = KS * u + part + first, blk = at >= units * KS ? at - units * KS : at;
         const uint32_t x0 = (uint32_t)(blk * C::ROW), xs = lds0 + (uint32_t)(stage * C::XSTAGE + wave * DX * 1024);
 #pragma unroll
         for (int i = 0; i < DX; ++i)
@@ -695,10 +697,26 @@ __global__ void __launch_bounds__(WV * 64) moe_rows_kernel(MoeParams p, int tile
                 stage = stage == C::STAGES - 1 ? 0 : stage + 1;
             }
         }
+        if constexpr (KS > 1) {                           // the groups join, by way of the last unit's weights, where nothing is on its way to
+            const int done = stage == 0 ? C::STAGES - 1 : stage - 1;
+            v4f* sums = reinterpret_cast<v4f*>(rows_lds + C::RING + C::W_OFF + (done * WV + wave) * C::WSTAGE) + lane;
+#pragma unroll
+            for (int i = 0; i < C::RT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+                    if (part == 1) sums[64 * (i * NT + j)] = acc[i][j];
+            wait_lgkm0();
+            barrier_nofence();
+#pragma unroll
+            for (int i = 0; i < C::RT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+                    if (part == 0) acc[i][j] += sums[64 * (i * NT + j)];
+        }
         const int n0 = (it.tile * WV + wave) * C::OUT + 4 * g;
 #pragma unroll
         for (int j = 0; j < NT; ++j)
-            if (16 * j + c < it.n) {
+            if (part == 0 && 16 * j + c < it.n) {
                 const int pair = R.pair[it.r0 + 16 * j + c];
                 if constexpr (UP) {
                     if (n0 < N) store_h(p, pair, n0, R.weight[it.r0 + 16 * j + c], acc[0][j], acc[1][j]);
@@ -738,15 +756,15 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(MoeParams p) {
     store_y(p, t, n, v, residual);
 }
 
-template <bool UP, bool FP16, int NT, int WV>
+template <bool UP, bool FP16, int NT, int WV, int KS>
 int launch_rows(const MoeParams& p, hipStream_t st) {
     constexpr int CT = 2, AH = 2;
-    using C = Rows<UP, NT, CT, WV, AH>;
+    using C = Rows<UP, NT, CT, WV, KS, AH>;
     const int out = WV * C::OUT, tiles = ((UP ? p.F : p.H) + out - 1) / out, P = p.T * p.k, most = std::min(p.E, P) + P / (16 * NT);
     const size_t lds = C::LDS + routed_bytes(p.E, P, UP);
     // 8 waves per CU
-    const int64_t grid = std::min<int64_t>(((int64_t)tiles * most + XCDS - 1) / XCDS * XCDS, std::max(XCDS, 8 / WV * h3host::cu_count() / XCDS * XCDS));
-    hipLaunchKernelGGL((moe_rows_kernel<UP, FP16, NT, CT, WV, AH>), dim3((unsigned)grid), dim3(WV * 64), lds, st, p, tiles);
+    const int64_t grid = std::min<int64_t>(((int64_t)tiles * most + XCDS - 1) / XCDS * XCDS, std::max(XCDS, 8 / (WV * KS) * h3host::cu_count() / XCDS * XCDS));
+    hipLaunchKernelGGL((moe_rows_kernel<UP, FP16, NT, CT, WV, KS, AH>), dim3((unsigned)grid), dim3(WV * KS * 64), lds, st, p, tiles);
     H3_CHECK_HIP(hipGetLastError());
     return H3FP8_OK;
 }
@@ -786,10 +804,20 @@ int run(const MoeParams& p, hipStream_t st) {
     // channels and all rows of an expert at least); else blocks of 16 and 4 waves.  us, 16 rows and 4 waves / 32 and 8, kernel 1 and
     // kernel 2: 32 experts of 4096 x 2048, 12 rows each 104 / 98 and 58 / 58, 16 110 / 122 and 64 / 71, 24 132 / 117 and 77 / 75,
     // 32 150 / 115 and 110 / 79; 8 experts of 2048 x 2048, 32 rows 27 / 22 and 19 / 25; 16 of 1200 x 1040, 32 rows 21 / 17 and 15 / 19.
-    const bool many = p.T * p.k > 20 * p.E;
-    int rc = many ? launch_rows<true, FP16, 2, 8>(p, st) : launch_rows<true, FP16, 1, 4>(p, st);
+    const bool many = p.T * p.k > 20 * p.E, wide = (int64_t)p.H * p.E >= 256 * h3host::cu_count();
+    // Two groups of 4 waves to an item where the items leave half the CUs alone and have 12 blocks of K or more.  us, one / two, kernel
+    // 1: 4 experts of 4096 x 1024 (64 items, 32 blocks) 21.7 / 17.5, 8 of 4096 x 512 (64) 21.8 / 17.4, but 8 of 2048 x 2048 (256 items,
+    // 16 blocks) 15.1 / 16.6, 2 of 1024 x 512 (16, 8) 8.9 / 8.4; kernel 2: 8 of 2048 x 2048 (128, 16) 13.7 / 11.7, 8 of 1536 x 2304
+    // (96, 18) 14.9 / 13.0, but 16 of 1024 x 512 (128, 4) 5.9 / 6.3, 12 of 1200 x 1040 (120, 9) 10.5 / 10.6.
+    const int blocks = std::max(std::min(p.E, p.T * p.k), p.T * p.k / 16);
+    const auto two = [&](int64_t tiles, int K) { return 2 * tiles * blocks <= h3host::cu_count() && K > 11 * BK; };
+    int rc = many                        ? launch_rows<true, FP16, 2, 8, 1>(p, st)
+             : two((p.F + 63) / 64, p.H) ? launch_rows<true, FP16, 1, 4, 2>(p, st)
+                                         : launch_rows<true, FP16, 1, 4, 1>(p, st);
     if (rc) return rc;
-    rc = many && (int64_t)p.H * p.E >= 256 * h3host::cu_count() ? launch_rows<false, false, 2, 8>(p, st) : launch_rows<false, false, 1, 4>(p, st);
+    rc = many && wide                  ? launch_rows<false, false, 2, 8, 1>(p, st)
+         : two((p.H + 127) / 128, p.F) ? launch_rows<false, false, 1, 4, 2>(p, st)
+                                       : launch_rows<false, false, 1, 4, 1>(p, st);
     return rc ? rc : launch_combine(p, st);
 }
 

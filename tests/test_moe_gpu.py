@@ -221,7 +221,8 @@ def test_layer_masks_and_uneven_experts(cuda):
 
 @pytest.mark.parametrize("T,E,k,H,F", [(128, 512, 16, 256, 128), (128, 102, 16, 672, 144), (128, 101, 16, 656, 144), (128, 32, 16, 2064, 272),
                                        (128, 16, 16, 144, 16), (8, 3, 1, 272, 144), (1, 12, 8, 272, 144), (2, 7, 4, 272, 144), (2, 9, 8, 272, 144),
-                                       (1, 20, 16, 400, 272), (2, 20, 9, 272, 144), (8, 2, 1, 4096, 2064)])
+                                       (1, 20, 16, 400, 272), (2, 20, 9, 272, 144), (8, 2, 1, 4096, 2064), (9, 2, 1, 1424, 1552),
+                                       (40, 3, 2, 1552, 2000), (20, 2, 2, 4096, 528)])
 def test_layer_at_its_limits(cuda, T, E, k, H, F):
     """Most tokens, choices and experts; around the rules; a few pairs with equal choices and without one."""
     g = torch.Generator(device=cuda).manual_seed(E)
