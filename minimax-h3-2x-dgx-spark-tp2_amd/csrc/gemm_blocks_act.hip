@@ -152,7 +152,7 @@ gemm_blocks_act_small_kernel(BlocksParams p, int tiles_n, int rt, ActParams a) {
 template <class T>
 int launch_tile(const BlocksParams& p, const ActParams& a, const char* who, hipStream_t st) {
     const int64_t tiles = row_tiles(p, T::TT) * ((p.N + T::TW - 1) / T::TW);
-    H3_REQUIRE(tiles < ((int64_t)1 << 31), "%s: too many tiles for one launch", who);
+    H3_REQUIRE(tiles > 0 && tiles < ((int64_t)1 << 31), "%s: %lld tiles for one launch", who, (long long)tiles);
     const dim3 grid((unsigned)std::min<int64_t>(tiles, h3host::cu_count())), block(T::WAVES * 64);
     if (p.fp16) hipLaunchKernelGGL((gemm_blocks_act_tile_kernel<T, true>), grid, block, 0, st, p, a);
     else hipLaunchKernelGGL((gemm_blocks_act_tile_kernel<T, false>), grid, block, 0, st, p, a);
@@ -163,7 +163,8 @@ int launch_tile(const BlocksParams& p, const ActParams& a, const char* who, hipS
 template <class T>
 int launch_small(const BlocksParams& p, const ActParams& a, const char* who, hipStream_t st) {
     const int64_t tiles_n = (p.N + T::TW - 1) / T::TW, rt = row_tiles(p, T::TT), tiles = rt * tiles_n;
-    H3_REQUIRE(tiles < ((int64_t)1 << 32) / (T::WAVES * 64), "%s: too many tiles for one launch", who);      // 2^32 threads
+    H3_REQUIRE(tiles > 0 && tiles < ((int64_t)1 << 32) / (T::WAVES * 64), "%s: %lld tiles for one launch", who,
+               (long long)tiles);                         // 2^32 threads
     const dim3 grid((unsigned)tiles), block(T::WAVES * 64);
     if (p.fp16) hipLaunchKernelGGL((gemm_blocks_act_small_kernel<T, true>), grid, block, T::LDS, st, p, (int)tiles_n, (int)rt, a);
     else hipLaunchKernelGGL((gemm_blocks_act_small_kernel<T, false>), grid, block, T::LDS, st, p, (int)tiles_n, (int)rt, a);
@@ -175,10 +176,15 @@ int launch_small(const BlocksParams& p, const ActParams& a, const char* who, hip
 // (the same sums) takes it in less than the round that it would cost.  us, in one launch / split, tiles left of 256 in brackets:
 // 6200 x 5376 x 7168 277 / 220 (21), 12 500 x 5376 x 5376 387 / 354 (21), 18 880 x 5376 x 14 336 1359 / 1306 (21), 18 880 x 14 336
 // x 5376 1381 / 1342 (56), 3800 x 5376 x 7168 183 / 148 (63), 16 740 x 9216 x 3328 545 / 540 (72), 4200 x 5376 x 7168 184 / 166 (105).
+// Where none is left over (the tiles fill their rounds, the last row tile full or not) it is one launch of all M rows: tiles that
+// are left are at least a row tile, so that rt * 256 < M.
 int64_t whole_rounds(int64_t M, int64_t N, int G) {
-    const int64_t cols = (N + 255) / 256, tiles = (M + 255) / 256 * cols, rt = tiles / G * G / cols;
-    return rt > 0 && 2 * (tiles - rt * cols) <= G ? rt * 256 : M;
+    const int64_t cols = (N + 255) / 256, tiles = (M + 255) / 256 * cols, rt = tiles / G * G / cols, left = tiles - rt * cols;
+    return rt > 0 && left > 0 && 2 * left <= G ? rt * 256 : M;
 }
+
+// Rows of the first launch.
+int64_t first_rows(int64_t M, int64_t N, int G) { return dense_form(M, N, G) == F_256x256 ? whole_rounds(M, N, G) : M; }
 
 int run_form(const BlocksParams& p, const ActParams& a, int form, const char* who, hipStream_t st) {
     const bool nt = streams(p);
@@ -203,7 +209,7 @@ int run_form(const BlocksParams& p, const ActParams& a, int form, const char* wh
 int run(const BlocksParams& p, const ActParams& a, const char* who, hipStream_t st) {
     if (p.M == 0 || p.N == 0) return H3FP8_OK;
     const int G = h3host::cu_count(), form = dense_form(p.M, p.N, G);
-    const int64_t rows = form == F_256x256 ? whole_rounds(p.M, p.N, G) : p.M;
+    const int64_t rows = first_rows(p.M, p.N, G);
     if (rows == p.M) return run_form(p, a, form, who, st);
     BlocksParams head = p, rest = p;
     ActParams b = a;
@@ -218,6 +224,11 @@ int run(const BlocksParams& p, const ActParams& a, const char* who, hipStream_t 
 }
 
 }  // namespace
+
+namespace h3host {
+// For the tests (host only): the rows of a call's first launch on G CUs; the others are a second one's.
+int64_t gemm_blocks_act_rows(int64_t M, int64_t N, int G) { return first_rows(M, N, G); }
+}  // namespace h3host
 
 extern "C" int h3fp8_gemm_blocks_act(const void* a, int64_t lda, const void* w, int64_t ldw, const float* sa, int64_t sa_m,
                                      int64_t sa_k, const float* sw, int64_t sw_n, int64_t sw_k, const void* bias, int act,
