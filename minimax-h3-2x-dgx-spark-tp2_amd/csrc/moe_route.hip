@@ -421,9 +421,15 @@ __device__ __forceinline__ void pick(const RouteArgs& a, const void* token, floa
         weight = (float)(mine64 * (double)a.scale);
     } else {
         float score = 0.0f;
-        if (expert >= 0) {
-            const float t = expf(a.sigmoid ? -fabsf(mine) : mine - xmax);
-            score = a.sigmoid ? (mine >= 0.0f ? 1.0f : t) / (1.0f + t) : t;
+        if (a.sigmoid) {
+            // over their sum the scores count by their quotients, which are ordinary numbers where fp32 cannot hold the scores
+            // themselves (subnormal from -87, 0 from -104 on): as multiples of exp(the best logit) where that is below 1.  From where
+            // float64 cannot hold one either, 1 + exp(-x) infinite, it is 0, as with a bias.
+            const float low = a.renorm ? fminf(xmax, 0.0f) : 0.0f, t = expf(-fabsf(mine));
+            const float up = mine >= 0.0f ? 1.0f : expf(mine - low);
+            if (expert >= 0 && mine > -709.78271484375f) score = up / (1.0f + t);
+        } else if (expert >= 0) {
+            score = expf(mine - xmax);
         }
         if (a.renorm) sum = sum16(score);
         else if (a.sigmoid) sum = 1.0f;
