@@ -500,7 +500,8 @@ PyObject* grouped_gemm_blocks(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// A residual of y's shape and type that is y itself or whose extent is apart from y's: its pointer and row stride (0: none).
+// A residual of y's shape and type that is y itself or whose extent is apart from y's: its pointer and row stride (0: none; a
+// single row's is its width, whatever stride it came with).
 bool residual_of(PyObject* arg, const at::Tensor& y, int64_t ldy, const void** p, int64_t* ld) {
     *p = nullptr;
     *ld = 0;
@@ -509,6 +510,7 @@ bool residual_of(PyObject* arg, const at::Tensor& y, int64_t ldy, const void** p
     if (!t || t->scalar_type() != y.scalar_type() || t->device() != y.device() || t->dim() != 2 || t->sizes() != y.sizes()) return false;
     *ld = row_stride(*t);
     if (*ld < 0) return false;
+    if (t->size(0) == 1) *ld = t->size(1);
     *p = t->data_ptr();
     const char *a = static_cast<const char*>(*p), *b = static_cast<const char*>(y.data_ptr());
     const int64_t span_a = ((t->size(0) - 1) * *ld + t->size(1)) * 2, span_b = ((y.size(0) - 1) * ldy + y.size(1)) * 2;
