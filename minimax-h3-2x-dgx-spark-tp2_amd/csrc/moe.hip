@@ -612,10 +612,12 @@ __global__ void __launch_bounds__(WV * KS * 64) moe_rows_kernel(MoeParams p, int
         for (int i = 0; i < DW; ++i)
             dma16_at(UP && i >= 2 ? qu : qw, __builtin_amdgcn_readfirstlane(ws + 1024u * i), cw[i & 1] < left ? vw[UP ? i & 1 : i] : OOB,
                      __builtin_amdgcn_readfirstlane(k0));
-        // the wave's scales (of the gate rows, of the up rows), by lanes of its own
-        const uint32_t sb = (uint32_t)(min(blk, kb - 1) * (UP ? p.s1_k : p.s2_k)) * 4u;
+        // the wave's scales (of the gate rows, of the up rows), by lanes of its own; past the last block 0, so that nothing times an
+        // infinite one is no NaN
+        const uint32_t sb = (uint32_t)(blk * (UP ? p.s1_k : p.s2_k)) * 4u;
         if (lane / C::SC == wave)
-            dma4(qs, __builtin_amdgcn_readfirstlane(lds0 + (uint32_t)(C::S_OFF + stage * 256)), (UP && (lane & 1) ? s_up : s_at) + sb);
+            dma4(qs, __builtin_amdgcn_readfirstlane(lds0 + (uint32_t)(C::S_OFF + stage * 256)),
+                 blk < blocks ? (UP && (lane & 1) ? s_up : s_at) + sb : OOB);
     };
     v4f acc[C::RT][NT];
     // a block of K on the first J blocks of 16 tokens
