@@ -333,7 +333,8 @@ int h3fp8_gemm_blocks_act(const void* a, int64_t lda, const void* w, int64_t ldw
  *   ([E], or NULL) of score + bias in 64 bits, the lower index first among equals; a -inf (of the logit or the sum) and a NaN are
  *   never chosen.
  *   weights [T, k] = the chosen scores (renorm: over their sum, 0 where that is 0) * scale; experts [T, k]; choices for which
- *   no expert is left: expert -1, weight 0.  A NaN among a token's logits makes its weights NaN.
+ *   no expert is left: expert -1, weight 0.  A NaN among a token's logits makes its weights NaN.  A score is 0 where exp(-x), or
+ *   exp(x - max), is past float64's range (sigmoid: x <= -709.7828).
  *   order [T k]: the pairs p = t k + j sorted by expert, ascending within one, those without an expert last; offsets [E + 1]: expert
  *   e has the places offsets[e] .. offsets[e + 1] - 1 (the rows of h3fp8_grouped_gemm_blocks); place [T k]: where p went.
  * E at most 512, k at most 16.  workspace: h3fp8_moe_route_workspace(T, E) bytes of device memory, 16-byte aligned (0 up to 128

@@ -280,8 +280,14 @@ __device__ __forceinline__ void pick(const RouteArgs& a, const void* token, floa
         for (int v = 0; v < V; ++v) sum += __builtin_amdgcn_exp2f((x[v] - xmax) * 1.4426950408889634f);
         sum = sum16(sum);
     }
-    // what the rounds go by: the logit, or score + bias in fp32, the score off by at most 2^-20 (hardware exponential and
-    // reciprocal), the sum by 2^-24 of it; beside an infinite logit there are no scores: those experts go by the bias
+    // what the rounds go by: the logit, or score + bias in fp32; beside an infinite logit there are no scores: those experts go by
+    // the bias.  Two scores of a token, s and s', are off against each other
+    //   - by their own exponentials, products and reciprocals (1 ulp each) and the rounding of the exponents' arguments (s |d| 2^-22.8,
+    //     where s is at most exp(-|d|)): 2^-21 in all, a sigmoid's, both of which may be near 1, 2^-20;
+    //   - with softmax by the sum: (V + 4) 2^-24 of it for the additions of a lane and between lanes, up to 2^-18.8, and 2^-20.8 for its
+    //     terms.  That is one factor of all scores, so it takes |s - s'| <= 1 times as much from their difference;
+    //   - by 2^-23 (1 + |sum|) for the two roundings of score + bias.
+    // All together 0.85 (1 + |sum|) 2^-18 at most: the margin of 2^-18 (1 + |sum|) below keeps every expert that 64 bits could choose.
     if constexpr (BIAS) {
         float b[V];
         load_bias<DT, V>(a, l16, b);

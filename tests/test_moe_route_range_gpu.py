@@ -1,4 +1,4 @@
-"""The router's weights at the ends of their range: logits whose sigmoid fp32 cannot hold."""
+"""The router's weights at the ends of their range: logits whose sigmoid fp32 cannot hold, scores that a sum of 512 terms brings off."""
 import pytest
 import torch
 
@@ -35,3 +35,22 @@ def test_sigmoid_where_float64_ends(cuda):
         r = ops.moe_route(x, 2, "sigmoid", bias=bias)
         same_route(r, route64(x, 2, "sigmoid", bias=bias), x)
         assert r.weights.tolist() == [[1.0, 0.0], [0.0, 0.0], [1.0, 0.0], [0.5, 0.5]]
+
+
+@pytest.mark.parametrize("at", [0, 5, 130, 511])
+@pytest.mark.parametrize("below", [16.65, 8.0])
+def test_route_with_bias_near_ties_of_512(cuda, at, below):
+    """One logit that outweighs 511 others, whose terms the fp32 sum rounds away, and a bias that makes scores equal but for its own
+    rounding: of some ten experts, of a third, and of all."""
+    g = torch.Generator(device=cuda).manual_seed(at)
+    E = 512
+    x = 0.01 * torch.randn(5, E, generator=g, device=cuda) - below
+    x[:, at] = 0.0
+    score = torch.softmax(x.double(), 1)
+    near = torch.arange(E, device=cuda)
+    for row in range(5):
+        bias = (0.75 - score[row]).float()
+        for keep in (near % 57 == at % 57, near % 3 == at % 3, near >= 0):
+            for k in (4, 8, 16):
+                kw = dict(scoring="softmax", bias=torch.where(keep, bias, bias - 1.0))
+                same_route(ops.moe_route(x, k, **kw), route64(x, k, **kw), x)
