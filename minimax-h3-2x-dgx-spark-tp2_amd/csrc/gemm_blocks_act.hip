@@ -7,13 +7,16 @@
 // written per element each.  A lane has 4 or 8 consecutive channels of a token, the piece that it stores: it reads the residual
 // in the same piece, so that the output may be the residual itself.
 //
-// us, here / the product alone with a bias: 1 x 5376 -> 21 504, gelu_tanh 20 / 20.4; 200 x 7168 -> 5376 fp16 onto a residual 20.4
-// (weights from HBM 25 / 25); 4100 x 5376 -> 14 336, gelu 309 to 318 / 292 to 309; 18 880 x 14 336 -> 5376 onto a residual 1255 to
-// 1316 (in one launch 1300 to 1359) / 1217 to 1290.  What bounds it is the product (gemm_blocks_core.h); the epilogue of the 256 x 256 tiles stands between two
-// tiles of its workgroup: the residual's 203 MB 35 us, gelu's 15 instructions an element 45 (silu and gelu_tanh 25, relu none).
-// Its registers are the k-steps' own: a value that only they used, kept in memory during them, was loaded again in every k-step
-// and waited for all the loads under way (1400 us in place of 1295 with a bias alone).  The activation's
-// branch is taken per piece: with one for the whole tile the compiler moves its 128 sums through memory (248 bytes a lane).
+// us, here / the product alone with a bias, calls back to back: 1 x 5376 -> 21 504, gelu_tanh 20 / 20.4; 200 x 7168 -> 5376 fp16 onto
+// a residual 20.4 (weights from HBM 25 / 25; the kernel traced 22); 4100 x 5376 -> 14 336, gelu 309 to 312 / 287 to 291 (the first
+// ten calls behind a pause, while the clock settles, 374; traced 329 then); 18 880 x 14 336 -> 5376 onto a residual 1250 to 1257 (in
+// one launch 1322 to 1332) / 1270 to 1276.  What bounds it is the product (gemm_blocks_core.h); the epilogue of the 256 x 256 tiles
+// stands between two tiles of its workgroup.  us on top of the product in one launch, bias alone or relu / silu / gelu_tanh / gelu /
+// residual: 4100 x 5376 -> 14 336 6 / 11 / 16 / 22 / 28, 18 880 x 14 336 -> 5376 16 / 40 / 50 / 55 / 58, 18 880 x 5376 -> 14 336
+// 30 / 70 / 90 / 116 / 118 (541 MB of residual).  Its registers are the k-steps' own: a value that only they used, kept in memory
+// during them, was loaded again in every k-step and waited for all the loads under way (1400 us in place of 1295 with a bias
+// alone).  The activation's branch is taken per piece: with one for the whole tile the compiler moves its 128 sums through memory
+// (248 bytes a lane).
 //
 // The activations take the hardware's exponential and reciprocal (1 ulp each; the exponent's argument, up to 64 in size where
 // the result counts, is rounded to 2^-18): relative errors below 2^-17, a 64th of the smallest rounding behind them.  sigmoid:
@@ -173,9 +176,10 @@ int launch_small(const BlocksParams& p, const ActParams& a, const char* who, hip
 }
 
 // The rows that fill whole rounds of 256 x 256 tiles on G CUs, where what is left is up to half a round: a launch of smaller tiles
-// (the same sums) takes it in less than the round that it would cost.  us, in one launch / split, tiles left of 256 in brackets:
-// 6200 x 5376 x 7168 277 / 220 (21), 12 500 x 5376 x 5376 387 / 354 (21), 18 880 x 5376 x 14 336 1359 / 1306 (21), 18 880 x 14 336
-// x 5376 1381 / 1342 (56), 3800 x 5376 x 7168 183 / 148 (63), 16 740 x 9216 x 3328 545 / 540 (72), 4200 x 5376 x 7168 184 / 166 (105).
+// (the same sums) takes it in less than the round that it would cost.  us with a bias, in one launch / split, tiles left of 256 in
+// brackets: 6200 x 5376 x 7168 263 / 212 (21), 12 500 x 5376 x 5376 354 / 327 (21), 18 880 x 5376 x 14 336 1289 / 1228 (21), 18 880 x
+// 14 336 x 5376 1259 / 1254 (56), 3800 x 5376 x 7168 170 / 141 (63), 16 740 x 9216 x 3328 487 / 485 (72), 4200 x 5376 x 7168 170 / 158
+// (105).
 // Where none is left over (the tiles fill their rounds, the last row tile full or not) it is one launch of all M rows: tiles that
 // are left are at least a row tile, so that rt * 256 < M.
 int64_t whole_rounds(int64_t M, int64_t N, int G) {

@@ -13,8 +13,8 @@
 // Past that a workgroup's waves share the tokens' values through LDS, and its items follow each other without a pause.
 //
 // us of a layer, and the weights' bytes over that: 4 experts of 4096 x 2048 (1 token) 24, 4.3 TB/s; 2 of 1536 x 2304 (1 token)
-// 13.5, 1.6; 12 of 1200 x 1040 (37 tokens, fp16) 24, 1.9; 23 to 28 of 4096 x 2048 (16 tokens) 113 to 134, 5.2; 32 of them (128
-// tokens, 1024 pairs) 186 to 206, 4.1.  A copy of 2 GiB runs at 5.0 TB/s, read and written together.
+// 13.5, 1.6; 12 of 1200 x 1040 (37 tokens, fp16) 24, 1.9; 23 to 28 of 4096 x 2048 (16 tokens) 113 to 136, 5.2; 32 of them (128
+// tokens, 1024 pairs) 186 to 215, 3.7 to 4.3.  A copy of 2 GiB runs at 5.0 TB/s, read and written together.
 #include <algorithm>
 #include <type_traits>
 
